@@ -1,0 +1,82 @@
+// Element types of the sequence-block kernels (layer norm, gated scan, linear_act, distillation): fp32, bf16, fp16 in
+// memory, fp32 in registers.  A granule is VEC consecutive elements moved by one load / store instruction.
+#pragma once
+#include "common.h"
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+template <typename T, int N> struct VecOf { typedef T type __attribute__((ext_vector_type(N))); };
+template <typename T> struct VecOf<T, 1> { typedef T type; };
+
+// raw granule -> floats (exact) and floats -> raw granule (one rounding to nearest even; bf16 on v_cvt_pk_bf16_f32)
+template <typename T, int VEC>
+struct Gran {
+    typedef typename VecOf<T, VEC>::type V;
+    V v;
+    __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const V*>(p); }
+    __device__ __forceinline__ void load_nt(const T* p) { v = __builtin_nontemporal_load(reinterpret_cast<const V*>(p)); }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<V*>(p) = v; }
+    __device__ __forceinline__ void store_nt(T* p) const { __builtin_nontemporal_store(v, reinterpret_cast<V*>(p)); }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (VEC == 1) return (float)v;
+        else return (float)v[i];
+    }
+    __device__ __forceinline__ void set(int i, float f) {
+        if constexpr (VEC == 1) v = (T)f;
+        else v[i] = (T)f;
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) set(i, 0.f);
+    }
+};
+
+// A parameter vector (norm weight, bias) whose type is the activations' T or fp32: elements [i, i + VEC) as floats
+template <typename T, int VEC>
+__device__ __forceinline__ void load_param(float (&o)[VEC], const void* p, bool f32, int64_t i) {
+    if (f32) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = reinterpret_cast<const float*>(p)[i + j];
+    } else {
+        Gran<T, VEC> g;
+        g.load(reinterpret_cast<const T*>(p) + i);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = g.get(j);
+    }
+}
+
+// Sum over the TPR neighbouring threads that share a row: within a wave by shuffles, over several waves through `red`
+// (one float per wave of the block).  Every thread of the block calls it; all threads of a row get the same sum.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+    constexpr int W = TPR < 64 ? TPR : 64;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if constexpr (TPR > 64) {
+        constexpr int NW = TPR / 64;
+        const int wave = threadIdx.x >> 6;
+        __syncthreads();  // the previous use of `red` has been read
+        if ((threadIdx.x & 63) == 0) red[wave] = v;
+        __syncthreads();
+        const int w0 = wave / NW * NW;
+        v = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) v += red[w0 + i];
+    }
+    return v;
+}
+
+static inline bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
+
+// Compute units (one kind of device per process; 256 without one: the host-side plans are tested there).
+static inline int device_cus() {
+    static const int cus = [] {
+        int n = 0;
+        return dssvae_device_cus(&n) == DSSVAE_OK && n > 0 ? n : 256;
+    }();
+    return cus;
+}
+
+static inline int elem_size(int dtype) { return dtype == DSSVAE_F32 ? 4 : 2; }
+static inline bool dtype_ok(int dtype) { return dtype >= DSSVAE_F32 && dtype <= DSSVAE_F16; }

@@ -38,6 +38,7 @@ class GruBwdInst(C.Structure):
 
 
 CELL_GRU, CELL_LSTM = 0, 1
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # DSSVAE_F32 / _BF16 / _F16
 
 
 GEMM_MAX_GROUP = 8
@@ -140,6 +141,9 @@ _SIGNATURES = {
     "dssvae_adam_step_dyn": ([_P, _P, _P, _P, _L, _P, _F, _F, _F, _P, _F, _P, _P], _I),
     "dssvae_batch_rows": ([_P, _P, _P, _I, _I, _I, _L, _L, _L, _P, _P, _P], _I),
     "dssvae_keep_rows": ([_P, _I, _I, _P, _I, _P], _I),
+    "dssvae_layer_norm_fwd": ([_P, _L, _I, _P, _P, _I, _L, _I, _F, _P, _L, _P, _P], _I),
+    "dssvae_layer_norm_bwd_workspace_bytes": ([_L, _I], _L),
+    "dssvae_layer_norm_bwd": ([_P, _L, _I, _P, _L, _P, _I, _P, _L, _I, _P, _L, _P, _P, _P, _L, _P], _I),
 }
 EXPORTS = tuple(_SIGNATURES)
 

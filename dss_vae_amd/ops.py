@@ -4,6 +4,7 @@ import ctypes as C
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import lib as L
 
@@ -1788,3 +1789,131 @@ def adam_step(p, g, m, v, lr, beta1, beta2, eps, step, sumsq_t, max_norm, skip_f
         L.check(L.load().dssvae_adam_step(L.ptr(p), L.ptr(g), L.ptr(m), L.ptr(v), p.numel(), lr, beta1, beta2, eps,
                                           step, L.ptr(sumsq_t), max_norm, None, L.ptr(skip_flag), L.stream()),
                 "dssvae_adam_step")
+
+
+# ----------------------------------------------------------------------------------------------
+# Sequence-block operators: layer norm, gated linear recurrence, linear with activation and residual, distillation.
+# fp32, bf16 or fp16 activations; statistics, states and sums in fp32.  Arguments are checked here and again in the
+# C-ABI; everything runs on the current stream of the inputs' device, workspaces come from torch's allocator (a graph
+# being captured gets its own).
+# ----------------------------------------------------------------------------------------------
+class _Here(object):
+    """the inputs' device as the current one (a launch goes to the current device's stream); free when it already is"""
+    __slots__ = ("dev", "guard")
+
+    def __init__(self, dev):
+        self.dev, self.guard = dev, None
+
+    def __enter__(self):
+        if self.dev.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(self.dev)
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def _typed(what, t):
+    """element type code of a floating tensor on the GPU"""
+    L.require_cuda(t)
+    code = L.DTYPES.get(t.dtype)
+    if code is None:
+        raise RuntimeError("%s: expected float32, bfloat16 or float16, got %s" % (what, t.dtype))
+    return code
+
+
+def _expect(what, name, t, shape, dtypes, device):
+    """an argument's shape, type and device, or a RuntimeError that names it"""
+    if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes or t.device != device:
+        raise RuntimeError("%s: %s must be %s of %s on %s, got %s of %s on %s" % (
+            what, name, list(shape), " or ".join(str(d) for d in dtypes), device, list(t.shape), t.dtype, t.device))
+    return t
+
+
+def _matrix(t):
+    """2-D tensor -> (tensor, row stride) with unit column stride and rows that do not overlap (copied if need be)"""
+    M, N = t.shape
+    if N > 1 and t.stride(1) != 1 or M > 1 and t.stride(0) < N:
+        t = t.contiguous()
+    return t, (t.stride(0) if M > 1 else N)
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _layer_norm_fwd(x2, ldx, code, w, b, eps, stats):
+    y = torch.empty(x2.shape, device=x2.device, dtype=x2.dtype)
+    R, D = x2.shape
+    p = w if w is not None else b
+    with _Here(x2.device), _Span("layer_norm_fwd_kernel", 8.0 * R * D, 2.0 * R * D * x2.element_size(),
+                                 detail="R=%d D=%d" % (R, D)):
+        L.check(L.load().dssvae_layer_norm_fwd(L.ptr(x2), ldx, code, L.ptr(w), L.ptr(b),
+                                               int(p is not None and p.dtype == torch.float32), R, D, eps, L.ptr(y), D,
+                                               L.ptr(stats), L.stream()), "dssvae_layer_norm_fwd")
+    return y
+
+
+class _LayerNormFn(Function):
+    @staticmethod
+    def forward(ctx, x, w, b, eps, code):
+        ctx.set_materialize_grads(False)
+        x2, ldx = _matrix(x.reshape(-1, x.size(-1)))
+        wc, bc = (None if p is None else p.contiguous() for p in (w, b))
+        stats = torch.empty(x2.size(0), 2, device=x.device, dtype=torch.float32)
+        y = _layer_norm_fwd(x2, ldx, code, wc, bc, eps, stats)
+        ctx.save_for_backward(x2, w, stats)
+        ctx.bias_ref, ctx.code, ctx.xshape = b, code, x.shape
+        return y.view(x.shape)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        if dy is None:
+            return (None,) * 5
+        x2, w, stats = ctx.saved_tensors
+        b = ctx.bias_ref
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        R, D = x2.shape
+        x2, ldx = _matrix(x2)
+        dy2, lddy = _matrix(dy.reshape(-1, D))
+        dev, lib = x2.device, L.load()
+        wc = None if w is None else w.contiguous()
+        p = w if w is not None else b
+        dx = torch.empty(R, D, device=dev, dtype=x2.dtype) if need_x else None
+        dw, db = (None if not need else _claim(t) for need, t in ((need_w, w), (need_b, b)))
+        dw = torch.empty(D, device=dev, dtype=w.dtype) if need_w and dw is None else dw
+        db = torch.empty(D, device=dev, dtype=b.dtype) if need_b and db is None else db
+        with _Here(dev), _Span("layer_norm_bwd_kernel", 12.0 * R * D, 3.0 * R * D * x2.element_size(),
+                               detail="R=%d D=%d" % (R, D)):
+            ws = None
+            if need_w or need_b:
+                ws = torch.empty(lib.dssvae_layer_norm_bwd_workspace_bytes(R, D), device=dev, dtype=torch.uint8)
+            L.check(lib.dssvae_layer_norm_bwd(L.ptr(x2), ldx, ctx.code, L.ptr(dy2), lddy, L.ptr(wc),
+                                              int(p is not None and p.dtype == torch.float32), L.ptr(stats), R, D,
+                                              L.ptr(dx), D, L.ptr(dw), L.ptr(db), L.ptr(ws),
+                                              0 if ws is None else ws.numel(), L.stream()), "dssvae_layer_norm_bwd")
+        return None if dx is None else dx.view(ctx.xshape), dw, db, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """(x - mean) / sqrt(var + eps) * weight + bias over the last axis (biased variance); weight / bias [D] of x's type
+    or both float32, either may be None (ones / zeros).  Any leading shape; rows may be strided."""
+    code = _typed("layer_norm", x)
+    if x.dim() < 1 or x.size(-1) < 1:
+        raise RuntimeError("layer_norm: x needs a last axis of at least one element, got %s" % (list(x.shape),))
+    D = x.size(-1)
+    if not eps >= 0.0:
+        raise RuntimeError("layer_norm: eps must not be negative, got %r" % (eps,))
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None:
+            _expect("layer_norm", name, p, (D,), (x.dtype, torch.float32), x.device)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise RuntimeError("layer_norm: weight is %s, bias is %s" % (weight.dtype, bias.dtype))
+    if _wants_grad(x, weight, bias):
+        return _LayerNormFn.apply(x, weight, bias, float(eps), code)
+    x2, ldx = _matrix(x.reshape(-1, D))
+    w, b = (None if p is None else p.contiguous() for p in (weight, bias))
+    return _layer_norm_fwd(x2, ldx, code, w, b, float(eps), None).view(x.shape)

@@ -549,6 +549,29 @@ int dssvae_batch_rows(const int64_t* flat_ids, const int64_t* offsets, const int
                       int64_t sos, int64_t eos, int64_t pad, int64_t* out, int32_t* lengths_out, void* stream);
 int dssvae_keep_rows(const int32_t* lengths, int B, int T, int64_t* keep, int n_keep, void* stream);
 
+/* =============================================================================================
+ * Sequence-block operators (no reference counterpart: the reference has nn.GRU / nn.LSTM and hard targets only).
+ * They extend ABI version 9.  Element type of the activations: a DSSVAE_F32 / _BF16 / _F16 code; sums, statistics and
+ * states are fp32 whatever the type, each output is rounded once.
+ * ============================================================================================= */
+#define DSSVAE_F32 0
+#define DSSVAE_BF16 1
+#define DSSVAE_F16 2
+
+/* ---------------------------------------------------------------------------------------------
+ * Layer norm over the last axis: y = (x - mean) * rstd * w + b, rstd = 1 / sqrt(var + eps), var = mean((x - mean)^2).
+ *   x, y, dy, dx: [rows, D] of `dtype` with row strides ldx .. (elements); w, b, dw, db: [D], fp32 if param_f32 else
+ *   `dtype`; w or b NULL = ones / zeros.  stats [rows, 2] fp32 = (mean, rstd) for the backward pass, or NULL.
+ * Backward: dx, dw, db may each be NULL; dw / db need the workspace (sums of the row groups, added in a fixed order).
+ * rows = 0 clears dw / db.
+ * ------------------------------------------------------------------------------------------- */
+int dssvae_layer_norm_fwd(const void* x, int64_t ldx, int dtype, const void* w, const void* b, int param_f32,
+                          int64_t rows, int D, float eps, void* y, int64_t ldy, float* stats, void* stream);
+int64_t dssvae_layer_norm_bwd_workspace_bytes(int64_t rows, int D);
+int dssvae_layer_norm_bwd(const void* x, int64_t ldx, int dtype, const void* dy, int64_t lddy, const void* w,
+                          int param_f32, const float* stats, int64_t rows, int D, void* dx, int64_t lddx, void* dw,
+                          void* db, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
