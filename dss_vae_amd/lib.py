@@ -144,6 +144,11 @@ _SIGNATURES = {
     "dssvae_layer_norm_fwd": ([_P, _L, _I, _P, _P, _I, _L, _I, _F, _P, _L, _P, _P], _I),
     "dssvae_layer_norm_bwd_workspace_bytes": ([_L, _I], _L),
     "dssvae_layer_norm_bwd": ([_P, _L, _I, _P, _L, _P, _I, _P, _L, _I, _P, _L, _P, _P, _P, _L, _P], _I),
+    "dssvae_gated_scan_chunks": ([_I], _I),
+    "dssvae_gated_scan_workspace_bytes": ([_I, _I, _I, _I], _L),
+    "dssvae_gated_scan_fwd": ([_P, _L, _L, _I, _P, _P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _P, _P, _L, _P], _I),
+    "dssvae_gated_scan_bwd": ([_P, _L, _L, _I, _P, _I, _I, _P, _P, _L, _L, _P, _I, _I, _I, _P, _L, _L, _P, _P, _L, _P], _I),
+    "dssvae_gated_step": ([_P, _L, _I, _P, _I, _I, _I, _P, _L, _P, _P], _I),
 }
 EXPORTS = tuple(_SIGNATURES)
 

@@ -1917,3 +1917,139 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     x2, ldx = _matrix(x.reshape(-1, D))
     w, b = (None if p is None else p.contiguous() for p in (weight, bias))
     return _layer_norm_fwd(x2, ldx, code, w, b, float(eps), None).view(x.shape)
+
+
+def _sequence(t):
+    """[B, T, W] tensor with unit inner stride and rows that do not overlap (copied if need be)"""
+    B, T, W = t.shape
+    if W > 1 and t.stride(2) != 1 or T > 1 and t.stride(1) < W or B > 1 and t.stride(0) < W:
+        t = t.contiguous()
+    return t
+
+
+def _scan_bytes(lib, B, T, H, code, dev):
+    n = lib.dssvae_gated_scan_workspace_bytes(B, T, H, code)
+    return (None, 0) if n <= 0 else (torch.empty(n, device=dev, dtype=torch.uint8), n)
+
+
+def _gated_scan_fwd(x, h0, lengths, reverse, tanh, code, keep):
+    """-> out, h_last, checkpoints (None unless `keep`)"""
+    B, T, H = x.size(0), x.size(1), x.size(2) // 2
+    dev, lib = x.device, L.load()
+    out = torch.empty(B, T, H, device=dev, dtype=x.dtype)
+    h_last = torch.empty(B, H, device=dev, dtype=torch.float32)
+    ckpt = torch.empty(B, lib.dssvae_gated_scan_chunks(T), H, device=dev, dtype=torch.float32) if keep else None
+    with _Here(dev), _Span("gated_scan_fwd_kernel", 12.0 * B * T * H, 3.0 * B * T * H * x.element_size(), T,
+                           detail="B%dT%dH%d" % (B, T, H)):
+        if T == 0:
+            h_last.zero_() if h0 is None else h_last.copy_(h0)
+        elif T == 1 and lengths is None and not keep:
+            L.check(lib.dssvae_gated_step(L.ptr(x), x.stride(0), code, L.ptr(h0), tanh, B, H, L.ptr(out), H, L.ptr(h_last),
+                                          L.stream()), "dssvae_gated_step")
+        else:
+            ws, n = _scan_bytes(lib, B, T, H, code, dev)
+            L.check(lib.dssvae_gated_scan_fwd(L.ptr(x), x.stride(0), x.stride(1), code, L.ptr(h0), L.ptr(lengths), reverse,
+                                              tanh, B, T, H, L.ptr(out), T * H, H, L.ptr(h_last), L.ptr(ckpt), L.ptr(ws), n,
+                                              L.stream()), "dssvae_gated_scan_fwd")
+    return out, h_last, ckpt
+
+
+class _GatedScanFn(Function):
+    @staticmethod
+    def forward(ctx, x, h0, lengths, reverse, tanh, code):
+        ctx.set_materialize_grads(False)
+        xs = _sequence(x)
+        h0 = None if h0 is None else h0.contiguous()
+        out, h_last, ckpt = _gated_scan_fwd(xs, h0, lengths, reverse, tanh, code, True)
+        ctx.save_for_backward(xs, lengths, ckpt)
+        ctx.meta = (reverse, tanh, code)
+        return out, h_last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dh):
+        if dout is None and dh is None:
+            return (None,) * 6
+        x, lengths, ckpt = ctx.saved_tensors
+        reverse, tanh, code = ctx.meta
+        B, T, H = x.size(0), x.size(1), x.size(2) // 2
+        dev, lib = x.device, L.load()
+        x = _sequence(x)
+        dout = None if dout is None else _sequence(dout)
+        dh = None if dh is None else dh.contiguous()
+        dx = torch.empty(B, T, 2 * H, device=dev, dtype=x.dtype)
+        dh0 = torch.empty(B, H, device=dev, dtype=torch.float32) if ctx.needs_input_grad[1] else None
+        with _Here(dev), _Span("gated_scan_bwd_kernel", 18.0 * B * T * H, 5.0 * B * T * H * x.element_size(), T,
+                               detail="B%dT%dH%d" % (B, T, H)):
+            if T == 0:
+                if dh0 is not None:
+                    dh0.zero_() if dh is None else dh0.copy_(dh)
+            else:
+                ws, n = _scan_bytes(lib, B, T, H, code, dev)
+                ob, ot = (0, 0) if dout is None else (dout.stride(0), dout.stride(1))
+                L.check(lib.dssvae_gated_scan_bwd(L.ptr(x), x.stride(0), x.stride(1), code, L.ptr(lengths), reverse, tanh,
+                                                  L.ptr(ckpt), L.ptr(dout), ob, ot, L.ptr(dh), B, T, H, L.ptr(dx),
+                                                  T * 2 * H, 2 * H, L.ptr(dh0), L.ptr(ws), n, L.stream()),
+                        "dssvae_gated_scan_bwd")
+        return dx if ctx.needs_input_grad[0] else None, dh0, None, None, None, None
+
+
+_CANDIDATES = {"tanh": 1, "linear": 0}
+
+
+def _candidate(what, name):
+    if name not in _CANDIDATES:
+        raise RuntimeError("%s: candidate must be one of %s, got %r" % (what, sorted(_CANDIDATES), name))
+    return _CANDIDATES[name]
+
+
+def gated_scan(xproj, h0=None, lengths=None, reverse=False, candidate="tanh"):
+    """Gated linear recurrence over precomputed projections xproj [B, T, 2H] = (z | v):
+    h_t = a_t h_{t-1} + (1 - a_t) n_t with a = sigmoid(z) and n = tanh(v) (candidate="tanh") or v ("linear"): the GRU's
+    update with neither reset gate nor recurrent weight, so that all steps are computed at once.
+    h0 [B, H] float32 (None = zeros); lengths [B] int32 on the device (packed-sequence semantics: values outside 0 .. T are
+    clamped, padding is never read, out is zero there and the state passes through); reverse walks t = T-1 .. 0.
+    -> (out [B, T, H] of xproj's type, h_last [B, H] float32)"""
+    code = _typed("gated_scan", xproj)
+    tanh = _candidate("gated_scan", candidate)
+    if xproj.dim() != 3 or xproj.size(2) < 2 or xproj.size(2) % 2:
+        raise RuntimeError("gated_scan: xproj must be [B, T, 2H], got %s" % (list(xproj.shape),))
+    B, H = xproj.size(0), xproj.size(2) // 2
+    if h0 is not None:
+        _expect("gated_scan", "h0", h0, (B, H), (torch.float32,), xproj.device)
+    if lengths is not None:
+        lengths = _expect("gated_scan", "lengths", lengths, (B,), (torch.int32,), xproj.device).contiguous()
+    if _wants_grad(xproj, h0):
+        return _GatedScanFn.apply(xproj, h0, lengths, int(bool(reverse)), tanh, code)
+    h0 = None if h0 is None else h0.contiguous()
+    return _gated_scan_fwd(_sequence(xproj), h0, lengths, int(bool(reverse)), tanh, code, False)[:2]
+
+
+def gated_step(xproj, h=None, candidate="tanh", h_out=None):
+    """one step of gated_scan for xproj [B, 2H] and the state h [B, H] float32 (None = zeros) -> (out [B, H] of xproj's
+    type, new state [B, H] float32).  h_out: a contiguous float32 buffer the new state is written to; it may be h itself
+    (then the state is updated in place), but must not overlap it otherwise."""
+    code = _typed("gated_step", xproj)
+    tanh = _candidate("gated_step", candidate)
+    if xproj.dim() != 2 or xproj.size(1) < 2 or xproj.size(1) % 2:
+        raise RuntimeError("gated_step: xproj must be [B, 2H], got %s" % (list(xproj.shape),))
+    B, H = xproj.size(0), xproj.size(1) // 2
+    if h is not None:
+        _expect("gated_step", "h", h, (B, H), (torch.float32,), xproj.device)
+    if h_out is not None:
+        _expect("gated_step", "h_out", h_out, (B, H), (torch.float32,), xproj.device)
+        if not h_out.is_contiguous():
+            raise RuntimeError("gated_step: h_out must be contiguous")
+    if _wants_grad(xproj, h):
+        if h_out is not None:
+            raise RuntimeError("gated_step: h_out is for serving (no gradients)")
+        out, hn = gated_scan(xproj.unsqueeze(1), h, None, False, candidate)
+        return out.squeeze(1), hn
+    x, ldx = _matrix(xproj)
+    h = None if h is None else h.contiguous()
+    out = torch.empty(B, H, device=x.device, dtype=x.dtype)
+    hn = torch.empty(B, H, device=x.device, dtype=torch.float32) if h_out is None else h_out
+    with _Here(x.device), _Span("gated_step_kernel", 12.0 * B * H, B * H * (3.0 * x.element_size() + 8.0)):
+        L.check(L.load().dssvae_gated_step(L.ptr(x), ldx, code, L.ptr(h), tanh, B, H, L.ptr(out), H, L.ptr(hn), L.stream()),
+                "dssvae_gated_step")
+    return out, hn

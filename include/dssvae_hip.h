@@ -572,6 +572,29 @@ int dssvae_layer_norm_bwd(const void* x, int64_t ldx, int dtype, const void* dy,
                           int param_f32, const float* stats, int64_t rows, int D, void* dx, int64_t lddx, void* dw,
                           void* db, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Gated linear recurrence (the GRU's update without its reset gate and W_hh: parallel in time)
+ *   a_t = sigmoid(z_t), n_t = tanh(v_t) if tanh_candidate else v_t, h_t = a_t h_{t-1} + (1 - a_t) n_t
+ *   x [B, T, 2H] = (z | v) of `dtype`, strides xb (sequence) and xt (step), unit stride inside; out, dout [B, T, H] with
+ *   ob, ot; dx [B, T, 2H] with gb, gt.  h0, h_last, dh_last, dh0 [B, H] fp32 contiguous; h0 / dh_last / dout NULL = zeros;
+ *   h_last / dh0 may be NULL.  reverse: walks t = T-1 .. 0.  lengths [B] int32 or NULL: steps t >= lengths[b] (clamped to
+ *   0 .. T) leave the state as it is, are not read, and out / dx are zero there.
+ *   checkpoints [B, dssvae_gated_scan_chunks(T), H] fp32: written by the forward pass (NULL: not kept), read by backward.
+ * The workspace (NULL where its size is 0) belongs to one call.  T = 0: nothing is written.
+ * dssvae_gated_step: one token per row, x [B, 2H] with row stride xb, out [B, H] with ob; h_out may be h.
+ * ------------------------------------------------------------------------------------------- */
+int dssvae_gated_scan_chunks(int T);
+int64_t dssvae_gated_scan_workspace_bytes(int B, int T, int H, int dtype);
+int dssvae_gated_scan_fwd(const void* x, int64_t xb, int64_t xt, int dtype, const float* h0, const int32_t* lengths,
+                          int reverse, int tanh_candidate, int B, int T, int H, void* out, int64_t ob, int64_t ot,
+                          float* h_last, float* checkpoints, void* workspace, int64_t workspace_bytes, void* stream);
+int dssvae_gated_scan_bwd(const void* x, int64_t xb, int64_t xt, int dtype, const int32_t* lengths, int reverse,
+                          int tanh_candidate, const float* checkpoints, const void* dout, int64_t ob, int64_t ot,
+                          const float* dh_last, int B, int T, int H, void* dx, int64_t gb, int64_t gt, float* dh0,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+int dssvae_gated_step(const void* x, int64_t xb, int dtype, const float* h, int tanh_candidate, int B, int H, void* out,
+                      int64_t ob, float* h_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
