@@ -6,21 +6,27 @@
 //   D_t = dout_t + E_{t+1}: dz = D (1 - a)(h_t - n), dv = D (1 - a)(1 - n^2 | 1)      (a (h_{t-1} - n) = h_t - n)
 //
 // Both recurrences are affine maps y -> A y + B per channel and compose: (A2, B2) after (A1, B1) = (A1 A2, A2 B1 + B2).
-// A block owns LPR * VEC neighbouring channels of one sequence and walks time in chunks of 128 steps: thread (g, l)
-// holds KT consecutive steps of VEC channels in registers, the block's groups are joined by a shuffle scan inside each
-// wave and through LDS across the waves, the chunk's state is carried in registers.  One read of x (and
-// dout), one write.  The forward pass leaves the state at each chunk's start ("checkpoint", 1/128 of out); backward rebuilds
-// h inside the chunk from it, in fp32, and never reads out.
-// Few sequences and channels, many steps: the time axis is cut into segments; a first launch reads the segment's inputs
-// for its (A, B) per channel, the second starts each segment from the composition of those before it (backward: behind it).
+// A block owns LPR * VEC neighbouring channels of one sequence and walks time in chunks: thread (g, l) holds KT consecutive
+// steps of VEC channels in registers (16 values), the block's groups are joined by a shuffle scan inside each wave and
+// through LDS across the waves, the chunk's state is carried in registers; the next chunk's loads are in flight meanwhile.
+// One read of x (and dout), one write.  The forward pass leaves the state at each chunk's start ("checkpoint"); backward
+// rebuilds h inside the chunk from it, in fp32, and never reads out.
+// A granule is only 4 bytes: the scan costs log2(64 / LPR) shuffled compositions per channel and thread, so many steps per
+// thread (KT = 8, fp32 16) beat wide granules (16-byte ones leave 2: 265 us for backward over 2 x 16384 x 2048 bf16, 8-byte
+// ones 213 us, this form 165 us = 4.1 TB/s; forward 109 / 97 / 82 us = 4.9 TB/s).
+// Too few tiles (128 bytes of channels each) to fill the chip: the time axis is cut into segments; a first launch reads the
+// segment's inputs for its (A, B) per channel, the second starts each segment from the composition of those before it
+// (backward: behind it).  Narrower tiles instead (32 bytes: no second read, but four blocks per cache line) took 192 us
+// forward where the two launches take 164 us.
 // Steps at or behind a sequence's length are the identity (A = 1, B = 0): the state is kept, out and dx are zero there.
 #include "elem.h"
 
 namespace {
 
-constexpr int CHUNK = 128;
-// threads of a block: a thread's share of a chunk is 16 values of a 16-byte granule in either width
+// lanes per row; threads of a block and steps per thread: 128 steps a chunk in either width
+constexpr int LPR = 32, CHUNK = 128;
 template <typename T> constexpr int NT = sizeof(T) == 4 ? 256 : 512;
+template <typename T> constexpr int KT = CHUNK * LPR / NT<T>;
 constexpr int STEP_THREADS = 256;
 
 __device__ __forceinline__ float sigmoid_f(float x) {
@@ -42,7 +48,7 @@ struct Dims {
 
 // what a block works on: channel tile, sequence, segment
 struct Where { int c0, b, seg, len; };
-template <int LPR, int VEC>
+template <int VEC>
 __device__ __forceinline__ Where where(const Dims& d) {
     const int wid = xcd_remap(blockIdx.x, gridDim.x);  // neighbouring tiles, which may share cache lines, on one XCD
     Where w;
@@ -61,7 +67,7 @@ __device__ __forceinline__ Where where(const Dims& d) {
 // ones.  Lanes scan their wave's groups by shuffles, the waves' totals meet in LDS (one barrier), and every wave runs the NW
 // totals over the carry by itself: 2 NW floats read per lane, where reading them per thread and channel cost VEC times that.
 // prod (or NULL): the product of the chunk's A, per channel.
-template <int NW, int LPR, int VEC, bool FWD>
+template <int NW, int VEC, bool FWD>
 __device__ __forceinline__ void block_scan(float (&A)[VEC], float (&B)[VEC], float& carry, float (&y)[VEC],
                                            float2* lds /* [NW][LPR * VEC] */, float* prod = nullptr) {
     constexpr int GW = 64 / LPR, CH = LPR * VEC;  // groups per wave, channels
@@ -111,219 +117,262 @@ __device__ __forceinline__ float enter(float y, const float* __restrict__ maps, 
     return y;
 }
 
-// One chunk's loads for this thread: granules of (z | v) of its KT steps; steps that are not live are not read.
-template <typename T, int VEC, int LPR, int KT, bool HALF>
+// This thread's steps of a chunk.  Pointers walk: one 64-bit add per row instead of a multiplication (which cost more than
+// the recurrence).  Bit k of `live`: step k is inside [lo, hi); steps that are not are neither read nor used.
+template <typename T, int VEC, bool HALF, bool GRAD>
 struct Steps {
-    Gran<T, VEC> z[KT], v[HALF ? 1 : KT], g[KT];
-    unsigned live;   // bit k: step k is live
-    __device__ __forceinline__ void load(const T* x, const T* dout, const Dims& d, const Where& w, int chunk, int c, bool on) {
+    Gran<T, VEC> z[KT<T>], v[HALF ? 1 : KT<T>], g[GRAD ? KT<T> : 1];
+    unsigned live;
+    __device__ __forceinline__ void load(const T* px, int64_t dx, const T* pg, int64_t dg, int H, int s0, int lo, int hi) {
         live = 0;
-        const int s0 = chunk * CHUNK + (int)(threadIdx.x / LPR) * KT;
 #pragma unroll
-        for (int k = 0; k < KT; ++k) {
-            const int s = s0 + k, t = d.reverse ? d.T - 1 - s : s;
-            const bool ok = on && s < d.T && t < w.len;
+        for (int k = 0; k < KT<T>; ++k) {
+            const bool ok = s0 + k >= lo && s0 + k < hi;
             live |= ok ? 1u << k : 0u;
             if (ok) {
-                const T* p = x + t * d.xt + c;
-                z[k].load(p);
-                if constexpr (!HALF) v[k].load(p + d.H);
-                if (dout) g[k].load(dout + t * d.ot + c);
-                else g[k].zero();
+                z[k].load(px);
+                if constexpr (!HALF) v[k].load(px + H);
+                if constexpr (GRAD) {
+                    if (pg) g[k].load(pg);
+                    else g[k].zero();
+                }
             } else {
                 z[k].zero();
                 if constexpr (!HALF) v[k].zero();
-                g[k].zero();
+                if constexpr (GRAD) g[k].zero();
             }
+            px += dx;
+            if constexpr (GRAD) pg += pg ? dg : 0;
         }
     }
 };
 
+// Where a thread stands: channels c.. (clamped for loads), first step s0 of chunk `first`, live steps [lo, hi) of the
+// sequence in walking order, and the carry's channel cc of its lane.
+template <typename T, int VEC>
+struct Thread {
+    Where w;
+    int c, cc, s0, lo, hi, first, last;
+    bool on, con, writer;
+    __device__ __forceinline__ explicit Thread(const Dims& d) {
+        w = where<VEC>(d);
+        c = w.c0 + (int)(threadIdx.x % LPR) * VEC;
+        on = c < d.H;
+        cc = w.c0 + (int)(threadIdx.x & 63) % (LPR * VEC);
+        con = cc < d.H;
+        writer = con && threadIdx.x < LPR * VEC;
+        s0 = (int)(threadIdx.x / LPR) * KT<T>;
+        lo = d.reverse ? d.T - w.len : 0;
+        hi = d.reverse ? d.T : w.len;
+        first = w.seg * d.seg_chunks;
+        last = min(d.nchunk, first + d.seg_chunks);
+    }
+    // row of this thread's first step of a chunk, for strides (sb, st) of a tensor; `step` = the walk's stride
+    __device__ __forceinline__ int64_t at(const Dims& d, int64_t sb, int64_t st, int chunk) const {
+        const int s = chunk * CHUNK + s0;
+        return w.b * sb + (int64_t)(d.reverse ? d.T - 1 - s : s) * st + (on ? c : 0);
+    }
+};
+#define DSSVAE_SCAN_LOAD(steps, chunk_, pg)                                                                               \
+    do {                                                                                                                  \
+        const T* px_ = x + th.at(d, d.xb, d.xt, chunk_);                                                                  \
+        const T* pg_ = (pg) ? (pg) + th.at(d, d.ob, d.ot, chunk_) : nullptr;                                              \
+        steps.load(px_, dxs, pg_, dgs, d.H, (chunk_) * CHUNK + th.s0, th.lo, th.hi);                                       \
+    } while (0)
+
 // ---- segment maps: (A, B) of the forward recurrence, or of E (BWD) ------------------------------------------------
-template <typename T, int VEC, int LPR, bool TANH, bool BWD>
+template <typename T, int VEC, bool TANH, bool BWD>
 __global__ __launch_bounds__(NT<T>) void gated_scan_maps_kernel(const T* __restrict__ x, const T* __restrict__ dout, Dims d,
-                                                                  float* __restrict__ maps) {
-    constexpr int NW = NT<T> / 64, KT = CHUNK * LPR / NT<T>;
+                                                                float* __restrict__ maps) {
+    constexpr int NW = NT<T> / 64, K = KT<T>;
     __shared__ float2 lds[2][NW * LPR * VEC];
-    const Where w = where<LPR, VEC>(d);
-    if (w.seg == (BWD ? 0 : d.segs - 1)) return;  // nobody starts behind the last one
-    const int l = threadIdx.x % LPR, c = w.c0 + l * VEC;
-    const bool on = c < d.H;
-    const T* xb = x + w.b * d.xb;
-    const T* gb = dout ? dout + w.b * d.ob : nullptr;
-    const int cc = w.c0 + (int)(threadIdx.x & 63) % (LPR * VEC);  // the channel whose carry this lane holds
-    const bool writer = cc < d.H && threadIdx.x < LPR * VEC;
+    const Thread<T, VEC> th(d);
+    if (th.w.seg == (BWD ? 0 : d.segs - 1)) return;  // nobody starts behind the last one
+    const int64_t dxs = d.reverse ? -d.xt : d.xt, dgs = d.reverse ? -d.ot : d.ot;
     float SA = 1.f, SB = 0.f;
-    const int first = w.seg * d.seg_chunks, last = min(d.nchunk, first + d.seg_chunks);
-    for (int i = 0; i < last - first; ++i) {
-        const int chunk = BWD ? last - 1 - i : first + i;
-        Steps<T, VEC, LPR, KT, BWD> s;
-        s.load(xb, BWD ? gb : nullptr, d, w, chunk, c, on);
+    Steps<T, VEC, BWD, BWD> s, next;
+    const int n = th.last - th.first;
+    DSSVAE_SCAN_LOAD(next, (BWD ? th.last - 1 : th.first), dout);
+    for (int i = 0; i < n; ++i) {
+        s = next;
+        if (i + 1 < n) {
+            const int chunk = BWD ? th.last - 2 - i : th.first + 1 + i;
+            DSSVAE_SCAN_LOAD(next, chunk, dout);
+        }
         float A[VEC], B[VEC], y[VEC];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) { A[v] = 1.f; B[v] = 0.f; }
 #pragma unroll
-        for (int kk = 0; kk < KT; ++kk) {
-            const int k = BWD ? KT - 1 - kk : kk;
+        for (int kk = 0; kk < K; ++kk) {
+            const int k = BWD ? K - 1 - kk : kk;
             const bool ok = (s.live >> k) & 1;
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 const float a = sigmoid_f(s.z[k].get(v));
-                if (ok) {
-                    if constexpr (BWD) {
-                        B[v] = a * (s.g[k].get(v) + B[v]);
-                    } else {
-                        const float n = TANH ? tanh_f(s.v[k].get(v)) : s.v[k].get(v);
-                        B[v] = a * B[v] + (1.f - a) * n;
-                    }
-                    A[v] *= a;
+                float b;
+                if constexpr (BWD) {
+                    b = a * (s.g[k].get(v) + B[v]);
+                } else {
+                    const float nn = TANH ? tanh_f(s.v[k].get(v)) : s.v[k].get(v);
+                    b = a * B[v] + (1.f - a) * nn;
                 }
+                B[v] = ok ? b : B[v];
+                A[v] = ok ? A[v] * a : A[v];
             }
         }
-        block_scan<NW, LPR, VEC, !BWD>(A, B, SB, y, lds[i & 1], &SA);
+        block_scan<NW, VEC, !BWD>(A, B, SB, y, lds[i & 1], &SA);
     }
-    if (writer) {
-        float* m = maps + ((int64_t)w.b * d.segs + w.seg) * 2 * d.H + cc;
+    if (th.writer) {
+        float* m = maps + ((int64_t)th.w.b * d.segs + th.w.seg) * 2 * d.H + th.cc;
         m[0] = SA;
         m[d.H] = SB;
     }
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------
-template <typename T, int VEC, int LPR, bool TANH>
-__global__ __launch_bounds__(NT<T>) void gated_scan_fwd_kernel(const T* __restrict__ x, Dims d, const float* __restrict__ h0,
-                                                                 const float* __restrict__ maps, T* __restrict__ out,
-                                                                 float* __restrict__ h_last, float* __restrict__ ckpt) {
-    constexpr int NW = NT<T> / 64, KT = CHUNK * LPR / NT<T>;
-    __shared__ float2 lds[2][NW * LPR * VEC];
-    const Where w = where<LPR, VEC>(d);
-    const int l = threadIdx.x % LPR, c = w.c0 + l * VEC;
-    const bool on = c < d.H;
-    const T* xb = x + w.b * d.xb;
-    T* ob = out + w.b * d.ob;
-    const int cc = w.c0 + (int)(threadIdx.x & 63) % (LPR * VEC);  // the channel whose carry this lane holds
-    const bool con = cc < d.H, writer = con && threadIdx.x < LPR * VEC;
-    float h = h0 && con ? h0[(int64_t)w.b * d.H + cc] : 0.f;
-    if (d.segs > 1 && con) h = enter(h, maps, d, w.b, w.seg, cc, true);
-    const int first = w.seg * d.seg_chunks, last = min(d.nchunk, first + d.seg_chunks);
-    Steps<T, VEC, LPR, KT, false> s, next;
-    next.load(xb, nullptr, d, w, first, c, on);
-    for (int chunk = first; chunk < last; ++chunk) {
-        s = next;
-        if (chunk + 1 < last) next.load(xb, nullptr, d, w, chunk + 1, c, on);
-        float a[KT][VEC], bn[KT][VEC], A[VEC], B[VEC], y[VEC];
+template <typename T, int VEC, bool TANH>
+__device__ __forceinline__ void fwd_chunk(const Steps<T, VEC, false, false>& s, const Thread<T, VEC>& th,
+                                          const Dims& d, int chunk, float& h, float2* lds, T* out) {
+    constexpr int NW = NT<T> / 64, K = KT<T>;
+    float a[K][VEC], bn[K][VEC], A[VEC], B[VEC], y[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) { A[v] = 1.f; B[v] = 0.f; }
+    for (int v = 0; v < VEC; ++v) { A[v] = 1.f; B[v] = 0.f; }
 #pragma unroll
-        for (int k = 0; k < KT; ++k) {
-            const bool ok = (s.live >> k) & 1;
+    for (int k = 0; k < K; ++k) {
+        const bool ok = (s.live >> k) & 1;
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float ak = sigmoid_f(s.z[k].get(v)), n = TANH ? tanh_f(s.v[k].get(v)) : s.v[k].get(v);
-                a[k][v] = ok ? ak : 1.f;
-                bn[k][v] = ok ? (1.f - ak) * n : 0.f;
-                B[v] = a[k][v] * B[v] + bn[k][v];
-                A[v] *= a[k][v];
-            }
-        }
-        if (ckpt && writer) ckpt[((int64_t)w.b * d.nchunk + chunk) * d.H + cc] = h;
-        block_scan<NW, LPR, VEC, true>(A, B, h, y, lds[chunk & 1]);
-        const int s0 = chunk * CHUNK + (int)(threadIdx.x / LPR) * KT;
-#pragma unroll
-        for (int k = 0; k < KT; ++k) {
-            const bool ok = (s.live >> k) & 1;
-            Gran<T, VEC> o;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                y[v] = a[k][v] * y[v] + bn[k][v];
-                o.set(v, ok ? y[v] : 0.f);
-            }
-            const int st = s0 + k, t = d.reverse ? d.T - 1 - st : st;
-            if (on && st < d.T) o.store(ob + t * d.ot + c);
+        for (int v = 0; v < VEC; ++v) {
+            const float ak = sigmoid_f(s.z[k].get(v)), n = TANH ? tanh_f(s.v[k].get(v)) : s.v[k].get(v);
+            a[k][v] = ok ? ak : 1.f;
+            bn[k][v] = ok ? (1.f - ak) * n : 0.f;
+            B[v] = a[k][v] * B[v] + bn[k][v];
+            A[v] *= a[k][v];
         }
     }
-    if (w.seg == d.segs - 1 && h_last && writer) h_last[(int64_t)w.b * d.H + cc] = h;
+    block_scan<NW, VEC, true>(A, B, h, y, lds);
+    const int64_t dos = d.reverse ? -d.ot : d.ot;
+    const int s0 = chunk * CHUNK + th.s0;
+    T* po = out + th.at(d, d.ob, d.ot, chunk);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const bool ok = (s.live >> k) & 1;
+        Gran<T, VEC> o;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            y[v] = a[k][v] * y[v] + bn[k][v];
+            o.set(v, ok ? y[v] : 0.f);
+        }
+        if (th.on && s0 + k < d.T) o.store(po);
+        po += dos;
+    }
+}
+
+template <typename T, int VEC, bool TANH>
+__global__ __launch_bounds__(NT<T>) void gated_scan_fwd_kernel(const T* __restrict__ x, Dims d, const float* __restrict__ h0,
+                                                               const float* __restrict__ maps, T* __restrict__ out,
+                                                               float* __restrict__ h_last, float* __restrict__ ckpt) {
+    constexpr int NW = NT<T> / 64;
+    __shared__ float2 lds[2][NW * LPR * VEC];
+    const Thread<T, VEC> th(d);
+    const int64_t dxs = d.reverse ? -d.xt : d.xt, dgs = 0, row = (int64_t)th.w.b * d.H + th.cc;
+    float h = h0 && th.con ? h0[row] : 0.f;
+    if (d.segs > 1 && th.con) h = enter(h, maps, d, th.w.b, th.w.seg, th.cc, true);
+    Steps<T, VEC, false, false> s, next;
+    const T* none = nullptr;
+    DSSVAE_SCAN_LOAD(next, th.first, none);
+    for (int chunk = th.first; chunk < th.last; ++chunk) {
+        s = next;
+        if (chunk + 1 < th.last) DSSVAE_SCAN_LOAD(next, (chunk + 1), none);
+        if (ckpt && th.writer) ckpt[((int64_t)th.w.b * d.nchunk + chunk) * d.H + th.cc] = h;
+        fwd_chunk<T, VEC, TANH>(s, th, d, chunk, h, lds[chunk & 1], out);
+    }
+    if (th.w.seg == d.segs - 1 && h_last && th.writer) h_last[row] = h;
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------------
-template <typename T, int VEC, int LPR, bool TANH>
-__global__ __launch_bounds__(NT<T>) void gated_scan_bwd_kernel(const T* __restrict__ x, const T* __restrict__ dout, Dims d,
-                                                                 const float* __restrict__ ckpt,
-                                                                 const float* __restrict__ dh_last,
-                                                                 const float* __restrict__ maps, T* __restrict__ dx,
-                                                                 float* __restrict__ dh0) {
-    constexpr int NW = NT<T> / 64, KT = CHUNK * LPR / NT<T>;
-    __shared__ float2 lds[2][2][NW * LPR * VEC];
-    const Where w = where<LPR, VEC>(d);
-    const int l = threadIdx.x % LPR, c = w.c0 + l * VEC;
-    const bool on = c < d.H;
-    const T* xb = x + w.b * d.xb;
-    const T* gb = dout ? dout + w.b * d.ob : nullptr;
-    T* db = dx + w.b * d.gb;
-    const int cc = w.c0 + (int)(threadIdx.x & 63) % (LPR * VEC);  // the channel whose carry this lane holds
-    const bool con = cc < d.H, writer = con && threadIdx.x < LPR * VEC;
-    float E = dh_last && con ? dh_last[(int64_t)w.b * d.H + cc] : 0.f;
-    if (d.segs > 1 && con) E = enter(E, maps, d, w.b, w.seg, cc, false);
-    const int first = w.seg * d.seg_chunks, last = min(d.nchunk, first + d.seg_chunks);
-    for (int chunk = last - 1; chunk >= first; --chunk) {
-        Steps<T, VEC, LPR, KT, false> s;
-        s.load(xb, gb, d, w, chunk, c, on);
-        float hc = con ? ckpt[((int64_t)w.b * d.nchunk + chunk) * d.H + cc] : 0.f;
-        float a[KT][VEC], n[KT][VEC], A[VEC], B[VEC], F[VEC], G[VEC], y[VEC], e[VEC];
+template <typename T, int VEC, bool TANH>
+__device__ __forceinline__ void bwd_chunk(const Steps<T, VEC, false, true>& s, const Thread<T, VEC>& th,
+                                          const Dims& d, int chunk, float hc, float& E, float2* lds0, float2* lds1, T* dx) {
+    constexpr int NW = NT<T> / 64, K = KT<T>;
+    float a[K][VEC], n[K][VEC], A[VEC], B[VEC], F[VEC], G[VEC], y[VEC], e[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) { A[v] = 1.f; B[v] = 0.f; G[v] = 0.f; }
+    for (int v = 0; v < VEC; ++v) { A[v] = 1.f; B[v] = 0.f; G[v] = 0.f; }
 #pragma unroll
-        for (int k = 0; k < KT; ++k) {
-            const bool ok = (s.live >> k) & 1;
+    for (int k = 0; k < K; ++k) {
+        const bool ok = (s.live >> k) & 1;
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float ak = sigmoid_f(s.z[k].get(v));
-                n[k][v] = TANH ? tanh_f(s.v[k].get(v)) : s.v[k].get(v);
-                a[k][v] = ok ? ak : 1.f;
-                B[v] = a[k][v] * B[v] + (ok ? (1.f - ak) * n[k][v] : 0.f);
-                A[v] *= a[k][v];
-            }
-        }
-#pragma unroll
-        for (int k = KT - 1; k >= 0; --k) {
-            const bool ok = (s.live >> k) & 1;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) G[v] = ok ? a[k][v] * (s.g[k].get(v) + G[v]) : G[v];
-        }
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) F[v] = A[v];
-        block_scan<NW, LPR, VEC, true>(A, B, hc, y, lds[chunk & 1][0]);
-        block_scan<NW, LPR, VEC, false>(F, G, E, e, lds[chunk & 1][1]);
-        float h[KT][VEC];  // h_t
-#pragma unroll
-        for (int k = 0; k < KT; ++k) {
-            const bool ok = (s.live >> k) & 1;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                y[v] = ok ? a[k][v] * y[v] + (1.f - a[k][v]) * n[k][v] : y[v];
-                h[k][v] = y[v];
-            }
-        }
-        const int s0 = chunk * CHUNK + (int)(threadIdx.x / LPR) * KT;
-#pragma unroll
-        for (int k = KT - 1; k >= 0; --k) {
-            const bool ok = (s.live >> k) & 1;
-            Gran<T, VEC> oz, on_;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float D = s.g[k].get(v) + e[v], q = D * (1.f - a[k][v]);
-                oz.set(v, ok ? q * (h[k][v] - n[k][v]) : 0.f);
-                on_.set(v, ok ? (TANH ? q * (1.f - n[k][v] * n[k][v]) : q) : 0.f);
-                e[v] = ok ? a[k][v] * D : e[v];
-            }
-            const int st = s0 + k, t = d.reverse ? d.T - 1 - st : st;
-            if (on && st < d.T) {
-                oz.store(db + t * d.gt + c);
-                on_.store(db + t * d.gt + d.H + c);
-            }
+        for (int v = 0; v < VEC; ++v) {
+            const float ak = sigmoid_f(s.z[k].get(v));
+            n[k][v] = TANH ? tanh_f(s.v[k].get(v)) : s.v[k].get(v);
+            a[k][v] = ok ? ak : 1.f;
+            B[v] = a[k][v] * B[v] + (ok ? (1.f - ak) * n[k][v] : 0.f);
+            A[v] *= a[k][v];
         }
     }
-    if (w.seg == 0 && dh0 && writer) dh0[(int64_t)w.b * d.H + cc] = E;
+#pragma unroll
+    for (int k = K - 1; k >= 0; --k) {
+        const bool ok = (s.live >> k) & 1;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) G[v] = ok ? a[k][v] * (s.g[k].get(v) + G[v]) : G[v];
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) F[v] = A[v];
+    block_scan<NW, VEC, true>(A, B, hc, y, lds0);
+    block_scan<NW, VEC, false>(F, G, E, e, lds1);
+    float h[K][VEC];  // h_t - n_t = a_t (h_{t-1} - n_t)
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const bool ok = (s.live >> k) & 1;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            h[k][v] = a[k][v] * (y[v] - n[k][v]);
+            y[v] = ok ? h[k][v] + n[k][v] : y[v];
+        }
+    }
+    const int64_t dgs = d.reverse ? -d.gt : d.gt;
+    const int s0 = chunk * CHUNK + th.s0;
+    T* pd = dx + th.at(d, d.gb, d.gt, chunk) + (K - 1) * dgs;
+#pragma unroll
+    for (int k = K - 1; k >= 0; --k) {
+        const bool ok = (s.live >> k) & 1;
+        Gran<T, VEC> oz, on_;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const float D = s.g[k].get(v) + e[v], q = D * (1.f - a[k][v]);
+            oz.set(v, ok ? q * h[k][v] : 0.f);
+            on_.set(v, ok ? (TANH ? q * (1.f - n[k][v] * n[k][v]) : q) : 0.f);
+            e[v] = ok ? a[k][v] * D : e[v];
+        }
+        if (th.on && s0 + k < d.T) {
+            oz.store(pd);
+            on_.store(pd + d.H);
+        }
+        pd -= dgs;
+    }
+}
+
+template <typename T, int VEC, bool TANH>
+__global__ __launch_bounds__(NT<T>) void gated_scan_bwd_kernel(const T* __restrict__ x, const T* __restrict__ dout, Dims d,
+                                                               const float* __restrict__ ckpt,
+                                                               const float* __restrict__ dh_last,
+                                                               const float* __restrict__ maps, T* __restrict__ dx,
+                                                               float* __restrict__ dh0) {
+    constexpr int NW = NT<T> / 64;
+    __shared__ float2 lds[2][2][NW * LPR * VEC];
+    const Thread<T, VEC> th(d);
+    const int64_t dxs = d.reverse ? -d.xt : d.xt, dgs = d.reverse ? -d.ot : d.ot, row = (int64_t)th.w.b * d.H + th.cc;
+    float E = dh_last && th.con ? dh_last[row] : 0.f;
+    if (d.segs > 1 && th.con) E = enter(E, maps, d, th.w.b, th.w.seg, th.cc, false);
+    Steps<T, VEC, false, true> s, next;
+    DSSVAE_SCAN_LOAD(next, (th.last - 1), dout);
+    for (int chunk = th.last - 1; chunk >= th.first; --chunk) {
+        s = next;
+        if (chunk > th.first) DSSVAE_SCAN_LOAD(next, (chunk - 1), dout);
+        const float hc = th.con ? ckpt[((int64_t)th.w.b * d.nchunk + chunk) * d.H + th.cc] : 0.f;
+        float2 *l0 = lds[chunk & 1][0], *l1 = lds[chunk & 1][1];
+        bwd_chunk<T, VEC, TANH>(s, th, d, chunk, hc, E, l0, l1, dx);
+    }
+    if (th.w.seg == 0 && dh0 && th.writer) dh0[row] = E;
 }
 
 // ---- one token: h' = a h + (1 - a) n, out = h' rounded to T; h_out may be h -------------------------------------------
@@ -352,76 +401,76 @@ __global__ __launch_bounds__(STEP_THREADS) void gated_step_kernel(const T* __res
     for (int j = 0; j < VEC; ++j) h_out[b * H + c + j] = hv[j];
 }
 
-// Segments of the time axis.  One while the tiles (128 bytes of channels each) alone give two blocks a CU: the segment maps
-// cost a second read of the inputs.
+// Segments of the time axis: one while the tiles alone give more than half the CUs a block (the segment maps cost a second
+// read of the inputs).  Measured, forward, T = 4096, bf16: 256 tiles 100 us whole, 147 us in segments; 128 tiles 82 / 76 us;
+// 5 tiles x 16384 steps 304 / 33 us.
 inline int plan_segs(int B, int T, int H, int es) {
-    const int64_t blocks = (int64_t)B * (((int64_t)H * es + 127) / 128), nchunk = ((int64_t)T + CHUNK - 1) / CHUNK;
-    const int64_t cus = device_cus();
-    if (blocks >= 2 * cus || nchunk <= 2) return 1;
-    int64_t segs = (4 * cus + blocks - 1) / blocks;
+    const int64_t cus = device_cus(), blocks = (int64_t)B * (((int64_t)H * es + 127) / 128);
+    const int64_t nchunk = ((int64_t)T + CHUNK - 1) / CHUNK;
+    if (blocks < 1 || 2 * blocks > cus || nchunk <= 2) return 1;
+    int64_t segs = 2 * cus / blocks;
     if (segs > nchunk) segs = nchunk;
     const int64_t per = (nchunk + segs - 1) / segs;
     return (int)((nchunk + per - 1) / per);
 }
 
+// 16-bit channels move in pairs where every row starts on 4 bytes
 inline int pick_vec(int es, int H, const void* const* ptrs, const int64_t* strides, int n) {
-    for (int bytes = 16; bytes >= 8; bytes /= 2) {
-        const int vec = bytes / es;
-        if (H % vec) continue;
-        bool ok = true;
-        for (int i = 0; i < n; ++i)
-            ok = ok && (!ptrs[i] || (aligned_to(ptrs[i], bytes) && strides[2 * i] % vec == 0 && strides[2 * i + 1] % vec == 0));
-        if (ok) return vec;
-    }
-    return 1;
+    if (es == 4 || H % 2) return 1;
+    for (int i = 0; i < n; ++i)
+        if (ptrs[i] && (!aligned_to(ptrs[i], 4) || strides[2 * i] % 2 || strides[2 * i + 1] % 2)) return 1;
+    return 2;
 }
 
-template <typename T, int VEC, int LPR, bool TANH>
+template <typename T, int VEC, bool TANH>
 int fwd_launch(const T* x, Dims d, const float* h0, T* out, float* h_last, float* ckpt, float* maps, hipStream_t s) {
     d.tiles = (d.H + LPR * VEC - 1) / (LPR * VEC);
     const int64_t grid = (int64_t)d.tiles * d.B * d.segs;
     if (grid > 0x7fffffff) return DSSVAE_ETOOBIG;
     if (d.segs > 1) {
-        hipLaunchKernelGGL((gated_scan_maps_kernel<T, VEC, LPR, TANH, false>), dim3((unsigned)grid), dim3(NT<T>), 0, s, x,
+        hipLaunchKernelGGL((gated_scan_maps_kernel<T, VEC, TANH, false>), dim3((unsigned)grid), dim3(NT<T>), 0, s, x,
                            (const T*)nullptr, d, maps);
         DSSVAE_CHECK_LAUNCH();
     }
-    hipLaunchKernelGGL((gated_scan_fwd_kernel<T, VEC, LPR, TANH>), dim3((unsigned)grid), dim3(NT<T>), 0, s, x, d, h0, maps, out,
+    hipLaunchKernelGGL((gated_scan_fwd_kernel<T, VEC, TANH>), dim3((unsigned)grid), dim3(NT<T>), 0, s, x, d, h0, maps, out,
                        h_last, ckpt);
     DSSVAE_CHECK_LAUNCH();
     return DSSVAE_OK;
 }
 
-template <typename T, int VEC, int LPR, bool TANH>
+template <typename T, int VEC, bool TANH>
 int bwd_launch(const T* x, const T* dout, Dims d, const float* ckpt, const float* dh_last, T* dx, float* dh0, float* maps,
                hipStream_t s) {
     d.tiles = (d.H + LPR * VEC - 1) / (LPR * VEC);
     const int64_t grid = (int64_t)d.tiles * d.B * d.segs;
     if (grid > 0x7fffffff) return DSSVAE_ETOOBIG;
     if (d.segs > 1) {
-        hipLaunchKernelGGL((gated_scan_maps_kernel<T, VEC, LPR, false, true>), dim3((unsigned)grid), dim3(NT<T>), 0, s, x, dout, d,
+        hipLaunchKernelGGL((gated_scan_maps_kernel<T, VEC, false, true>), dim3((unsigned)grid), dim3(NT<T>), 0, s, x, dout, d,
                            maps);
         DSSVAE_CHECK_LAUNCH();
     }
-    hipLaunchKernelGGL((gated_scan_bwd_kernel<T, VEC, LPR, TANH>), dim3((unsigned)grid), dim3(NT<T>), 0, s, x, dout, d, ckpt,
+    hipLaunchKernelGGL((gated_scan_bwd_kernel<T, VEC, TANH>), dim3((unsigned)grid), dim3(NT<T>), 0, s, x, dout, d, ckpt,
                        dh_last, maps, dx, dh0);
     DSSVAE_CHECK_LAUNCH();
     return DSSVAE_OK;
 }
 
-// a granule of 16 bytes: 8 lanes cover 128 bytes of channels; 8 bytes or one element: 16 lanes
-#define DSSVAE_SCAN_VECS(CALL, T, V16, V8)                       \
-    do {                                                         \
-        if (vec == V16) { if (tanh) return CALL(T, V16, 8, true); return CALL(T, V16, 8, false); }   \
-        if (vec == V8) { if (tanh) return CALL(T, V8, 16, true); return CALL(T, V8, 16, false); }    \
-        if (tanh) return CALL(T, 1, 16, true);                   \
-        return CALL(T, 1, 16, false);                            \
-    } while (0)
-#define DSSVAE_SCAN_TYPES(CALL)                                  \
-    do {                                                         \
-        if (dtype == DSSVAE_F32) DSSVAE_SCAN_VECS(CALL, float, 4, 2);    \
-        if (dtype == DSSVAE_BF16) DSSVAE_SCAN_VECS(CALL, bf16_t, 8, 4);  \
-        DSSVAE_SCAN_VECS(CALL, f16_t, 8, 4);                     \
+#define DSSVAE_SCAN_TYPES(CALL)                                          \
+    do {                                                                 \
+        if (dtype == DSSVAE_F32) {                                       \
+            if (tanh) return CALL(float, 1, true);                       \
+            return CALL(float, 1, false);                                \
+        }                                                                \
+        if (dtype == DSSVAE_BF16) {                                      \
+            if (vec == 2 && tanh) return CALL(bf16_t, 2, true);          \
+            if (vec == 2) return CALL(bf16_t, 2, false);                 \
+            if (tanh) return CALL(bf16_t, 1, true);                      \
+            return CALL(bf16_t, 1, false);                               \
+        }                                                                \
+        if (vec == 2 && tanh) return CALL(f16_t, 2, true);               \
+        if (vec == 2) return CALL(f16_t, 2, false);                      \
+        if (tanh) return CALL(f16_t, 1, true);                           \
+        return CALL(f16_t, 1, false);                                    \
     } while (0)
 
 int bad_dims(int dtype, int B, int T, int H, int64_t xb, int64_t xt) {
@@ -434,7 +483,7 @@ Dims make_dims(const int32_t* lengths, int B, int T, int H, int reverse, int es)
     Dims d{};
     d.lengths = lengths;
     d.B = B; d.T = T; d.H = H; d.reverse = reverse != 0;
-    d.nchunk = (T + CHUNK - 1) / CHUNK;
+    d.nchunk = (int)(((int64_t)T + CHUNK - 1) / CHUNK);
     d.segs = plan_segs(B, T, H, es);
     d.seg_chunks = (d.nchunk + d.segs - 1) / d.segs;
     return d;
@@ -442,7 +491,7 @@ Dims make_dims(const int32_t* lengths, int B, int T, int H, int reverse, int es)
 
 }  // namespace
 
-extern "C" int dssvae_gated_scan_chunks(int T) { return T < 0 ? DSSVAE_EINVAL : (T + CHUNK - 1) / CHUNK; }
+extern "C" int dssvae_gated_scan_chunks(int T) { return T < 0 ? DSSVAE_EINVAL : (int)(((int64_t)T + CHUNK - 1) / CHUNK); }
 
 extern "C" int64_t dssvae_gated_scan_workspace_bytes(int B, int T, int H, int dtype) {
     if (!dtype_ok(dtype) || B < 0 || T < 0 || H < 1) return DSSVAE_EINVAL;
@@ -465,7 +514,7 @@ extern "C" int dssvae_gated_scan_fwd(const void* x, int64_t xb, int64_t xt, int 
     const int64_t strides[] = {B > 1 ? xb : 0, T > 1 ? xt : 0, B > 1 ? ob : 0, T > 1 ? ot : 0};
     const int vec = pick_vec(es, H, ptrs, strides, 2), tanh = tanh_candidate != 0;
     hipStream_t s = (hipStream_t)stream;
-#define CALL(T_, V, L, TH) fwd_launch<T_, V, L, TH>((const T_*)x, d, h0, (T_*)out, h_last, checkpoints, (float*)workspace, s)
+#define CALL(T_, V, TH) fwd_launch<T_, V, TH>((const T_*)x, d, h0, (T_*)out, h_last, checkpoints, (float*)workspace, s)
     DSSVAE_SCAN_TYPES(CALL);
 #undef CALL
 }
@@ -486,8 +535,8 @@ extern "C" int dssvae_gated_scan_bwd(const void* x, int64_t xb, int64_t xt, int 
     const int64_t strides[] = {B > 1 ? xb : 0, T > 1 ? xt : 0, B > 1 ? ob : 0, T > 1 ? ot : 0, B > 1 ? gb : 0, T > 1 ? gt : 0};
     const int vec = pick_vec(es, H, ptrs, strides, 3), tanh = tanh_candidate != 0;
     hipStream_t s = (hipStream_t)stream;
-#define CALL(T_, V, L, TH)                                                                                             \
-    bwd_launch<T_, V, L, TH>((const T_*)x, (const T_*)dout, d, checkpoints, dh_last, (T_*)dx, dh0, (float*)workspace, s)
+#define CALL(T_, V, TH)                                                                                             \
+    bwd_launch<T_, V, TH>((const T_*)x, (const T_*)dout, d, checkpoints, dh_last, (T_*)dx, dh0, (float*)workspace, s)
     DSSVAE_SCAN_TYPES(CALL);
 #undef CALL
 }
@@ -510,11 +559,18 @@ extern "C" int dssvae_gated_step(const void* x, int64_t xb, int dtype, const flo
     if (bad_dims(dtype, B, 1, H, xb, 2 * (int64_t)H) || (B > 1 && ob < H)) return DSSVAE_EINVAL;
     if (B == 0) return DSSVAE_OK;
     if (!x || !out || !h_out) return DSSVAE_EINVAL;
-    const void* ptrs[] = {x, out};
-    const int64_t strides[] = {B > 1 ? xb : 0, 0, B > 1 ? ob : 0, 0};
-    const int vec = pick_vec(elem_size(dtype), H, ptrs, strides, 2), tanh = tanh_candidate != 0;
+    const int es = elem_size(dtype), wide = 16 / es;
+    // 16-byte granules where rows allow them, else single elements
+    const bool ok = H % wide == 0 && aligned_to(x, 16) && aligned_to(out, 16) && (B == 1 || (xb % wide == 0 && ob % wide == 0));
     hipStream_t s = (hipStream_t)stream;
-#define CALL(T_, V, L, TH) step_launch<T_, V, TH>((const T_*)x, xb, h, B, H, (T_*)out, ob, h_out, s)
-    DSSVAE_SCAN_TYPES(CALL);
-#undef CALL
+#define GO(T, V)                                                                                                       \
+    do {                                                                                                               \
+        if (tanh_candidate) return step_launch<T, V, true>((const T*)x, xb, h, B, H, (T*)out, ob, h_out, s);           \
+        return step_launch<T, V, false>((const T*)x, xb, h, B, H, (T*)out, ob, h_out, s);                              \
+    } while (0)
+    if (dtype == DSSVAE_F32) { if (ok) GO(float, 4); GO(float, 1); }
+    if (dtype == DSSVAE_BF16) { if (ok) GO(bf16_t, 8); GO(bf16_t, 1); }
+    if (ok) GO(f16_t, 8);
+    GO(f16_t, 1);
+#undef GO
 }
