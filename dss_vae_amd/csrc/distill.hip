@@ -1,0 +1,304 @@
+// Distillation from a teacher's top logits (HBM-bound: one read of the student's logits, one write of their gradient).
+//
+//   p = softmax(teacher / tau) over the row's valid slots, q = softmax(logits / tau) over the vocabulary
+//   row = tau^2 sum_j p_j (log p_j - log q[id_j]) ; total = sum_i w_i row_i ; dlogits = w tau (q - scatter(p))
+//
+// One block per row.  The weight of a row is known at the call, so the gradient leaves in the SAME pass: a row stays in
+// registers (NV granules of 16 bytes per thread) between its read, its maximum, its sum and the store; wider rows than
+// 16 granules x 1024 threads are read twice.  Rows may start at any element: up to VEC - 1 elements in front of the first
+// 16-byte boundary and behind the last granule are "edge" elements, one per thread.
+// The k teacher slots are wave 0's: softmax by shuffles while the block loads.  The k gradient entries are written over the
+// dense store behind a barrier, by the first slot of each distinct id with the sum of its probabilities: no atomics, and
+// repeated ids add up in slot order.
+#include "elem.h"
+
+namespace {
+
+constexpr int MAX_TOP = DSSVAE_DISTILL_MAX_TOP;
+constexpr float LOG2E = 1.4426950408889634f, NINF = -__builtin_huge_valf();
+
+__device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <int NT, bool MAX>
+__device__ __forceinline__ float block_reduce(float v, float* red /* [NT / 64] */) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const float u = __shfl_xor(v, o, 64);
+        v = MAX ? fmaxf(v, u) : v + u;
+    }
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int i = 1; i < NT / 64; ++i) v = MAX ? fmaxf(v, red[i]) : v + red[i];
+    return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+// The granules stay in their 16 bytes between the walks over them: the compiler may not keep them as floats as well, which
+// would double a 16-bit row's registers (and spill).
+template <typename T, int VEC, int N>
+__device__ __forceinline__ void keep_raw(Gran<T, VEC> (&v)[N]) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        u32x4 r = __builtin_bit_cast(u32x4, v[i].v);
+        asm volatile("" : "+v"(r));
+        v[i].v = __builtin_bit_cast(typename Gran<T, VEC>::V, r);
+    }
+}
+
+// NV granules per thread in registers; NV = 0: any width, the row is read twice
+template <typename T, int NT, int NV>
+__global__ __launch_bounds__(NT, NT == 1024 && NV <= 8 ? 8 : 4) void distill_kernel(
+    const T* __restrict__ z, int64_t ldz, int V, const int64_t* __restrict__ ids, const float* __restrict__ teacher, int k,
+    float tau, const float* __restrict__ weight, float w_all, T* __restrict__ dz, int64_t lddz, float* __restrict__ rows) {
+    constexpr int VEC = 16 / (int)sizeof(T);
+    constexpr int NR = NV > 0 ? NV : 1;
+    __shared__ float red_max[NT / 64], red_sum[NT / 64];
+    __shared__ int s_id[MAX_TOP];
+    __shared__ float s_p[MAX_TOP];
+    __shared__ float s_mass;  // 1, 0 (no valid slot) or NaN (an id outside the vocabulary, a NaN or +inf among the teacher's logits)
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const float w = weight ? weight[row] : w_all, c = LOG2E / tau;
+    const T* zr = z + row * ldz;
+    T* dr = dz ? dz + row * lddz : nullptr;
+    const int mis = (int)((reinterpret_cast<uintptr_t>(zr) & 15u) / sizeof(T));
+    const int head = min((VEC - mis) % VEC, V), nvec = (V - head) / VEC, tail = V - head - nvec * VEC;
+    const int edge = tid < head ? tid : tid - head < tail ? V - tail + (tid - head) : -1;
+    const T* zb = zr + head;
+
+    bool dead = w == 0.f;  // nothing is read, nothing but zeros is written
+    Gran<T, VEC> v[NR];
+    float ev = NINF;
+    if (!dead) {
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int g = i * NT + tid;
+                if (g < nvec) {
+                    v[i].load(zb + (int64_t)g * VEC);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) v[i].set(j, NINF);
+                }
+            }
+        }
+        if (edge >= 0) ev = (float)zr[edge];
+        if (tid < 64) {
+            float top = NINF;
+            bool bad = false;
+            for (int j = tid; j < k; j += 64) {
+                const int64_t id = ids[row * k + j];
+                const float t = id >= 0 ? teacher[row * k + j] : NINF;
+                bad |= id >= V || !(t < -NINF);
+                s_id[j] = id >= 0 && id < V ? (int)id : -1;
+                s_p[j] = t;
+                top = fmaxf(top, t);
+            }
+            top = wave_max(top);
+            float sum = 0.f;
+            for (int j = tid; j < k; j += 64) sum += exp2_f((s_p[j] - top) * c);
+            sum = wave_sum(sum);
+            const bool any_bad = __any(bad), none = top == NINF;
+            for (int j = tid; j < k; j += 64) s_p[j] = none ? 0.f : exp2_f((s_p[j] - top) * c) / sum;
+            if (tid == 0) s_mass = any_bad ? __builtin_nanf("") : none ? 0.f : 1.f;
+        }
+    }
+    float m = ev, s = 0.f;
+    if (!dead) {
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) m = fmaxf(m, v[i].get(j));
+        } else {
+            // running maximum and sum of this thread
+            s = edge >= 0 ? 1.f : 0.f;
+            for (int64_t g = tid; g < nvec; g += NT) {
+                v[0].load(zb + g * VEC);
+                float top = m;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) top = fmaxf(top, v[0].get(j));
+                if (top == NINF) {
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) s = v[0].get(j) != v[0].get(j) ? v[0].get(j) : s;
+                    continue;
+                }
+                s *= exp2_f((m - top) * c);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) s += exp2_f((v[0].get(j) - top) * c);
+                m = top;
+            }
+        }
+    }
+    const float M = block_reduce<NT, true>(m, red_max);
+    if constexpr (NV > 0) keep_raw(v);
+    const float mass = dead ? 0.f : s_mass;
+    if (mass == 0.f) {  // (the whole block alike)
+        if (tid == 0) rows[row] = 0.f;
+        if (!dr) return;
+        Gran<T, VEC> o;
+        o.zero();
+        T* db = dr + head;
+        for (int64_t g = tid; g < nvec; g += NT) o.store(db + g * VEC);
+        if (edge >= 0) dr[edge] = (T)0.f;
+        return;
+    }
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) s += exp2_f((v[i].get(j) - M) * c);
+        if (edge >= 0) s += exp2_f((ev - M) * c);
+    } else {
+        s = m == NINF ? (s != s ? s : 0.f) : s * exp2_f((m - M) * c);
+    }
+    const float S = block_reduce<NT, false>(s, red_sum);
+    if constexpr (NV > 0) keep_raw(v);
+    if (tid < 64) {
+        float part = 0.f;
+        for (int j = tid; j < k; j += 64) {
+            const float p = s_p[j];
+            if (p > 0.f && s_id[j] >= 0) part += p * (logf(p) - ((float)zr[s_id[j]] - M) / tau);
+        }
+        part = wave_sum(part);
+        if (tid == 0) rows[row] = tau * tau * (part + logf(S)) * mass;
+    }
+    if (!dr) return;
+    const float a = w * tau * mass / S;
+    T* db = dr + head;
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int g = i * NT + tid;
+            if (g >= nvec) continue;
+            Gran<T, VEC> o;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) o.set(j, a * exp2_f((v[i].get(j) - M) * c));
+            o.store(db + (int64_t)g * VEC);
+        }
+    } else {
+        for (int64_t g = tid; g < nvec; g += NT) {
+            Gran<T, VEC> o;
+            v[0].load(zb + g * VEC);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) o.set(j, a * exp2_f((v[0].get(j) - M) * c));
+            o.store(db + g * VEC);
+        }
+    }
+    if (edge >= 0) dr[edge] = (T)(a * exp2_f((ev - M) * c));
+    __syncthreads();  // the dense stores come before the k entries written over them
+    for (int j = tid; j < k; j += NT) {
+        const int id = s_id[j];
+        if (id < 0) continue;
+        float p = 0.f;
+        bool first = true;
+        for (int i = 0; i < k; ++i) {
+            const bool same = s_id[i] == id;
+            first = first && !(same && i < j);
+            p += same ? s_p[i] : 0.f;
+        }
+        if (first) dr[id] = (T)(a * exp2_f(((float)zr[id] - M) * c) - w * tau * p * mass);
+    }
+}
+
+// total = sum of w_i row_i in a fixed order (64-bit sums)
+__global__ __launch_bounds__(1024) void distill_total_kernel(const float* __restrict__ rows, const float* __restrict__ weight,
+                                                             float w_all, int64_t n, float* __restrict__ total) {
+    __shared__ double red[16];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+        const float w = weight ? weight[i] : w_all;
+        if (w != 0.f) s += (double)w * rows[i];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 16; ++i) s += red[i];
+        *total = (float)s;
+    }
+}
+
+// x *= *g; *g = 1 (the usual upstream gradient of a loss) costs one scalar read
+template <typename T>
+__global__ __launch_bounds__(256) void scale_kernel(T* __restrict__ x, int64_t ld, int64_t rows, int V,
+                                                    const float* __restrict__ g) {
+    const float f = *g;
+    if (f == 1.f) return;
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
+        for (int64_t c = threadIdx.x; c < V; c += 256) x[r * ld + c] = (T)((float)x[r * ld + c] * f);
+}
+
+template <typename T>
+int launch(const T* z, int64_t ldz, int64_t N, int V, const int64_t* ids, const float* teacher, int k, float tau,
+           const float* weight, float w_all, T* dz, int64_t lddz, float* rows, hipStream_t s) {
+    constexpr int VEC = 16 / (int)sizeof(T);
+    const int64_t gran = ((int64_t)V + VEC - 1) / VEC;
+#define GO(NT, NV)                                                                                                     \
+    do {                                                                                                               \
+        hipLaunchKernelGGL((distill_kernel<T, NT, NV>), dim3((unsigned)N), dim3(NT), 0, s, z, ldz, V, ids, teacher, k, tau, weight, \
+                           w_all, dz, lddz, rows);                                                                     \
+        DSSVAE_CHECK_LAUNCH();                                                                                         \
+        return DSSVAE_OK;                                                                                              \
+    } while (0)
+    if (gran <= 256) GO(256, 1);
+    if (gran <= 256 * 4) GO(256, 4);
+    if (gran <= 1024 * 4) GO(1024, 4);
+    if (gran <= 1024 * 8) GO(1024, 8);
+    if (gran <= 1024 * 16) GO(1024, 16);
+    GO(1024, 0);
+#undef GO
+}
+
+}  // namespace
+
+extern "C" int dssvae_distill(const void* logits, int64_t ldz, int dtype, int64_t N, int V, const int64_t* ids,
+                              const float* teacher, int k, float tau, const float* weight, float weight_all, void* dlogits,
+                              int64_t lddz, float* rows, float* total, void* stream) {
+    if (!dtype_ok(dtype) || N < 0 || N > 0x7fffffff || V < 1 || V > (1 << 30) || k < 1 || k > MAX_TOP || ldz < V ||
+        !(tau > 0.f) || !(tau < __builtin_huge_valf()) || !total || (dlogits && lddz < V))
+        return DSSVAE_EINVAL;
+    if (N > 0 && (!logits || !ids || !teacher || !rows)) return DSSVAE_EINVAL;
+    const int es = elem_size(dtype);
+    if (!aligned_to(logits, es) || !aligned_to(dlogits, es)) return DSSVAE_EINVAL;
+    // a granule of the gradient is stored where its logits were loaded: same offset from the 16-byte boundary in every row
+    if (dlogits && N > 0 && ((reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(dlogits)) % 16 != 0 ||
+                             (N > 1 && (ldz - lddz) % (16 / es) != 0)))
+        return DSSVAE_EINVAL;
+    hipStream_t s = (hipStream_t)stream;
+    if (N > 0) {
+        int e;
+        if (dtype == DSSVAE_F32)
+            e = launch<float>((const float*)logits, ldz, N, V, ids, teacher, k, tau, weight, weight_all, (float*)dlogits, lddz, rows, s);
+        else if (dtype == DSSVAE_BF16)
+            e = launch<bf16_t>((const bf16_t*)logits, ldz, N, V, ids, teacher, k, tau, weight, weight_all, (bf16_t*)dlogits, lddz, rows, s);
+        else
+            e = launch<f16_t>((const f16_t*)logits, ldz, N, V, ids, teacher, k, tau, weight, weight_all, (f16_t*)dlogits, lddz, rows, s);
+        if (e != DSSVAE_OK) return e;
+    }
+    hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(1024), 0, s, rows, weight, weight_all, N, total);
+    DSSVAE_CHECK_LAUNCH();
+    return DSSVAE_OK;
+}
+
+extern "C" int dssvae_scale_rows(void* x, int64_t ld, int dtype, int64_t rows, int V, const float* factor, void* stream) {
+    if (!dtype_ok(dtype) || rows < 0 || V < 1 || ld < V || !factor) return DSSVAE_EINVAL;
+    if (rows == 0) return DSSVAE_OK;
+    if (!x) return DSSVAE_EINVAL;
+    const int64_t most = 16 * (int64_t)device_cus();
+    const dim3 grid((unsigned)(rows < most ? rows : most));
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == DSSVAE_F32) hipLaunchKernelGGL((scale_kernel<float>), grid, dim3(256), 0, s, (float*)x, ld, rows, V, factor);
+    else if (dtype == DSSVAE_BF16) hipLaunchKernelGGL((scale_kernel<bf16_t>), grid, dim3(256), 0, s, (bf16_t*)x, ld, rows, V, factor);
+    else hipLaunchKernelGGL((scale_kernel<f16_t>), grid, dim3(256), 0, s, (f16_t*)x, ld, rows, V, factor);
+    DSSVAE_CHECK_LAUNCH();
+    return DSSVAE_OK;
+}

@@ -38,6 +38,7 @@ class GruBwdInst(C.Structure):
 
 
 CELL_GRU, CELL_LSTM = 0, 1
+DISTILL_MAX_TOP = 1024
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # DSSVAE_F32 / _BF16 / _F16
 
 
@@ -149,6 +150,8 @@ _SIGNATURES = {
     "dssvae_gated_scan_fwd": ([_P, _L, _L, _I, _P, _P, _I, _I, _I, _I, _I, _P, _L, _L, _P, _P, _P, _L, _P], _I),
     "dssvae_gated_scan_bwd": ([_P, _L, _L, _I, _P, _I, _I, _P, _P, _L, _L, _P, _I, _I, _I, _P, _L, _L, _P, _P, _L, _P], _I),
     "dssvae_gated_step": ([_P, _L, _I, _P, _I, _I, _I, _P, _L, _P, _P], _I),
+    "dssvae_distill": ([_P, _L, _I, _L, _I, _P, _P, _I, _F, _P, _F, _P, _L, _P, _P, _P], _I),
+    "dssvae_scale_rows": ([_P, _L, _I, _L, _I, _P, _P], _I),
 }
 EXPORTS = tuple(_SIGNATURES)
 

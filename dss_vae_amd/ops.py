@@ -2053,3 +2053,90 @@ def gated_step(xproj, h=None, candidate="tanh", h_out=None):
         L.check(L.load().dssvae_gated_step(L.ptr(x), ldx, code, L.ptr(h), tanh, B, H, L.ptr(out), H, L.ptr(hn), L.stream()),
                 "dssvae_gated_step")
     return out, hn
+
+
+def _like_rows(z, ldz):
+    """uninitialised [N, V] whose rows start at the same offset from a 16-byte boundary as those of z"""
+    N, V = z.shape
+    per = 16 // z.element_size()
+    off, pitch = z.data_ptr() % 16 // z.element_size(), V + (ldz - V) % per
+    return torch.empty(off + N * pitch, device=z.device, dtype=z.dtype).as_strided((N, V), (pitch, 1), off)
+
+
+def _distill(z, ldz, code, ids, teacher, tau, weight, want_grad):
+    """-> total, rows, dlogits (None unless wanted)"""
+    N, V = z.shape
+    rows = torch.empty(N, device=z.device, dtype=torch.float32)
+    total = torch.empty((), device=z.device, dtype=torch.float32)
+    dz = _like_rows(z, ldz) if want_grad else None
+    with _Here(z.device), _Span("distill_kernel", 8.0 * N * V, (2.0 if want_grad else 1.0) * N * V * z.element_size(),
+                                detail="N=%d V=%d k=%d" % (N, V, ids.size(1))):
+        L.check(L.load().dssvae_distill(L.ptr(z), ldz, code, N, V, L.ptr(ids), L.ptr(teacher), ids.size(1), tau,
+                                        L.ptr(weight), 1.0 / max(N, 1), L.ptr(dz), 0 if dz is None else dz.stride(0),
+                                        L.ptr(rows), L.ptr(total), L.stream()), "dssvae_distill")
+    return total, rows, dz
+
+
+class _DistillFn(Function):
+    """the gradient is written by the forward pass (the rows' weights are its arguments) and scaled by the upstream
+    scalar in backward, which costs nothing where that is 1"""
+
+    @staticmethod
+    def forward(ctx, logits, ids, teacher, weight, tau, code):
+        ctx.set_materialize_grads(False)
+        z, ldz = _matrix(logits.reshape(-1, logits.size(-1)))
+        total, rows, ctx.dz = _distill(z, ldz, code, ids, teacher, tau, weight, True)
+        ctx.shape, ctx.code = logits.shape, code
+        rows = rows.view(logits.shape[:-1])
+        ctx.mark_non_differentiable(rows)
+        return total, rows
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, _grows):
+        if g is None:
+            ctx.dz = None
+            return (None,) * 6
+        dz, ctx.dz = ctx.dz, None
+        if dz is None:
+            raise RuntimeError("distill_loss keeps its gradient for ONE backward pass (retain_graph / a second backward "
+                               "is not supported)")
+        if dz.size(0):
+            with _Here(dz.device):
+                L.check(L.load().dssvae_scale_rows(L.ptr(dz), dz.stride(0), ctx.code, dz.size(0), dz.size(1),
+                                                   L.ptr(g.contiguous()), L.stream()), "dssvae_scale_rows")
+        return dz.view(ctx.shape) if dz.is_contiguous() else dz.unflatten(0, ctx.shape[:-1]), None, None, None, None, None
+
+
+def distill_loss(logits, ids, teacher, temperature=1.0, weight=None):
+    """Distillation from a teacher's k top logits: per row tau^2 KL(p || q) between p = softmax(teacher / tau) over the
+    row's valid slots and q = softmax(logits / tau) over the whole vocabulary.
+    logits [..., V]; ids [..., k] int64, an id < 0 is an empty slot (an id >= V makes its row NaN), the same id twice adds
+    up; teacher [..., k] float32 or of the logits' type (logits or log-probabilities alike); weight [...] float32, None =
+    1 / rows each.  Rows of weight 0 and rows without a valid slot are not read: loss 0, gradient 0.
+    -> (total = sum of weight * row, a differentiable float32 scalar; rows [...] float32, for reporting only).
+    The gradient of `total` is computed in the forward pass and kept for ONE backward pass."""
+    code = _typed("distill_loss", logits)
+    if logits.dim() < 2 or logits.size(-1) < 1:
+        raise RuntimeError("distill_loss: logits must be [..., V], got %s" % (list(logits.shape),))
+    lead = tuple(logits.shape[:-1])
+    if ids.dim() != logits.dim() or not 1 <= ids.size(-1) <= L.DISTILL_MAX_TOP:
+        raise RuntimeError("distill_loss: ids must be [..., k] with 1 <= k <= %d, got %s" % (L.DISTILL_MAX_TOP,
+                                                                                             list(ids.shape)))
+    k = ids.size(-1)
+    _expect("distill_loss", "ids", ids, lead + (k,), (torch.int64,), logits.device)
+    _expect("distill_loss", "teacher", teacher, lead + (k,), (torch.float32, logits.dtype), logits.device)
+    if weight is not None:
+        _expect("distill_loss", "weight", weight, lead, (torch.float32,), logits.device)
+    tau = float(temperature)
+    if not 0.0 < tau < float("inf"):
+        raise RuntimeError("distill_loss: temperature must be positive and finite, got %r" % (temperature,))
+    if _wants_grad(teacher, weight):
+        raise RuntimeError("distill_loss: gradients go to the logits only (detach teacher and weight)")
+    ids2, t2 = ids.reshape(-1, k).contiguous(), teacher.detach().reshape(-1, k).float().contiguous()
+    w2 = None if weight is None else weight.detach().reshape(-1).contiguous()
+    if _wants_grad(logits):
+        return _DistillFn.apply(logits, ids2, t2, w2, tau, code)
+    z, ldz = _matrix(logits.reshape(-1, logits.size(-1)))
+    total, rows, _ = _distill(z, ldz, code, ids2, t2, tau, w2, False)
+    return total, rows.view(lead)

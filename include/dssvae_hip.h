@@ -595,6 +595,23 @@ int dssvae_gated_scan_bwd(const void* x, int64_t xb, int64_t xt, int dtype, cons
 int dssvae_gated_step(const void* x, int64_t xb, int dtype, const float* h, int tanh_candidate, int B, int H, void* out,
                       int64_t ob, float* h_out, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Distillation from a teacher's top logits.
+ *   p = softmax(teacher / tau) over a row's valid slots, q = softmax(logits / tau) over the vocabulary
+ *   rows[i] = tau^2 sum_j p_j (log p_j - log q[ids_j]); *total = sum_i w_i rows[i]; dlogits = w_i tau (q - scatter(p))
+ *   logits, dlogits [N, V] of `dtype`, row strides ldz / lddz; ids [N, k] int64 and teacher [N, k] fp32 contiguous,
+ *   1 <= k <= DSSVAE_DISTILL_MAX_TOP; an id < 0 is an empty slot, the same id twice adds up, an id >= V, a NaN or +inf
+ *   teacher logit makes its row (loss and gradient) NaN.  A row without a valid slot, all teacher logits -inf among it, and one of
+ *   weight 0 is not read: loss 0, gradient 0.  weight [N] fp32, or NULL: weight_all for every row.
+ *   dlogits NULL: no gradient.  Its rows must start at the same offset from a 16-byte boundary as those of logits.
+ * dssvae_scale_rows: x[r, :V] *= *factor (fp32 on the device), without touching memory where that is 1.
+ * ------------------------------------------------------------------------------------------- */
+#define DSSVAE_DISTILL_MAX_TOP 1024
+int dssvae_distill(const void* logits, int64_t ldz, int dtype, int64_t N, int V, const int64_t* ids, const float* teacher,
+                   int k, float tau, const float* weight, float weight_all, void* dlogits, int64_t lddz, float* rows,
+                   float* total, void* stream);
+int dssvae_scale_rows(void* x, int64_t ld, int dtype, int64_t rows, int V, const float* factor, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
