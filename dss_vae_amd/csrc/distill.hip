@@ -4,8 +4,10 @@
 //   row = tau^2 sum_j p_j (log p_j - log q[id_j]) ; total = sum_i w_i row_i ; dlogits = w tau (q - scatter(p))
 //
 // One block per row.  The weight of a row is known at the call, so the gradient leaves in the SAME pass: a row stays in
-// registers (NV granules of 16 bytes per thread) between its read, its maximum, its sum and the store; wider rows than
-// 16 granules x 1024 threads are read twice.  Rows may start at any element: up to VEC - 1 elements in front of the first
+// registers (NV granules of 16 bytes per thread) between its read and the store; wider rows than 16 granules x 1024 threads
+// are read twice.  Maximum and sum are one walk, granule by granule as they arrive: two walks left the memory idle for the
+// second where only one block fits a CU (2048 x 100003 bf16, NV = 16: 222 us, now 181 us = 4.3 TB/s).  Up to NV = 8 two
+// blocks share a CU (64 registers) and fill each other's gaps: 7936 x 30000 fp32 in 345 us = 5.2 TB/s.  Rows may start at any element: up to VEC - 1 elements in front of the first
 // 16-byte boundary and behind the last granule are "edge" elements, one per thread.
 // The k teacher slots are wave 0's: softmax by shuffles while the block loads.  The k gradient entries are written over the
 // dense store behind a barrier, by the first slot of each distinct id with the sum of its probabilities: no atomics, and
@@ -19,37 +21,33 @@ constexpr float LOG2E = 1.4426950408889634f, NINF = -__builtin_huge_valf();
 
 __device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
 
-template <int NT, bool MAX>
-__device__ __forceinline__ float block_reduce(float v, float* red /* [NT / 64] */) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float u = __shfl_xor(v, o, 64);
-        v = MAX ? fmaxf(v, u) : v + u;
-    }
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int i = 1; i < NT / 64; ++i) v = MAX ? fmaxf(v, red[i]) : v + red[i];
-    return v;
-}
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
     return v;
 }
 
+// Running maximum m and sum s of exp((x - m) / tau): one more granule
+template <typename T, int VEC>
+__device__ __forceinline__ void online(const Gran<T, VEC>& v, float c, float& m, float& s) {
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) top = fmaxf(top, v.get(j));
+    const float ref = top == NINF ? 0.f : top;  // (all -inf so far: every term is 0; a NaN stays one)
+    s *= exp2_f((m - ref) * c);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s += exp2_f((v.get(j) - ref) * c);
+    m = top;
+}
+
 // The granules stay in their 16 bytes between the walks over them: the compiler may not keep them as floats as well, which
 // would double a 16-bit row's registers (and spill).
-template <typename T, int VEC, int N>
-__device__ __forceinline__ void keep_raw(Gran<T, VEC> (&v)[N]) {
+template <typename T, int VEC>
+__device__ __forceinline__ void keep_raw(Gran<T, VEC>& v) {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        u32x4 r = __builtin_bit_cast(u32x4, v[i].v);
-        asm volatile("" : "+v"(r));
-        v[i].v = __builtin_bit_cast(typename Gran<T, VEC>::V, r);
-    }
+    u32x4 r = __builtin_bit_cast(u32x4, v.v);
+    asm volatile("" : "+v"(r));
+    v.v = __builtin_bit_cast(typename Gran<T, VEC>::V, r);
 }
 
 // NV granules per thread in registers; NV = 0: any width, the row is read twice
@@ -59,7 +57,7 @@ __global__ __launch_bounds__(NT, NT == 1024 && NV <= 8 ? 8 : 4) void distill_ker
     float tau, const float* __restrict__ weight, float w_all, T* __restrict__ dz, int64_t lddz, float* __restrict__ rows) {
     constexpr int VEC = 16 / (int)sizeof(T);
     constexpr int NR = NV > 0 ? NV : 1;
-    __shared__ float red_max[NT / 64], red_sum[NT / 64];
+    __shared__ float2 red[NT / 64];  // (maximum, sum) of each wave
     __shared__ int s_id[MAX_TOP];
     __shared__ float s_p[MAX_TOP];
     __shared__ float s_mass;  // 1, 0 (no valid slot) or NaN (an id outside the vocabulary, a NaN or +inf among the teacher's logits)
@@ -82,7 +80,7 @@ __global__ __launch_bounds__(NT, NT == 1024 && NV <= 8 ? 8 : 4) void distill_ker
             for (int i = 0; i < NV; ++i) {
                 const int g = i * NT + tid;
                 if (g < nvec) {
-                    v[i].load(zb + (int64_t)g * VEC);
+                    v[i].load(zb + (unsigned)(g * VEC));
                 } else {
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) v[i].set(j, NINF);
@@ -110,35 +108,27 @@ __global__ __launch_bounds__(NT, NT == 1024 && NV <= 8 ? 8 : 4) void distill_ker
             if (tid == 0) s_mass = any_bad ? __builtin_nanf("") : none ? 0.f : 1.f;
         }
     }
-    float m = ev, s = 0.f;
+    // maximum and sum in ONE walk that consumes the granules in the order they arrive, the later ones still in flight
+    float m = ev, s = ev == NINF ? 0.f : 1.f;
     if (!dead) {
         if constexpr (NV > 0) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) m = fmaxf(m, v[i].get(j));
+            for (int i = 0; i < NV; ++i) {
+                online(v[i], c, m, s);
+                keep_raw(v[i]);
+            }
         } else {
-            // running maximum and sum of this thread
-            s = edge >= 0 ? 1.f : 0.f;
             for (int64_t g = tid; g < nvec; g += NT) {
                 v[0].load(zb + g * VEC);
-                float top = m;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) top = fmaxf(top, v[0].get(j));
-                if (top == NINF) {
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) s = v[0].get(j) != v[0].get(j) ? v[0].get(j) : s;
-                    continue;
-                }
-                s *= exp2_f((m - top) * c);
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) s += exp2_f((v[0].get(j) - top) * c);
-                m = top;
+                online(v[0], c, m, s);
             }
         }
     }
-    const float M = block_reduce<NT, true>(m, red_max);
-    if constexpr (NV > 0) keep_raw(v);
+    const float mw = wave_max(m);
+    s *= exp2_f((m - (mw == NINF ? 0.f : mw)) * c);
+    s = wave_sum(s);
+    if ((tid & 63) == 0) red[tid >> 6] = make_float2(mw, s);
+    __syncthreads();
     const float mass = dead ? 0.f : s_mass;
     if (mass == 0.f) {  // (the whole block alike)
         if (tid == 0) rows[row] = 0.f;
@@ -150,17 +140,13 @@ __global__ __launch_bounds__(NT, NT == 1024 && NV <= 8 ? 8 : 4) void distill_ker
         if (edge >= 0) dr[edge] = (T)0.f;
         return;
     }
-    if constexpr (NV > 0) {
+    const float2 r = red[tid % (NT / 64)];  // every NT / 64 neighbouring lanes hold all the waves' pairs
+    float M = r.x;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+    for (int o = NT / 128; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    float S = r.y * exp2_f((r.x - M) * c);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s += exp2_f((v[i].get(j) - M) * c);
-        if (edge >= 0) s += exp2_f((ev - M) * c);
-    } else {
-        s = m == NINF ? (s != s ? s : 0.f) : s * exp2_f((m - M) * c);
-    }
-    const float S = block_reduce<NT, false>(s, red_sum);
-    if constexpr (NV > 0) keep_raw(v);
+    for (int o = NT / 128; o > 0; o >>= 1) S += __shfl_xor(S, o, 64);
     if (tid < 64) {
         float part = 0.f;
         for (int j = tid; j < k; j += 64) {
@@ -181,7 +167,7 @@ __global__ __launch_bounds__(NT, NT == 1024 && NV <= 8 ? 8 : 4) void distill_ker
             Gran<T, VEC> o;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) o.set(j, a * exp2_f((v[i].get(j) - M) * c));
-            o.store(db + (int64_t)g * VEC);
+            o.store(db + (unsigned)(g * VEC));
         }
     } else {
         for (int64_t g = tid; g < nvec; g += NT) {
@@ -199,6 +185,7 @@ __global__ __launch_bounds__(NT, NT == 1024 && NV <= 8 ? 8 : 4) void distill_ker
         if (id < 0) continue;
         float p = 0.f;
         bool first = true;
+#pragma unroll 4
         for (int i = 0; i < k; ++i) {
             const bool same = s_id[i] == id;
             first = first && !(same && i < j);
