@@ -1,0 +1,680 @@
+// Linear layer with its epilogue:  z = x w^T + b,  y = act(z) + residual,  and its backward pass
+//   dz = dy act'(z),  dx = dz w,  dw = dz^T x,  db = sum_rows dz,  dresidual = dy.
+//
+// fp32 products run on dssvae_gemm_f32 (v_mfma_f32_32x32x2_f32) with the epilogue as one pass behind them.  bf16 / fp16
+// products are this file's: v_mfma_f32_32x32x16, fp32 accumulation, one rounding per output.
+//
+// The 16-bit tile kernel: C[M, N] = A[M, K] . B[N, K]^T, both operands contiguous along K.  A BM x BN block walks K in
+// steps of 64; operand tiles go global -> LDS directly (16 bytes a lane, no registers), double buffered.  LDS row r keeps its
+// 16-byte chunk c at place c ^ (r & 7): the eight rows a quarter wave reads at one chunk then cover all banks (rows are 128
+// bytes apart, unswizzled they would share one).  The pipeline is rotated: fragments of the step's first half are already in
+// registers when it begins; one barrier per step, passed between the halves: by then the next tile has landed and every
+// wave has read all of this one, so its buffer takes the tile after next while the second half multiplies.
+// The backward operands that are contiguous the other way (w and x along the summed axis, dz for dw) are transposed into the
+// workspace first: dz in both orders by the pass that forms it, which also leaves the column sums for db.
+// Few output tiles: K is split over blocks, fp32 partials go to the workspace and a second launch adds them in order and
+// applies the epilogue (no atomics: same bits every time).
+#include "elem.h"
+
+namespace {
+
+constexpr int BK = 64;
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+// ---- activations --------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float sigmoid_f(float x) {
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+}
+__device__ __forceinline__ float tanh_f(float x) {
+    return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.8853900817779268f * x));
+}
+__device__ __forceinline__ float act_f(int act, float z) {
+    switch (act) {
+        case DSSVAE_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
+        case DSSVAE_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+        case DSSVAE_ACT_SILU: return z * sigmoid_f(z);
+        case DSSVAE_ACT_TANH: return tanh_f(z);
+        default: return z;
+    }
+}
+__device__ __forceinline__ float act_slope(int act, float z) {
+    switch (act) {
+        case DSSVAE_ACT_RELU: return z > 0.f ? 1.f : (z != z ? z : 0.f);
+        case DSSVAE_ACT_GELU:
+            return 0.5f * (1.f + erff(z * 0.70710678118654752f)) +
+                   z * 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
+        case DSSVAE_ACT_SILU: {
+            const float s = sigmoid_f(z);
+            return s * (1.f + z * (1.f - s));
+        }
+        case DSSVAE_ACT_TANH: {
+            const float t = tanh_f(z);
+            return 1.f - t * t;
+        }
+        default: return 1.f;
+    }
+}
+
+// z is kept for backward in the activations' type: rounded, and held below the type's infinity (the slopes of a huge finite z
+// are exact there, those of an infinity would be 0 * inf)
+template <typename T> __device__ __forceinline__ float keep_z(float z) { return z; }
+template <> __device__ __forceinline__ float keep_z<f16_t>(float z) { return z > 65504.f ? 65504.f : z < -65504.f ? -65504.f : z; }
+
+// What happens to an accumulated element on its way out
+struct Epilogue {
+    const void* bias; int bias_f32;   // [N] or NULL
+    const void* res; int64_t ldr;     // [M, N] or NULL
+    void* z; int64_t ldz;             // pre-activation, or NULL
+    void* y; int64_t ldy;
+    int act, vec;                     // vec: rows of res, z, y may be moved 16 bytes at a time
+};
+
+template <typename T>
+__device__ __forceinline__ float bias_at(const Epilogue& e, int64_t n) {
+    if (!e.bias) return 0.f;
+    return e.bias_f32 ? reinterpret_cast<const float*>(e.bias)[n] : (float)reinterpret_cast<const T*>(e.bias)[n];
+}
+
+// eight consecutive columns n .. of row m (those below N), acc without bias
+template <typename T>
+__device__ __forceinline__ void finish8(const Epilogue& e, f32x8 a, int64_t m, int n, int N) {
+    T* y = reinterpret_cast<T*>(e.y) + m * e.ldy + n;
+    T* z = e.z ? reinterpret_cast<T*>(e.z) + m * e.ldz + n : nullptr;
+    const T* r = e.res ? reinterpret_cast<const T*>(e.res) + m * e.ldr + n : nullptr;
+    if (e.vec && n + 8 <= N) {
+        Gran<T, 8> g;
+        if (r) g.load(r);
+        Gran<T, 8> gz, gy;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float zz = a[j] + bias_at<T>(e, n + j);
+            gz.set(j, keep_z<T>(zz));
+            gy.set(j, act_f(e.act, zz) + (r ? g.get(j) : 0.f));
+        }
+        if (z) gz.store(z);
+        gy.store(y);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (n + j >= N) continue;
+            const float zz = a[j] + bias_at<T>(e, n + j);
+            if (z) z[j] = (T)keep_z<T>(zz);
+            y[j] = (T)(act_f(e.act, zz) + (r ? (float)r[j] : 0.f));
+        }
+    }
+}
+
+// ---- the 16-bit tile kernel ---------------------------------------------------------------------------------------
+typedef __attribute__((address_space(1))) const void* gptr_t;
+typedef __attribute__((address_space(3))) void* lptr_t;
+
+__device__ const uint4 zero_granule = {0, 0, 0, 0};
+
+template <typename T> struct Mfma;
+template <> struct Mfma<bf16_t> {
+    typedef bf16_t V __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x16 go(V a, V b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mfma<f16_t> {
+    typedef f16_t V __attribute__((ext_vector_type(8)));
+    static __device__ __forceinline__ f32x16 go(V a, V b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+
+// One operand's share of a tile load: R rows x 64 k, TH threads, 16 bytes a lane.  A thread's granules all lie in the same
+// place of their rows (rows TH / 8 apart, a multiple of 8: the swizzle is the same), so only the row pointer differs.
+template <typename T, int R, int TH>
+struct Loader {
+    static constexpr int NR = R * 8 / TH;
+    const T* p[NR];
+    int k;  // k of this thread's granule inside a tile
+    __device__ __forceinline__ void init(const T* base, int64_t ld, int64_t r0, int64_t rows) {
+        const int row = threadIdx.x >> 3;
+        k = (int)((threadIdx.x & 7) ^ (row & 7)) * 8;
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            int64_t r = r0 + row + i * (TH / 8);
+            r = r < rows ? r : rows - 1;  // rows behind the last are computed from it and never stored
+            p[i] = base + r * ld + k;
+        }
+    }
+    // k0: first k of the tile; granules at or behind K come from a granule of zeros
+    __device__ __forceinline__ void load(T* lds, int64_t k0, int64_t K) const {
+        const int wave = threadIdx.x >> 6;
+        const bool in = k0 + k < K;
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            const T* src = in ? p[i] + k0 : reinterpret_cast<const T*>(&zero_granule);
+            __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(lds + (i * TH + wave * 64) * 8), 16, 0, 0);
+        }
+    }
+};
+
+// MI x NI blocks of 32 x 32 of this wave's tile: the operands of K half `h` (two MFMA steps of 16)
+template <typename T, int MI, int NI>
+struct Frags {
+    typename Mfma<T>::V a[2][MI], b[2][NI];
+    __device__ __forceinline__ void read(const T* sa, const T* sb, int ra, int rb, int h) {
+        const int lane = threadIdx.x & 63, r = lane & 31;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int c = ((h * 4 + s * 2 + (lane >> 5)) ^ (r & 7)) * 8;  // (tile rows start at multiples of 8)
+#pragma unroll
+            for (int i = 0; i < MI; ++i) a[s][i] = *reinterpret_cast<const typename Mfma<T>::V*>(sa + (ra + i * 32 + r) * BK + c);
+#pragma unroll
+            for (int j = 0; j < NI; ++j) b[s][j] = *reinterpret_cast<const typename Mfma<T>::V*>(sb + (rb + j * 32 + r) * BK + c);
+        }
+    }
+    __device__ __forceinline__ void multiply(f32x16 (&acc)[MI][NI]) const {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) acc[i][j] = Mfma<T>::go(a[s][i], b[s][j], acc[i][j]);
+    }
+};
+
+struct Shape {
+    const void* A; int64_t lda;
+    const void* B; int64_t ldb;
+    int64_t M; int N; int64_t K;
+    int tiles_m, tiles_n, ksplit;
+    int64_t ktiles;      // k-tiles per split
+    float* part;         // [ksplit][M][N] where ksplit > 1
+};
+
+// output tile of work item `wid`: groups of 8 tile rows, column by column inside a group, so that the blocks of an XCD that run
+// together share operand panels in its L2
+__device__ __forceinline__ void tile_of(const Shape& s, int t, int& tm, int& tn) {
+    constexpr int G = 8;
+    const int per = G * s.tiles_n, g = t / per, first = g * G, rows = min(G, s.tiles_m - first), in = t - g * per;
+    tm = first + in % rows;
+    tn = in / rows;
+}
+
+template <typename T, int BM, int BN, int WR, int WC>
+__global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, Epilogue e) {
+    constexpr int TH = 64 * WR * WC, MI = BM / WR / 32, NI = BN / WC / 32;
+    static_assert(NI == 2, "the epilogue moves 64 columns of a wave at a time");
+    __shared__ __attribute__((aligned(16))) T sa0[BM * BK], sa1[BM * BK], sb0[BN * BK], sb1[BN * BK];
+    const int wid = xcd_remap(blockIdx.x, gridDim.x), tiles = s.tiles_m * s.tiles_n;
+    const int split = wid / tiles;
+    int tm, tn;
+    tile_of(s, wid - split * tiles, tm, tn);
+    const int64_t m0 = (int64_t)tm * BM;
+    const int n0 = tn * BN;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int ra = wave / WC * (BM / WR), rb = wave % WC * (BN / WC);
+    const int64_t nk = (s.K + BK - 1) / BK, kt0 = split * s.ktiles, kt1 = min(nk, kt0 + s.ktiles);
+
+    f32x16 acc[MI][NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+    Loader<T, BM, TH> la;
+    Loader<T, BN, TH> lb;
+    la.init((const T*)s.A, s.lda, m0, s.M);
+    lb.init((const T*)s.B, s.ldb, n0, s.N);
+    // a tile at or behind kt1 is loaded from zeros (nobody multiplies it)
+    const int64_t kend = min(s.K, kt1 * BK);
+    if (kt0 < kt1) {
+        la.load(sa0, kt0 * BK, kend);
+        lb.load(sb0, kt0 * BK, kend);
+        la.load(sa1, (kt0 + 1) * BK, kend);
+        lb.load(sb1, (kt0 + 1) * BK, kend);
+        __syncthreads();
+        Frags<T, MI, NI> f0, f1;
+        f0.read(sa0, sb0, ra, rb, 0);
+        for (int64_t kt = kt0;; kt += 2) {
+            f1.read(sa0, sb0, ra, rb, 1);
+            f0.multiply(acc);
+            __syncthreads();  // everyone has read buffer 0, tile kt + 1 has landed in buffer 1
+            if (kt + 2 < kt1) {
+                la.load(sa0, (kt + 2) * BK, kend);
+                lb.load(sb0, (kt + 2) * BK, kend);
+            }
+            f0.read(sa1, sb1, ra, rb, 0);
+            f1.multiply(acc);
+            if (kt + 1 >= kt1) break;
+            f1.read(sa1, sb1, ra, rb, 1);
+            f0.multiply(acc);
+            __syncthreads();
+            if (kt + 3 < kt1) {
+                la.load(sa1, (kt + 3) * BK, kend);
+                lb.load(sb1, (kt + 3) * BK, kend);
+            }
+            f0.read(sa0, sb0, ra, rb, 0);
+            f1.multiply(acc);
+            if (kt + 2 >= kt1) break;
+        }
+        __syncthreads();  // operand buffers are free (and no load is in flight)
+    }
+
+    // 32 rows x 64 columns of this wave at a time through 8 KiB of LDS of its own, read back along rows
+    constexpr int HALF = WR * WC / 2;
+    float* stage = reinterpret_cast<float*>(wave < HALF ? sa0 : sa1) + (wave % HALF) * 32 * 64;
+    static_assert(HALF * 32 * 64 * 4 <= (int)sizeof(sa0), "the waves' staging rows fit the operand buffers");
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                stage[((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * 64 + j * 32 + (lane & 31)] = acc[i][j][r];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int row = q * 8 + (lane >> 3), col = (lane & 7) * 8;
+            const f32x8 v = *reinterpret_cast<const f32x8*>(stage + row * 64 + col);
+            const int64_t m = m0 + ra + i * 32 + row;
+            const int n = n0 + rb + col;
+            if (m >= s.M || n >= s.N) continue;
+            if (s.ksplit > 1) {
+                float* o = s.part + ((int64_t)split * s.M + m) * s.N + n;
+                if (n + 8 <= s.N && s.N % 4 == 0) {
+                    reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+                    reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (n + j < s.N) o[j] = v[j];
+                }
+            } else {
+                finish8<T>(e, v, m, n, s.N);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+
+// partials of the K splits, added in order, then the epilogue: 8 columns a thread
+template <typename T>
+__global__ __launch_bounds__(256) void linear_join_kernel(const float* __restrict__ part, int ksplit, int64_t M, int N,
+                                                          Epilogue e) {
+    const int per = (N + 7) / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= M * per) return;
+    const int64_t m = i / per;
+    const int n = (int)(i % per) * 8;
+    f32x8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    for (int k = 0; k < ksplit; ++k) {
+        const float* p = part + ((int64_t)k * M + m) * N + n;
+        if (n + 8 <= N && N % 4 == 0) {
+            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+            v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+            v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (n + j < N) v[j] += p[j];
+        }
+    }
+    finish8<T>(e, v, m, n, N);
+}
+
+// ---- operands into the form the tile kernel takes -----------------------------------------------------------------
+// dst [R, ldd] = src [R, C], columns C .. ldd zero
+template <typename T>
+__global__ __launch_bounds__(256) void linear_pack_kernel(const T* __restrict__ src, int64_t ld, int64_t R, int64_t C,
+                                                          T* __restrict__ dst, int64_t ldd) {
+    for (int64_t r = blockIdx.x; r < R; r += gridDim.x)
+        for (int64_t c = threadIdx.x; c < ldd; c += 256) dst[r * ldd + c] = c < C ? src[r * ld + c] : (T)0.f;
+}
+
+// One pass over a [R, C] matrix in 64 x 64 tiles (a block walks the row tiles blockIdx.y, + gridDim.y of one column tile):
+//   v = src                      (z NULL)
+//   v = src * act'(z)            else
+// out [R, ldo] (NULL: not wanted) gets v, columns C .. ldo zero; outT [C, ldt] (NULL) its transpose, columns R .. ldt zero;
+// sums [gridDim.y][C] (NULL) the block's column sums of the unrounded v.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_turn_kernel(const T* __restrict__ src, int64_t ld, const T* __restrict__ z,
+                                                          int64_t ldz, int act, int64_t R, int64_t C, T* __restrict__ out,
+                                                          int64_t ldo, T* __restrict__ outT, int64_t ldt,
+                                                          float* __restrict__ sums) {
+    __shared__ T tile[64][66];
+    __shared__ float red[4][64];
+    const int64_t c0 = (int64_t)blockIdx.x * 64;
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const int64_t rtiles = (R + 63) / 64;
+    float sum = 0.f;
+    for (int64_t rt = blockIdx.y; rt < rtiles; rt += gridDim.y) {
+        const int64_t r0 = rt * 64;
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+            const int64_t r = r0 + i * 4 + ty, c = c0 + tx;
+            float v = 0.f;
+            if (r < R && c < C) {
+                v = (float)src[r * ld + c];
+                if (z) v *= act_slope(act, (float)z[r * ldz + c]);
+            }
+            sum += v;
+            if (out && r < R && c < ldo) out[r * ldo + c] = (T)v;
+            if (outT) tile[i * 4 + ty][tx] = (T)v;
+        }
+        if (outT) {
+            __syncthreads();
+#pragma unroll 4
+            for (int i = 0; i < 16; ++i) {
+                const int64_t c = c0 + i * 4 + ty, r = r0 + tx;
+                if (c < C && r < ldt) outT[c * ldt + r] = tile[tx][i * 4 + ty];
+            }
+            __syncthreads();
+        }
+    }
+    if (!sums) return;
+    red[ty][tx] = sum;
+    __syncthreads();
+    if (ty == 0 && c0 + tx < C) sums[(int64_t)blockIdx.y * C + c0 + tx] = red[0][tx] + red[1][tx] + red[2][tx] + red[3][tx];
+}
+
+// db [C] = sum of n rows of partial sums, in order
+template <typename T>
+__global__ __launch_bounds__(256) void linear_db_kernel(const float* __restrict__ sums, int n, int64_t C, void* db, int f32) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= C) return;
+    float s = 0.f;
+    for (int i = 0; i < n; ++i) s += sums[(int64_t)i * C + c];
+    if (f32) reinterpret_cast<float*>(db)[c] = s;
+    else reinterpret_cast<T*>(db)[c] = (T)s;
+}
+
+// fp32: y = act(z) + res over the product's output
+__global__ __launch_bounds__(256) void linear_epilogue_f32_kernel(const float* z, int64_t ldz, const float* __restrict__ res,
+                                                                  int64_t ldr, int act, int64_t M, int N, float* y, int64_t ldy) {
+    for (int64_t m = blockIdx.x; m < M; m += gridDim.x)
+        for (int n = threadIdx.x; n < N; n += 256)
+            y[m * ldy + n] = act_f(act, z[m * ldz + n]) + (res ? res[m * ldr + n] : 0.f);
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------
+inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// Tile width and K split: the smallest of a cost in units of one 128 x 128 x 64 step of a CU.  Two 128-wide blocks share a CU
+// and their steps read twice the LDS per product (a step costs 1.35); partials cost their traffic.
+struct Plan { bool wide; int ksplit; };
+inline Plan plan(int64_t M, int64_t N, int64_t K) {
+    const double cus = device_cus();
+    const int64_t nk = up(K, BK) / BK;
+    Plan best{false, 1};
+    double least = -1;
+    for (int wide = 0; wide < 2; ++wide)
+        for (int ks = 1; ks <= 16; ks *= 2) {
+            if (ks > 1 && nk / ks < 4) break;
+            const int b = wide ? 256 : 128;
+            const double tiles = (double)(up(M, b) / b) * (double)(up(N, b) / b) * ks, steps = (double)((nk + ks - 1) / ks);
+            const double slots = wide ? cus : 2 * cus, rounds = (double)(int64_t)((tiles + slots - 1) / slots);
+            double cost = wide ? rounds * (steps * 4 + 12) : rounds * (2 * 1.35 * steps + 6);
+            if (ks > 1) cost += 10 + (double)(2 * ks) * M * N * 4 / 2e6;
+            if (least < 0 || cost < least) {
+                least = cost;
+                best = Plan{wide != 0, ks};
+            }
+        }
+    return best;
+}
+
+inline int64_t part_bytes(int64_t M, int64_t N, int64_t K) {
+    const Plan p = plan(M, N, K);
+    return p.ksplit > 1 ? up((int64_t)p.ksplit * M * N * 4, 256) : 0;
+}
+
+// operand rows usable as they are: 16-byte granules
+inline bool direct(const void* p, int64_t ld, int64_t K) { return aligned_to(p, 16) && ld % 8 == 0 && K % 8 == 0; }
+
+inline bool epilogue_vec(const Epilogue& e) {
+    return aligned_to(e.y, 16) && e.ldy % 8 == 0 && (!e.z || (aligned_to(e.z, 16) && e.ldz % 8 == 0)) &&
+           (!e.res || (aligned_to(e.res, 16) && e.ldr % 8 == 0));
+}
+
+template <typename T>
+int product(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K, Epilogue e, void* part,
+            hipStream_t st) {
+    if (M == 0 || N == 0) return DSSVAE_OK;
+    const Plan p = plan(M, N, K);
+    const int b = p.wide ? 256 : 128;
+    Shape s;
+    s.A = A; s.lda = lda; s.B = B; s.ldb = ldb; s.M = M; s.N = (int)N; s.K = K;
+    const int64_t tm = up(M, b) / b, tn = up(N, b) / b;
+    if (tm * tn * p.ksplit > 0x7fffffff) return DSSVAE_ETOOBIG;
+    s.tiles_m = (int)tm; s.tiles_n = (int)tn; s.ksplit = p.ksplit;
+    const int64_t nk = up(K, BK) / BK;
+    s.ktiles = (nk + p.ksplit - 1) / p.ksplit;
+    s.part = (float*)part;
+    e.vec = epilogue_vec(e);
+    const dim3 grid((unsigned)(tm * tn * p.ksplit));
+    if (p.wide) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, 4>), grid, dim3(512), 0, st, s, e);
+    else hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, 2>), grid, dim3(256), 0, st, s, e);
+    DSSVAE_CHECK_LAUNCH();
+    if (p.ksplit > 1) {
+        const int64_t n = M * ((N + 7) / 8), blocks = (n + 255) / 256;
+        if (blocks > 0x7fffffff) return DSSVAE_ETOOBIG;
+        hipLaunchKernelGGL((linear_join_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, st, s.part, p.ksplit, M, (int)N, e);
+        DSSVAE_CHECK_LAUNCH();
+    }
+    return DSSVAE_OK;
+}
+
+template <typename T>
+int pack(const void* src, int64_t ld, int64_t R, int64_t C, void* dst, int64_t ldd, hipStream_t st) {
+    if (R == 0) return DSSVAE_OK;
+    const int64_t most = 16 * (int64_t)device_cus();
+    hipLaunchKernelGGL((linear_pack_kernel<T>), dim3((unsigned)(R < most ? R : most)), dim3(256), 0, st, (const T*)src, ld, R, C,
+                       (T*)dst, ldd);
+    DSSVAE_CHECK_LAUNCH();
+    return DSSVAE_OK;
+}
+
+// blocks along the rows of linear_turn_kernel: enough to fill the chip
+inline int64_t turn_rows(int64_t R, int64_t C) {
+    const int64_t ct = (C + 63) / 64, rt = (R + 63) / 64, want = (8 * (int64_t)device_cus() + ct - 1) / ct;
+    return rt < 1 ? 1 : rt < want ? rt : want;
+}
+template <typename T>
+int turn(const void* src, int64_t ld, const void* z, int64_t ldz, int act, int64_t R, int64_t C, void* out, int64_t ldo, void* outT,
+         int64_t ldt, float* sums, hipStream_t st) {
+    const dim3 grid((unsigned)((C + 63) / 64), (unsigned)turn_rows(R, C));
+    hipLaunchKernelGGL((linear_turn_kernel<T>), grid, dim3(256), 0, st, (const T*)src, ld, (const T*)z, ldz, act, R, C, (T*)out, ldo,
+                       (T*)outT, ldt, sums);
+    DSSVAE_CHECK_LAUNCH();
+    return DSSVAE_OK;
+}
+
+// workspace pieces, each on a 256-byte boundary
+struct Space {
+    char* p; int64_t used, size;
+    void* take(int64_t bytes) {
+        void* r = p ? p + used : nullptr;
+        used += up(bytes, 256);
+        return r;
+    }
+};
+
+bool bad_args(int dtype, int act, int64_t M, int N, int K) {
+    return !dtype_ok(dtype) || act < DSSVAE_ACT_NONE || act > DSSVAE_ACT_TANH || M < 0 || M > 0x7fffffff || N < 1 || K < 1 ||
+           N > (1 << 30) || K > (1 << 30);
+}
+
+template <typename T>
+int fwd16(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int N, int K, const Epilogue& e, Space& sp, hipStream_t st,
+          bool dry) {
+    const int64_t ldk = up(K, 8);
+    if (!direct(x, ldx, K)) {
+        void* d = sp.take(M * ldk * 2);
+        if (!dry) { const int rc = pack<T>(x, ldx, M, K, d, ldk, st); if (rc) return rc; }
+        x = d; ldx = ldk;
+    }
+    if (!direct(w, ldw, K)) {
+        void* d = sp.take((int64_t)N * ldk * 2);
+        if (!dry) { const int rc = pack<T>(w, ldw, N, K, d, ldk, st); if (rc) return rc; }
+        w = d; ldw = ldk;
+    }
+    void* part = sp.take(part_bytes(M, N, ldk));
+    return dry ? DSSVAE_OK : product<T>(x, ldx, w, ldw, M, N, ldk, e, part, st);
+}
+
+struct BwdArgs {
+    const void *dy, *z, *x, *w;
+    int64_t lddy, ldz, ldx, ldw, lddx, lddw;
+    void *dx, *dw, *db;
+    int db_f32, act;
+    int64_t M; int N, K;
+};
+
+template <typename T>
+int bwd16(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
+    const int64_t M = a.M, N = a.N, K = a.K, ldn = up(N, 8), ldm = up(M, 8);
+    int rc = DSSVAE_OK;
+    // dz: a copy where it differs from dy or dy's rows cannot be loaded as they are
+    const bool copy = a.dx && (a.z || !direct(a.dy, a.lddy, N));
+    const void* dz = a.dy;
+    int64_t lddz = a.lddy;
+    void *dzc = nullptr, *dzt = nullptr;
+    if (copy) { dzc = sp.take(M * ldn * 2); dz = dzc; lddz = ldn; }
+    if (a.dw) dzt = sp.take(N * ldm * 2);
+    float* sums = a.db ? (float*)sp.take(turn_rows(M, N) * N * 4) : nullptr;
+    if (copy || a.dw || a.db) {
+        if (!dry) {
+            if ((rc = turn<T>(a.dy, a.lddy, a.z, a.ldz, a.act, M, N, dzc, ldn, dzt, ldm, sums, st))) return rc;
+            if (a.db) {
+                hipLaunchKernelGGL((linear_db_kernel<T>), dim3((unsigned)((N + 255) / 256)), dim3(256), 0, st, sums,
+                                   (int)turn_rows(M, N), N, a.db, a.db_f32);
+                DSSVAE_CHECK_LAUNCH();
+            }
+        }
+    }
+    if (a.dx) {
+        void* wt = sp.take(K * ldn * 2);
+        void* part = sp.take(part_bytes(M, K, ldn));
+        if (!dry) {
+            if ((rc = turn<T>(a.w, a.ldw, nullptr, 0, 0, N, K, nullptr, 0, wt, ldn, nullptr, st))) return rc;
+            Epilogue e{};
+            e.y = a.dx; e.ldy = a.lddx;
+            if ((rc = product<T>(dz, lddz, wt, ldn, M, K, ldn, e, part, st))) return rc;
+        }
+    }
+    if (a.dw) {
+        void* xt = sp.take(K * ldm * 2);
+        void* part = sp.take(part_bytes(N, K, ldm));
+        if (!dry) {
+            if ((rc = turn<T>(a.x, a.ldx, nullptr, 0, 0, M, K, nullptr, 0, xt, ldm, nullptr, st))) return rc;
+            Epilogue e{};
+            e.y = a.dw; e.ldy = a.lddw;
+            if ((rc = product<T>(dzt, ldm, xt, ldm, N, K, ldm, e, part, st))) return rc;
+        }
+    }
+    return rc;
+}
+
+int bwd32(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
+    const float* dz = (const float*)a.dy;
+    int64_t lddz = a.lddy;
+    float *dzc = nullptr, *sums = nullptr;
+    int rc = DSSVAE_OK;
+    if (a.z && (a.dx || a.dw)) {
+        dzc = (float*)sp.take(a.M * a.N * 4);
+        dz = dzc; lddz = a.N;
+    }
+    if (a.db) sums = (float*)sp.take(turn_rows(a.M, a.N) * a.N * 4);
+    if (dry) return rc;
+    if (dzc || sums) {
+        if ((rc = turn<float>(a.dy, a.lddy, a.z, a.ldz, a.act, a.M, a.N, dzc, a.N, nullptr, 0, sums, st))) return rc;
+        if (a.db) {
+            hipLaunchKernelGGL((linear_db_kernel<float>), dim3((unsigned)((a.N + 255) / 256)), dim3(256), 0, st, sums,
+                               (int)turn_rows(a.M, a.N), a.N, a.db, 1);
+            DSSVAE_CHECK_LAUNCH();
+        }
+    }
+    const int M = (int)a.M;
+    if (a.dx && M > 0 && (rc = dssvae_gemm_f32(dz, lddz, 0, nullptr, (const float*)a.w, a.ldw, 1, (float*)a.dx, a.lddx, nullptr, M, a.K,
+                                               a.N, 1.f, 0.f, st)))
+        return rc;
+    if (a.dw) {
+        if (M == 0) return dssvae_zero2d((float*)a.dw, a.lddw, a.N, a.K, st);
+        return dssvae_gemm_f32(dz, lddz, 1, nullptr, (const float*)a.x, a.ldx, 1, (float*)a.dw, a.lddw, nullptr, a.N, a.K, M, 1.f, 0.f, st);
+    }
+    return rc;
+}
+
+int bwd_any(int dtype, const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
+    if (dtype == DSSVAE_F32) return bwd32(a, sp, st, dry);
+    return dtype == DSSVAE_BF16 ? bwd16<bf16_t>(a, sp, st, dry) : bwd16<f16_t>(a, sp, st, dry);
+}
+
+}  // namespace
+
+extern "C" int64_t dssvae_linear_act_fwd_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype,
+                                                         int64_t M, int N, int K) {
+    if (bad_args(dtype, DSSVAE_ACT_NONE, M, N, K)) return DSSVAE_EINVAL;
+    if (dtype == DSSVAE_F32) return 0;
+    Space sp{nullptr, 0, 0};
+    fwd16<bf16_t>(x, ldx, w, ldw, M, N, K, Epilogue{}, sp, nullptr, true);
+    return sp.used;
+}
+
+extern "C" int dssvae_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_f32,
+                                     const void* res, int64_t ldr, int dtype, int act, int64_t M, int N, int K, void* y,
+                                     int64_t ldy, void* z, int64_t ldz, void* workspace, int64_t workspace_bytes,
+                                     void* stream) {
+    if (bad_args(dtype, act, M, N, K) || ldx < K || ldw < K || ldy < N || (res && ldr < N) || (z && ldz < N)) return DSSVAE_EINVAL;
+    if (M == 0) return DSSVAE_OK;
+    if (!x || !w || !y || (z && z == y)) return DSSVAE_EINVAL;
+    const int64_t need = dssvae_linear_act_fwd_workspace_bytes(x, ldx, w, ldw, dtype, M, N, K);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))) return DSSVAE_EINVAL;
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == DSSVAE_F32) {
+        const bool plain = act == DSSVAE_ACT_NONE && !res;
+        float* zz = z ? (float*)z : (float*)y;
+        const int64_t ldzz = z ? ldz : ldy;
+        const int rc = dssvae_gemm_f32((const float*)x, ldx, 0, nullptr, (const float*)w, ldw, 0, zz, ldzz, (const float*)bias, (int)M, N,
+                                       K, 1.f, 0.f, stream);
+        if (rc || (plain && !z)) return rc;
+        const int64_t most = 16 * (int64_t)device_cus();
+        hipLaunchKernelGGL(linear_epilogue_f32_kernel, dim3((unsigned)(M < most ? M : most)), dim3(256), 0, st, zz, ldzz,
+                           (const float*)res, ldr, act, M, N, (float*)y, ldy);
+        DSSVAE_CHECK_LAUNCH();
+        return DSSVAE_OK;
+    }
+    Epilogue e{};
+    e.bias = bias; e.bias_f32 = bias_f32; e.res = res; e.ldr = ldr; e.z = z; e.ldz = ldz; e.y = y; e.ldy = ldy; e.act = act;
+    Space sp{(char*)workspace, 0, workspace_bytes};
+    if (dtype == DSSVAE_BF16) return fwd16<bf16_t>(x, ldx, w, ldw, M, N, K, e, sp, st, false);
+    return fwd16<f16_t>(x, ldx, w, ldw, M, N, K, e, sp, st, false);
+}
+
+extern "C" int64_t dssvae_linear_act_bwd_workspace_bytes(const void* dy, int64_t lddy, int has_z, int dtype, int64_t M, int N, int K,
+                                                         int want_dx, int want_dw, int want_db) {
+    if (bad_args(dtype, DSSVAE_ACT_NONE, M, N, K)) return DSSVAE_EINVAL;
+    static char some;
+    BwdArgs a{};
+    a.dy = dy; a.lddy = lddy; a.z = has_z ? &some : nullptr; a.M = M; a.N = N; a.K = K;
+    a.dx = want_dx ? &some : nullptr; a.dw = want_dw ? &some : nullptr; a.db = want_db ? &some : nullptr;
+    Space sp{nullptr, 0, 0};
+    bwd_any(dtype, a, sp, nullptr, true);
+    return sp.used;
+}
+
+extern "C" int dssvae_linear_act_bwd(const void* dy, int64_t lddy, const void* z, int64_t ldz, const void* x, int64_t ldx,
+                                     const void* w, int64_t ldw, int dtype, int act, int64_t M, int N, int K, void* dx,
+                                     int64_t lddx, void* dw, int64_t lddw, void* db, int db_f32, void* workspace,
+                                     int64_t workspace_bytes, void* stream) {
+    if (bad_args(dtype, act, M, N, K) || lddy < N || (z && ldz < N) || (dw && (ldx < K || lddw < K)) || (dx && (ldw < K || lddx < K)))
+        return DSSVAE_EINVAL;
+    if (act != DSSVAE_ACT_NONE && !z && M > 0) return DSSVAE_EINVAL;
+    if ((M > 0 && (!dy || (dw && !x))) || (dx && !w)) return DSSVAE_EINVAL;
+    BwdArgs a{};
+    a.dy = dy; a.lddy = lddy; a.z = act == DSSVAE_ACT_NONE ? nullptr : z; a.ldz = ldz; a.x = x; a.ldx = ldx; a.w = w; a.ldw = ldw;
+    a.dx = M > 0 ? dx : nullptr; a.lddx = lddx; a.dw = dw; a.lddw = lddw; a.db = db; a.db_f32 = db_f32 || dtype == DSSVAE_F32;
+    a.act = act; a.M = M; a.N = N; a.K = K;
+    Space need{nullptr, 0, 0};
+    bwd_any(dtype, a, need, nullptr, true);
+    if (need.used > 0 && (!workspace || workspace_bytes < need.used || !aligned_to(workspace, 16))) return DSSVAE_EINVAL;
+    Space sp{(char*)workspace, 0, workspace_bytes};
+    return bwd_any(dtype, a, sp, (hipStream_t)stream, false);
+}

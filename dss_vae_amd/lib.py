@@ -39,6 +39,7 @@ class GruBwdInst(C.Structure):
 
 CELL_GRU, CELL_LSTM = 0, 1
 DISTILL_MAX_TOP = 1024
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "tanh": 4}  # DSSVAE_ACT_*
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # DSSVAE_F32 / _BF16 / _F16
 
 
@@ -152,6 +153,10 @@ _SIGNATURES = {
     "dssvae_gated_step": ([_P, _L, _I, _P, _I, _I, _I, _P, _L, _P, _P], _I),
     "dssvae_distill": ([_P, _L, _I, _L, _I, _P, _P, _I, _F, _P, _F, _P, _L, _P, _P, _P], _I),
     "dssvae_scale_rows": ([_P, _L, _I, _L, _I, _P, _P], _I),
+    "dssvae_linear_act_fwd_workspace_bytes": ([_P, _L, _P, _L, _I, _L, _I, _I], _L),
+    "dssvae_linear_act_fwd": ([_P, _L, _P, _L, _P, _I, _P, _L, _I, _I, _L, _I, _I, _P, _L, _P, _L, _P, _L, _P], _I),
+    "dssvae_linear_act_bwd_workspace_bytes": ([_P, _L, _I, _I, _L, _I, _I, _I, _I, _I], _L),
+    "dssvae_linear_act_bwd": ([_P, _L, _P, _L, _P, _L, _P, _L, _I, _I, _L, _I, _I, _P, _L, _P, _L, _P, _I, _P, _L, _P], _I),
 }
 EXPORTS = tuple(_SIGNATURES)
 

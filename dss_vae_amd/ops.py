@@ -2140,3 +2140,91 @@ def distill_loss(logits, ids, teacher, temperature=1.0, weight=None):
     z, ldz = _matrix(logits.reshape(-1, logits.size(-1)))
     total, rows, _ = _distill(z, ldz, code, ids2, t2, tau, w2, False)
     return total, rows.view(lead)
+
+
+def _linear_act_fwd(x2, ldx, w, ldw, b, act, r, code, keep_z):
+    """-> y, z (the pre-activation in x's type; None unless `keep_z`)"""
+    M, K = x2.shape
+    N, dev, lib = w.size(0), x2.device, L.load()
+    y = torch.empty(M, N, device=dev, dtype=x2.dtype)
+    z = torch.empty(M, N, device=dev, dtype=x2.dtype) if keep_z else None
+    r, ldr = (None, 0) if r is None else _matrix(r)
+    with _Here(dev), _Span("linear_tile_kernel" if code else "gemm_store_kernel", 2.0 * M * N * K,
+                           (M * K + N * K + M * N) * float(x2.element_size()), detail="M=%d N=%d K=%d" % (M, N, K)):
+        n = lib.dssvae_linear_act_fwd_workspace_bytes(L.ptr(x2), ldx, L.ptr(w), ldw, code, M, N, K)
+        ws = torch.empty(n, device=dev, dtype=torch.uint8) if n > 0 else None
+        L.check(lib.dssvae_linear_act_fwd(L.ptr(x2), ldx, L.ptr(w), ldw, L.ptr(b), int(b is not None and b.dtype == torch.float32),
+                                          L.ptr(r), ldr, code, act, M, N, K, L.ptr(y), N, L.ptr(z), N, L.ptr(ws), max(n, 0),
+                                          L.stream()), "dssvae_linear_act_fwd")
+    return y, z
+
+
+class _LinearActFn(Function):
+    @staticmethod
+    def forward(ctx, x, w, b, residual, act, code):
+        ctx.set_materialize_grads(False)
+        N = w.size(0)
+        x2, ldx = _matrix(x.reshape(-1, x.size(-1)))
+        wc, ldw = _matrix(w)
+        bc = None if b is None else b.contiguous()
+        keep = act != 0 and any(ctx.needs_input_grad[:3])
+        y, z = _linear_act_fwd(x2, ldx, wc, ldw, bc, act, None if residual is None else residual.reshape(-1, N), code, keep)
+        ctx.save_for_backward(x2, w, z)
+        ctx.bias_ref, ctx.act, ctx.code, ctx.xshape = b, act, code, x.shape
+        return y.view(*x.shape[:-1], N)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        if dy is None:
+            return (None,) * 6
+        x2, w, z = ctx.saved_tensors
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if need_x or need_w or need_b:
+            M, K = x2.shape
+            N, dev, lib = w.size(0), x2.device, L.load()
+            x2, ldx = _matrix(x2)
+            wc, ldw = _matrix(w)
+            dy2, lddy = _matrix(dy.reshape(-1, N))
+            b = ctx.bias_ref
+            dx = torch.empty(M, K, device=dev, dtype=x2.dtype) if need_x else None
+            dw, db = (None if not need else _claim(t) for need, t in ((need_w, w), (need_b, b)))
+            dw = torch.empty(N, K, device=dev, dtype=w.dtype) if need_w and dw is None else dw
+            db = torch.empty(N, device=dev, dtype=b.dtype) if need_b and db is None else db
+            with _Here(dev), _Span("linear_act_bwd", 2.0 * M * N * K * (int(need_x) + int(need_w)),
+                                   4.0 * M * N * x2.element_size(), detail="M=%d N=%d K=%d" % (M, N, K)):
+                n = lib.dssvae_linear_act_bwd_workspace_bytes(L.ptr(dy2), lddy, int(z is not None), ctx.code, M, N, K, int(need_x and M > 0),
+                                                              int(need_w), int(need_b))
+                ws = torch.empty(n, device=dev, dtype=torch.uint8) if n > 0 else None
+                L.check(lib.dssvae_linear_act_bwd(L.ptr(dy2), lddy, L.ptr(z), N, L.ptr(x2), ldx, L.ptr(wc), ldw, ctx.code, ctx.act, M,
+                                                  N, K, L.ptr(dx), K, L.ptr(dw), K, L.ptr(db),
+                                                  int(db is not None and db.dtype == torch.float32), L.ptr(ws), max(n, 0),
+                                                  L.stream()), "dssvae_linear_act_bwd")
+            dx = None if dx is None else dx.view(ctx.xshape)
+        return dx, dw, db, dy if need_r else None, None, None
+
+
+def linear_act(x, w, b=None, act="none", residual=None):
+    """act(x w^T + b) + residual: x [..., K], w [N, K] and residual [..., N] of one type (float32, bfloat16, float16),
+    b [N] of that type or float32; act "none", "relu", "gelu" (the exact form), "silu" or "tanh".  Products accumulate in
+    fp32 and every output is rounded once; for training in 16 bits the pre-activation is kept in x's type."""
+    code = _typed("linear_act", x)
+    if act not in L.ACTIVATIONS:
+        raise RuntimeError("linear_act: act must be one of %s, got %r" % (sorted(L.ACTIVATIONS), act))
+    if x.dim() < 1 or w.dim() != 2 or x.size(-1) != w.size(1) or w.size(0) < 1 or w.size(1) < 1:
+        raise RuntimeError("linear_act: x [..., K] and w [N, K] do not fit: %s, %s" % (list(x.shape), list(w.shape)))
+    N, K = w.shape
+    _expect("linear_act", "w", w, (N, K), (x.dtype,), x.device)
+    if b is not None:
+        _expect("linear_act", "b", b, (N,), (x.dtype, torch.float32), x.device)
+    if residual is not None:
+        _expect("linear_act", "residual", residual, tuple(x.shape[:-1]) + (N,), (x.dtype,), x.device)
+    a = L.ACTIVATIONS[act]
+    if _wants_grad(x, w, b, residual):
+        return _LinearActFn.apply(x, w, b, residual, a, code)
+    x2, ldx = _matrix(x.reshape(-1, K))
+    w2, ldw = _matrix(w)
+    r = None if residual is None else residual.reshape(-1, N)
+    y, _ = _linear_act_fwd(x2, ldx, w2, ldw, None if b is None else b.contiguous(), a, r, code, False)
+    return y.view(*x.shape[:-1], N)

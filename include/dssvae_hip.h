@@ -612,6 +612,33 @@ int dssvae_distill(const void* logits, int64_t ldz, int dtype, int64_t N, int V,
                    float* total, void* stream);
 int dssvae_scale_rows(void* x, int64_t ld, int dtype, int64_t rows, int V, const float* factor, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Linear layer with bias, activation and residual:  z = x w^T + bias,  y = act(z) + res
+ *   x [M, K], w [N, K], res / y / z [M, N] of `dtype` with their row strides; bias [N] fp32 if bias_f32 else `dtype`, or
+ *   NULL; res NULL: none; z NULL: the pre-activation is not kept (backward needs it unless act is DSSVAE_ACT_NONE).
+ *   y must not overlap x, w or z; it may be res.  DSSVAE_ACT_GELU is the exact form, z Phi(z).
+ * Backward: dz = dy act'(z); dx = dz w; dw = dz^T x; db = sum over rows of dz; dx, dw, db may each be NULL, z only where act
+ * is DSSVAE_ACT_NONE.  (The residual's gradient is dy.)  M = 0 clears dw and db.
+ * 16-bit types: fp32 accumulation, dz and z rounded to the type (the slopes and the products of backward start from those
+ * roundings); sums in a fixed order.  fp32: dssvae_gemm_f32's order.
+ * The workspace sizes depend on where the operands start: the query takes the pointers and strides of the call.
+ * ------------------------------------------------------------------------------------------- */
+#define DSSVAE_ACT_NONE 0
+#define DSSVAE_ACT_RELU 1
+#define DSSVAE_ACT_GELU 2
+#define DSSVAE_ACT_SILU 3
+#define DSSVAE_ACT_TANH 4
+int64_t dssvae_linear_act_fwd_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int64_t M,
+                                              int N, int K);
+int dssvae_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_f32,
+                          const void* res, int64_t ldr, int dtype, int act, int64_t M, int N, int K, void* y, int64_t ldy,
+                          void* z, int64_t ldz, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t dssvae_linear_act_bwd_workspace_bytes(const void* dy, int64_t lddy, int has_z, int dtype, int64_t M, int N, int K,
+                                              int want_dx, int want_dw, int want_db);
+int dssvae_linear_act_bwd(const void* dy, int64_t lddy, const void* z, int64_t ldz, const void* x, int64_t ldx, const void* w,
+                          int64_t ldw, int dtype, int act, int64_t M, int N, int K, void* dx, int64_t lddx, void* dw,
+                          int64_t lddw, void* db, int db_f32, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,245 @@
+"""ops.linear_act against its definition in 64 bits: every activation and type, sizes at and around the tile, granule and split
+borders, rows at every alignment, missing and frozen inputs, graph replay, run-to-run equality."""
+import math
+
+import pytest
+import torch
+
+from blocks_util import DEV, TYPES, U32, bits, check, half_step, rnd
+
+pytestmark = pytest.mark.gpu
+ACTS = ["none", "relu", "gelu", "silu", "tanh"]
+
+
+def act(z, name):
+    """-> act(z), act'(z) in 64 bits"""
+    if name == "relu":
+        return z.clamp(min=0), (z > 0).double()
+    if name == "gelu":
+        c = 0.5 * torch.erfc(-z / math.sqrt(2))
+        return z * c, c + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    if name == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s * (1 + z * (1 - s))
+    if name == "tanh":
+        return torch.tanh(z), 1 - torch.tanh(z) ** 2
+    return z, torch.ones_like(z)
+
+
+def reference(x, w, b, res, name, dy):
+    """-> dict of outputs and dict of error scales in units of 2^-24, in 64 bits.
+
+    z: a sum of K products and the bias in fp32: at most K + 1 roundings of partial sums; random signs and blocked order keep
+    it far below, 3 sqrt(K) + 8 units of sum |x||w| hold for every order of these random inputs.  The activations are Lipschitz
+    with a constant below 1.13 and add at most 8 units of max(1, |z|) of their own (exp2 / rcp / erf).
+    16-bit types: backward sees z rounded to the type (the slope moves by at most u max|act''| |z|, max|act''| <= 0.8 (gelu, at
+    0), and across 0 for relu not at all: the sign is kept) and dz rounded to the type: each dz is off by u (1 + 0.8 |z|) |dy|."""
+    u = 0.0 if x.dtype == torch.float32 else half_step(x.dtype)
+    x, w, dy = x.double(), w.double(), dy.double()
+    K, M, N = x.size(1), x.size(0), w.size(0)
+    z, mag = x @ w.t(), x.abs() @ w.abs().t()
+    if b is not None:
+        z, mag = z + b.double(), mag + b.double().abs()
+    zerr = (3 * math.sqrt(K) + 8) * mag
+    y, slope = act(z, name)
+    yerr = 1.2 * zerr + 8 * z.abs().clamp(min=1)
+    if res is not None:
+        y, yerr = y + res.double(), yerr + 2 * res.double().abs()
+    out, err = {"y": y}, {"y": yerr}
+    dz = dy * slope
+    # what the type's roundings and the fp32 error of z do to dz (relu: z close to 0 may fall on either side)
+    zoff = U32 * zerr + u * z.abs()
+    flip = ((z.abs() <= U32 * zerr) & (z != 0)).double() * dy.abs() if name == "relu" else 0.0
+    curve = 0.0 if name in ("none", "relu") else 0.8
+    dzerr = (flip + dy.abs() * (curve * zoff + 16 * U32) + u * dz.abs()) / U32
+    out["dx"], err["dx"] = dz @ w, dzerr @ w.abs() + (3 * math.sqrt(N) + 8) * (dz.abs() @ w.abs())
+    out["dw"], err["dw"] = dz.t() @ x, dzerr.t() @ x.abs() + (3 * math.sqrt(M) + 8) * (dz.abs().t() @ x.abs())
+    out["db"], err["db"] = dz.sum(0), dzerr.sum(0) + (3 * math.sqrt(M) + 8) * dz.abs().sum(0)
+    return out, err
+
+
+def case(M, N, K, dtype, seed=0, bias32=False):
+    return (rnd(M, K, seed=seed, dtype=dtype), rnd(N, K, seed=seed + 1, scale=K ** -0.5, dtype=dtype),
+            rnd(N, seed=seed + 2, scale=0.3, dtype=torch.float32 if bias32 else dtype), rnd(M, N, seed=seed + 3, dtype=dtype),
+            rnd(M, N, seed=seed + 4, dtype=dtype))
+
+
+def run(x, w, b, res, name, dy):
+    from dss_vae_amd import ops
+    leaves = {k: None if t is None else t.detach().to(DEV, copy=True).requires_grad_() for k, t in (("dx", x), ("dw", w), ("db", b), ("dr", res))}
+    y = ops.linear_act(leaves["dx"], leaves["dw"], leaves["db"], name, leaves["dr"])
+    y.backward(dy.to(DEV))
+    return {"y": y, **{k: t.grad for k, t in leaves.items() if t is not None}}
+
+
+def compare(x, w, b, res, name, dy, got):
+    want, err = reference(x, w, b, res, name, dy)
+    for k in want:
+        if k in got:
+            check(got[k], want[k], err[k], 1.0, (k, name, tuple(x.shape), w.size(0), x.dtype))
+    if "dr" in got:
+        assert torch.equal(got["dr"].cpu(), dy)
+
+
+SIZES = [(1, 1, 1), (2, 3, 5), (7, 9, 8), (16, 33, 64), (50, 40, 72), (33, 130, 130), (128, 128, 64), (129, 127, 65), (1, 300, 600),
+         (300, 8, 1000), (64, 257, 512), (257, 513, 200), (700, 300, 300), (5, 2048, 1024), (1030, 264, 56), (90, 72, 4104)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_sizes(dtype, M, N, K):
+    name = ACTS[(M + N + K) % 5]
+    x, w, b, res, dy = case(M, N, K, dtype, seed=M + N + K)
+    compare(x, w, b, res, name, dy, run(x, w, b, res, name, dy))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", ACTS)
+def test_activations(dtype, name):
+    x, w, b, res, dy = case(96, 200, 136, dtype, seed=3, bias32=True)
+    x *= 3  # z over the activations' whole range
+    compare(x, w, b, res, name, dy, run(x, w, b, res, name, dy))
+    compare(x, w, None, None, name, dy, run(x, w, None, None, name, dy))
+
+
+def test_large_tiles_and_splits():
+    """shapes of the 256-wide tiles (whole, ragged) and of the K splits"""
+    for M, N, K, dtype in ((4096, 4096, 128, torch.bfloat16), (4000, 4100, 72, torch.float16), (256, 256, 16384, torch.bfloat16),
+                           (130, 136, 9000, torch.float16)):
+        x, w, b, res, dy = case(M, N, K, dtype, seed=M)
+        got = run(x, w, b, res, "silu", dy)
+        compare(x, w, b, res, "silu", dy, got)
+        again = run(x, w, b, res, "silu", dy)
+        for k in got:
+            assert torch.equal(bits(got[k].detach()), bits(again[k].detach())), k
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_and_alignment(dtype):
+    from dss_vae_amd import ops
+    M, N, K = 70, 88, 96
+    x, w, b, res, dy = case(M, N, K, dtype, seed=4)
+    for off, pad in ((0, 0), (1, 0), (3, 5), (8, 8), (4, 4)):
+        xs, ws, rs = (torch.full((r, off + c + pad), float("nan"), dtype=dtype) for r, c in ((M, K), (N, K), (M, N)))
+        xs[:, off:off + K], ws[:, off:off + K], rs[:, off:off + N] = x, w, res
+        xl, wl, rl = (t.to(DEV).requires_grad_() for t in (xs, ws, rs))
+        bl = b.to(DEV).requires_grad_()
+        y = ops.linear_act(xl[:, off:off + K], wl[:, off:off + K], bl, "gelu", rl[:, off:off + N])
+        gx, gw, gb = torch.autograd.grad(y, (xl, wl, bl), dy.to(DEV))
+        assert (gx[:, :off] == 0).all() and (gw[:, off + K:] == 0).all()
+        compare(x, w, b, res, "gelu", dy, {"y": y, "dx": gx[:, off:off + K], "dw": gw[:, off:off + K], "db": gb})
+    y = ops.linear_act(x.t().contiguous().to(DEV).t(), w.t().contiguous().to(DEV).t(), b.to(DEV))
+    compare(x, w, b, None, "none", dy, {"y": y})
+    y = ops.linear_act(x[:1].to(DEV).expand(M, K), w.to(DEV), b.to(DEV), "none", res[:1].to(DEV).expand(M, N))
+    compare(x[:1].expand(M, K), w, b, res[:1].expand(M, N), "none", dy, {"y": y})
+    x3 = x.to(DEV).view(7, 10, K).requires_grad_()
+    y = ops.linear_act(x3, w.to(DEV), b.to(DEV), "tanh", res.to(DEV).view(7, 10, N))
+    assert y.shape == (7, 10, N)
+    y.sum().backward()  # an expanded scalar as the upstream gradient
+    compare(x, w, b, res, "tanh", torch.ones(M, N, dtype=dtype), {"y": y.reshape(M, N), "dx": x3.grad.reshape(M, K)})
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_frozen_inputs_and_no_rows(dtype):
+    from dss_vae_amd import ops
+    x, w, b, res, dy = (t.to(DEV) for t in case(40, 24, 32, dtype, seed=5))
+    full = run(x, w, b, res, "gelu", dy)
+    for which in range(4):
+        leaves = [t.clone().requires_grad_(i == which) for i, t in enumerate((x, w, b, res))]
+        y = ops.linear_act(leaves[0], leaves[1], leaves[2], "gelu", leaves[3])
+        g, = torch.autograd.grad(y, leaves[which], dy)
+        assert torch.equal(bits(y.detach()), bits(full["y"].detach()))
+        key = ("dx", "dw", "db", "dr")[which]
+        if dtype != torch.float32 or key in ("db", "dr"):
+            assert torch.equal(bits(g), bits(full[key]))
+    wl, bl = w.clone().requires_grad_(), b.clone().requires_grad_()
+    y = ops.linear_act(x[:0], wl, bl, "gelu", res[:0])
+    assert y.shape == (0, 24)
+    y.sum().backward()
+    assert (wl.grad == 0).all() and (bl.grad == 0).all() and wl.grad.shape == w.shape
+    with torch.no_grad():
+        assert torch.equal(bits(ops.linear_act(x, wl, bl, "gelu", res)), bits(full["y"].detach()))
+
+
+def test_values_that_are_not_finite_stay_in_their_rows():
+    from dss_vae_amd import ops
+    for dtype in TYPES:
+        x, w, b, _, _ = (t.to(DEV) for t in case(200, 140, 100, dtype, seed=6))
+        clean = ops.linear_act(x, w, b, "relu")
+        x[17], x[130, 3] = float("nan"), float("inf")
+        got = ops.linear_act(x, w, b, "relu")
+        keep = [i for i in range(200) if i not in (17, 130)]
+        assert torch.equal(got[keep], clean[keep]) and got[17].isnan().all()
+
+
+def test_huge_pre_activations_have_finite_slopes():
+    """fp16: z beyond the type's range in fp32: y is infinite, its slope 0 or 1, no NaN"""
+    from dss_vae_amd import ops
+    x = torch.full((4, 64), 200.0, dtype=torch.float16, device=DEV, requires_grad=True)
+    w = torch.full((8, 64), 100.0, dtype=torch.float16, device=DEV)
+    w[4:] = -100.0
+    for name in ("silu", "gelu", "tanh", "relu"):
+        y = ops.linear_act(x, w, None, name)
+        g, = torch.autograd.grad(y, x, torch.full_like(y, 2.0 ** -10))
+        assert not g.isnan().any(), name
+
+
+def test_gradient_against_differences():
+    x, w, b, res, dy = case(3, 4, 5, torch.float32, seed=7)
+    for name in ("gelu", "silu", "tanh"):
+        got = run(x, w, b, res, name, dy)
+
+        def f(xx, ww, bb):
+            return float((act(xx.double() @ ww.double().t() + bb.double(), name)[0] * dy.double()).sum())
+
+        h = 1e-6
+        for k, t in (("dx", x), ("dw", w), ("db", b)):
+            for i in range(t.numel()):
+                up, down = t.double().clone(), t.double().clone()
+                up.view(-1)[i] += h
+                down.view(-1)[i] -= h
+                a = [up if t is s else s.double() for s in (x, w, b)]
+                c = [down if t is s else s.double() for s in (x, w, b)]
+                assert abs((f(*a) - f(*c)) / (2 * h) - float(got[k].view(-1)[i])) < 1e-4
+
+
+def test_replayed_graph():
+    from dss_vae_amd import ops
+    x, w, b, res, dy = (t.to(DEV) for t in case(500, 120, 1000, torch.bfloat16, seed=8))
+    xs, ws, bs = (t.clone().requires_grad_() for t in (x, w, b))
+
+    def step(a, c, d):
+        y = ops.linear_act(a, c, d, "gelu", res)
+        return (y,) + torch.autograd.grad(y, (a, c, d), dy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(xs, ws, bs)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(xs, ws, bs)
+    for n in range(3):
+        xs.data.copy_(x * (1 + n))
+        want = step(*(t.detach().clone().requires_grad_() for t in (xs, ws, bs)))
+        for o in out:
+            o.detach().fill_(3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(out, want):
+            assert torch.equal(bits(a.detach()), bits(c.detach())), n
+
+
+def test_refusals():
+    from dss_vae_amd import ops
+    x, w, b = torch.zeros(4, 8, device=DEV), torch.zeros(3, 8, device=DEV), torch.zeros(3, device=DEV)
+    for bad in (lambda: ops.linear_act(x.cpu(), w), lambda: ops.linear_act(x.double(), w.double()),
+                lambda: ops.linear_act(x, w.half()), lambda: ops.linear_act(x, w[:, :7]), lambda: ops.linear_act(x, w[0]),
+                lambda: ops.linear_act(x, w[:0]), lambda: ops.linear_act(x[:, :0], w[:, :0]), lambda: ops.linear_act(x, w, b[:2]),
+                lambda: ops.linear_act(x, w, b.half()), lambda: ops.linear_act(x.half(), w.half(), b.bfloat16()),
+                lambda: ops.linear_act(x, w, b, "elu"), lambda: ops.linear_act(x, w, b, "none", torch.zeros(4, 1, device=DEV)),
+                lambda: ops.linear_act(x, w, b, "none", torch.zeros(4, 3, device=DEV).half()),
+                lambda: ops.linear_act(x, w.cpu(), b)):
+        with pytest.raises(RuntimeError):
+            bad()
