@@ -29,10 +29,19 @@ __device__ __forceinline__ float sigmoid_f(float x) {
 __device__ __forceinline__ float tanh_f(float x) {
     return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.8853900817779268f * x));
 }
+// Phi(z) of the normal distribution, given e = exp(-z^2 / 2): the five-term rational form of Abramowitz & Stegun 7.1.26
+// (|error of erf| <= 1.5e-7).  The epilogue is bound by the vector ALUs: this is 20 lane cycles where erff is about 45.
+__device__ __forceinline__ float normal_cdf(float z, float e) {
+    const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678118654752f * fabsf(z));
+    const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    const float q = 0.5f * p * e;
+    return z < 0.f ? q : 1.f - q;
+}
+__device__ __forceinline__ float normal_exp(float z) { return __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z); }
 __device__ __forceinline__ float act_f(int act, float z) {
     switch (act) {
         case DSSVAE_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
-        case DSSVAE_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+        case DSSVAE_ACT_GELU: return z * normal_cdf(z, normal_exp(z));
         case DSSVAE_ACT_SILU: return z * sigmoid_f(z);
         case DSSVAE_ACT_TANH: return tanh_f(z);
         default: return z;
@@ -41,9 +50,10 @@ __device__ __forceinline__ float act_f(int act, float z) {
 __device__ __forceinline__ float act_slope(int act, float z) {
     switch (act) {
         case DSSVAE_ACT_RELU: return z > 0.f ? 1.f : (z != z ? z : 0.f);
-        case DSSVAE_ACT_GELU:
-            return 0.5f * (1.f + erff(z * 0.70710678118654752f)) +
-                   z * 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
+        case DSSVAE_ACT_GELU: {
+            const float e = normal_exp(z);
+            return normal_cdf(z, e) + z * 0.3989422804014327f * e;
+        }
         case DSSVAE_ACT_SILU: {
             const float s = sigmoid_f(z);
             return s * (1.f + z * (1.f - s));
@@ -76,9 +86,17 @@ __device__ __forceinline__ float bias_at(const Epilogue& e, int64_t n) {
     return e.bias_f32 ? reinterpret_cast<const float*>(e.bias)[n] : (float)reinterpret_cast<const T*>(e.bias)[n];
 }
 
-// eight consecutive columns n .. of row m (those below N), acc without bias
 template <typename T>
-__device__ __forceinline__ void finish8(const Epilogue& e, f32x8 a, int64_t m, int n, int N) {
+__device__ __forceinline__ f32x8 bias8(const Epilogue& e, int n, int N) {
+    f32x8 b;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) b[j] = n + j < N ? bias_at<T>(e, n + j) : 0.f;
+    return b;
+}
+
+// eight consecutive columns n .. of row m (those below N): a without the bias b
+template <typename T>
+__device__ __forceinline__ void finish8(const Epilogue& e, f32x8 a, f32x8 b, int64_t m, int n, int N) {
     T* y = reinterpret_cast<T*>(e.y) + m * e.ldy + n;
     T* z = e.z ? reinterpret_cast<T*>(e.z) + m * e.ldz + n : nullptr;
     const T* r = e.res ? reinterpret_cast<const T*>(e.res) + m * e.ldr + n : nullptr;
@@ -88,7 +106,7 @@ __device__ __forceinline__ void finish8(const Epilogue& e, f32x8 a, int64_t m, i
         Gran<T, 8> gz, gy;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float zz = a[j] + bias_at<T>(e, n + j);
+            const float zz = a[j] + b[j];
             gz.set(j, keep_z<T>(zz));
             gy.set(j, act_f(e.act, zz) + (r ? g.get(j) : 0.f));
         }
@@ -98,7 +116,7 @@ __device__ __forceinline__ void finish8(const Epilogue& e, f32x8 a, int64_t m, i
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             if (n + j >= N) continue;
-            const float zz = a[j] + bias_at<T>(e, n + j);
+            const float zz = a[j] + b[j];
             if (z) z[j] = (T)keep_z<T>(zz);
             y[j] = (T)(act_f(e.act, zz) + (r ? (float)r[j] : 0.f));
         }
@@ -259,20 +277,25 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, E
     constexpr int HALF = WR * WC / 2;
     float* stage = reinterpret_cast<float*>(wave < HALF ? sa0 : sa1) + (wave % HALF) * 32 * 64;
     static_assert(HALF * 32 * 64 * 4 <= (int)sizeof(sa0), "the waves' staging rows fit the operand buffers");
-#pragma unroll
+    const int col = (lane & 7) * 8, n = n0 + rb + col;  // the lane's columns in every row
+    const f32x8 bias = bias8<T>(e, n, s.N);
+#pragma unroll 1
     for (int i = 0; i < MI; ++i) {
 #pragma unroll
-        for (int j = 0; j < NI; ++j)
+        for (int ii = 0; ii < MI; ++ii) {  // (accumulators are only ever named by constants: else they go to memory)
+            if (ii != i) continue;
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                stage[((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * 64 + j * 32 + (lane & 31)] = acc[i][j][r];
+            for (int j = 0; j < NI; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    stage[((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * 64 + j * 32 + (lane & 31)] = acc[ii][j][r];
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const int row = q * 8 + (lane >> 3), col = (lane & 7) * 8;
+            const int row = q * 8 + (lane >> 3);
             const f32x8 v = *reinterpret_cast<const f32x8*>(stage + row * 64 + col);
             const int64_t m = m0 + ra + i * 32 + row;
-            const int n = n0 + rb + col;
             if (m >= s.M || n >= s.N) continue;
             if (s.ksplit > 1) {
                 float* o = s.part + ((int64_t)split * s.M + m) * s.N + n;
@@ -285,7 +308,7 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, E
                         if (n + j < s.N) o[j] = v[j];
                 }
             } else {
-                finish8<T>(e, v, m, n, s.N);
+                finish8<T>(e, v, bias, m, n, s.N);
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -316,7 +339,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const float* __restric
                 if (n + j < N) v[j] += p[j];
         }
     }
-    finish8<T>(e, v, m, n, N);
+    finish8<T>(e, v, bias8<T>(e, n, N), m, n, N);
 }
 
 // ---- operands into the form the tile kernel takes -----------------------------------------------------------------
@@ -333,54 +356,110 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const T* __restrict__ 
 //   v = src * act'(z)            else
 // out [R, ldo] (NULL: not wanted) gets v, columns C .. ldo zero; outT [C, ldt] (NULL) its transpose, columns R .. ldt zero;
 // sums [gridDim.y][C] (NULL) the block's column sums of the unrounded v.
+// A thread moves granules of 8 elements (16-bit) in rows of 64: `vec` where rows of src, z and out start on granules, else by
+// elements.  The tile's granule (r, chunk) lies at chunk ^ (r / 8): the eight lanes that gather one column's 64 rows then
+// read eight different banks.  outT rows always start on granules (ldt % 8 == 0).
 template <typename T>
 __global__ __launch_bounds__(256) void linear_turn_kernel(const T* __restrict__ src, int64_t ld, const T* __restrict__ z,
                                                           int64_t ldz, int act, int64_t R, int64_t C, T* __restrict__ out,
                                                           int64_t ldo, T* __restrict__ outT, int64_t ldt,
-                                                          float* __restrict__ sums) {
-    __shared__ T tile[64][66];
-    __shared__ float red[4][64];
+                                                          float* __restrict__ sums, int vec) {
+    __shared__ __attribute__((aligned(16))) T tile[64 * 64];
+    __shared__ float red[32][64];
     const int64_t c0 = (int64_t)blockIdx.x * 64;
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    const int64_t rtiles = (R + 63) / 64;
-    float sum = 0.f;
+    const int ch = threadIdx.x & 7, rr = threadIdx.x >> 3;
+    const int64_t rtiles = (R + 63) / 64, c = c0 + ch * 8;
+    float sum[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[j] = 0.f;
     for (int64_t rt = blockIdx.y; rt < rtiles; rt += gridDim.y) {
         const int64_t r0 = rt * 64;
-#pragma unroll 4
-        for (int i = 0; i < 16; ++i) {
-            const int64_t r = r0 + i * 4 + ty, c = c0 + tx;
-            float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int tr = i * 32 + rr;
+            const int64_t r = r0 + tr;
+            float v[8];
+            Gran<T, 8> g;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = 0.f;
             if (r < R && c < C) {
-                v = (float)src[r * ld + c];
-                if (z) v *= act_slope(act, (float)z[r * ldz + c]);
+                if (vec && c + 8 <= C) {
+                    g.load(src + r * ld + c);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = g.get(j);
+                    if (z) {
+                        g.load(z + r * ldz + c);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] *= act_slope(act, g.get(j));
+                    }
+                } else {
+                    for (int j = 0; j < 8 && c + j < C; ++j) {
+                        float u = (float)src[r * ld + c + j];
+                        if (z) u *= act_slope(act, (float)z[r * ldz + c + j]);
+#pragma unroll
+                        for (int jj = 0; jj < 8; ++jj) v[jj] = jj == j ? u : v[jj];
+                    }
+                }
             }
-            sum += v;
-            if (out && r < R && c < ldo) out[r * ldo + c] = (T)v;
-            if (outT) tile[i * 4 + ty][tx] = (T)v;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                sum[j] += v[j];
+                g.set(j, v[j]);
+            }
+            if (out && r < R) {
+                if (vec && c + 8 <= ldo) {
+                    g.store(out + r * ldo + c);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (c + j < ldo) out[r * ldo + c + j] = (T)v[j];
+                }
+            }
+            if (outT) g.store(tile + tr * 64 + (ch ^ (tr >> 3)) * 8);
         }
         if (outT) {
             __syncthreads();
-#pragma unroll 4
-            for (int i = 0; i < 16; ++i) {
-                const int64_t c = c0 + i * 4 + ty, r = r0 + tx;
-                if (c < C && r < ldt) outT[c * ldt + r] = tile[tx][i * 4 + ty];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                // lane ch gathers rows 8 ch .. of column i * 32 + rr
+                const int tc = i * 32 + rr;
+                Gran<T, 8> g;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const T t = tile[(ch * 8 + j) * 64 + ((tc >> 3) ^ ch) * 8 + (tc & 7)];
+                    if constexpr (sizeof(T) == 2) g.v[j] = t;
+                }
+                const int64_t r = r0 + ch * 8;
+                if (c0 + tc < C && r < ldt) g.store(outT + (c0 + tc) * ldt + r);
             }
             __syncthreads();
         }
     }
     if (!sums) return;
-    red[ty][tx] = sum;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) red[rr][ch * 8 + j] = sum[j];
     __syncthreads();
-    if (ty == 0 && c0 + tx < C) sums[(int64_t)blockIdx.y * C + c0 + tx] = red[0][tx] + red[1][tx] + red[2][tx] + red[3][tx];
+    if (threadIdx.x < 64 && c0 + threadIdx.x < C) {
+        float s = 0.f;
+        for (int i = 0; i < 32; ++i) s += red[i][threadIdx.x];
+        sums[(int64_t)blockIdx.y * C + c0 + threadIdx.x] = s;
+    }
 }
 
-// db [C] = sum of n rows of partial sums, in order
+// db [C] = sum of n rows of partial sums in a fixed order: 32 columns per block, 32 threads share a column
 template <typename T>
-__global__ __launch_bounds__(256) void linear_db_kernel(const float* __restrict__ sums, int n, int64_t C, void* db, int f32) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= C) return;
+__global__ __launch_bounds__(1024) void linear_db_kernel(const float* __restrict__ sums, int n, int64_t C, void* db, int f32) {
+    __shared__ float red[32][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + tx;
     float s = 0.f;
-    for (int i = 0; i < n; ++i) s += sums[(int64_t)i * C + c];
+    if (c < C)
+        for (int i = ty; i < n; i += 32) s += sums[(int64_t)i * C + c];
+    red[ty][tx] = s;
+    __syncthreads();
+    if (ty != 0 || c >= C) return;
+#pragma unroll
+    for (int i = 1; i < 32; ++i) s += red[i][tx];
     if (f32) reinterpret_cast<float*>(db)[c] = s;
     else reinterpret_cast<T*>(db)[c] = (T)s;
 }
@@ -480,8 +559,11 @@ template <typename T>
 int turn(const void* src, int64_t ld, const void* z, int64_t ldz, int act, int64_t R, int64_t C, void* out, int64_t ldo, void* outT,
          int64_t ldt, float* sums, hipStream_t st) {
     const dim3 grid((unsigned)((C + 63) / 64), (unsigned)turn_rows(R, C));
+    const int per = 8, align = per * (int)sizeof(T);  // (a fp32 granule of 8 is two 16-byte moves)
+    const int vec = aligned_to(src, align) && ld % per == 0 && (!z || (aligned_to(z, align) && ldz % per == 0)) &&
+                    (!out || (aligned_to(out, align) && ldo % per == 0));
     hipLaunchKernelGGL((linear_turn_kernel<T>), grid, dim3(256), 0, st, (const T*)src, ld, (const T*)z, ldz, act, R, C, (T*)out, ldo,
-                       (T*)outT, ldt, sums);
+                       (T*)outT, ldt, sums, vec);
     DSSVAE_CHECK_LAUNCH();
     return DSSVAE_OK;
 }
@@ -543,7 +625,7 @@ int bwd16(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
         if (!dry) {
             if ((rc = turn<T>(a.dy, a.lddy, a.z, a.ldz, a.act, M, N, dzc, ldn, dzt, ldm, sums, st))) return rc;
             if (a.db) {
-                hipLaunchKernelGGL((linear_db_kernel<T>), dim3((unsigned)((N + 255) / 256)), dim3(256), 0, st, sums,
+                hipLaunchKernelGGL((linear_db_kernel<T>), dim3((unsigned)((N + 31) / 32)), dim3(1024), 0, st, sums,
                                    (int)turn_rows(M, N), N, a.db, a.db_f32);
                 DSSVAE_CHECK_LAUNCH();
             }
@@ -586,7 +668,7 @@ int bwd32(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
     if (dzc || sums) {
         if ((rc = turn<float>(a.dy, a.lddy, a.z, a.ldz, a.act, a.M, a.N, dzc, a.N, nullptr, 0, sums, st))) return rc;
         if (a.db) {
-            hipLaunchKernelGGL((linear_db_kernel<float>), dim3((unsigned)((a.N + 255) / 256)), dim3(256), 0, st, sums,
+            hipLaunchKernelGGL((linear_db_kernel<float>), dim3((unsigned)((a.N + 31) / 32)), dim3(1024), 0, st, sums,
                                (int)turn_rows(a.M, a.N), a.N, a.db, 1);
             DSSVAE_CHECK_LAUNCH();
         }
