@@ -140,31 +140,39 @@ template <> struct Mfma<f16_t> {
 };
 
 // One operand's share of a tile load: R rows x 64 k, TH threads, 16 bytes a lane.  A thread's granules all lie in the same
-// place of their rows (rows TH / 8 apart, a multiple of 8: the swizzle is the same), so only the row pointer differs.
+// place of their rows (rows TH / 8 apart, a multiple of 8: the swizzle is the same).  Rows behind the last are loaded from
+// it and never stored.  `base` is uniform: row r0 of the operand at the tile's first k.
 template <typename T, int R, int TH>
 struct Loader {
     static constexpr int NR = R * 8 / TH;
-    const T* p[NR];
-    int k;  // k of this thread's granule inside a tile
-    __device__ __forceinline__ void init(const T* base, int64_t ld, int64_t r0, int64_t rows) {
+    unsigned off[NR];  // bytes behind base
+    __device__ __forceinline__ static int k_of() {
         const int row = threadIdx.x >> 3;
-        k = (int)((threadIdx.x & 7) ^ (row & 7)) * 8;
+        return (int)((threadIdx.x & 7) ^ (row & 7)) * 8;
+    }
+    __device__ __forceinline__ void init(int64_t ld, int64_t rows_left) {
+        const int row = threadIdx.x >> 3;
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
-            int64_t r = r0 + row + i * (TH / 8);
-            r = r < rows ? r : rows - 1;  // rows behind the last are computed from it and never stored
-            p[i] = base + r * ld + k;
+            int64_t r = row + i * (TH / 8);
+            r = r < rows_left ? r : rows_left - 1;
+            off[i] = (unsigned)((r * ld + k_of()) * (int64_t)sizeof(T));
         }
     }
-    // k0: first k of the tile; granules at or behind K come from a granule of zeros
-    __device__ __forceinline__ void load(T* lds, int64_t k0, int64_t K) const {
-        const int wave = threadIdx.x >> 6;
-        const bool in = k0 + k < K;
+    __device__ __forceinline__ void load(T* lds, const T* base) const {
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
-            const T* src = in ? p[i] + k0 : reinterpret_cast<const T*>(&zero_granule);
-            __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(lds + (i * TH + wave * 64) * 8), 16, 0, 0);
-        }
+        for (int i = 0; i < NR; ++i) put(lds, i, reinterpret_cast<const char*>(base) + off[i]);
+    }
+    // a tile that may reach behind K: granules there come from a granule of zeros
+    __device__ __forceinline__ void load_last(T* lds, const T* base, int64_t left) const {
+        const bool in = k_of() < left;
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            put(lds, i, in ? reinterpret_cast<const char*>(base) + off[i] : reinterpret_cast<const char*>(&zero_granule));
+    }
+    static __device__ __forceinline__ void put(T* lds, int i, const char* src) {
+        const int wave = threadIdx.x >> 6;
+        __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(lds + (i * TH + wave * 64) * 8), 16, 0, 0);
     }
 };
 
@@ -172,7 +180,8 @@ struct Loader {
 template <typename T, int MI, int NI>
 struct Frags {
     typename Mfma<T>::V a[2][MI], b[2][NI];
-    __device__ __forceinline__ void read(const T* sa, const T* sb, int ra, int rb, int h) {
+    __device__ __forceinline__ void read(const T* __restrict__ sa, int b_at, int ra, int rb, int h) {
+        const T* sb = sa + b_at;
         const int lane = threadIdx.x & 63, r = lane & 31;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -211,11 +220,53 @@ __device__ __forceinline__ void tile_of(const Shape& s, int t, int& tm, int& tn)
     tn = in / rows;
 }
 
+// Loads the tile at (a, b) into the buffer `lds`: BM rows of A, then BN rows of B.  (One restrict pointer per buffer: the
+// compiler's bookkeeping of loads that write LDS distinguishes few destinations; past those it waits for all of them in
+// front of every LDS read.)
+template <typename T, int BM, int BN, int TH>
+__device__ __forceinline__ void tile_load(T* __restrict__ lds, const Loader<T, BM, TH>& la, const Loader<T, BN, TH>& lb, const T* a,
+                                          const T* b) {
+    la.load(lds, a);
+    lb.load(lds + BM * BK, b);
+}
+
+// Barrier that also waits for this wave's loads into LDS (a workgroup fence alone does not order them).
+__device__ __forceinline__ void tile_barrier() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
+// The k-tile in `cur`, whose first half is in f0: multiplies it, starts the load of the tile after next (at a, b) into its
+// place and leaves the first half of the next tile in f0.  The instruction groups keep the matrix pipe fed: an LDS read (or
+// a load) between two MFMAs, all of them issued half a step before their data is needed.
+template <typename T, int BM, int BN, int TH, int MI, int NI>
+__device__ __forceinline__ void k_step(Frags<T, MI, NI>& f0, Frags<T, MI, NI>& f1, f32x16 (&acc)[MI][NI], const Loader<T, BM, TH>& la,
+                                       const Loader<T, BN, TH>& lb, T* cur, const T* next, int ra, int rb, const T* a, const T* b) {
+    constexpr int READS = 2 * (MI + NI), MULS = 2 * MI * NI, LOADS = Loader<T, BM, TH>::NR + Loader<T, BN, TH>::NR;
+    f1.read(cur, BM * BK, ra, rb, 1);
+    f0.multiply(acc);
+#pragma unroll
+    for (int i = 0; i < MULS; ++i) {
+        if (i < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+    tile_barrier();  // this tile has been read by every wave, the next one has landed
+    tile_load<T, BM, BN, TH>(cur, la, lb, a, b);
+    f0.read(next, BM * BK, ra, rb, 0);
+    f1.multiply(acc);
+#pragma unroll
+    for (int i = 0; i < MULS; ++i) {
+        if (i < LOADS) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+        if (i < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+}
+
 template <typename T, int BM, int BN, int WR, int WC>
 __global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, Epilogue e) {
     constexpr int TH = 64 * WR * WC, MI = BM / WR / 32, NI = BN / WC / 32;
     static_assert(NI == 2, "the epilogue moves 64 columns of a wave at a time");
-    __shared__ __attribute__((aligned(16))) T sa0[BM * BK], sa1[BM * BK], sb0[BN * BK], sb1[BN * BK];
+    __shared__ __attribute__((aligned(16))) T buf0[(BM + BN) * BK], buf1[(BM + BN) * BK];
     const int wid = xcd_remap(blockIdx.x, gridDim.x), tiles = s.tiles_m * s.tiles_n;
     const int split = wid / tiles;
     int tm, tn;
@@ -234,49 +285,43 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, E
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-    Loader<T, BM, TH> la;
-    Loader<T, BN, TH> lb;
-    la.init((const T*)s.A, s.lda, m0, s.M);
-    lb.init((const T*)s.B, s.ldb, n0, s.N);
-    // a tile at or behind kt1 is loaded from zeros (nobody multiplies it)
-    const int64_t kend = min(s.K, kt1 * BK);
     if (kt0 < kt1) {
-        la.load(sa0, kt0 * BK, kend);
-        lb.load(sb0, kt0 * BK, kend);
-        la.load(sa1, (kt0 + 1) * BK, kend);
-        lb.load(sb1, (kt0 + 1) * BK, kend);
-        __syncthreads();
+        Loader<T, BM, TH> la;
+        Loader<T, BN, TH> lb;
+        la.init(s.lda, s.M - m0);
+        lb.init(s.ldb, s.N - n0);
+        const T* A = (const T*)s.A + m0 * s.lda;
+        const T* B = (const T*)s.B + (int64_t)n0 * s.ldb;
+        // The order of the tiles is free: the last one, which alone may reach behind K, goes first, then kt0 .. kt1 - 2, so that
+        // the loop's loads need no test.  A tile behind the end is the one before it again (loaded, never multiplied).
+        const int64_t kl = (kt1 - 1) * BK, n = kt1 - kt0;
+        la.load_last(buf0, A + kl, s.K - kl);
+        lb.load_last(buf0 + BM * BK, B + kl, s.K - kl);
+        const int64_t most = n > 1 ? kt1 - 2 : kt0;
+        if (n > 1) tile_load<T, BM, BN, TH>(buf1, la, lb, A + kt0 * BK, B + kt0 * BK);
+        tile_barrier();
         Frags<T, MI, NI> f0, f1;
-        f0.read(sa0, sb0, ra, rb, 0);
-        for (int64_t kt = kt0;; kt += 2) {
-            f1.read(sa0, sb0, ra, rb, 1);
-            f0.multiply(acc);
-            __syncthreads();  // everyone has read buffer 0, tile kt + 1 has landed in buffer 1
-            if (kt + 2 < kt1) {
-                la.load(sa0, (kt + 2) * BK, kend);
-                lb.load(sb0, (kt + 2) * BK, kend);
+        f0.read(buf0, BM * BK, ra, rb, 0);
+        // step i multiplies the i-th tile in that order and loads the (i + 2)-th: kt0 + i + 1
+        int64_t i = 0;
+        if (n > 1) {
+            for (; i + 1 < n; i += 2) {
+                const int64_t k2 = min(kt0 + i + 1, most) * BK, k3 = min(kt0 + i + 2, most) * BK;
+                k_step<T, BM, BN, TH, MI, NI>(f0, f1, acc, la, lb, buf0, buf1, ra, rb, A + k2, B + k2);
+                k_step<T, BM, BN, TH, MI, NI>(f0, f1, acc, la, lb, buf1, buf0, ra, rb, A + k3, B + k3);
             }
-            f0.read(sa1, sb1, ra, rb, 0);
-            f1.multiply(acc);
-            if (kt + 1 >= kt1) break;
-            f1.read(sa1, sb1, ra, rb, 1);
-            f0.multiply(acc);
-            __syncthreads();
-            if (kt + 3 < kt1) {
-                la.load(sa1, (kt + 3) * BK, kend);
-                lb.load(sb1, (kt + 3) * BK, kend);
-            }
-            f0.read(sa0, sb0, ra, rb, 0);
-            f1.multiply(acc);
-            if (kt + 2 >= kt1) break;
         }
-        __syncthreads();  // operand buffers are free (and no load is in flight)
+        if (i < n) {  // an odd tile is left: nothing behind it
+            f1.read(buf0, BM * BK, ra, rb, 1);
+            f0.multiply(acc);
+            f1.multiply(acc);
+        }
+        tile_barrier();  // operand buffers are free (and no load is in flight)
     }
 
     // 32 rows x 64 columns of this wave at a time through 8 KiB of LDS of its own, read back along rows
-    constexpr int HALF = WR * WC / 2;
-    float* stage = reinterpret_cast<float*>(wave < HALF ? sa0 : sa1) + (wave % HALF) * 32 * 64;
-    static_assert(HALF * 32 * 64 * 4 <= (int)sizeof(sa0), "the waves' staging rows fit the operand buffers");
+    float* stage = reinterpret_cast<float*>(buf0) + wave * 32 * 64;
+    static_assert(WR * WC * 32 * 64 * 4 <= (int)sizeof(buf0), "the waves' staging rows fit an operand buffer");
     const int col = (lane & 7) * 8, n = n0 + rb + col;  // the lane's columns in every row
     const f32x8 bias = bias8<T>(e, n, s.N);
 #pragma unroll 1
@@ -504,8 +549,8 @@ inline int64_t part_bytes(int64_t M, int64_t N, int64_t K) {
     return p.ksplit > 1 ? up((int64_t)p.ksplit * M * N * 4, 256) : 0;
 }
 
-// operand rows usable as they are: 16-byte granules
-inline bool direct(const void* p, int64_t ld, int64_t K) { return aligned_to(p, 16) && ld % 8 == 0 && K % 8 == 0; }
+// operand rows usable as they are: 16-byte granules, and the 256 rows of a tile within 32-bit byte offsets
+inline bool direct(const void* p, int64_t ld, int64_t K) { return aligned_to(p, 16) && ld % 8 == 0 && K % 8 == 0 && ld < (1 << 22); }
 
 inline bool epilogue_vec(const Epilogue& e) {
     return aligned_to(e.y, 16) && e.ldy % 8 == 0 && (!e.z || (aligned_to(e.z, 16) && e.ldz % 8 == 0)) &&
