@@ -32,6 +32,15 @@ struct Gran {
     }
 };
 
+// The same without alignment beyond the element's: still one 16-byte instruction (global memory takes any address), a little
+// dearer where it crosses a cache line
+template <typename T, int VEC>
+struct GranU : Gran<T, VEC> {
+    typedef typename Gran<T, VEC>::V U __attribute__((aligned(sizeof(T))));
+    __device__ __forceinline__ void load(const T* p) { this->v = *reinterpret_cast<const U*>(p); }
+    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<U*>(p) = this->v; }
+};
+
 // A parameter vector (norm weight, bias) whose type is the activations' T or fp32: elements [i, i + VEC) as floats
 template <typename T, int VEC>
 __device__ __forceinline__ void load_param(float (&o)[VEC], const void* p, bool f32, int64_t i) {

@@ -1,11 +1,11 @@
 // Linear layer with its epilogue:  z = x w^T + b,  y = act(z) + residual,  and its backward pass
 //   dz = dy act'(z),  dx = dz w,  dw = dz^T x,  db = sum_rows dz,  dresidual = dy.
 //
-// fp32 products run on dssvae_gemm_f32 (v_mfma_f32_32x32x2_f32) with the epilogue as one pass behind them.  bf16 / fp16
-// products are this file's: v_mfma_f32_32x32x16, fp32 accumulation, one rounding per output.
+// Products run on one tile kernel: v_mfma_f32_32x32x16 for bf16 / fp16, v_mfma_f32_32x32x2_f32 for fp32 (exact products),
+// fp32 accumulation, one rounding per output.
 //
-// The 16-bit tile kernel: C[M, N] = A[M, K] . B[N, K]^T, both operands contiguous along K.  A BM x BN block walks K in
-// steps of 64; operand tiles go global -> LDS directly (16 bytes a lane, no registers), double buffered.  LDS row r keeps its
+// The tile kernel: C[M, N] = A[M, K] . B[N, K]^T, both operands contiguous along K.  A BM x BN block walks K in steps of
+// 128 bytes (64 or 32 elements); operand tiles go global -> LDS directly (16 bytes a lane, no registers), double buffered.  LDS row r keeps its
 // 16-byte chunk c at place c ^ (r & 7): the eight rows a quarter wave reads at one chunk then cover all banks (rows are 128
 // bytes apart, unswizzled they would share one).  The pipeline is rotated: fragments of the step's first half are already in
 // registers when it begins; one barrier per step, passed between the halves: by then the next tile has landed and every
@@ -18,7 +18,9 @@
 
 namespace {
 
-constexpr int BK = 64;
+// elements of a k-tile's row (128 bytes) and of a 16-byte granule
+template <typename T> constexpr int BK = 128 / (int)sizeof(T);
+template <typename T> constexpr int GR = 16 / (int)sizeof(T);
 
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
@@ -77,7 +79,7 @@ struct Epilogue {
     const void* res; int64_t ldr;     // [M, N] or NULL
     void* z; int64_t ldz;             // pre-activation, or NULL
     void* y; int64_t ldy;
-    int act, vec;                     // vec: rows of res, z, y may be moved 16 bytes at a time
+    int act;
 };
 
 template <typename T>
@@ -100,10 +102,9 @@ __device__ __forceinline__ void finish8(const Epilogue& e, f32x8 a, f32x8 b, int
     T* y = reinterpret_cast<T*>(e.y) + m * e.ldy + n;
     T* z = e.z ? reinterpret_cast<T*>(e.z) + m * e.ldz + n : nullptr;
     const T* r = e.res ? reinterpret_cast<const T*>(e.res) + m * e.ldr + n : nullptr;
-    if (e.vec && n + 8 <= N) {
-        Gran<T, 8> g;
+    if (n + 8 <= N) {
+        GranU<T, 8> g, gz, gy;
         if (r) g.load(r);
-        Gran<T, 8> gz, gy;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float zz = a[j] + b[j];
@@ -123,23 +124,37 @@ __device__ __forceinline__ void finish8(const Epilogue& e, f32x8 a, f32x8 b, int
     }
 }
 
-// ---- the 16-bit tile kernel ---------------------------------------------------------------------------------------
+// ---- the tile kernel -----------------------------------------------------------------------------------------
 typedef __attribute__((address_space(1))) const void* gptr_t;
 typedef __attribute__((address_space(3))) void* lptr_t;
 
 __device__ const uint4 zero_granule = {0, 0, 0, 0};
 
+// V: what a lane holds of a 32-row block's granule pair (16 bytes of its row, lanes 32.. the second granule); go: the product
+// over both granules.  fp32 takes one float per lane and instruction: which k a (step, lane half) pair multiplies is free as
+// long as A and B agree, so four steps use up the 16 bytes.
 template <typename T> struct Mfma;
+template <> struct Mfma<float> {
+    typedef f32x4 V;
+    static constexpr int N = 4;  // instructions
+    static __device__ __forceinline__ f32x16 go(V a, V b, f32x16 c) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+        return c;
+    }
+};
 template <> struct Mfma<bf16_t> {
     typedef bf16_t V __attribute__((ext_vector_type(8)));
+    static constexpr int N = 1;
     static __device__ __forceinline__ f32x16 go(V a, V b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mfma<f16_t> {
     typedef f16_t V __attribute__((ext_vector_type(8)));
+    static constexpr int N = 1;
     static __device__ __forceinline__ f32x16 go(V a, V b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 
-// One operand's share of a tile load: R rows x 64 k, TH threads, 16 bytes a lane.  A thread's granules all lie in the same
+// One operand's share of a tile load: R rows x 128 bytes, TH threads, 16 bytes a lane.  A thread's granules all lie in the same
 // place of their rows (rows TH / 8 apart, a multiple of 8: the swizzle is the same).  Rows behind the last are loaded from
 // it and never stored.  `base` is uniform: row r0 of the operand at the tile's first k.
 template <typename T, int R, int TH>
@@ -148,7 +163,7 @@ struct Loader {
     unsigned off[NR];  // bytes behind base
     __device__ __forceinline__ static int k_of() {
         const int row = threadIdx.x >> 3;
-        return (int)((threadIdx.x & 7) ^ (row & 7)) * 8;
+        return (int)((threadIdx.x & 7) ^ (row & 7)) * GR<T>;
     }
     __device__ __forceinline__ void init(int64_t ld, int64_t rows_left) {
         const int row = threadIdx.x >> 3;
@@ -172,11 +187,11 @@ struct Loader {
     }
     static __device__ __forceinline__ void put(T* lds, int i, const char* src) {
         const int wave = threadIdx.x >> 6;
-        __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(lds + (i * TH + wave * 64) * 8), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(lds + (i * TH + wave * 64) * GR<T>), 16, 0, 0);
     }
 };
 
-// MI x NI blocks of 32 x 32 of this wave's tile: the operands of K half `h` (two MFMA steps of 16)
+// MI x NI blocks of 32 x 32 of this wave's tile: the operands of K half `h` (two granule pairs)
 template <typename T, int MI, int NI>
 struct Frags {
     typename Mfma<T>::V a[2][MI], b[2][NI];
@@ -185,11 +200,11 @@ struct Frags {
         const int lane = threadIdx.x & 63, r = lane & 31;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const int c = ((h * 4 + s * 2 + (lane >> 5)) ^ (r & 7)) * 8;  // (tile rows start at multiples of 8)
+            const int c = ((h * 4 + s * 2 + (lane >> 5)) ^ (r & 7)) * GR<T>;  // (tile rows start at multiples of 8)
 #pragma unroll
-            for (int i = 0; i < MI; ++i) a[s][i] = *reinterpret_cast<const typename Mfma<T>::V*>(sa + (ra + i * 32 + r) * BK + c);
+            for (int i = 0; i < MI; ++i) a[s][i] = *reinterpret_cast<const typename Mfma<T>::V*>(sa + (ra + i * 32 + r) * BK<T> + c);
 #pragma unroll
-            for (int j = 0; j < NI; ++j) b[s][j] = *reinterpret_cast<const typename Mfma<T>::V*>(sb + (rb + j * 32 + r) * BK + c);
+            for (int j = 0; j < NI; ++j) b[s][j] = *reinterpret_cast<const typename Mfma<T>::V*>(sb + (rb + j * 32 + r) * BK<T> + c);
         }
     }
     __device__ __forceinline__ void multiply(f32x16 (&acc)[MI][NI]) const {
@@ -227,7 +242,7 @@ template <typename T, int BM, int BN, int TH>
 __device__ __forceinline__ void tile_load(T* __restrict__ lds, const Loader<T, BM, TH>& la, const Loader<T, BN, TH>& lb, const T* a,
                                           const T* b) {
     la.load(lds, a);
-    lb.load(lds + BM * BK, b);
+    lb.load(lds + BM * BK<T>, b);
 }
 
 // Barrier that also waits for this wave's loads into LDS (a workgroup fence alone does not order them).
@@ -242,8 +257,8 @@ __device__ __forceinline__ void tile_barrier() {
 template <typename T, int BM, int BN, int TH, int MI, int NI>
 __device__ __forceinline__ void k_step(Frags<T, MI, NI>& f0, Frags<T, MI, NI>& f1, f32x16 (&acc)[MI][NI], const Loader<T, BM, TH>& la,
                                        const Loader<T, BN, TH>& lb, T* cur, const T* next, int ra, int rb, const T* a, const T* b) {
-    constexpr int READS = 2 * (MI + NI), MULS = 2 * MI * NI, LOADS = Loader<T, BM, TH>::NR + Loader<T, BN, TH>::NR;
-    f1.read(cur, BM * BK, ra, rb, 1);
+    constexpr int READS = 2 * (MI + NI), MULS = 2 * MI * NI * Mfma<T>::N, LOADS = Loader<T, BM, TH>::NR + Loader<T, BN, TH>::NR;
+    f1.read(cur, BM * BK<T>, ra, rb, 1);
     f0.multiply(acc);
 #pragma unroll
     for (int i = 0; i < MULS; ++i) {
@@ -252,7 +267,7 @@ __device__ __forceinline__ void k_step(Frags<T, MI, NI>& f0, Frags<T, MI, NI>& f
     }
     tile_barrier();  // this tile has been read by every wave, the next one has landed
     tile_load<T, BM, BN, TH>(cur, la, lb, a, b);
-    f0.read(next, BM * BK, ra, rb, 0);
+    f0.read(next, BM * BK<T>, ra, rb, 0);
     f1.multiply(acc);
 #pragma unroll
     for (int i = 0; i < MULS; ++i) {
@@ -266,7 +281,7 @@ template <typename T, int BM, int BN, int WR, int WC>
 __global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, Epilogue e) {
     constexpr int TH = 64 * WR * WC, MI = BM / WR / 32, NI = BN / WC / 32;
     static_assert(NI == 2, "the epilogue moves 64 columns of a wave at a time");
-    __shared__ __attribute__((aligned(16))) T buf0[(BM + BN) * BK], buf1[(BM + BN) * BK];
+    __shared__ __attribute__((aligned(16))) T buf0[(BM + BN) * BK<T>], buf1[(BM + BN) * BK<T>];
     const int wid = xcd_remap(blockIdx.x, gridDim.x), tiles = s.tiles_m * s.tiles_n;
     const int split = wid / tiles;
     int tm, tn;
@@ -275,7 +290,7 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, E
     const int n0 = tn * BN;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int ra = wave / WC * (BM / WR), rb = wave % WC * (BN / WC);
-    const int64_t nk = (s.K + BK - 1) / BK, kt0 = split * s.ktiles, kt1 = min(nk, kt0 + s.ktiles);
+    const int64_t nk = (s.K + BK<T> - 1) / BK<T>, kt0 = split * s.ktiles, kt1 = min(nk, kt0 + s.ktiles);
 
     f32x16 acc[MI][NI];
 #pragma unroll
@@ -294,25 +309,25 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, E
         const T* B = (const T*)s.B + (int64_t)n0 * s.ldb;
         // The order of the tiles is free: the last one, which alone may reach behind K, goes first, then kt0 .. kt1 - 2, so that
         // the loop's loads need no test.  A tile behind the end is the one before it again (loaded, never multiplied).
-        const int64_t kl = (kt1 - 1) * BK, n = kt1 - kt0;
+        const int64_t kl = (kt1 - 1) * BK<T>, n = kt1 - kt0;
         la.load_last(buf0, A + kl, s.K - kl);
-        lb.load_last(buf0 + BM * BK, B + kl, s.K - kl);
+        lb.load_last(buf0 + BM * BK<T>, B + kl, s.K - kl);
         const int64_t most = n > 1 ? kt1 - 2 : kt0;
-        if (n > 1) tile_load<T, BM, BN, TH>(buf1, la, lb, A + kt0 * BK, B + kt0 * BK);
+        if (n > 1) tile_load<T, BM, BN, TH>(buf1, la, lb, A + kt0 * BK<T>, B + kt0 * BK<T>);
         tile_barrier();
         Frags<T, MI, NI> f0, f1;
-        f0.read(buf0, BM * BK, ra, rb, 0);
+        f0.read(buf0, BM * BK<T>, ra, rb, 0);
         // step i multiplies the i-th tile in that order and loads the (i + 2)-th: kt0 + i + 1
         int64_t i = 0;
         if (n > 1) {
             for (; i + 1 < n; i += 2) {
-                const int64_t k2 = min(kt0 + i + 1, most) * BK, k3 = min(kt0 + i + 2, most) * BK;
+                const int64_t k2 = min(kt0 + i + 1, most) * BK<T>, k3 = min(kt0 + i + 2, most) * BK<T>;
                 k_step<T, BM, BN, TH, MI, NI>(f0, f1, acc, la, lb, buf0, buf1, ra, rb, A + k2, B + k2);
                 k_step<T, BM, BN, TH, MI, NI>(f0, f1, acc, la, lb, buf1, buf0, ra, rb, A + k3, B + k3);
             }
         }
         if (i < n) {  // an odd tile is left: nothing behind it
-            f1.read(buf0, BM * BK, ra, rb, 1);
+            f1.read(buf0, BM * BK<T>, ra, rb, 1);
             f0.multiply(acc);
             f1.multiply(acc);
         }
@@ -401,14 +416,13 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const T* __restrict__ 
 //   v = src * act'(z)            else
 // out [R, ldo] (NULL: not wanted) gets v, columns C .. ldo zero; outT [C, ldt] (NULL) its transpose, columns R .. ldt zero;
 // sums [gridDim.y][C] (NULL) the block's column sums of the unrounded v.
-// A thread moves granules of 8 elements (16-bit) in rows of 64: `vec` where rows of src, z and out start on granules, else by
-// elements.  The tile's granule (r, chunk) lies at chunk ^ (r / 8): the eight lanes that gather one column's 64 rows then
-// read eight different banks.  outT rows always start on granules (ldt % 8 == 0).
+// A thread moves eight neighbouring elements of a row.  The tile keeps its eight (r, chunk) at chunk ^ (r / 8): the eight lanes
+// that gather one column's 64 rows then read eight different banks.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_turn_kernel(const T* __restrict__ src, int64_t ld, const T* __restrict__ z,
                                                           int64_t ldz, int act, int64_t R, int64_t C, T* __restrict__ out,
                                                           int64_t ldo, T* __restrict__ outT, int64_t ldt,
-                                                          float* __restrict__ sums, int vec) {
+                                                          float* __restrict__ sums) {
     __shared__ __attribute__((aligned(16))) T tile[64 * 64];
     __shared__ float red[32][64];
     const int64_t c0 = (int64_t)blockIdx.x * 64;
@@ -424,11 +438,11 @@ __global__ __launch_bounds__(256) void linear_turn_kernel(const T* __restrict__ 
             const int tr = i * 32 + rr;
             const int64_t r = r0 + tr;
             float v[8];
-            Gran<T, 8> g;
+            GranU<T, 8> g;
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = 0.f;
             if (r < R && c < C) {
-                if (vec && c + 8 <= C) {
+                if (c + 8 <= C) {
                     g.load(src + r * ld + c);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] = g.get(j);
@@ -452,7 +466,7 @@ __global__ __launch_bounds__(256) void linear_turn_kernel(const T* __restrict__ 
                 g.set(j, v[j]);
             }
             if (out && r < R) {
-                if (vec && c + 8 <= ldo) {
+                if (c + 8 <= ldo) {
                     g.store(out + r * ldo + c);
                 } else {
 #pragma unroll
@@ -468,14 +482,20 @@ __global__ __launch_bounds__(256) void linear_turn_kernel(const T* __restrict__ 
             for (int i = 0; i < 2; ++i) {
                 // lane ch gathers rows 8 ch .. of column i * 32 + rr
                 const int tc = i * 32 + rr;
-                Gran<T, 8> g;
+                GranU<T, 8> g;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const T t = tile[(ch * 8 + j) * 64 + ((tc >> 3) ^ ch) * 8 + (tc & 7)];
-                    if constexpr (sizeof(T) == 2) g.v[j] = t;
-                }
+                for (int j = 0; j < 8; ++j) g.v[j] = tile[(ch * 8 + j) * 64 + ((tc >> 3) ^ ch) * 8 + (tc & 7)];
                 const int64_t r = r0 + ch * 8;
-                if (c0 + tc < C && r < ldt) g.store(outT + (c0 + tc) * ldt + r);
+                T* o = outT + (c0 + tc) * ldt + r;
+                if (c0 + tc < C) {
+                    if (r + 8 <= ldt) {
+                        g.store(o);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (r + j < ldt) o[j] = g.v[j];
+                    }
+                }
             }
             __syncthreads();
         }
@@ -509,72 +529,75 @@ __global__ __launch_bounds__(1024) void linear_db_kernel(const float* __restrict
     else reinterpret_cast<T*>(db)[c] = (T)s;
 }
 
-// fp32: y = act(z) + res over the product's output
-__global__ __launch_bounds__(256) void linear_epilogue_f32_kernel(const float* z, int64_t ldz, const float* __restrict__ res,
-                                                                  int64_t ldr, int act, int64_t M, int N, float* y, int64_t ldy) {
-    for (int64_t m = blockIdx.x; m < M; m += gridDim.x)
-        for (int n = threadIdx.x; n < N; n += 256)
-            y[m * ldy + n] = act_f(act, z[m * ldz + n]) + (res ? res[m * ldr + n] : 0.f);
-}
-
 // ---- host ---------------------------------------------------------------------------------------------------------
 inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Tile width and K split: the smallest of a cost in units of one 128 x 128 x 64 step of a CU.  Two 128-wide blocks share a CU
-// and their steps read twice the LDS per product (a step costs 1.35); partials cost their traffic.
-struct Plan { bool wide; int ksplit; };
+// Tile width and K split: the smallest of a modelled time in microseconds.  u: a 128 x 128 step of a CU at the rate that the
+// 256-wide (fp32: 128-wide) kernel reaches.  Narrower tiles read more LDS per product, a lone 64-wide block has two waves
+// for four SIMDs; every round of blocks has a latency of its own; partials cost their traffic and a launch.
+struct Plan { int tile, ksplit; };
+template <typename T>
 inline Plan plan(int64_t M, int64_t N, int64_t K) {
-    const double cus = device_cus();
-    const int64_t nk = up(K, BK) / BK;
-    Plan best{false, 1};
+    static const int splits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+    const bool f32 = sizeof(T) == 4;
+    const double cus = device_cus(), u = f32 ? 2.0 : 0.42;
+    const int64_t nk = up(K, BK<T>) / BK<T>;
+    Plan best{64, 1};
     double least = -1;
-    for (int wide = 0; wide < 2; ++wide)
-        for (int ks = 1; ks <= 16; ks *= 2) {
+    for (int tile = f32 ? 128 : 256; tile >= 64; tile /= 2)
+        for (int ks : splits) {
             if (ks > 1 && nk / ks < 4) break;
-            const int b = wide ? 256 : 128;
-            const double tiles = (double)(up(M, b) / b) * (double)(up(N, b) / b) * ks, steps = (double)((nk + ks - 1) / ks);
-            const double slots = wide ? cus : 2 * cus, rounds = (double)(int64_t)((tiles + slots - 1) / slots);
-            double cost = wide ? rounds * (steps * 4 + 12) : rounds * (2 * 1.35 * steps + 6);
-            if (ks > 1) cost += 10 + (double)(2 * ks) * M * N * 4 / 2e6;
+            const double per = tile == 256 ? 4 * u : tile == 128 ? (f32 ? u : 1.35 * u) : (f32 ? 0.27 * u : 0.5 * u);
+            const double wait = tile == 256 ? 6 : tile == 128 ? 4 : 3;
+            const int resident = tile == 256 ? 1 : tile == 128 ? 2 : 4;
+            const double tiles = (double)(up(M, tile) / tile) * (double)(up(N, tile) / tile) * ks;
+            const double load = (double)(int64_t)((tiles + cus - 1) / cus);  // blocks of the fullest CU
+            double cost = load * (double)((nk + ks - 1) / ks) * per * (tile == 64 && load < 2 ? 2 : 1) +
+                          (double)(int64_t)((load + resident - 1) / resident) * wait;
+            if (ks > 1) cost += 4 + (double)(2 * ks + 1) * M * N * 4 / 4e6;
             if (least < 0 || cost < least) {
                 least = cost;
-                best = Plan{wide != 0, ks};
+                best = Plan{tile, ks};
             }
         }
     return best;
 }
 
+template <typename T>
 inline int64_t part_bytes(int64_t M, int64_t N, int64_t K) {
-    const Plan p = plan(M, N, K);
+    const Plan p = plan<T>(M, N, K);
     return p.ksplit > 1 ? up((int64_t)p.ksplit * M * N * 4, 256) : 0;
 }
 
 // operand rows usable as they are: 16-byte granules, and the 256 rows of a tile within 32-bit byte offsets
-inline bool direct(const void* p, int64_t ld, int64_t K) { return aligned_to(p, 16) && ld % 8 == 0 && K % 8 == 0 && ld < (1 << 22); }
-
-inline bool epilogue_vec(const Epilogue& e) {
-    return aligned_to(e.y, 16) && e.ldy % 8 == 0 && (!e.z || (aligned_to(e.z, 16) && e.ldz % 8 == 0)) &&
-           (!e.res || (aligned_to(e.res, 16) && e.ldr % 8 == 0));
+constexpr int64_t MAX_LD = 1 << 21;
+template <typename T>
+inline bool direct(const void* p, int64_t ld, int64_t K) {
+    return aligned_to(p, 16) && ld % GR<T> == 0 && K % GR<T> == 0 && ld <= MAX_LD;
 }
 
 template <typename T>
 int product(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K, Epilogue e, void* part,
             hipStream_t st) {
     if (M == 0 || N == 0) return DSSVAE_OK;
-    const Plan p = plan(M, N, K);
-    const int b = p.wide ? 256 : 128;
+    const Plan p = plan<T>(M, N, K);
+    const int b = p.tile;
     Shape s;
     s.A = A; s.lda = lda; s.B = B; s.ldb = ldb; s.M = M; s.N = (int)N; s.K = K;
     const int64_t tm = up(M, b) / b, tn = up(N, b) / b;
     if (tm * tn * p.ksplit > 0x7fffffff) return DSSVAE_ETOOBIG;
     s.tiles_m = (int)tm; s.tiles_n = (int)tn; s.ksplit = p.ksplit;
-    const int64_t nk = up(K, BK) / BK;
+    const int64_t nk = up(K, BK<T>) / BK<T>;
     s.ktiles = (nk + p.ksplit - 1) / p.ksplit;
     s.part = (float*)part;
-    e.vec = epilogue_vec(e);
     const dim3 grid((unsigned)(tm * tn * p.ksplit));
-    if (p.wide) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, 4>), grid, dim3(512), 0, st, s, e);
-    else hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, 2>), grid, dim3(256), 0, st, s, e);
+    if (b == 256) {
+        if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, 4>), grid, dim3(512), 0, st, s, e);
+    } else if (b == 128) {
+        hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, 2>), grid, dim3(256), 0, st, s, e);
+    } else {
+        hipLaunchKernelGGL((linear_tile_kernel<T, 64, 64, 2, 1>), grid, dim3(128), 0, st, s, e);
+    }
     DSSVAE_CHECK_LAUNCH();
     if (p.ksplit > 1) {
         const int64_t n = M * ((N + 7) / 8), blocks = (n + 255) / 256;
@@ -604,11 +627,8 @@ template <typename T>
 int turn(const void* src, int64_t ld, const void* z, int64_t ldz, int act, int64_t R, int64_t C, void* out, int64_t ldo, void* outT,
          int64_t ldt, float* sums, hipStream_t st) {
     const dim3 grid((unsigned)((C + 63) / 64), (unsigned)turn_rows(R, C));
-    const int per = 8, align = per * (int)sizeof(T);  // (a fp32 granule of 8 is two 16-byte moves)
-    const int vec = aligned_to(src, align) && ld % per == 0 && (!z || (aligned_to(z, align) && ldz % per == 0)) &&
-                    (!out || (aligned_to(out, align) && ldo % per == 0));
     hipLaunchKernelGGL((linear_turn_kernel<T>), grid, dim3(256), 0, st, (const T*)src, ld, (const T*)z, ldz, act, R, C, (T*)out, ldo,
-                       (T*)outT, ldt, sums, vec);
+                       (T*)outT, ldt, sums);
     DSSVAE_CHECK_LAUNCH();
     return DSSVAE_OK;
 }
@@ -629,20 +649,20 @@ bool bad_args(int dtype, int act, int64_t M, int N, int K) {
 }
 
 template <typename T>
-int fwd16(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int N, int K, const Epilogue& e, Space& sp, hipStream_t st,
+int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int N, int K, const Epilogue& e, Space& sp, hipStream_t st,
           bool dry) {
-    const int64_t ldk = up(K, 8);
-    if (!direct(x, ldx, K)) {
-        void* d = sp.take(M * ldk * 2);
+    const int64_t ldk = up(K, GR<T>), es = sizeof(T);
+    if (!direct<T>(x, ldx, K)) {
+        void* d = sp.take(M * ldk * es);
         if (!dry) { const int rc = pack<T>(x, ldx, M, K, d, ldk, st); if (rc) return rc; }
         x = d; ldx = ldk;
     }
-    if (!direct(w, ldw, K)) {
-        void* d = sp.take((int64_t)N * ldk * 2);
+    if (!direct<T>(w, ldw, K)) {
+        void* d = sp.take((int64_t)N * ldk * es);
         if (!dry) { const int rc = pack<T>(w, ldw, N, K, d, ldk, st); if (rc) return rc; }
         w = d; ldw = ldk;
     }
-    void* part = sp.take(part_bytes(M, N, ldk));
+    void* part = sp.take(part_bytes<T>(M, N, ldk));
     return dry ? DSSVAE_OK : product<T>(x, ldx, w, ldw, M, N, ldk, e, part, st);
 }
 
@@ -655,16 +675,16 @@ struct BwdArgs {
 };
 
 template <typename T>
-int bwd16(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
-    const int64_t M = a.M, N = a.N, K = a.K, ldn = up(N, 8), ldm = up(M, 8);
+int backward(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
+    const int64_t M = a.M, N = a.N, K = a.K, ldn = up(N, GR<T>), ldm = up(M, GR<T>), es = sizeof(T);
     int rc = DSSVAE_OK;
     // dz: a copy where it differs from dy or dy's rows cannot be loaded as they are
-    const bool copy = a.dx && (a.z || !direct(a.dy, a.lddy, N));
+    const bool copy = a.dx && (a.z || !direct<T>(a.dy, a.lddy, N));
     const void* dz = a.dy;
     int64_t lddz = a.lddy;
     void *dzc = nullptr, *dzt = nullptr;
-    if (copy) { dzc = sp.take(M * ldn * 2); dz = dzc; lddz = ldn; }
-    if (a.dw) dzt = sp.take(N * ldm * 2);
+    if (copy) { dzc = sp.take(M * ldn * es); dz = dzc; lddz = ldn; }
+    if (a.dw) dzt = sp.take(N * ldm * es);
     float* sums = a.db ? (float*)sp.take(turn_rows(M, N) * N * 4) : nullptr;
     if (copy || a.dw || a.db) {
         if (!dry) {
@@ -677,8 +697,8 @@ int bwd16(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
         }
     }
     if (a.dx) {
-        void* wt = sp.take(K * ldn * 2);
-        void* part = sp.take(part_bytes(M, K, ldn));
+        void* wt = sp.take(K * ldn * es);
+        void* part = sp.take(part_bytes<T>(M, K, ldn));
         if (!dry) {
             if ((rc = turn<T>(a.w, a.ldw, nullptr, 0, 0, N, K, nullptr, 0, wt, ldn, nullptr, st))) return rc;
             Epilogue e{};
@@ -687,8 +707,8 @@ int bwd16(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
         }
     }
     if (a.dw) {
-        void* xt = sp.take(K * ldm * 2);
-        void* part = sp.take(part_bytes(N, K, ldm));
+        void* xt = sp.take(K * ldm * es);
+        void* part = sp.take(part_bytes<T>(N, K, ldm));
         if (!dry) {
             if ((rc = turn<T>(a.x, a.ldx, nullptr, 0, 0, M, K, nullptr, 0, xt, ldm, nullptr, st))) return rc;
             Epilogue e{};
@@ -699,39 +719,9 @@ int bwd16(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
     return rc;
 }
 
-int bwd32(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
-    const float* dz = (const float*)a.dy;
-    int64_t lddz = a.lddy;
-    float *dzc = nullptr, *sums = nullptr;
-    int rc = DSSVAE_OK;
-    if (a.z && (a.dx || a.dw)) {
-        dzc = (float*)sp.take(a.M * a.N * 4);
-        dz = dzc; lddz = a.N;
-    }
-    if (a.db) sums = (float*)sp.take(turn_rows(a.M, a.N) * a.N * 4);
-    if (dry) return rc;
-    if (dzc || sums) {
-        if ((rc = turn<float>(a.dy, a.lddy, a.z, a.ldz, a.act, a.M, a.N, dzc, a.N, nullptr, 0, sums, st))) return rc;
-        if (a.db) {
-            hipLaunchKernelGGL((linear_db_kernel<float>), dim3((unsigned)((a.N + 31) / 32)), dim3(1024), 0, st, sums,
-                               (int)turn_rows(a.M, a.N), a.N, a.db, 1);
-            DSSVAE_CHECK_LAUNCH();
-        }
-    }
-    const int M = (int)a.M;
-    if (a.dx && M > 0 && (rc = dssvae_gemm_f32(dz, lddz, 0, nullptr, (const float*)a.w, a.ldw, 1, (float*)a.dx, a.lddx, nullptr, M, a.K,
-                                               a.N, 1.f, 0.f, st)))
-        return rc;
-    if (a.dw) {
-        if (M == 0) return dssvae_zero2d((float*)a.dw, a.lddw, a.N, a.K, st);
-        return dssvae_gemm_f32(dz, lddz, 1, nullptr, (const float*)a.x, a.ldx, 1, (float*)a.dw, a.lddw, nullptr, a.N, a.K, M, 1.f, 0.f, st);
-    }
-    return rc;
-}
-
 int bwd_any(int dtype, const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
-    if (dtype == DSSVAE_F32) return bwd32(a, sp, st, dry);
-    return dtype == DSSVAE_BF16 ? bwd16<bf16_t>(a, sp, st, dry) : bwd16<f16_t>(a, sp, st, dry);
+    if (dtype == DSSVAE_F32) return backward<float>(a, sp, st, dry);
+    return dtype == DSSVAE_BF16 ? backward<bf16_t>(a, sp, st, dry) : backward<f16_t>(a, sp, st, dry);
 }
 
 }  // namespace
@@ -739,9 +729,9 @@ int bwd_any(int dtype, const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
 extern "C" int64_t dssvae_linear_act_fwd_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype,
                                                          int64_t M, int N, int K) {
     if (bad_args(dtype, DSSVAE_ACT_NONE, M, N, K)) return DSSVAE_EINVAL;
-    if (dtype == DSSVAE_F32) return 0;
     Space sp{nullptr, 0, 0};
-    fwd16<bf16_t>(x, ldx, w, ldw, M, N, K, Epilogue{}, sp, nullptr, true);
+    if (dtype == DSSVAE_F32) forward<float>(x, ldx, w, ldw, M, N, K, Epilogue{}, sp, nullptr, true);
+    else forward<bf16_t>(x, ldx, w, ldw, M, N, K, Epilogue{}, sp, nullptr, true);  // (fp16: the same sizes)
     return sp.used;
 }
 
@@ -751,28 +741,17 @@ extern "C" int dssvae_linear_act_fwd(const void* x, int64_t ldx, const void* w, 
                                      void* stream) {
     if (bad_args(dtype, act, M, N, K) || ldx < K || ldw < K || ldy < N || (res && ldr < N) || (z && ldz < N)) return DSSVAE_EINVAL;
     if (M == 0) return DSSVAE_OK;
+    if (K > MAX_LD) return DSSVAE_ETOOBIG;
     if (!x || !w || !y || (z && z == y)) return DSSVAE_EINVAL;
     const int64_t need = dssvae_linear_act_fwd_workspace_bytes(x, ldx, w, ldw, dtype, M, N, K);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))) return DSSVAE_EINVAL;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == DSSVAE_F32) {
-        const bool plain = act == DSSVAE_ACT_NONE && !res;
-        float* zz = z ? (float*)z : (float*)y;
-        const int64_t ldzz = z ? ldz : ldy;
-        const int rc = dssvae_gemm_f32((const float*)x, ldx, 0, nullptr, (const float*)w, ldw, 0, zz, ldzz, (const float*)bias, (int)M, N,
-                                       K, 1.f, 0.f, stream);
-        if (rc || (plain && !z)) return rc;
-        const int64_t most = 16 * (int64_t)device_cus();
-        hipLaunchKernelGGL(linear_epilogue_f32_kernel, dim3((unsigned)(M < most ? M : most)), dim3(256), 0, st, zz, ldzz,
-                           (const float*)res, ldr, act, M, N, (float*)y, ldy);
-        DSSVAE_CHECK_LAUNCH();
-        return DSSVAE_OK;
-    }
     Epilogue e{};
-    e.bias = bias; e.bias_f32 = bias_f32; e.res = res; e.ldr = ldr; e.z = z; e.ldz = ldz; e.y = y; e.ldy = ldy; e.act = act;
+    e.bias = bias; e.bias_f32 = bias_f32 || dtype == DSSVAE_F32; e.res = res; e.ldr = ldr; e.z = z; e.ldz = ldz; e.y = y; e.ldy = ldy; e.act = act;
     Space sp{(char*)workspace, 0, workspace_bytes};
-    if (dtype == DSSVAE_BF16) return fwd16<bf16_t>(x, ldx, w, ldw, M, N, K, e, sp, st, false);
-    return fwd16<f16_t>(x, ldx, w, ldw, M, N, K, e, sp, st, false);
+    if (dtype == DSSVAE_F32) return forward<float>(x, ldx, w, ldw, M, N, K, e, sp, st, false);
+    if (dtype == DSSVAE_BF16) return forward<bf16_t>(x, ldx, w, ldw, M, N, K, e, sp, st, false);
+    return forward<f16_t>(x, ldx, w, ldw, M, N, K, e, sp, st, false);
 }
 
 extern "C" int64_t dssvae_linear_act_bwd_workspace_bytes(const void* dy, int64_t lddy, int has_z, int dtype, int64_t M, int N, int K,
@@ -795,6 +774,7 @@ extern "C" int dssvae_linear_act_bwd(const void* dy, int64_t lddy, const void* z
         return DSSVAE_EINVAL;
     if (act != DSSVAE_ACT_NONE && !z && M > 0) return DSSVAE_EINVAL;
     if ((M > 0 && (!dy || (dw && !x))) || (dx && !w)) return DSSVAE_EINVAL;
+    if ((dx && N > MAX_LD) || (dw && M > MAX_LD)) return DSSVAE_ETOOBIG;
     BwdArgs a{};
     a.dy = dy; a.lddy = lddy; a.z = act == DSSVAE_ACT_NONE ? nullptr : z; a.ldz = ldz; a.x = x; a.ldx = ldx; a.w = w; a.ldw = ldw;
     a.dx = M > 0 ? dx : nullptr; a.lddx = lddx; a.dw = dw; a.lddw = lddw; a.db = db; a.db_f32 = db_f32 || dtype == DSSVAE_F32;

@@ -619,8 +619,8 @@ int dssvae_scale_rows(void* x, int64_t ld, int dtype, int64_t rows, int V, const
  *   y must not overlap x, w or z; it may be res.  DSSVAE_ACT_GELU is the exact form, z Phi(z).
  * Backward: dz = dy act'(z); dx = dz w; dw = dz^T x; db = sum over rows of dz; dx, dw, db may each be NULL, z only where act
  * is DSSVAE_ACT_NONE.  (The residual's gradient is dy.)  M = 0 clears dw and db.
- * 16-bit types: fp32 accumulation, dz and z rounded to the type (the slopes and the products of backward start from those
- * roundings); sums in a fixed order.  fp32: dssvae_gemm_f32's order.
+ * fp32 accumulation in a fixed order; 16-bit types: dz and z are rounded to the type (the slopes and the products of backward
+ * start from those roundings).  A summed axis (K forward, N for dx, M for dw) has at most 2097152 elements: DSSVAE_ETOOBIG.
  * The workspace sizes depend on where the operands start: the query takes the pointers and strides of the call.
  * ------------------------------------------------------------------------------------------- */
 #define DSSVAE_ACT_NONE 0
