@@ -97,19 +97,20 @@ __device__ __forceinline__ f32x8 bias8(const Epilogue& e, int n, int N) {
 }
 
 // eight consecutive columns n .. of row m (those below N): a without the bias b
-template <typename T>
-__device__ __forceinline__ void finish8(const Epilogue& e, f32x8 a, f32x8 b, int64_t m, int n, int N) {
+template <typename T, int ACT>
+__device__ __forceinline__ void finish8_act(const Epilogue& e, f32x8 a, f32x8 b, int64_t m, int n, int N) {
     T* y = reinterpret_cast<T*>(e.y) + m * e.ldy + n;
     T* z = e.z ? reinterpret_cast<T*>(e.z) + m * e.ldz + n : nullptr;
     const T* r = e.res ? reinterpret_cast<const T*>(e.res) + m * e.ldr + n : nullptr;
     if (n + 8 <= N) {
         GranU<T, 8> g, gz, gy;
         if (r) g.load(r);
+        else g.zero();
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float zz = a[j] + b[j];
             gz.set(j, keep_z<T>(zz));
-            gy.set(j, act_f(e.act, zz) + (r ? g.get(j) : 0.f));
+            gy.set(j, act_f(ACT, zz) + g.get(j));
         }
         if (z) gz.store(z);
         gy.store(y);
@@ -119,8 +120,19 @@ __device__ __forceinline__ void finish8(const Epilogue& e, f32x8 a, f32x8 b, int
             if (n + j >= N) continue;
             const float zz = a[j] + b[j];
             if (z) z[j] = (T)keep_z<T>(zz);
-            y[j] = (T)(act_f(e.act, zz) + (r ? (float)r[j] : 0.f));
+            y[j] = (T)(act_f(ACT, zz) + (r ? (float)r[j] : 0.f));
         }
+    }
+}
+// (one branch on the activation per eight elements, not one per element)
+template <typename T>
+__device__ __forceinline__ void finish8(const Epilogue& e, f32x8 a, f32x8 b, int64_t m, int n, int N) {
+    switch (e.act) {
+        case DSSVAE_ACT_RELU: finish8_act<T, DSSVAE_ACT_RELU>(e, a, b, m, n, N); break;
+        case DSSVAE_ACT_GELU: finish8_act<T, DSSVAE_ACT_GELU>(e, a, b, m, n, N); break;
+        case DSSVAE_ACT_SILU: finish8_act<T, DSSVAE_ACT_SILU>(e, a, b, m, n, N); break;
+        case DSSVAE_ACT_TANH: finish8_act<T, DSSVAE_ACT_TANH>(e, a, b, m, n, N); break;
+        default: finish8_act<T, DSSVAE_ACT_NONE>(e, a, b, m, n, N);
     }
 }
 
@@ -280,7 +292,6 @@ __device__ __forceinline__ void k_step(Frags<T, MI, NI>& f0, Frags<T, MI, NI>& f
 template <typename T, int BM, int BN, int WR, int WC>
 __global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, Epilogue e) {
     constexpr int TH = 64 * WR * WC, MI = BM / WR / 32, NI = BN / WC / 32;
-    static_assert(NI == 2, "the epilogue moves 64 columns of a wave at a time");
     __shared__ __attribute__((aligned(16))) T buf0[(BM + BN) * BK<T>], buf1[(BM + BN) * BK<T>];
     const int wid = xcd_remap(blockIdx.x, gridDim.x), tiles = s.tiles_m * s.tiles_n;
     const int split = wid / tiles;
@@ -334,10 +345,11 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, E
         tile_barrier();  // operand buffers are free (and no load is in flight)
     }
 
-    // 32 rows x 64 columns of this wave at a time through 8 KiB of LDS of its own, read back along rows
-    float* stage = reinterpret_cast<float*>(buf0) + wave * 32 * 64;
-    static_assert(WR * WC * 32 * 64 * 4 <= (int)sizeof(buf0), "the waves' staging rows fit an operand buffer");
-    const int col = (lane & 7) * 8, n = n0 + rb + col;  // the lane's columns in every row
+    // 32 rows x CW columns of this wave at a time through LDS of its own, read back along rows
+    constexpr int CW = 32 * NI, LR = CW / 8, RP = 64 / LR;  // columns, lanes per row, rows per pass
+    float* stage = reinterpret_cast<float*>(buf0) + wave * 32 * CW;
+    static_assert(WR * WC * 32 * CW * 4 <= (int)sizeof(buf0), "the waves' staging rows fit an operand buffer");
+    const int col = (lane % LR) * 8, n = n0 + rb + col;  // the lane's columns in every row
     const f32x8 bias = bias8<T>(e, n, s.N);
 #pragma unroll 1
     for (int i = 0; i < MI; ++i) {
@@ -348,13 +360,13 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, E
             for (int j = 0; j < NI; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    stage[((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * 64 + j * 32 + (lane & 31)] = acc[ii][j][r];
+                    stage[((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * CW + j * 32 + (lane & 31)] = acc[ii][j][r];
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int row = q * 8 + (lane >> 3);
-            const f32x8 v = *reinterpret_cast<const f32x8*>(stage + row * 64 + col);
+        for (int q = 0; q < 32 / RP; ++q) {
+            const int row = q * RP + lane / LR;
+            const f32x8 v = *reinterpret_cast<const f32x8*>(stage + row * CW + col);
             const int64_t m = m0 + ra + i * 32 + row;
             if (m >= s.M || n >= s.N) continue;
             if (s.ksplit > 1) {
@@ -418,9 +430,9 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const T* __restrict__ 
 // sums [gridDim.y][C] (NULL) the block's column sums of the unrounded v.
 // A thread moves eight neighbouring elements of a row.  The tile keeps its eight (r, chunk) at chunk ^ (r / 8): the eight lanes
 // that gather one column's 64 rows then read eight different banks.
-template <typename T>
+template <typename T, int ACT>
 __global__ __launch_bounds__(256) void linear_turn_kernel(const T* __restrict__ src, int64_t ld, const T* __restrict__ z,
-                                                          int64_t ldz, int act, int64_t R, int64_t C, T* __restrict__ out,
+                                                          int64_t ldz, int64_t R, int64_t C, T* __restrict__ out,
                                                           int64_t ldo, T* __restrict__ outT, int64_t ldt,
                                                           float* __restrict__ sums) {
     __shared__ __attribute__((aligned(16))) T tile[64 * 64];
@@ -449,12 +461,12 @@ __global__ __launch_bounds__(256) void linear_turn_kernel(const T* __restrict__ 
                     if (z) {
                         g.load(z + r * ldz + c);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) v[j] *= act_slope(act, g.get(j));
+                        for (int j = 0; j < 8; ++j) v[j] *= act_slope(ACT, g.get(j));
                     }
                 } else {
                     for (int j = 0; j < 8 && c + j < C; ++j) {
                         float u = (float)src[r * ld + c + j];
-                        if (z) u *= act_slope(act, (float)z[r * ldz + c + j]);
+                        if (z) u *= act_slope(ACT, (float)z[r * ldz + c + j]);
 #pragma unroll
                         for (int jj = 0; jj < 8; ++jj) v[jj] = jj == j ? u : v[jj];
                     }
@@ -533,8 +545,9 @@ __global__ __launch_bounds__(1024) void linear_db_kernel(const float* __restrict
 inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 // Tile width and K split: the smallest of a modelled time in microseconds.  u: a 128 x 128 step of a CU at the rate that the
-// 256-wide (fp32: 128-wide) kernel reaches.  Narrower tiles read more LDS per product, a lone 64-wide block has two waves
-// for four SIMDs; every round of blocks has a latency of its own; partials cost their traffic and a launch.
+// 256-wide (fp32: 128-wide) kernel reaches.  Narrower tiles read more LDS per product; a step takes at least the latency of the
+// loads it waits for; every round of blocks has a prologue and an epilogue; partials cost their traffic and a launch.  (A sweep
+// over 17 shapes and all choices in both widths: within 10 % of the best one for all but the smallest.)
 struct Plan { int tile, ksplit; };
 template <typename T>
 inline Plan plan(int64_t M, int64_t N, int64_t K) {
@@ -547,13 +560,14 @@ inline Plan plan(int64_t M, int64_t N, int64_t K) {
     for (int tile = f32 ? 128 : 256; tile >= 64; tile /= 2)
         for (int ks : splits) {
             if (ks > 1 && nk / ks < 4) break;
-            const double per = tile == 256 ? 4 * u : tile == 128 ? (f32 ? u : 1.35 * u) : (f32 ? 0.27 * u : 0.5 * u);
-            const double wait = tile == 256 ? 6 : tile == 128 ? 4 : 3;
+            const double per = tile == 256 ? 4 * u : tile == 128 ? (f32 ? u : 1.35 * u) : (f32 ? 0.3 * u : 0.5 * u);
+            const double least_step = tile == 256 ? 1.7 : tile == 128 ? 0.8 : 0.35;  // a step's load latency
+            const double wait = tile == 256 ? 8 : tile == 128 ? 5 : 3;
             const int resident = tile == 256 ? 1 : tile == 128 ? 2 : 4;
             const double tiles = (double)(up(M, tile) / tile) * (double)(up(N, tile) / tile) * ks;
             const double load = (double)(int64_t)((tiles + cus - 1) / cus);  // blocks of the fullest CU
-            double cost = load * (double)((nk + ks - 1) / ks) * per * (tile == 64 && load < 2 ? 2 : 1) +
-                          (double)(int64_t)((load + resident - 1) / resident) * wait;
+            const double step = load * per > least_step ? load * per : least_step;
+            double cost = step * (double)((nk + ks - 1) / ks) + (double)(int64_t)((load + resident - 1) / resident) * wait;
             if (ks > 1) cost += 4 + (double)(2 * ks + 1) * M * N * 4 / 4e6;
             if (least < 0 || cost < least) {
                 least = cost;
@@ -596,7 +610,7 @@ int product(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, i
     } else if (b == 128) {
         hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, 2>), grid, dim3(256), 0, st, s, e);
     } else {
-        hipLaunchKernelGGL((linear_tile_kernel<T, 64, 64, 2, 1>), grid, dim3(128), 0, st, s, e);
+        hipLaunchKernelGGL((linear_tile_kernel<T, 64, 64, 2, 2>), grid, dim3(256), 0, st, s, e);
     }
     DSSVAE_CHECK_LAUNCH();
     if (p.ksplit > 1) {
@@ -627,8 +641,12 @@ template <typename T>
 int turn(const void* src, int64_t ld, const void* z, int64_t ldz, int act, int64_t R, int64_t C, void* out, int64_t ldo, void* outT,
          int64_t ldt, float* sums, hipStream_t st) {
     const dim3 grid((unsigned)((C + 63) / 64), (unsigned)turn_rows(R, C));
-    hipLaunchKernelGGL((linear_turn_kernel<T>), grid, dim3(256), 0, st, (const T*)src, ld, (const T*)z, ldz, act, R, C, (T*)out, ldo,
-                       (T*)outT, ldt, sums);
+#define GO(ACT)                                                                                                        \
+    if (act == ACT)                                                                                                    \
+    hipLaunchKernelGGL((linear_turn_kernel<T, ACT>), grid, dim3(256), 0, st, (const T*)src, ld, (const T*)z, ldz, R, C, (T*)out, ldo, \
+                       (T*)outT, ldt, sums)
+    GO(DSSVAE_ACT_NONE); GO(DSSVAE_ACT_RELU); GO(DSSVAE_ACT_GELU); GO(DSSVAE_ACT_SILU); GO(DSSVAE_ACT_TANH);
+#undef GO
     DSSVAE_CHECK_LAUNCH();
     return DSSVAE_OK;
 }
