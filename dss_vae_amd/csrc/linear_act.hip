@@ -68,16 +68,49 @@ __device__ __forceinline__ float act_slope(int act, float z) {
     }
 }
 
-// z is kept for backward in the activations' type: rounded, and held below the type's infinity (the slopes of a huge finite z
-// are exact there, those of an infinity would be 0 * inf)
-template <typename T> __device__ __forceinline__ float keep_z(float z) { return z; }
-template <> __device__ __forceinline__ float keep_z<f16_t>(float z) { return z > 65504.f ? 65504.f : z < -65504.f ? -65504.f : z; }
+// The pre-activation as backward needs it.  fp32: itself.  16-bit types: a 16-bit code of the slope's argument, evenly spaced over
+// the range in which the slope moves (beyond it the slope is 0 or 1 to 2e-6): |z| <= 8, silu 16, in steps of range / 32767,
+// i.e. off by at most 1.2e-4 (silu 2.4e-4).  z rounded to bf16 would be off by 4e-3 at |z| = 2 and z rounded to fp16 lost a
+// gradient's last bit; the code takes one instruction for two values.  relu keeps z > 0 only.  NaN has a code of its own.
+constexpr int16_t CODE_NAN = -32768;
+__device__ __forceinline__ float code_range(int act) { return act == DSSVAE_ACT_SILU ? 16.f : 8.f; }
+template <int ACT>
+__device__ __forceinline__ void encode8(const float (&z)[8], int16_t (&q)[8]) {
+    const float c = 1.f / code_range(ACT);
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        sum += z[j] + z[j + 1];
+        if constexpr (ACT == DSSVAE_ACT_RELU) {
+            q[j] = z[j] > 0.f;
+            q[j + 1] = z[j + 1] > 0.f;
+        } else {
+            typedef short s16x2 __attribute__((ext_vector_type(2)));
+            const s16x2 p = __builtin_bit_cast(s16x2, __builtin_amdgcn_cvt_pknorm_i16(z[j] * c, z[j + 1] * c));
+            q[j] = p.x;
+            q[j + 1] = p.y;
+        }
+    }
+    if (sum != sum) {  // a NaN (or infinities of both signs) among them
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = z[j] != z[j] ? CODE_NAN : q[j];
+    }
+}
+__device__ __forceinline__ float decode(int act, int16_t q) {
+    return q == CODE_NAN ? __builtin_nanf("") : (float)q * (code_range(act) / 32767.f);
+}
+// act'(z) from what forward kept
+template <typename T, int ACT>
+__device__ __forceinline__ float slope_kept(const T* z, int64_t i) {
+    if constexpr (sizeof(T) == 4) return act_slope(ACT, (float)z[i]);
+    else return act_slope(ACT, decode(ACT, reinterpret_cast<const int16_t*>(z)[i]));
+}
 
 // What happens to an accumulated element on its way out
 struct Epilogue {
     const void* bias; int bias_f32;   // [N] or NULL
     const void* res; int64_t ldr;     // [M, N] or NULL
-    void* z; int64_t ldz;             // pre-activation, or NULL
+    void* z; int64_t ldz;             // pre-activation as backward needs it, or NULL
     void* y; int64_t ldy;
     int act;
 };
@@ -103,24 +136,44 @@ __device__ __forceinline__ void finish8_act(const Epilogue& e, f32x8 a, f32x8 b,
     T* z = e.z ? reinterpret_cast<T*>(e.z) + m * e.ldz + n : nullptr;
     const T* r = e.res ? reinterpret_cast<const T*>(e.res) + m * e.ldr + n : nullptr;
     if (n + 8 <= N) {
-        GranU<T, 8> g, gz, gy;
+        GranU<T, 8> g, gy;
         if (r) g.load(r);
         else g.zero();
+        float zz[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float zz = a[j] + b[j];
-            gz.set(j, keep_z<T>(zz));
-            gy.set(j, act_f(ACT, zz) + g.get(j));
+            zz[j] = a[j] + b[j];
+            gy.set(j, act_f(ACT, zz[j]) + g.get(j));
         }
-        if (z) gz.store(z);
+        if (z) {
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) g.set(j, zz[j]);
+                g.store(z);
+            } else {
+                int16_t q[8];
+                encode8<ACT>(zz, q);
+                GranU<int16_t, 8> gq;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) gq.v[j] = q[j];
+                gq.store(reinterpret_cast<int16_t*>(z));
+            }
+        }
         gy.store(y);
     } else {
+        float zz[8];
+        int16_t q[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) zz[j] = a[j] + b[j];
+        if constexpr (sizeof(T) == 2) encode8<ACT>(zz, q);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             if (n + j >= N) continue;
-            const float zz = a[j] + b[j];
-            if (z) z[j] = (T)keep_z<T>(zz);
-            y[j] = (T)(act_f(ACT, zz) + (r ? (float)r[j] : 0.f));
+            if (z) {
+                if constexpr (sizeof(T) == 4) z[j] = zz[j];
+                else reinterpret_cast<int16_t*>(z)[j] = q[j];
+            }
+            y[j] = (T)(act_f(ACT, zz[j]) + (r ? (float)r[j] : 0.f));
         }
     }
 }
@@ -425,7 +478,7 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const T* __restrict__ 
 
 // One pass over a [R, C] matrix in 64 x 64 tiles (a block walks the row tiles blockIdx.y, + gridDim.y of one column tile):
 //   v = src                      (z NULL)
-//   v = src * act'(z)            else
+//   v = src * act'(z)            else (z as linear_tile_kernel's epilogue kept it)
 // out [R, ldo] (NULL: not wanted) gets v, columns C .. ldo zero; outT [C, ldt] (NULL) its transpose, columns R .. ldt zero;
 // sums [gridDim.y][C] (NULL) the block's column sums of the unrounded v.
 // A thread moves eight neighbouring elements of a row.  The tile keeps its eight (r, chunk) at chunk ^ (r / 8): the eight lanes
@@ -459,14 +512,21 @@ __global__ __launch_bounds__(256) void linear_turn_kernel(const T* __restrict__ 
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] = g.get(j);
                     if (z) {
-                        g.load(z + r * ldz + c);
+                        if constexpr (sizeof(T) == 4) {
+                            g.load(z + r * ldz + c);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) v[j] *= act_slope(ACT, g.get(j));
+                            for (int j = 0; j < 8; ++j) v[j] *= act_slope(ACT, g.get(j));
+                        } else {
+                            GranU<int16_t, 8> gq;
+                            gq.load(reinterpret_cast<const int16_t*>(z) + r * ldz + c);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) v[j] *= act_slope(ACT, decode(ACT, gq.v[j]));
+                        }
                     }
                 } else {
                     for (int j = 0; j < 8 && c + j < C; ++j) {
                         float u = (float)src[r * ld + c + j];
-                        if (z) u *= act_slope(ACT, (float)z[r * ldz + c + j]);
+                        if (z) u *= slope_kept<T, ACT>(z, r * ldz + c + j);
 #pragma unroll
                         for (int jj = 0; jj < 8; ++jj) v[jj] = jj == j ? u : v[jj];
                     }

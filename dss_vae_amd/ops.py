@@ -1,12 +1,20 @@
 """autograd wrappers over the C-ABI (include/dssvae_hip.h).  Every op launches hand-written HIP
 kernels on the current stream; torch is used for memory and tiny glue only.  No CPU path."""
 import ctypes as C
+import os
 
 import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import lib as L
+
+# Backward passes run on the thread that asks for them.  One process drives one GPU here: autograd's worker thread per device has
+# nothing to run beside, and the two hand-overs per backward call (the caller sleeps meanwhile) cost 50-70 us of a small step:
+# layer_norm forward and backward of 7936 x 300 fp32 125 -> 57 us, gated_scan of 256 x 90 x 300 114 -> 54 us.  The setting belongs to
+# the importing thread; DSSVAE_AUTOGRAD_THREADS=1 (or torch.autograd.set_multithreading_enabled(True) later) keeps torch's default.
+if os.environ.get("DSSVAE_AUTOGRAD_THREADS", "0") != "1":
+    torch.autograd.set_multithreading_enabled(False)
 
 _CUS = None
 
@@ -1797,22 +1805,37 @@ def adam_step(p, g, m, v, lr, beta1, beta2, eps, step, sumsq_t, max_norm, skip_f
 # C-ABI; everything runs on the current stream of the inputs' device, workspaces come from torch's allocator (a graph
 # being captured gets its own).
 # ----------------------------------------------------------------------------------------------
-class _Here(object):
-    """the inputs' device as the current one (a launch goes to the current device's stream); free when it already is"""
-    __slots__ = ("dev", "guard")
+_FN = {}  # entry points by name
 
-    def __init__(self, dev):
-        self.dev, self.guard = dev, None
 
-    def __enter__(self):
-        if self.dev.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.dev)
-            self.guard.__enter__()
+def _go(name, dev, args, span=None):
+    """one C-ABI call (its arguments without the stream) on the current stream of `dev`; span() -> the arguments of _Span.
+    Written for few Python operations: small calls are bound by the host."""
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(L.load(), name)
+    if dev.index != torch._C._cuda_getDevice():  # a launch goes to the current device
+        with torch.cuda.device(dev):
+            return _go(name, dev, args, span)
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    if PROFILE is None or span is None:
+        rc = fn(*args, stream)
+    else:
+        with _Span(*span()):
+            rc = fn(*args, stream)
+    if rc:
+        L.check(rc, name)
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _space(n, dev):
+    """workspace of n bytes (None where a call needs none; a negative size is an error code)"""
+    if n < 0:
+        L.check(n, "workspace size")
+    return None if n == 0 else torch.empty(n, device=dev, dtype=torch.uint8)
 
 
 def _typed(what, t):
@@ -1826,7 +1849,7 @@ def _typed(what, t):
 
 def _expect(what, name, t, shape, dtypes, device):
     """an argument's shape, type and device, or a RuntimeError that names it"""
-    if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes or t.device != device:
+    if t.shape != shape or t.dtype not in dtypes or t.device != device:
         raise RuntimeError("%s: %s must be %s of %s on %s, got %s of %s on %s" % (
             what, name, list(shape), " or ".join(str(d) for d in dtypes), device, list(t.shape), t.dtype, t.device))
     return t
@@ -1841,18 +1864,25 @@ def _matrix(t):
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _contig(t):
+    return None if t is None else t.contiguous()
 
 
 def _layer_norm_fwd(x2, ldx, code, w, b, eps, stats):
-    y = torch.empty(x2.shape, device=x2.device, dtype=x2.dtype)
     R, D = x2.shape
+    y = torch.empty(R, D, device=x2.device, dtype=x2.dtype)
     p = w if w is not None else b
-    with _Here(x2.device), _Span("layer_norm_fwd_kernel", 8.0 * R * D, 2.0 * R * D * x2.element_size(),
-                                 detail="R=%d D=%d" % (R, D)):
-        L.check(L.load().dssvae_layer_norm_fwd(L.ptr(x2), ldx, code, L.ptr(w), L.ptr(b),
-                                               int(p is not None and p.dtype == torch.float32), R, D, eps, L.ptr(y), D,
-                                               L.ptr(stats), L.stream()), "dssvae_layer_norm_fwd")
+    _go("dssvae_layer_norm_fwd", x2.device,
+        (x2.data_ptr(), ldx, code, _p(w), _p(b), int(p is not None and p.dtype == torch.float32), R, D, eps, y.data_ptr(), D,
+         _p(stats)),
+        lambda: ("layer_norm_fwd_kernel", 8.0 * R * D, 2.0 * R * D * x2.element_size(), 0, "R=%d D=%d" % (R, D)))
     return y
 
 
@@ -1861,9 +1891,8 @@ class _LayerNormFn(Function):
     def forward(ctx, x, w, b, eps, code):
         ctx.set_materialize_grads(False)
         x2, ldx = _matrix(x.reshape(-1, x.size(-1)))
-        wc, bc = (None if p is None else p.contiguous() for p in (w, b))
         stats = torch.empty(x2.size(0), 2, device=x.device, dtype=torch.float32)
-        y = _layer_norm_fwd(x2, ldx, code, wc, bc, eps, stats)
+        y = _layer_norm_fwd(x2, ldx, code, _contig(w), _contig(b), eps, stats)
         ctx.save_for_backward(x2, w, stats)
         ctx.bias_ref, ctx.code, ctx.xshape = b, code, x.shape
         return y.view(x.shape)
@@ -1877,24 +1906,22 @@ class _LayerNormFn(Function):
         b = ctx.bias_ref
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         R, D = x2.shape
+        dev, es = x2.device, x2.element_size()
         x2, ldx = _matrix(x2)
         dy2, lddy = _matrix(dy.reshape(-1, D))
-        dev, lib = x2.device, L.load()
-        wc = None if w is None else w.contiguous()
-        p = w if w is not None else b
+        wc, p = _contig(w), (w if w is not None else b)
         dx = torch.empty(R, D, device=dev, dtype=x2.dtype) if need_x else None
-        dw, db = (None if not need else _claim(t) for need, t in ((need_w, w), (need_b, b)))
-        dw = torch.empty(D, device=dev, dtype=w.dtype) if need_w and dw is None else dw
-        db = torch.empty(D, device=dev, dtype=b.dtype) if need_b and db is None else db
-        with _Here(dev), _Span("layer_norm_bwd_kernel", 12.0 * R * D, 3.0 * R * D * x2.element_size(),
-                               detail="R=%d D=%d" % (R, D)):
-            ws = None
-            if need_w or need_b:
-                ws = torch.empty(lib.dssvae_layer_norm_bwd_workspace_bytes(R, D), device=dev, dtype=torch.uint8)
-            L.check(lib.dssvae_layer_norm_bwd(L.ptr(x2), ldx, ctx.code, L.ptr(dy2), lddy, L.ptr(wc),
-                                              int(p is not None and p.dtype == torch.float32), L.ptr(stats), R, D,
-                                              L.ptr(dx), D, L.ptr(dw), L.ptr(db), L.ptr(ws),
-                                              0 if ws is None else ws.numel(), L.stream()), "dssvae_layer_norm_bwd")
+        dw, db = _claim(w, need_w), _claim(b, need_b)
+        if need_w and dw is None:
+            dw = torch.empty(D, device=dev, dtype=w.dtype)
+        if need_b and db is None:
+            db = torch.empty(D, device=dev, dtype=b.dtype)
+        n = L.load().dssvae_layer_norm_bwd_workspace_bytes(R, D) if need_w or need_b else 0
+        ws = _space(n, dev)
+        _go("dssvae_layer_norm_bwd", dev,
+            (x2.data_ptr(), ldx, ctx.code, dy2.data_ptr(), lddy, _p(wc), int(p is not None and p.dtype == torch.float32),
+             stats.data_ptr(), R, D, _p(dx), D, _p(dw), _p(db), _p(ws), n),
+            lambda: ("layer_norm_bwd_kernel", 12.0 * R * D, 3.0 * R * D * es, 0, "R=%d D=%d" % (R, D)))
         return None if dx is None else dx.view(ctx.xshape), dw, db, None, None
 
 
@@ -1915,8 +1942,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     if _wants_grad(x, weight, bias):
         return _LayerNormFn.apply(x, weight, bias, float(eps), code)
     x2, ldx = _matrix(x.reshape(-1, D))
-    w, b = (None if p is None else p.contiguous() for p in (weight, bias))
-    return _layer_norm_fwd(x2, ldx, code, w, b, float(eps), None).view(x.shape)
+    return _layer_norm_fwd(x2, ldx, code, _contig(weight), _contig(bias), float(eps), None).view(x.shape)
 
 
 def _sequence(t):
@@ -1927,30 +1953,31 @@ def _sequence(t):
     return t
 
 
-def _scan_bytes(lib, B, T, H, code, dev):
-    n = lib.dssvae_gated_scan_workspace_bytes(B, T, H, code)
-    return (None, 0) if n <= 0 else (torch.empty(n, device=dev, dtype=torch.uint8), n)
+def _gated_step(x, ldx, code, h, tanh, out, h_out):
+    B, H = x.size(0), x.size(-1) // 2
+    _go("dssvae_gated_step", x.device, (x.data_ptr(), ldx, code, _p(h), tanh, B, H, out.data_ptr(), H, h_out.data_ptr()),
+        lambda: ("gated_step_kernel", 12.0 * B * H, B * H * (3.0 * x.element_size() + 8.0)))
 
 
 def _gated_scan_fwd(x, h0, lengths, reverse, tanh, code, keep):
     """-> out, h_last, checkpoints (None unless `keep`)"""
-    B, T, H = x.size(0), x.size(1), x.size(2) // 2
-    dev, lib = x.device, L.load()
+    B, T, H2 = x.shape
+    H, dev, lib = H2 // 2, x.device, L.load()
     out = torch.empty(B, T, H, device=dev, dtype=x.dtype)
     h_last = torch.empty(B, H, device=dev, dtype=torch.float32)
     ckpt = torch.empty(B, lib.dssvae_gated_scan_chunks(T), H, device=dev, dtype=torch.float32) if keep else None
-    with _Here(dev), _Span("gated_scan_fwd_kernel", 12.0 * B * T * H, 3.0 * B * T * H * x.element_size(), T,
-                           detail="B%dT%dH%d" % (B, T, H)):
-        if T == 0:
-            h_last.zero_() if h0 is None else h_last.copy_(h0)
-        elif T == 1 and lengths is None and not keep:
-            L.check(lib.dssvae_gated_step(L.ptr(x), x.stride(0), code, L.ptr(h0), tanh, B, H, L.ptr(out), H, L.ptr(h_last),
-                                          L.stream()), "dssvae_gated_step")
-        else:
-            ws, n = _scan_bytes(lib, B, T, H, code, dev)
-            L.check(lib.dssvae_gated_scan_fwd(L.ptr(x), x.stride(0), x.stride(1), code, L.ptr(h0), L.ptr(lengths), reverse,
-                                              tanh, B, T, H, L.ptr(out), T * H, H, L.ptr(h_last), L.ptr(ckpt), L.ptr(ws), n,
-                                              L.stream()), "dssvae_gated_scan_fwd")
+    if T == 0:
+        h_last.zero_() if h0 is None else h_last.copy_(h0)
+    elif T == 1 and lengths is None and not keep:
+        _gated_step(x, x.stride(0), code, h0, tanh, out, h_last)
+    else:
+        n = lib.dssvae_gated_scan_workspace_bytes(B, T, H, code)
+        ws = _space(n, dev)
+        _go("dssvae_gated_scan_fwd", dev,
+            (x.data_ptr(), x.stride(0), x.stride(1), code, _p(h0), _p(lengths), reverse, tanh, B, T, H, out.data_ptr(), T * H,
+             H, h_last.data_ptr(), _p(ckpt), _p(ws), n),
+            lambda: ("gated_scan_fwd_kernel", 12.0 * B * T * H, 3.0 * B * T * H * x.element_size(), T,
+                     "B%dT%dH%d" % (B, T, H)))
     return out, h_last, ckpt
 
 
@@ -1959,8 +1986,7 @@ class _GatedScanFn(Function):
     def forward(ctx, x, h0, lengths, reverse, tanh, code):
         ctx.set_materialize_grads(False)
         xs = _sequence(x)
-        h0 = None if h0 is None else h0.contiguous()
-        out, h_last, ckpt = _gated_scan_fwd(xs, h0, lengths, reverse, tanh, code, True)
+        out, h_last, ckpt = _gated_scan_fwd(xs, _contig(h0), lengths, reverse, tanh, code, True)
         ctx.save_for_backward(xs, lengths, ckpt)
         ctx.meta = (reverse, tanh, code)
         return out, h_last
@@ -1972,25 +1998,25 @@ class _GatedScanFn(Function):
             return (None,) * 6
         x, lengths, ckpt = ctx.saved_tensors
         reverse, tanh, code = ctx.meta
-        B, T, H = x.size(0), x.size(1), x.size(2) // 2
-        dev, lib = x.device, L.load()
+        B, T, H2 = x.shape
+        H, dev, lib = H2 // 2, x.device, L.load()
         x = _sequence(x)
         dout = None if dout is None else _sequence(dout)
-        dh = None if dh is None else dh.contiguous()
-        dx = torch.empty(B, T, 2 * H, device=dev, dtype=x.dtype)
+        dh = _contig(dh)
+        dx = torch.empty(B, T, H2, device=dev, dtype=x.dtype)
         dh0 = torch.empty(B, H, device=dev, dtype=torch.float32) if ctx.needs_input_grad[1] else None
-        with _Here(dev), _Span("gated_scan_bwd_kernel", 18.0 * B * T * H, 5.0 * B * T * H * x.element_size(), T,
-                               detail="B%dT%dH%d" % (B, T, H)):
-            if T == 0:
-                if dh0 is not None:
-                    dh0.zero_() if dh is None else dh0.copy_(dh)
-            else:
-                ws, n = _scan_bytes(lib, B, T, H, code, dev)
-                ob, ot = (0, 0) if dout is None else (dout.stride(0), dout.stride(1))
-                L.check(lib.dssvae_gated_scan_bwd(L.ptr(x), x.stride(0), x.stride(1), code, L.ptr(lengths), reverse, tanh,
-                                                  L.ptr(ckpt), L.ptr(dout), ob, ot, L.ptr(dh), B, T, H, L.ptr(dx),
-                                                  T * 2 * H, 2 * H, L.ptr(dh0), L.ptr(ws), n, L.stream()),
-                        "dssvae_gated_scan_bwd")
+        if T == 0:
+            if dh0 is not None:
+                dh0.zero_() if dh is None else dh0.copy_(dh)
+        else:
+            n = lib.dssvae_gated_scan_workspace_bytes(B, T, H, code)
+            ws = _space(n, dev)
+            ob, ot = (0, 0) if dout is None else (dout.stride(0), dout.stride(1))
+            _go("dssvae_gated_scan_bwd", dev,
+                (x.data_ptr(), x.stride(0), x.stride(1), code, _p(lengths), reverse, tanh, ckpt.data_ptr(), _p(dout), ob, ot,
+                 _p(dh), B, T, H, dx.data_ptr(), T * H2, H2, _p(dh0), _p(ws), n),
+                lambda: ("gated_scan_bwd_kernel", 18.0 * B * T * H, 5.0 * B * T * H * x.element_size(), T,
+                         "B%dT%dH%d" % (B, T, H)))
         return dx if ctx.needs_input_grad[0] else None, dh0, None, None, None, None
 
 
@@ -2021,8 +2047,7 @@ def gated_scan(xproj, h0=None, lengths=None, reverse=False, candidate="tanh"):
         lengths = _expect("gated_scan", "lengths", lengths, (B,), (torch.int32,), xproj.device).contiguous()
     if _wants_grad(xproj, h0):
         return _GatedScanFn.apply(xproj, h0, lengths, int(bool(reverse)), tanh, code)
-    h0 = None if h0 is None else h0.contiguous()
-    return _gated_scan_fwd(_sequence(xproj), h0, lengths, int(bool(reverse)), tanh, code, False)[:2]
+    return _gated_scan_fwd(_sequence(xproj), _contig(h0), lengths, int(bool(reverse)), tanh, code, False)[:2]
 
 
 def gated_step(xproj, h=None, candidate="tanh", h_out=None):
@@ -2046,12 +2071,9 @@ def gated_step(xproj, h=None, candidate="tanh", h_out=None):
         out, hn = gated_scan(xproj.unsqueeze(1), h, None, False, candidate)
         return out.squeeze(1), hn
     x, ldx = _matrix(xproj)
-    h = None if h is None else h.contiguous()
     out = torch.empty(B, H, device=x.device, dtype=x.dtype)
     hn = torch.empty(B, H, device=x.device, dtype=torch.float32) if h_out is None else h_out
-    with _Here(x.device), _Span("gated_step_kernel", 12.0 * B * H, B * H * (3.0 * x.element_size() + 8.0)):
-        L.check(L.load().dssvae_gated_step(L.ptr(x), ldx, code, L.ptr(h), tanh, B, H, L.ptr(out), H, L.ptr(hn), L.stream()),
-                "dssvae_gated_step")
+    _gated_step(x, ldx, code, _contig(h), tanh, out, hn)
     return out, hn
 
 
@@ -2069,11 +2091,12 @@ def _distill(z, ldz, code, ids, teacher, tau, weight, want_grad):
     rows = torch.empty(N, device=z.device, dtype=torch.float32)
     total = torch.empty((), device=z.device, dtype=torch.float32)
     dz = _like_rows(z, ldz) if want_grad else None
-    with _Here(z.device), _Span("distill_kernel", 8.0 * N * V, (2.0 if want_grad else 1.0) * N * V * z.element_size(),
-                                detail="N=%d V=%d k=%d" % (N, V, ids.size(1))):
-        L.check(L.load().dssvae_distill(L.ptr(z), ldz, code, N, V, L.ptr(ids), L.ptr(teacher), ids.size(1), tau,
-                                        L.ptr(weight), 1.0 / max(N, 1), L.ptr(dz), 0 if dz is None else dz.stride(0),
-                                        L.ptr(rows), L.ptr(total), L.stream()), "dssvae_distill")
+    k = ids.size(1)
+    _go("dssvae_distill", z.device,
+        (z.data_ptr(), ldz, code, N, V, ids.data_ptr(), teacher.data_ptr(), k, tau, _p(weight), 1.0 / max(N, 1), _p(dz),
+         0 if dz is None else dz.stride(0), rows.data_ptr(), total.data_ptr()),
+        lambda: ("distill_kernel", 8.0 * N * V, (2.0 if want_grad else 1.0) * N * V * z.element_size(), 0,
+                 "N=%d V=%d k=%d" % (N, V, k)))
     return total, rows, dz
 
 
@@ -2102,9 +2125,7 @@ class _DistillFn(Function):
             raise RuntimeError("distill_loss keeps its gradient for ONE backward pass (retain_graph / a second backward "
                                "is not supported)")
         if dz.size(0):
-            with _Here(dz.device):
-                L.check(L.load().dssvae_scale_rows(L.ptr(dz), dz.stride(0), ctx.code, dz.size(0), dz.size(1),
-                                                   L.ptr(g.contiguous()), L.stream()), "dssvae_scale_rows")
+            _go("dssvae_scale_rows", dz.device, (dz.data_ptr(), dz.stride(0), ctx.code, dz.size(0), dz.size(1), g.data_ptr()))
         return dz.view(ctx.shape) if dz.is_contiguous() else dz.unflatten(0, ctx.shape[:-1]), None, None, None, None, None
 
 
@@ -2143,19 +2164,21 @@ def distill_loss(logits, ids, teacher, temperature=1.0, weight=None):
 
 
 def _linear_act_fwd(x2, ldx, w, ldw, b, act, r, code, keep_z):
-    """-> y, z (the pre-activation in x's type; None unless `keep_z`)"""
+    """-> y, z (the pre-activation as backward needs it; None unless `keep_z`)"""
     M, K = x2.shape
-    N, dev, lib = w.size(0), x2.device, L.load()
+    N, dev = w.size(0), x2.device
     y = torch.empty(M, N, device=dev, dtype=x2.dtype)
-    z = torch.empty(M, N, device=dev, dtype=x2.dtype) if keep_z else None
+    # (fp32: the values; 16 bits: codes of the kernel's own)
+    z = torch.empty(M, N, device=dev, dtype=torch.float32 if code == 0 else torch.int16) if keep_z else None
     r, ldr = (None, 0) if r is None else _matrix(r)
-    with _Here(dev), _Span("linear_tile_kernel" if code else "gemm_store_kernel", 2.0 * M * N * K,
-                           (M * K + N * K + M * N) * float(x2.element_size()), detail="M=%d N=%d K=%d" % (M, N, K)):
-        n = lib.dssvae_linear_act_fwd_workspace_bytes(L.ptr(x2), ldx, L.ptr(w), ldw, code, M, N, K)
-        ws = torch.empty(n, device=dev, dtype=torch.uint8) if n > 0 else None
-        L.check(lib.dssvae_linear_act_fwd(L.ptr(x2), ldx, L.ptr(w), ldw, L.ptr(b), int(b is not None and b.dtype == torch.float32),
-                                          L.ptr(r), ldr, code, act, M, N, K, L.ptr(y), N, L.ptr(z), N, L.ptr(ws), max(n, 0),
-                                          L.stream()), "dssvae_linear_act_fwd")
+    xp, wp = x2.data_ptr(), w.data_ptr()
+    n = L.load().dssvae_linear_act_fwd_workspace_bytes(xp, ldx, wp, ldw, code, M, N, K)
+    ws = _space(n, dev)
+    _go("dssvae_linear_act_fwd", dev,
+        (xp, ldx, wp, ldw, _p(b), int(b is not None and b.dtype == torch.float32), _p(r), ldr, code, act, M, N, K, y.data_ptr(),
+         N, _p(z), N, _p(ws), n),
+        lambda: ("linear_tile_kernel", 2.0 * M * N * K, (M * K + N * K + M * N) * float(x2.element_size()), 0,
+                 "M=%d N=%d K=%d" % (M, N, K)))
     return y, z
 
 
@@ -2166,7 +2189,7 @@ class _LinearActFn(Function):
         N = w.size(0)
         x2, ldx = _matrix(x.reshape(-1, x.size(-1)))
         wc, ldw = _matrix(w)
-        bc = None if b is None else b.contiguous()
+        bc = _contig(b)
         keep = act != 0 and any(ctx.needs_input_grad[:3])
         y, z = _linear_act_fwd(x2, ldx, wc, ldw, bc, act, None if residual is None else residual.reshape(-1, N), code, keep)
         ctx.save_for_backward(x2, w, z)
@@ -2183,24 +2206,25 @@ class _LinearActFn(Function):
         dx = dw = db = None
         if need_x or need_w or need_b:
             M, K = x2.shape
-            N, dev, lib = w.size(0), x2.device, L.load()
+            N, dev, es, code, act = w.size(0), x2.device, x2.element_size(), ctx.code, ctx.act
             x2, ldx = _matrix(x2)
             wc, ldw = _matrix(w)
             dy2, lddy = _matrix(dy.reshape(-1, N))
             b = ctx.bias_ref
             dx = torch.empty(M, K, device=dev, dtype=x2.dtype) if need_x else None
-            dw, db = (None if not need else _claim(t) for need, t in ((need_w, w), (need_b, b)))
-            dw = torch.empty(N, K, device=dev, dtype=w.dtype) if need_w and dw is None else dw
-            db = torch.empty(N, device=dev, dtype=b.dtype) if need_b and db is None else db
-            with _Here(dev), _Span("linear_act_bwd", 2.0 * M * N * K * (int(need_x) + int(need_w)),
-                                   4.0 * M * N * x2.element_size(), detail="M=%d N=%d K=%d" % (M, N, K)):
-                n = lib.dssvae_linear_act_bwd_workspace_bytes(L.ptr(dy2), lddy, int(z is not None), ctx.code, M, N, K, int(need_x and M > 0),
-                                                              int(need_w), int(need_b))
-                ws = torch.empty(n, device=dev, dtype=torch.uint8) if n > 0 else None
-                L.check(lib.dssvae_linear_act_bwd(L.ptr(dy2), lddy, L.ptr(z), N, L.ptr(x2), ldx, L.ptr(wc), ldw, ctx.code, ctx.act, M,
-                                                  N, K, L.ptr(dx), K, L.ptr(dw), K, L.ptr(db),
-                                                  int(db is not None and db.dtype == torch.float32), L.ptr(ws), max(n, 0),
-                                                  L.stream()), "dssvae_linear_act_bwd")
+            dw, db = _claim(w, need_w), _claim(b, need_b)
+            if need_w and dw is None:
+                dw = torch.empty(N, K, device=dev, dtype=w.dtype)
+            if need_b and db is None:
+                db = torch.empty(N, device=dev, dtype=b.dtype)
+            n = L.load().dssvae_linear_act_bwd_workspace_bytes(dy2.data_ptr(), lddy, int(z is not None), code, M, N, K,
+                                                               int(need_x and M > 0), int(need_w), int(need_b))
+            ws = _space(n, dev)
+            _go("dssvae_linear_act_bwd", dev,
+                (dy2.data_ptr(), lddy, _p(z), N, x2.data_ptr(), ldx, wc.data_ptr(), ldw, code, act, M, N, K, _p(dx), K, _p(dw), K,
+                 _p(db), int(db is not None and db.dtype == torch.float32), _p(ws), n),
+                lambda: ("linear_act_bwd", 2.0 * M * N * K * (int(need_x) + int(need_w)), 4.0 * M * N * es, 0,
+                         "M=%d N=%d K=%d" % (M, N, K)))
             dx = None if dx is None else dx.view(ctx.xshape)
         return dx, dw, db, dy if need_r else None, None, None
 
@@ -2208,7 +2232,8 @@ class _LinearActFn(Function):
 def linear_act(x, w, b=None, act="none", residual=None):
     """act(x w^T + b) + residual: x [..., K], w [N, K] and residual [..., N] of one type (float32, bfloat16, float16),
     b [N] of that type or float32; act "none", "relu", "gelu" (the exact form), "silu" or "tanh".  Products accumulate in
-    fp32 and every output is rounded once; for training in 16 bits the pre-activation is kept in x's type."""
+    fp32 in a fixed order and every output is rounded once.  For training in 16 bits the slope's argument is kept in 16 bits
+    (evenly spaced, finer than either type where slopes move) and the products of backward take dy act'(z) rounded to the type."""
     code = _typed("linear_act", x)
     if act not in L.ACTIVATIONS:
         raise RuntimeError("linear_act: act must be one of %s, got %r" % (sorted(L.ACTIVATIONS), act))
@@ -2226,5 +2251,5 @@ def linear_act(x, w, b=None, act="none", residual=None):
     x2, ldx = _matrix(x.reshape(-1, K))
     w2, ldw = _matrix(w)
     r = None if residual is None else residual.reshape(-1, N)
-    y, _ = _linear_act_fwd(x2, ldx, w2, ldw, None if b is None else b.contiguous(), a, r, code, False)
+    y, _ = _linear_act_fwd(x2, ldx, w2, ldw, _contig(b), a, r, code, False)
     return y.view(*x.shape[:-1], N)

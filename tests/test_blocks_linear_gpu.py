@@ -32,8 +32,9 @@ def reference(x, w, b, res, name, dy):
     z: a sum of K products and the bias in fp32: at most K + 1 roundings of partial sums; random signs and blocked order keep
     it far below, 3 sqrt(K) + 8 units of sum |x||w| hold for every order of these random inputs.  The activations are Lipschitz
     with a constant below 1.13 and add at most 8 units of max(1, |z|) of their own (exp2 / rcp / erf).
-    16-bit types: backward sees z rounded to the type (the slope moves by at most u max|act''| |z|, max|act''| <= 0.8 (gelu, at
-    0), and across 0 for relu not at all: the sign is kept) and dz rounded to the type: each dz is off by u (1 + 0.8 |z|) |dy|."""
+    16-bit types: backward sees a code of z, off by half of range / 32767 (8, silu 16; beyond the range the slope is within
+    2e-6 of its limit), which moves the slope by at most max|act''| <= 0.8 (gelu, at 0) times that, and dz rounded to the
+    type: off by u |dz|.  relu keeps the sign."""
     u = 0.0 if x.dtype == torch.float32 else half_step(x.dtype)
     x, w, dy = x.double(), w.double(), dy.double()
     K, M, N = x.size(1), x.size(0), w.size(0)
@@ -48,10 +49,11 @@ def reference(x, w, b, res, name, dy):
     out, err = {"y": y}, {"y": yerr}
     dz = dy * slope
     # what the type's roundings and the fp32 error of z do to dz (relu: z close to 0 may fall on either side)
-    zoff = U32 * zerr + u * z.abs()
+    step = 0.0 if u == 0.0 or name in ("none", "relu") else (16.0 if name == "silu" else 8.0) / 32767
+    zoff = U32 * zerr + step / 2
     flip = ((z.abs() <= U32 * zerr) & (z != 0)).double() * dy.abs() if name == "relu" else 0.0
     curve = 0.0 if name in ("none", "relu") else 0.8
-    dzerr = (flip + dy.abs() * (curve * zoff + 16 * U32) + u * dz.abs()) / U32
+    dzerr = (flip + dy.abs() * (curve * zoff + 16 * U32 + (2e-6 if step else 0.0)) + u * dz.abs()) / U32
     out["dx"], err["dx"] = dz @ w, dzerr @ w.abs() + (3 * math.sqrt(N) + 8) * (dz.abs() @ w.abs())
     out["dw"], err["dw"] = dz.t() @ x, dzerr.t() @ x.abs() + (3 * math.sqrt(M) + 8) * (dz.abs().t() @ x.abs())
     out["db"], err["db"] = dz.sum(0), dzerr.sum(0) + (3 * math.sqrt(M) + 8) * dz.abs().sum(0)
