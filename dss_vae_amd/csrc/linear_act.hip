@@ -476,27 +476,44 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(const T* __restrict__ 
         for (int64_t c = threadIdx.x; c < ldd; c += 256) dst[r * ldd + c] = c < C ? src[r * ld + c] : (T)0.f;
 }
 
-// One pass over a [R, C] matrix in 64 x 64 tiles (a block walks the row tiles blockIdx.y, + gridDim.y of one column tile):
+// One pass over a [R, C] matrix in 64 x 64 tiles (a block walks the row tiles first, + stride, .. of one column tile):
 //   v = src                      (z NULL)
 //   v = src * act'(z)            else (z as linear_tile_kernel's epilogue kept it)
 // out [R, ldo] (NULL: not wanted) gets v, columns C .. ldo zero; outT [C, ldt] (NULL) its transpose, columns R .. ldt zero;
-// sums [gridDim.y][C] (NULL) the block's column sums of the unrounded v.
+// sums [stride][C] (NULL) the block's column sums of the unrounded v.
 // A thread moves eight neighbouring elements of a row.  The tile keeps its eight (r, chunk) at chunk ^ (r / 8): the eight lanes
 // that gather one column's 64 rows then read eight different banks.
+// A launch makes several such passes (dy, w and x of one backward call): blocks begin[i] .. begin[i + 1] belong to the i-th.
+struct Turn {
+    const void* src; int64_t ld;
+    const void* z; int64_t ldz;
+    int64_t R, C;
+    void* out; int64_t ldo;
+    void* outT; int64_t ldt;
+    float* sums;
+    int stride;  // blocks along the rows
+};
+struct Turns { Turn job[3]; int begin[4]; };
+
 template <typename T, int ACT>
-__global__ __launch_bounds__(256) void linear_turn_kernel(const T* __restrict__ src, int64_t ld, const T* __restrict__ z,
-                                                          int64_t ldz, int64_t R, int64_t C, T* __restrict__ out,
-                                                          int64_t ldo, T* __restrict__ outT, int64_t ldt,
-                                                          float* __restrict__ sums) {
+__global__ __launch_bounds__(256) void linear_turn_kernel(Turns jobs) {
     __shared__ __attribute__((aligned(16))) T tile[64 * 64];
     __shared__ float red[32][64];
-    const int64_t c0 = (int64_t)blockIdx.x * 64;
+    int which = 0;
+    while ((int)blockIdx.x >= jobs.begin[which + 1]) ++which;
+    const Turn& t = jobs.job[which];
+    const T *__restrict__ src = (const T*)t.src, *__restrict__ z = (const T*)t.z;
+    T *__restrict__ out = (T*)t.out, *__restrict__ outT = (T*)t.outT;
+    float* __restrict__ sums = t.sums;
+    const int64_t ld = t.ld, ldz = t.ldz, R = t.R, C = t.C, ldo = t.ldo, ldt = t.ldt;
+    const int block = (int)blockIdx.x - jobs.begin[which], stride = t.stride, first = block % stride;
+    const int64_t c0 = (int64_t)(block / stride) * 64;
     const int ch = threadIdx.x & 7, rr = threadIdx.x >> 3;
     const int64_t rtiles = (R + 63) / 64, c = c0 + ch * 8;
     float sum[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum[j] = 0.f;
-    for (int64_t rt = blockIdx.y; rt < rtiles; rt += gridDim.y) {
+    for (int64_t rt = first; rt < rtiles; rt += stride) {
         const int64_t r0 = rt * 64;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -579,7 +596,7 @@ __global__ __launch_bounds__(256) void linear_turn_kernel(const T* __restrict__ 
     if (threadIdx.x < 64 && c0 + threadIdx.x < C) {
         float s = 0.f;
         for (int i = 0; i < 32; ++i) s += red[i][threadIdx.x];
-        sums[(int64_t)blockIdx.y * C + c0 + threadIdx.x] = s;
+        sums[(int64_t)first * C + c0 + threadIdx.x] = s;
     }
 }
 
@@ -695,16 +712,27 @@ int pack(const void* src, int64_t ld, int64_t R, int64_t C, void* dst, int64_t l
 // blocks along the rows of linear_turn_kernel: enough to fill the chip
 inline int64_t turn_rows(int64_t R, int64_t C) {
     const int64_t ct = (C + 63) / 64, rt = (R + 63) / 64, want = (8 * (int64_t)device_cus() + ct - 1) / ct;
-    return rt < 1 ? 1 : rt < want ? rt : want;
+    return rt < 1 ? 1 : rt < want ? rt : want;  // (at most 8 blocks a CU and one per column tile: begin[] stays small)
 }
+struct TurnList {
+    Turns t{};
+    int n = 0;
+    void add(const void* src, int64_t ld, const void* z, int64_t ldz, int64_t R, int64_t C, void* out, int64_t ldo, void* outT, int64_t ldt,
+             float* sums) {
+        const int64_t rows = turn_rows(R, C);
+        t.job[n] = Turn{src, ld, z, ldz, R, C, out, ldo, outT, ldt, sums, (int)rows};
+        t.begin[n + 1] = t.begin[n] + (int)(rows * ((C + 63) / 64));
+        ++n;
+    }
+};
 template <typename T>
-int turn(const void* src, int64_t ld, const void* z, int64_t ldz, int act, int64_t R, int64_t C, void* out, int64_t ldo, void* outT,
-         int64_t ldt, float* sums, hipStream_t st) {
-    const dim3 grid((unsigned)((C + 63) / 64), (unsigned)turn_rows(R, C));
+int turn(const TurnList& l, int act, hipStream_t st) {
+    if (l.n == 0) return DSSVAE_OK;
+    Turns t = l.t;
+    for (int i = l.n; i < 3; ++i) t.begin[i + 1] = t.begin[l.n];
+    const dim3 grid((unsigned)t.begin[l.n]);
 #define GO(ACT)                                                                                                        \
-    if (act == ACT)                                                                                                    \
-    hipLaunchKernelGGL((linear_turn_kernel<T, ACT>), grid, dim3(256), 0, st, (const T*)src, ld, (const T*)z, ldz, R, C, (T*)out, ldo, \
-                       (T*)outT, ldt, sums)
+    if (act == ACT) hipLaunchKernelGGL((linear_turn_kernel<T, ACT>), grid, dim3(256), 0, st, t)
     GO(DSSVAE_ACT_NONE); GO(DSSVAE_ACT_RELU); GO(DSSVAE_ACT_GELU); GO(DSSVAE_ACT_SILU); GO(DSSVAE_ACT_TANH);
 #undef GO
     DSSVAE_CHECK_LAUNCH();
@@ -764,35 +792,29 @@ int backward(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
     if (copy) { dzc = sp.take(M * ldn * es); dz = dzc; lddz = ldn; }
     if (a.dw) dzt = sp.take(N * ldm * es);
     float* sums = a.db ? (float*)sp.take(turn_rows(M, N) * N * 4) : nullptr;
-    if (copy || a.dw || a.db) {
-        if (!dry) {
-            if ((rc = turn<T>(a.dy, a.lddy, a.z, a.ldz, a.act, M, N, dzc, ldn, dzt, ldm, sums, st))) return rc;
-            if (a.db) {
-                hipLaunchKernelGGL((linear_db_kernel<T>), dim3((unsigned)((N + 31) / 32)), dim3(1024), 0, st, sums,
-                                   (int)turn_rows(M, N), N, a.db, a.db_f32);
-                DSSVAE_CHECK_LAUNCH();
-            }
-        }
+    void* wt = a.dx ? sp.take(K * ldn * es) : nullptr;
+    void* xt = a.dw ? sp.take(K * ldm * es) : nullptr;
+    void* part_x = a.dx ? sp.take(part_bytes<T>(M, K, ldn)) : nullptr;
+    void* part_w = a.dw ? sp.take(part_bytes<T>(N, K, ldm)) : nullptr;
+    if (dry) return rc;
+    TurnList l;
+    if (copy || a.dw || a.db) l.add(a.dy, a.lddy, a.z, a.ldz, M, N, dzc, ldn, dzt, ldm, sums);
+    if (a.dx) l.add(a.w, a.ldw, nullptr, 0, N, K, nullptr, 0, wt, ldn, nullptr);
+    if (a.dw) l.add(a.x, a.ldx, nullptr, 0, M, K, nullptr, 0, xt, ldm, nullptr);
+    if ((rc = turn<T>(l, a.act, st))) return rc;
+    if (a.db) {
+        hipLaunchKernelGGL((linear_db_kernel<T>), dim3((unsigned)((N + 31) / 32)), dim3(1024), 0, st, sums, (int)turn_rows(M, N), N, a.db,
+                           a.db_f32);
+        DSSVAE_CHECK_LAUNCH();
     }
+    Epilogue e{};
     if (a.dx) {
-        void* wt = sp.take(K * ldn * es);
-        void* part = sp.take(part_bytes<T>(M, K, ldn));
-        if (!dry) {
-            if ((rc = turn<T>(a.w, a.ldw, nullptr, 0, 0, N, K, nullptr, 0, wt, ldn, nullptr, st))) return rc;
-            Epilogue e{};
-            e.y = a.dx; e.ldy = a.lddx;
-            if ((rc = product<T>(dz, lddz, wt, ldn, M, K, ldn, e, part, st))) return rc;
-        }
+        e.y = a.dx; e.ldy = a.lddx;
+        if ((rc = product<T>(dz, lddz, wt, ldn, M, K, ldn, e, part_x, st))) return rc;
     }
     if (a.dw) {
-        void* xt = sp.take(K * ldm * es);
-        void* part = sp.take(part_bytes<T>(N, K, ldm));
-        if (!dry) {
-            if ((rc = turn<T>(a.x, a.ldx, nullptr, 0, 0, M, K, nullptr, 0, xt, ldm, nullptr, st))) return rc;
-            Epilogue e{};
-            e.y = a.dw; e.ldy = a.lddw;
-            if ((rc = product<T>(dzt, ldm, xt, ldm, N, K, ldm, e, part, st))) return rc;
-        }
+        e.y = a.dw; e.ldy = a.lddw;
+        if ((rc = product<T>(dzt, ldm, xt, ldm, N, K, ldm, e, part_w, st))) return rc;
     }
     return rc;
 }
