@@ -474,7 +474,7 @@ int bwd_launch(const T* x, const T* dout, Dims d, const float* ckpt, const float
     } while (0)
 
 int bad_dims(int dtype, int B, int T, int H, int64_t xb, int64_t xt) {
-    if (!dtype_ok(dtype) || B < 0 || T < 0 || H < 1 || H > (1 << 29)) return 1;
+    if (!dtype_ok(dtype) || B < 0 || T < 0 || T > (1 << 30) || H < 1 || H > (1 << 29)) return 1;
     if (T > 1 && xt < 2 * (int64_t)H) return 1;
     return B > 1 && xb < 2 * (int64_t)H;
 }
