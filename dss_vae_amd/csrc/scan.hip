@@ -13,11 +13,11 @@
 // rebuilds h inside the chunk from it, in fp32, and never reads out.
 // A granule is only 4 bytes: the scan costs log2(64 / LPR) shuffled compositions per channel and thread, so many steps per
 // thread (KT = 8, fp32 16) beat wide granules (16-byte ones leave 2: 265 us for backward over 2 x 16384 x 2048 bf16, 8-byte
-// ones 213 us, this form 165 us = 4.1 TB/s; forward 109 / 97 / 82 us = 4.9 TB/s).
+// ones 213 us, this form 150 us = 4.5 TB/s; forward 109 / 97 / 81 us = 4.9 TB/s).
 // Too few tiles (128 bytes of channels each) to fill the chip: the time axis is cut into segments; a first launch reads the
 // segment's inputs for its (A, B) per channel, the second starts each segment from the composition of those before it
 // (backward: behind it).  Narrower tiles instead (32 bytes: no second read, but four blocks per cache line) took 192 us
-// forward where the two launches take 164 us.
+// forward where the two launches take 158 us.
 // Steps at or behind a sequence's length are the identity (A = 1, B = 0): the state is kept, out and dx are zero there.
 #include "elem.h"
 
@@ -118,7 +118,9 @@ __device__ __forceinline__ float enter(float y, const float* __restrict__ maps, 
 }
 
 // This thread's steps of a chunk.  Pointers walk: one 64-bit add per row instead of a multiplication (which cost more than
-// the recurrence).  Bit k of `live`: step k is inside [lo, hi); steps that are not are neither read nor used.
+// the recurrence).  Bit k of `live`: step k is inside [lo, hi).  Steps that are not are never read: z = +inf, v = 0 and dout = 0
+// stand in their place, which makes a = 1 and (1 - a) n = 0 exactly, the identity, without a select in the arithmetic (these
+// kernels are bound by the vector ALUs as much as by memory); only what is stored there is chosen.
 template <typename T, int VEC, bool HALF, bool GRAD>
 struct Steps {
     Gran<T, VEC> z[KT<T>], v[HALF ? 1 : KT<T>], g[GRAD ? KT<T> : 1];
@@ -137,7 +139,8 @@ struct Steps {
                     else g[k].zero();
                 }
             } else {
-                z[k].zero();
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) z[k].set(j, __builtin_huge_valf());
                 if constexpr (!HALF) v[k].zero();
                 if constexpr (GRAD) g[k].zero();
             }
@@ -205,19 +208,16 @@ __global__ __launch_bounds__(NT<T>) void gated_scan_maps_kernel(const T* __restr
 #pragma unroll
         for (int kk = 0; kk < K; ++kk) {
             const int k = BWD ? K - 1 - kk : kk;
-            const bool ok = (s.live >> k) & 1;
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
                 const float a = sigmoid_f(s.z[k].get(v));
-                float b;
                 if constexpr (BWD) {
-                    b = a * (s.g[k].get(v) + B[v]);
+                    B[v] = a * (s.g[k].get(v) + B[v]);
                 } else {
-                    const float nn = TANH ? tanh_f(s.v[k].get(v)) : s.v[k].get(v);
-                    b = a * B[v] + (1.f - a) * nn;
+                    const float n = TANH ? tanh_f(s.v[k].get(v)) : s.v[k].get(v);
+                    B[v] = a * B[v] + (1.f - a) * n;
                 }
-                B[v] = ok ? b : B[v];
-                A[v] = ok ? A[v] * a : A[v];
+                A[v] *= a;
             }
         }
         block_scan<NW, VEC, !BWD>(A, B, SB, y, lds[i & 1], &SA);
@@ -239,12 +239,11 @@ __device__ __forceinline__ void fwd_chunk(const Steps<T, VEC, false, false>& s, 
     for (int v = 0; v < VEC; ++v) { A[v] = 1.f; B[v] = 0.f; }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const bool ok = (s.live >> k) & 1;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             const float ak = sigmoid_f(s.z[k].get(v)), n = TANH ? tanh_f(s.v[k].get(v)) : s.v[k].get(v);
-            a[k][v] = ok ? ak : 1.f;
-            bn[k][v] = ok ? (1.f - ak) * n : 0.f;
+            a[k][v] = ak;
+            bn[k][v] = (1.f - ak) * n;
             B[v] = a[k][v] * B[v] + bn[k][v];
             A[v] *= a[k][v];
         }
@@ -260,8 +259,9 @@ __device__ __forceinline__ void fwd_chunk(const Steps<T, VEC, false, false>& s, 
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             y[v] = a[k][v] * y[v] + bn[k][v];
-            o.set(v, ok ? y[v] : 0.f);
+            o.set(v, y[v]);
         }
+        if (!ok) o.zero();
         if (th.on && s0 + k < d.T) o.store(po);
         po += dos;
     }
@@ -299,21 +299,18 @@ __device__ __forceinline__ void bwd_chunk(const Steps<T, VEC, false, true>& s, c
     for (int v = 0; v < VEC; ++v) { A[v] = 1.f; B[v] = 0.f; G[v] = 0.f; }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const bool ok = (s.live >> k) & 1;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            const float ak = sigmoid_f(s.z[k].get(v));
+            a[k][v] = sigmoid_f(s.z[k].get(v));
             n[k][v] = TANH ? tanh_f(s.v[k].get(v)) : s.v[k].get(v);
-            a[k][v] = ok ? ak : 1.f;
-            B[v] = a[k][v] * B[v] + (ok ? (1.f - ak) * n[k][v] : 0.f);
+            B[v] = a[k][v] * B[v] + (1.f - a[k][v]) * n[k][v];
             A[v] *= a[k][v];
         }
     }
 #pragma unroll
     for (int k = K - 1; k >= 0; --k) {
-        const bool ok = (s.live >> k) & 1;
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) G[v] = ok ? a[k][v] * (s.g[k].get(v) + G[v]) : G[v];
+        for (int v = 0; v < VEC; ++v) G[v] = a[k][v] * (s.g[k].get(v) + G[v]);
     }
 #pragma unroll
     for (int v = 0; v < VEC; ++v) F[v] = A[v];
@@ -322,11 +319,10 @@ __device__ __forceinline__ void bwd_chunk(const Steps<T, VEC, false, true>& s, c
     float h[K][VEC];  // h_t - n_t = a_t (h_{t-1} - n_t)
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const bool ok = (s.live >> k) & 1;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             h[k][v] = a[k][v] * (y[v] - n[k][v]);
-            y[v] = ok ? h[k][v] + n[k][v] : y[v];
+            y[v] = h[k][v] + n[k][v];
         }
     }
     const int64_t dgs = d.reverse ? -d.gt : d.gt;
@@ -339,9 +335,13 @@ __device__ __forceinline__ void bwd_chunk(const Steps<T, VEC, false, true>& s, c
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             const float D = s.g[k].get(v) + e[v], q = D * (1.f - a[k][v]);
-            oz.set(v, ok ? q * h[k][v] : 0.f);
-            on_.set(v, ok ? (TANH ? q * (1.f - n[k][v] * n[k][v]) : q) : 0.f);
-            e[v] = ok ? a[k][v] * D : e[v];
+            oz.set(v, q * h[k][v]);
+            on_.set(v, TANH ? q * (1.f - n[k][v] * n[k][v]) : q);
+            e[v] = a[k][v] * D;
+        }
+        if (!ok) {
+            oz.zero();
+            on_.zero();
         }
         if (th.on && s0 + k < d.T) {
             oz.store(pd);
