@@ -15,9 +15,7 @@ struct Gran {
     typedef typename VecOf<T, VEC>::type V;
     V v;
     __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const V*>(p); }
-    __device__ __forceinline__ void load_nt(const T* p) { v = __builtin_nontemporal_load(reinterpret_cast<const V*>(p)); }
     __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<V*>(p) = v; }
-    __device__ __forceinline__ void store_nt(T* p) const { __builtin_nontemporal_store(v, reinterpret_cast<V*>(p)); }
     __device__ __forceinline__ float get(int i) const {
         if constexpr (VEC == 1) return (float)v;
         else return (float)v[i];
@@ -39,6 +37,7 @@ struct GranU : Gran<T, VEC> {
     typedef typename Gran<T, VEC>::V U __attribute__((aligned(sizeof(T))));
     __device__ __forceinline__ void load(const T* p) { this->v = *reinterpret_cast<const U*>(p); }
     __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<U*>(p) = this->v; }
+    __device__ __forceinline__ void store_nt(T* p) const { __builtin_nontemporal_store(this->v, reinterpret_cast<U*>(p)); }
 };
 
 // A parameter vector (norm weight, bias) whose type is the activations' T or fp32: elements [i, i + VEC) as floats

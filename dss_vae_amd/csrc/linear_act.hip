@@ -492,6 +492,7 @@ struct Turn {
     void* outT; int64_t ldt;
     float* sums;
     int stride;  // blocks along the rows
+    int stream;  // the outputs are larger than what the caches keep until the products read them: streaming stores
 };
 struct Turns { Turn job[3]; int begin[4]; };
 
@@ -556,7 +557,8 @@ __global__ __launch_bounds__(256) void linear_turn_kernel(Turns jobs) {
             }
             if (out && r < R) {
                 if (c + 8 <= ldo) {
-                    g.store(out + r * ldo + c);
+                    if (t.stream) g.store_nt(out + r * ldo + c);
+                    else g.store(out + r * ldo + c);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
@@ -578,7 +580,8 @@ __global__ __launch_bounds__(256) void linear_turn_kernel(Turns jobs) {
                 T* o = outT + (c0 + tc) * ldt + r;
                 if (c0 + tc < C) {
                     if (r + 8 <= ldt) {
-                        g.store(o);
+                        if (t.stream) g.store_nt(o);
+                        else g.store(o);
                     } else {
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
@@ -715,12 +718,15 @@ inline int64_t turn_rows(int64_t R, int64_t C) {
     return rt < 1 ? 1 : rt < want ? rt : want;  // (at most 8 blocks a CU and one per column tile: begin[] stays small)
 }
 struct TurnList {
+    int64_t es;
     Turns t{};
     int n = 0;
     void add(const void* src, int64_t ld, const void* z, int64_t ldz, int64_t R, int64_t C, void* out, int64_t ldo, void* outT, int64_t ldt,
              float* sums) {
         const int64_t rows = turn_rows(R, C);
-        t.job[n] = Turn{src, ld, z, ldz, R, C, out, ldo, outT, ldt, sums, (int)rows};
+        // (streaming stores: 8192 x 16384 bf16, two outputs, 302 -> 268 us; at 10-20 MB they cost the product behind it 13 us of 43)
+        const int stream = R * C * es * ((out != nullptr) + (outT != nullptr)) > (int64_t)128 << 20;
+        t.job[n] = Turn{src, ld, z, ldz, R, C, out, ldo, outT, ldt, sums, (int)rows, stream};
         t.begin[n + 1] = t.begin[n] + (int)(rows * ((C + 63) / 64));
         ++n;
     }
@@ -797,7 +803,7 @@ int backward(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
     void* part_x = a.dx ? sp.take(part_bytes<T>(M, K, ldn)) : nullptr;
     void* part_w = a.dw ? sp.take(part_bytes<T>(N, K, ldm)) : nullptr;
     if (dry) return rc;
-    TurnList l;
+    TurnList l{es};
     if (copy || a.dw || a.db) l.add(a.dy, a.lddy, a.z, a.ldz, M, N, dzc, ldn, dzt, ldm, sums);
     if (a.dx) l.add(a.w, a.ldw, nullptr, 0, N, K, nullptr, 0, wt, ldn, nullptr);
     if (a.dw) l.add(a.x, a.ldx, nullptr, 0, M, K, nullptr, 0, xt, ldm, nullptr);

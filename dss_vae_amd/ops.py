@@ -1863,6 +1863,11 @@ def _matrix(t):
     return t, (t.stride(0) if M > 1 else N)
 
 
+def _flat(t):
+    """[..., N] -> [rows, N]"""
+    return t if t.dim() == 2 else t.reshape(-1, t.size(-1))
+
+
 def _wants_grad(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
@@ -1877,7 +1882,7 @@ def _contig(t):
 
 def _layer_norm_fwd(x2, ldx, code, w, b, eps, stats):
     R, D = x2.shape
-    y = torch.empty(R, D, device=x2.device, dtype=x2.dtype)
+    y = x2.new_empty((R, D))
     p = w if w is not None else b
     _go("dssvae_layer_norm_fwd", x2.device,
         (x2.data_ptr(), ldx, code, _p(w), _p(b), int(p is not None and p.dtype == torch.float32), R, D, eps, y.data_ptr(), D,
@@ -1890,12 +1895,12 @@ class _LayerNormFn(Function):
     @staticmethod
     def forward(ctx, x, w, b, eps, code):
         ctx.set_materialize_grads(False)
-        x2, ldx = _matrix(x.reshape(-1, x.size(-1)))
-        stats = torch.empty(x2.size(0), 2, device=x.device, dtype=torch.float32)
+        x2, ldx = _matrix(_flat(x))
+        stats = torch.empty((x2.size(0), 2), device=x.device, dtype=torch.float32)
         y = _layer_norm_fwd(x2, ldx, code, _contig(w), _contig(b), eps, stats)
         ctx.save_for_backward(x2, w, stats)
         ctx.bias_ref, ctx.code, ctx.xshape = b, code, x.shape
-        return y.view(x.shape)
+        return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
     @once_differentiable
@@ -1908,21 +1913,23 @@ class _LayerNormFn(Function):
         R, D = x2.shape
         dev, es = x2.device, x2.element_size()
         x2, ldx = _matrix(x2)
-        dy2, lddy = _matrix(dy.reshape(-1, D))
+        dy2, lddy = _matrix(_flat(dy))
         wc, p = _contig(w), (w if w is not None else b)
-        dx = torch.empty(R, D, device=dev, dtype=x2.dtype) if need_x else None
+        dx = x2.new_empty((R, D)) if need_x else None
         dw, db = _claim(w, need_w), _claim(b, need_b)
         if need_w and dw is None:
-            dw = torch.empty(D, device=dev, dtype=w.dtype)
+            dw = w.new_empty((D,))
         if need_b and db is None:
-            db = torch.empty(D, device=dev, dtype=b.dtype)
+            db = b.new_empty((D,))
         n = L.load().dssvae_layer_norm_bwd_workspace_bytes(R, D) if need_w or need_b else 0
         ws = _space(n, dev)
         _go("dssvae_layer_norm_bwd", dev,
             (x2.data_ptr(), ldx, ctx.code, dy2.data_ptr(), lddy, _p(wc), int(p is not None and p.dtype == torch.float32),
              stats.data_ptr(), R, D, _p(dx), D, _p(dw), _p(db), _p(ws), n),
             lambda: ("layer_norm_bwd_kernel", 12.0 * R * D, 3.0 * R * D * es, 0, "R=%d D=%d" % (R, D)))
-        return None if dx is None else dx.view(ctx.xshape), dw, db, None, None
+        if dx is not None and len(ctx.xshape) != 2:
+            dx = dx.view(ctx.xshape)
+        return dx, dw, db, None, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -1941,8 +1948,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
         raise RuntimeError("layer_norm: weight is %s, bias is %s" % (weight.dtype, bias.dtype))
     if _wants_grad(x, weight, bias):
         return _LayerNormFn.apply(x, weight, bias, float(eps), code)
-    x2, ldx = _matrix(x.reshape(-1, D))
-    return _layer_norm_fwd(x2, ldx, code, _contig(weight), _contig(bias), float(eps), None).view(x.shape)
+    x2, ldx = _matrix(_flat(x))
+    y = _layer_norm_fwd(x2, ldx, code, _contig(weight), _contig(bias), float(eps), None)
+    return y if x.dim() == 2 else y.view(x.shape)
 
 
 def _sequence(t):
@@ -1963,9 +1971,9 @@ def _gated_scan_fwd(x, h0, lengths, reverse, tanh, code, keep):
     """-> out, h_last, checkpoints (None unless `keep`)"""
     B, T, H2 = x.shape
     H, dev, lib = H2 // 2, x.device, L.load()
-    out = torch.empty(B, T, H, device=dev, dtype=x.dtype)
-    h_last = torch.empty(B, H, device=dev, dtype=torch.float32)
-    ckpt = torch.empty(B, lib.dssvae_gated_scan_chunks(T), H, device=dev, dtype=torch.float32) if keep else None
+    out = x.new_empty((B, T, H))
+    h_last = torch.empty((B, H), device=dev, dtype=torch.float32)
+    ckpt = h_last.new_empty((B, lib.dssvae_gated_scan_chunks(T), H)) if keep else None
     if T == 0:
         h_last.zero_() if h0 is None else h_last.copy_(h0)
     elif T == 1 and lengths is None and not keep:
@@ -2003,8 +2011,8 @@ class _GatedScanFn(Function):
         x = _sequence(x)
         dout = None if dout is None else _sequence(dout)
         dh = _contig(dh)
-        dx = torch.empty(B, T, H2, device=dev, dtype=x.dtype)
-        dh0 = torch.empty(B, H, device=dev, dtype=torch.float32) if ctx.needs_input_grad[1] else None
+        dx = x.new_empty((B, T, H2))
+        dh0 = ckpt.new_empty((B, H)) if ctx.needs_input_grad[1] else None
         if T == 0:
             if dh0 is not None:
                 dh0.zero_() if dh is None else dh0.copy_(dh)
@@ -2071,8 +2079,8 @@ def gated_step(xproj, h=None, candidate="tanh", h_out=None):
         out, hn = gated_scan(xproj.unsqueeze(1), h, None, False, candidate)
         return out.squeeze(1), hn
     x, ldx = _matrix(xproj)
-    out = torch.empty(B, H, device=x.device, dtype=x.dtype)
-    hn = torch.empty(B, H, device=x.device, dtype=torch.float32) if h_out is None else h_out
+    out = x.new_empty((B, H))
+    hn = torch.empty((B, H), device=x.device, dtype=torch.float32) if h_out is None else h_out
     _gated_step(x, ldx, code, _contig(h), tanh, out, hn)
     return out, hn
 
@@ -2088,8 +2096,8 @@ def _like_rows(z, ldz):
 def _distill(z, ldz, code, ids, teacher, tau, weight, want_grad):
     """-> total, rows, dlogits (None unless wanted)"""
     N, V = z.shape
-    rows = torch.empty(N, device=z.device, dtype=torch.float32)
-    total = torch.empty((), device=z.device, dtype=torch.float32)
+    rows = torch.empty((N,), device=z.device, dtype=torch.float32)
+    total = rows.new_empty(())
     dz = _like_rows(z, ldz) if want_grad else None
     k = ids.size(1)
     _go("dssvae_distill", z.device,
@@ -2107,10 +2115,11 @@ class _DistillFn(Function):
     @staticmethod
     def forward(ctx, logits, ids, teacher, weight, tau, code):
         ctx.set_materialize_grads(False)
-        z, ldz = _matrix(logits.reshape(-1, logits.size(-1)))
+        z, ldz = _matrix(_flat(logits))
         total, rows, ctx.dz = _distill(z, ldz, code, ids, teacher, tau, weight, True)
         ctx.shape, ctx.code = logits.shape, code
-        rows = rows.view(logits.shape[:-1])
+        if logits.dim() != 2:
+            rows = rows.view(logits.shape[:-1])
         ctx.mark_non_differentiable(rows)
         return total, rows
 
@@ -2126,7 +2135,9 @@ class _DistillFn(Function):
                                "is not supported)")
         if dz.size(0):
             _go("dssvae_scale_rows", dz.device, (dz.data_ptr(), dz.stride(0), ctx.code, dz.size(0), dz.size(1), g.data_ptr()))
-        return dz.view(ctx.shape) if dz.is_contiguous() else dz.unflatten(0, ctx.shape[:-1]), None, None, None, None, None
+        if len(ctx.shape) != 2:
+            dz = dz.view(ctx.shape) if dz.is_contiguous() else dz.unflatten(0, ctx.shape[:-1])
+        return dz, None, None, None, None, None
 
 
 def distill_loss(logits, ids, teacher, temperature=1.0, weight=None):
@@ -2154,22 +2165,24 @@ def distill_loss(logits, ids, teacher, temperature=1.0, weight=None):
         raise RuntimeError("distill_loss: temperature must be positive and finite, got %r" % (temperature,))
     if _wants_grad(teacher, weight):
         raise RuntimeError("distill_loss: gradients go to the logits only (detach teacher and weight)")
-    ids2, t2 = ids.reshape(-1, k).contiguous(), teacher.detach().reshape(-1, k).float().contiguous()
-    w2 = None if weight is None else weight.detach().reshape(-1).contiguous()
+    ids2, t2 = _flat(ids).contiguous(), _flat(teacher).contiguous()
+    if t2.dtype != torch.float32:
+        t2 = t2.float()
+    w2 = None if weight is None else weight.reshape(-1).contiguous()
     if _wants_grad(logits):
         return _DistillFn.apply(logits, ids2, t2, w2, tau, code)
-    z, ldz = _matrix(logits.reshape(-1, logits.size(-1)))
+    z, ldz = _matrix(_flat(logits))
     total, rows, _ = _distill(z, ldz, code, ids2, t2, tau, w2, False)
-    return total, rows.view(lead)
+    return total, rows if logits.dim() == 2 else rows.view(lead)
 
 
 def _linear_act_fwd(x2, ldx, w, ldw, b, act, r, code, keep_z):
     """-> y, z (the pre-activation as backward needs it; None unless `keep_z`)"""
     M, K = x2.shape
     N, dev = w.size(0), x2.device
-    y = torch.empty(M, N, device=dev, dtype=x2.dtype)
+    y = x2.new_empty((M, N))
     # (fp32: the values; 16 bits: codes of the kernel's own)
-    z = torch.empty(M, N, device=dev, dtype=torch.float32 if code == 0 else torch.int16) if keep_z else None
+    z = torch.empty((M, N), device=dev, dtype=torch.float32 if code == 0 else torch.int16) if keep_z else None
     r, ldr = (None, 0) if r is None else _matrix(r)
     xp, wp = x2.data_ptr(), w.data_ptr()
     n = L.load().dssvae_linear_act_fwd_workspace_bytes(xp, ldx, wp, ldw, code, M, N, K)
@@ -2187,14 +2200,13 @@ class _LinearActFn(Function):
     def forward(ctx, x, w, b, residual, act, code):
         ctx.set_materialize_grads(False)
         N = w.size(0)
-        x2, ldx = _matrix(x.reshape(-1, x.size(-1)))
+        x2, ldx = _matrix(_flat(x))
         wc, ldw = _matrix(w)
-        bc = _contig(b)
         keep = act != 0 and any(ctx.needs_input_grad[:3])
-        y, z = _linear_act_fwd(x2, ldx, wc, ldw, bc, act, None if residual is None else residual.reshape(-1, N), code, keep)
+        y, z = _linear_act_fwd(x2, ldx, wc, ldw, _contig(b), act, None if residual is None else _flat(residual), code, keep)
         ctx.save_for_backward(x2, w, z)
         ctx.bias_ref, ctx.act, ctx.code, ctx.xshape = b, act, code, x.shape
-        return y.view(*x.shape[:-1], N)
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
     @staticmethod
     @once_differentiable
@@ -2209,14 +2221,14 @@ class _LinearActFn(Function):
             N, dev, es, code, act = w.size(0), x2.device, x2.element_size(), ctx.code, ctx.act
             x2, ldx = _matrix(x2)
             wc, ldw = _matrix(w)
-            dy2, lddy = _matrix(dy.reshape(-1, N))
+            dy2, lddy = _matrix(_flat(dy))
             b = ctx.bias_ref
-            dx = torch.empty(M, K, device=dev, dtype=x2.dtype) if need_x else None
+            dx = x2.new_empty((M, K)) if need_x else None
             dw, db = _claim(w, need_w), _claim(b, need_b)
             if need_w and dw is None:
-                dw = torch.empty(N, K, device=dev, dtype=w.dtype)
+                dw = w.new_empty((N, K))
             if need_b and db is None:
-                db = torch.empty(N, device=dev, dtype=b.dtype)
+                db = b.new_empty((N,))
             n = L.load().dssvae_linear_act_bwd_workspace_bytes(dy2.data_ptr(), lddy, int(z is not None), code, M, N, K,
                                                                int(need_x and M > 0), int(need_w), int(need_b))
             ws = _space(n, dev)
@@ -2225,7 +2237,8 @@ class _LinearActFn(Function):
                  _p(db), int(db is not None and db.dtype == torch.float32), _p(ws), n),
                 lambda: ("linear_act_bwd", 2.0 * M * N * K * (int(need_x) + int(need_w)), 4.0 * M * N * es, 0,
                          "M=%d N=%d K=%d" % (M, N, K)))
-            dx = None if dx is None else dx.view(ctx.xshape)
+            if dx is not None and len(ctx.xshape) != 2:
+                dx = dx.view(ctx.xshape)
         return dx, dw, db, dy if need_r else None, None, None
 
 
@@ -2248,8 +2261,7 @@ def linear_act(x, w, b=None, act="none", residual=None):
     a = L.ACTIVATIONS[act]
     if _wants_grad(x, w, b, residual):
         return _LinearActFn.apply(x, w, b, residual, a, code)
-    x2, ldx = _matrix(x.reshape(-1, K))
+    x2, ldx = _matrix(_flat(x))
     w2, ldw = _matrix(w)
-    r = None if residual is None else residual.reshape(-1, N)
-    y, _ = _linear_act_fwd(x2, ldx, w2, ldw, _contig(b), a, r, code, False)
-    return y.view(*x.shape[:-1], N)
+    y, _ = _linear_act_fwd(x2, ldx, w2, ldw, _contig(b), a, None if residual is None else _flat(residual), code, False)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
