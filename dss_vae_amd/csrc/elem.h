@@ -40,15 +40,75 @@ struct GranU : Gran<T, VEC> {
     __device__ __forceinline__ void store_nt(T* p) const { __builtin_nontemporal_store(this->v, reinterpret_cast<U*>(p)); }
 };
 
-// A parameter vector (norm weight, bias) whose type is the activations' T or fp32: elements [i, i + VEC) as floats
-template <typename T, int VEC>
-__device__ __forceinline__ void load_param(float (&o)[VEC], const void* p, bool f32, int64_t i) {
-    if (f32) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) o[j] = reinterpret_cast<const float*>(p)[i + j];
+// The granule at column c of a row of D elements: what lies behind D reads as zero and is not stored.  WHOLE: D is a multiple
+// of VEC, a granule is inside or outside.
+template <bool WHOLE, typename T, int VEC>
+__device__ __forceinline__ void load_cols(GranU<T, VEC>& g, const T* row, int c, int D) {
+    if (WHOLE ? c < D : c + VEC <= D) {
+        g.load(row + c);
     } else {
-        Gran<T, VEC> g;
-        g.load(reinterpret_cast<const T*>(p) + i);
+        g.zero();
+        if (!WHOLE) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                if (c + j < D) g.set(j, (float)row[c + j]);
+        }
+    }
+}
+template <bool WHOLE, typename T, int VEC>
+__device__ __forceinline__ void store_cols(const GranU<T, VEC>& g, T* row, int c, int D) {
+    if (WHOLE ? c < D : c + VEC <= D) {
+        g.store(row + c);
+    } else if (!WHOLE) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (c + j < D) row[c + j] = (T)g.get(j);
+    }
+}
+
+// The same in two steps, so that nothing waits between the loads of a row: load_near takes a granule that is always whole,
+// trim puts its columns in place (columns behind D: zero, or with ZERO false the value of some column of the row).
+// Rows narrower than a granule go by elements.
+template <typename T, int VEC>
+__device__ __forceinline__ void load_near(GranU<T, VEC>& g, const T* row, int c, int D) {
+    if (D >= VEC) {
+        g.load(row + (c + VEC <= D ? c : D - VEC));
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) g.set(j, (float)row[c + j < D ? c + j : D - 1]);
+    }
+}
+template <bool ZERO, typename T, int VEC>
+__device__ __forceinline__ void trim(GranU<T, VEC>& g, int c, int D) {
+    static_assert(VEC * sizeof(T) == 16, "16-byte granules");
+    if (c + VEC <= D) return;
+    const int out = c + VEC - D;  // columns behind the row's end
+    if (D >= VEC && out < VEC) {
+        const unsigned __int128 raw = __builtin_bit_cast(unsigned __int128, g.v);
+        const int bits = out * 8 * (int)sizeof(T);
+        g.v = __builtin_bit_cast(typename Gran<T, VEC>::V, ZERO ? raw >> bits : raw >> bits | raw << (128 - bits));
+    } else if (ZERO) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+            if (c + j >= D) g.set(j, 0.f);
+    }
+}
+
+// A parameter vector [D] (norm weight, bias) whose type is the activations' T or fp32, `none` where it is NULL: elements
+// [c, c + VEC) as floats, zero behind D
+template <bool WHOLE, typename T, int VEC>
+__device__ __forceinline__ void load_param(float (&o)[VEC], const void* p, bool f32, int c, int D, float none) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) o[j] = c + j < D ? none : 0.f;
+    if (!p || c >= D) return;
+    if (f32) {
+        GranU<float, VEC> g;
+        load_cols<WHOLE, float, VEC>(g, reinterpret_cast<const float*>(p), c, D);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = g.get(j);
+    } else {
+        GranU<T, VEC> g;
+        load_cols<WHOLE, T, VEC>(g, reinterpret_cast<const T*>(p), c, D);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) o[j] = g.get(j);
     }
