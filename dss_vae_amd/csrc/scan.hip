@@ -25,8 +25,10 @@ namespace {
 
 // lanes per row; threads of a block and steps per thread: 128 steps a chunk in either width
 constexpr int LPR = 32, CHUNK = 128;
-template <typename T> constexpr int NT = sizeof(T) == 4 ? 256 : 512;
-template <typename T> constexpr int KT = CHUNK * LPR / NT<T>;
+template <typename T> constexpr int KT = sizeof(T) == 4 ? 16 : 8;
+// Threads of a block: 256 or 512, and half or a quarter of that where the sequence ends in that part of its only chunk
+// (512 x 30 x 2048 bf16, forward / backward: 128 / 230 us with the whole chunk, 36 / 66 us with a quarter of it)
+template <typename T, int DIV> constexpr int NT = CHUNK / DIV * LPR / KT<T>;
 constexpr int STEP_THREADS = 256;
 
 __device__ __forceinline__ float sigmoid_f(float x) {
@@ -185,9 +187,9 @@ struct Thread {
 
 // ---- segment maps: (A, B) of the forward recurrence, or of E (BWD) ------------------------------------------------
 template <typename T, int VEC, bool TANH, bool BWD>
-__global__ __launch_bounds__(NT<T>) void gated_scan_maps_kernel(const T* __restrict__ x, const T* __restrict__ dout, Dims d,
+__global__ __launch_bounds__((NT<T, 1>)) void gated_scan_maps_kernel(const T* __restrict__ x, const T* __restrict__ dout, Dims d,
                                                                 float* __restrict__ maps) {
-    constexpr int NW = NT<T> / 64, K = KT<T>;
+    constexpr int NW = NT<T, 1> / 64, K = KT<T>;
     __shared__ float2 lds[2][NW * LPR * VEC];
     const Thread<T, VEC> th(d);
     if (th.w.seg == (BWD ? 0 : d.segs - 1)) return;  // nobody starts behind the last one
@@ -230,10 +232,10 @@ __global__ __launch_bounds__(NT<T>) void gated_scan_maps_kernel(const T* __restr
 }
 
 // ---- forward ---------------------------------------------------------------------------------------------------------
-template <typename T, int VEC, bool TANH>
+template <typename T, int VEC, bool TANH, int DIV>
 __device__ __forceinline__ void fwd_chunk(const Steps<T, VEC, false, false>& s, const Thread<T, VEC>& th,
                                           const Dims& d, int chunk, float& h, float2* lds, T* out) {
-    constexpr int NW = NT<T> / 64, K = KT<T>;
+    constexpr int NW = NT<T, DIV> / 64, K = KT<T>;
     float a[K][VEC], bn[K][VEC], A[VEC], B[VEC], y[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) { A[v] = 1.f; B[v] = 0.f; }
@@ -267,11 +269,11 @@ __device__ __forceinline__ void fwd_chunk(const Steps<T, VEC, false, false>& s, 
     }
 }
 
-template <typename T, int VEC, bool TANH>
-__global__ __launch_bounds__(NT<T>) void gated_scan_fwd_kernel(const T* __restrict__ x, Dims d, const float* __restrict__ h0,
+template <typename T, int VEC, bool TANH, int DIV>
+__global__ __launch_bounds__((NT<T, DIV>)) void gated_scan_fwd_kernel(const T* __restrict__ x, Dims d, const float* __restrict__ h0,
                                                                const float* __restrict__ maps, T* __restrict__ out,
                                                                float* __restrict__ h_last, float* __restrict__ ckpt) {
-    constexpr int NW = NT<T> / 64;
+    constexpr int NW = NT<T, DIV> / 64;
     __shared__ float2 lds[2][NW * LPR * VEC];
     const Thread<T, VEC> th(d);
     const int64_t dxs = d.reverse ? -d.xt : d.xt, dgs = 0, row = (int64_t)th.w.b * d.H + th.cc;
@@ -284,16 +286,16 @@ __global__ __launch_bounds__(NT<T>) void gated_scan_fwd_kernel(const T* __restri
         s = next;
         if (chunk + 1 < th.last) DSSVAE_SCAN_LOAD(next, (chunk + 1), none);
         if (ckpt && th.writer) ckpt[((int64_t)th.w.b * d.nchunk + chunk) * d.H + th.cc] = h;
-        fwd_chunk<T, VEC, TANH>(s, th, d, chunk, h, lds[chunk & 1], out);
+        fwd_chunk<T, VEC, TANH, DIV>(s, th, d, chunk, h, lds[chunk & 1], out);
     }
     if (th.w.seg == d.segs - 1 && h_last && th.writer) h_last[row] = h;
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------------
-template <typename T, int VEC, bool TANH>
+template <typename T, int VEC, bool TANH, int DIV>
 __device__ __forceinline__ void bwd_chunk(const Steps<T, VEC, false, true>& s, const Thread<T, VEC>& th,
                                           const Dims& d, int chunk, float hc, float& E, float2* lds0, float2* lds1, T* dx) {
-    constexpr int NW = NT<T> / 64, K = KT<T>;
+    constexpr int NW = NT<T, DIV> / 64, K = KT<T>;
     float a[K][VEC], n[K][VEC], A[VEC], B[VEC], F[VEC], G[VEC], y[VEC], e[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) { A[v] = 1.f; B[v] = 0.f; G[v] = 0.f; }
@@ -351,13 +353,13 @@ __device__ __forceinline__ void bwd_chunk(const Steps<T, VEC, false, true>& s, c
     }
 }
 
-template <typename T, int VEC, bool TANH>
-__global__ __launch_bounds__(NT<T>) void gated_scan_bwd_kernel(const T* __restrict__ x, const T* __restrict__ dout, Dims d,
+template <typename T, int VEC, bool TANH, int DIV>
+__global__ __launch_bounds__((NT<T, DIV>)) void gated_scan_bwd_kernel(const T* __restrict__ x, const T* __restrict__ dout, Dims d,
                                                                const float* __restrict__ ckpt,
                                                                const float* __restrict__ dh_last,
                                                                const float* __restrict__ maps, T* __restrict__ dx,
                                                                float* __restrict__ dh0) {
-    constexpr int NW = NT<T> / 64;
+    constexpr int NW = NT<T, DIV> / 64;
     __shared__ float2 lds[2][2][NW * LPR * VEC];
     const Thread<T, VEC> th(d);
     const int64_t dxs = d.reverse ? -d.xt : d.xt, dgs = d.reverse ? -d.ot : d.ot, row = (int64_t)th.w.b * d.H + th.cc;
@@ -370,7 +372,7 @@ __global__ __launch_bounds__(NT<T>) void gated_scan_bwd_kernel(const T* __restri
         if (chunk > th.first) DSSVAE_SCAN_LOAD(next, (chunk - 1), dout);
         const float hc = th.con ? ckpt[((int64_t)th.w.b * d.nchunk + chunk) * d.H + th.cc] : 0.f;
         float2 *l0 = lds[chunk & 1][0], *l1 = lds[chunk & 1][1];
-        bwd_chunk<T, VEC, TANH>(s, th, d, chunk, hc, E, l0, l1, dx);
+        bwd_chunk<T, VEC, TANH, DIV>(s, th, d, chunk, hc, E, l0, l1, dx);
     }
     if (th.w.seg == 0 && dh0 && th.writer) dh0[row] = E;
 }
@@ -428,12 +430,17 @@ int fwd_launch(const T* x, Dims d, const float* h0, T* out, float* h_last, float
     const int64_t grid = (int64_t)d.tiles * d.B * d.segs;
     if (grid > 0x7fffffff) return DSSVAE_ETOOBIG;
     if (d.segs > 1) {
-        hipLaunchKernelGGL((gated_scan_maps_kernel<T, VEC, TANH, false>), dim3((unsigned)grid), dim3(NT<T>), 0, s, x,
+        hipLaunchKernelGGL((gated_scan_maps_kernel<T, VEC, TANH, false>), dim3((unsigned)grid), dim3((NT<T, 1>)), 0, s, x,
                            (const T*)nullptr, d, maps);
         DSSVAE_CHECK_LAUNCH();
     }
-    hipLaunchKernelGGL((gated_scan_fwd_kernel<T, VEC, TANH>), dim3((unsigned)grid), dim3(NT<T>), 0, s, x, d, h0, maps, out,
-                       h_last, ckpt);
+#define GO(DIV)                                                                                                     \
+    hipLaunchKernelGGL((gated_scan_fwd_kernel<T, VEC, TANH, DIV>), dim3((unsigned)grid), dim3((NT<T, DIV>)), 0, s, x, d, h0, maps, \
+                       out, h_last, ckpt)
+    if (d.T <= CHUNK / 4) GO(4);
+    else if (d.T <= CHUNK / 2) GO(2);
+    else GO(1);
+#undef GO
     DSSVAE_CHECK_LAUNCH();
     return DSSVAE_OK;
 }
@@ -445,12 +452,17 @@ int bwd_launch(const T* x, const T* dout, Dims d, const float* ckpt, const float
     const int64_t grid = (int64_t)d.tiles * d.B * d.segs;
     if (grid > 0x7fffffff) return DSSVAE_ETOOBIG;
     if (d.segs > 1) {
-        hipLaunchKernelGGL((gated_scan_maps_kernel<T, VEC, false, true>), dim3((unsigned)grid), dim3(NT<T>), 0, s, x, dout, d,
+        hipLaunchKernelGGL((gated_scan_maps_kernel<T, VEC, false, true>), dim3((unsigned)grid), dim3((NT<T, 1>)), 0, s, x, dout, d,
                            maps);
         DSSVAE_CHECK_LAUNCH();
     }
-    hipLaunchKernelGGL((gated_scan_bwd_kernel<T, VEC, TANH>), dim3((unsigned)grid), dim3(NT<T>), 0, s, x, dout, d, ckpt,
-                       dh_last, maps, dx, dh0);
+#define GO(DIV)                                                                                                     \
+    hipLaunchKernelGGL((gated_scan_bwd_kernel<T, VEC, TANH, DIV>), dim3((unsigned)grid), dim3((NT<T, DIV>)), 0, s, x, dout, d, ckpt, \
+                       dh_last, maps, dx, dh0)
+    if (d.T <= CHUNK / 4) GO(4);
+    else if (d.T <= CHUNK / 2) GO(2);
+    else GO(1);
+#undef GO
     DSSVAE_CHECK_LAUNCH();
     return DSSVAE_OK;
 }
