@@ -1,8 +1,12 @@
 // Linear layer with its epilogue:  z = x w^T + b,  y = act(z) + residual,  and its backward pass
 //   dz = dy act'(z),  dx = dz w,  dw = dz^T x,  db = sum_rows dz,  dresidual = dy.
 //
-// Products run on one tile kernel: v_mfma_f32_32x32x16 for bf16 / fp16, v_mfma_f32_32x32x2_f32 for fp32 (exact products),
-// fp32 accumulation, one rounding per output.
+// Products run on one tile kernel: v_mfma_f32_32x32x16 for bf16 / fp16, fp32 accumulation, one rounding per output.
+// fp32 operands are taken apart into three bf16 each (24 bits, exact) as they come out of LDS, and six of the nine products of
+// the parts are added: what is left out is below 2^-22 of a product, and on the mean of random inputs the sums are closer to
+// the exact ones than v_mfma_f32_32x32x2_f32's order gives (K = 7936: 7e-7 of the norm; the library's fp32 product 1.6e-6).  The
+// fp32 instruction does a sixteenth of the bf16 one's work: a library product of 4096^3 takes 0.91 ms, this one 0.70 ms; the 704 vector
+// instructions that take 64 k apart cost as much time as the 96 MFMAs behind them, interleaved or not.
 //
 // The tile kernel: C[M, N] = A[M, K] . B[N, K]^T, both operands contiguous along K.  A BM x BN block walks K in steps of
 // 128 bytes (64 or 32 elements); operand tiles go global -> LDS directly (16 bytes a lane, no registers), double buffered.  LDS row r keeps its
@@ -256,6 +260,35 @@ struct Loader {
     }
 };
 
+// Eight fp32 values as sums of three bf16 each, x = p0 + p1 + p2 exactly (the first rounded to nearest, so that the rest has
+// either sign, the others cut off; p2 runs out of exponent below 2^-110: what is smaller than 2^-134 is dropped).  Infinities, and
+// the last 0.4 % below the largest finite value, become NaN.
+struct Split {
+    Mfma<bf16_t>::V p[3];
+    __device__ __forceinline__ void of(f32x4 lo, f32x4 hi) {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        u32x4 q[3];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float x = j < 2 ? lo[2 * j] : hi[2 * j - 4], y = j < 2 ? lo[2 * j + 1] : hi[2 * j - 3];
+            q[0][j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, bf16x2));
+            x -= __builtin_bit_cast(float, q[0][j] << 16);
+            y -= __builtin_bit_cast(float, q[0][j] & 0xffff0000u);
+#pragma unroll
+            for (int t = 1; t < 3; ++t) {
+                const uint32_t bx = __builtin_bit_cast(uint32_t, x), by = __builtin_bit_cast(uint32_t, y);
+                q[t][j] = __builtin_amdgcn_perm(by, bx, 0x07060302u);  // the upper halves
+                x -= __builtin_bit_cast(float, bx & 0xffff0000u);
+                y -= __builtin_bit_cast(float, by & 0xffff0000u);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 3; ++t) p[t] = __builtin_bit_cast(Mfma<bf16_t>::V, q[t]);
+    }
+};
+
 // MI x NI blocks of 32 x 32 of this wave's tile: the operands of K half `h` (two granule pairs)
 template <typename T, int MI, int NI>
 struct Frags {
@@ -279,6 +312,29 @@ struct Frags {
             for (int i = 0; i < MI; ++i)
 #pragma unroll
                 for (int j = 0; j < NI; ++j) acc[i][j] = Mfma<T>::go(a[s][i], b[s][j], acc[i][j]);
+    }
+};
+
+// A K half of fp32 operands (16 elements a row) as bf16 triples
+template <int MI, int NI>
+struct Planes {
+    Split a[MI], b[NI];
+    __device__ __forceinline__ void of(const Frags<float, MI, NI>& f) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) a[i].of(f.a[0][i], f.a[1][i]);
+#pragma unroll
+        for (int j = 0; j < NI; ++j) b[j].of(f.b[0][j], f.b[1][j]);
+    }
+    // smallest terms first; p1 p2, p2 p1 and p2 p2 are left out: |p1| <= 2^-8 |x|, |p2| < 2^-15 |x|, both signs: below 2^-22 of x y together
+    __device__ __forceinline__ void multiply(f32x16 (&acc)[MI][NI]) const {
+        constexpr int TERMS[6][2] = {{0, 2}, {2, 0}, {1, 1}, {0, 1}, {1, 0}, {0, 0}};
+#pragma unroll
+        for (int t = 0; t < 6; ++t)
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+                    acc[i][j] = Mfma<bf16_t>::go(a[i].p[TERMS[t][0]], b[j].p[TERMS[t][1]], acc[i][j]);
     }
 };
 
@@ -342,47 +398,91 @@ __device__ __forceinline__ void k_step(Frags<T, MI, NI>& f0, Frags<T, MI, NI>& f
     }
 }
 
-template <typename T, int BM, int BN, int WR, int WC>
-__global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, Epilogue e) {
-    constexpr int TH = 64 * WR * WC, MI = BM / WR / 32, NI = BN / WC / 32;
-    __shared__ __attribute__((aligned(16))) T buf0[(BM + BN) * BK<T>], buf1[(BM + BN) * BK<T>];
-    const int wid = xcd_remap(blockIdx.x, gridDim.x), tiles = s.tiles_m * s.tiles_n;
-    const int split = wid / tiles;
-    int tm, tn;
-    tile_of(s, wid - split * tiles, tm, tn);
-    const int64_t m0 = (int64_t)tm * BM;
-    const int n0 = tn * BN;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int ra = wave / WC * (BM / WR), rb = wave % WC * (BN / WC);
-    const int64_t nk = (s.K + BK<T> - 1) / BK<T>, kt0 = split * s.ktiles, kt1 = min(nk, kt0 + s.ktiles);
+// The same for fp32 operands as bf16 triples.  On entry p0 holds the first half of the tile in `cur` and f1 the second as it is,
+// and so of the next tile when it ends: a half is taken apart (11 vector instructions for two elements) behind the MFMAs of
+// the half before it, about 7 to an MFMA (4096^3: 0.77 ms with the two one after the other, 0.71 ms so).
+template <int BM, int BN, int TH, int MI, int NI>
+__device__ __forceinline__ void k_step_split(Planes<MI, NI>& p0, Frags<float, MI, NI>& f1, f32x16 (&acc)[MI][NI],
+                                             const Loader<float, BM, TH>& la, const Loader<float, BN, TH>& lb, float* cur, const float* next,
+                                             int ra, int rb, const float* a, const float* b) {
+    constexpr int READS = 2 * (MI + NI), MULS = 6 * MI * NI, OPS = 44 * (MI + NI), LOADS = Loader<float, BM, TH>::NR + Loader<float, BN, TH>::NR;
+    Planes<MI, NI> p1;
+    p1.of(f1);
+    p0.multiply(acc);
+#pragma unroll
+    for (int i = 0; i < MULS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, (OPS + MULS - 1) / MULS, 0);
+    }
+    tile_barrier();  // this tile has been read by every wave, the next one has landed
+    Frags<float, MI, NI> f0;
+    f0.read(next, BM * BK<float>, ra, rb, 0);
+    tile_load<float, BM, BN, TH>(cur, la, lb, a, b);
+    f1.read(next, BM * BK<float>, ra, rb, 1);
+    p0.of(f0);
+    p1.multiply(acc);
+    constexpr int AHEAD = MULS / 6;  // MFMAs that cover the first reads
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+    for (int i = 0; i < MULS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i < LOADS) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+        if (i < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        if (i >= AHEAD) __builtin_amdgcn_sched_group_barrier(0x002, (OPS + MULS - AHEAD - 1) / (MULS - AHEAD), 0);
+    }
+}
 
-    f32x16 acc[MI][NI];
+// acc = this wave's part of the output tile at (m0, n0), over the k-tiles kt0 .. kt1 - 1
+template <typename T, int BM, int BN, int WR, int WC, bool SPLIT>
+__device__ __forceinline__ void tile_product(const Shape& s, int64_t m0, int n0, int64_t kt0, int64_t kt1, T* __restrict__ buf0,
+                                             T* __restrict__ buf1, f32x16 (&acc)[BM / WR / 32][BN / WC / 32]) {
+    constexpr int TH = 64 * WR * WC, MI = BM / WR / 32, NI = BN / WC / 32;
+    const int wave = threadIdx.x >> 6;
+    const int ra = wave / WC * (BM / WR), rb = wave % WC * (BN / WC);
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-
-    if (kt0 < kt1) {
-        Loader<T, BM, TH> la;
-        Loader<T, BN, TH> lb;
-        la.init(s.lda, s.M - m0);
-        lb.init(s.ldb, s.N - n0);
-        const T* A = (const T*)s.A + m0 * s.lda;
-        const T* B = (const T*)s.B + (int64_t)n0 * s.ldb;
-        // The order of the tiles is free: the last one, which alone may reach behind K, goes first, then kt0 .. kt1 - 2, so that
-        // the loop's loads need no test.  A tile behind the end is the one before it again (loaded, never multiplied).
-        const int64_t kl = (kt1 - 1) * BK<T>, n = kt1 - kt0;
-        la.load_last(buf0, A + kl, s.K - kl);
-        lb.load_last(buf0 + BM * BK<T>, B + kl, s.K - kl);
-        const int64_t most = n > 1 ? kt1 - 2 : kt0;
-        if (n > 1) tile_load<T, BM, BN, TH>(buf1, la, lb, A + kt0 * BK<T>, B + kt0 * BK<T>);
-        tile_barrier();
+    if (kt0 >= kt1) return;
+    Loader<T, BM, TH> la;
+    Loader<T, BN, TH> lb;
+    la.init(s.lda, s.M - m0);
+    lb.init(s.ldb, s.N - n0);
+    const T* A = (const T*)s.A + m0 * s.lda;
+    const T* B = (const T*)s.B + (int64_t)n0 * s.ldb;
+    // The order of the tiles is free: the last one, which alone may reach behind K, goes first, then kt0 .. kt1 - 2, so that
+    // the loop's loads need no test.  A tile behind the end is the one before it again (loaded, never multiplied).
+    const int64_t kl = (kt1 - 1) * BK<T>, n = kt1 - kt0;
+    la.load_last(buf0, A + kl, s.K - kl);
+    lb.load_last(buf0 + BM * BK<T>, B + kl, s.K - kl);
+    const int64_t most = n > 1 ? kt1 - 2 : kt0;
+    if (n > 1) tile_load<T, BM, BN, TH>(buf1, la, lb, A + kt0 * BK<T>, B + kt0 * BK<T>);
+    tile_barrier();
+    // step i multiplies the i-th tile in that order and loads the (i + 2)-th: kt0 + i + 1
+    int64_t i = 0;
+    if constexpr (SPLIT) {
+        Frags<T, MI, NI> f0, f1;
+        Planes<MI, NI> p0, p1;
+        f0.read(buf0, BM * BK<T>, ra, rb, 0);
+        f1.read(buf0, BM * BK<T>, ra, rb, 1);
+        p0.of(f0);
+        if (n > 1) {
+            for (; i + 1 < n; i += 2) {
+                const int64_t k2 = min(kt0 + i + 1, most) * BK<T>, k3 = min(kt0 + i + 2, most) * BK<T>;
+                k_step_split<BM, BN, TH, MI, NI>(p0, f1, acc, la, lb, buf0, buf1, ra, rb, A + k2, B + k2);
+                k_step_split<BM, BN, TH, MI, NI>(p0, f1, acc, la, lb, buf1, buf0, ra, rb, A + k3, B + k3);
+            }
+        }
+        if (i < n) {
+            p1.of(f1);
+            p0.multiply(acc);
+            p1.multiply(acc);
+        }
+    } else {
         Frags<T, MI, NI> f0, f1;
         f0.read(buf0, BM * BK<T>, ra, rb, 0);
-        // step i multiplies the i-th tile in that order and loads the (i + 2)-th: kt0 + i + 1
-        int64_t i = 0;
         if (n > 1) {
             for (; i + 1 < n; i += 2) {
                 const int64_t k2 = min(kt0 + i + 1, most) * BK<T>, k3 = min(kt0 + i + 2, most) * BK<T>;
@@ -395,7 +495,46 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, E
             f0.multiply(acc);
             f1.multiply(acc);
         }
-        tile_barrier();  // operand buffers are free (and no load is in flight)
+    }
+    tile_barrier();  // operand buffers are free (and no load is in flight)
+}
+
+template <typename T, int BM, int BN, int WR, int WC>
+__global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, Epilogue e) {
+    constexpr int MI = BM / WR / 32, NI = BN / WC / 32;
+    __shared__ __attribute__((aligned(16))) T buf0[(BM + BN) * BK<T>], buf1[(BM + BN) * BK<T>];
+    const int wid = xcd_remap(blockIdx.x, gridDim.x), tiles = s.tiles_m * s.tiles_n;
+    const int split = wid / tiles;
+    int tm, tn;
+    tile_of(s, wid - split * tiles, tm, tn);
+    const int64_t m0 = (int64_t)tm * BM;
+    const int n0 = tn * BN;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int ra = wave / WC * (BM / WR), rb = wave % WC * (BN / WC);
+    const int64_t nk = (s.K + BK<T> - 1) / BK<T>, kt0 = split * s.ktiles, kt1 = min(nk, kt0 + s.ktiles);
+
+    f32x16 acc[MI][NI];
+    if constexpr (sizeof(T) == 4) {
+        tile_product<T, BM, BN, WR, WC, true>(s, m0, n0, kt0, kt1, buf0, buf1, acc);
+        float odd = 0.f;  // NaN once a sum is not finite
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) odd += 0.f * acc[i][j][r];
+        if (__syncthreads_or(odd != odd)) {  // infinities have no triple: those sums, and no others, from fp32 products
+            f32x16 whole[MI][NI];
+            tile_product<T, BM, BN, WR, WC, false>(s, m0, n0, kt0, kt1, buf0, buf1, whole);
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[i][j][r] = fabsf(acc[i][j][r]) < __builtin_huge_valf() ? acc[i][j][r] : whole[i][j][r];
+        }
+    } else {
+        tile_product<T, BM, BN, WR, WC, false>(s, m0, n0, kt0, kt1, buf0, buf1, acc);
     }
 
     // 32 rows x CW columns of this wave at a time through LDS of its own, read back along rows

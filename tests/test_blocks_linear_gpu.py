@@ -245,3 +245,42 @@ def test_refusals():
                 lambda: ops.linear_act(x, w.cpu(), b)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+def test_fp32_products_over_the_exponent_range():
+    """fp32: rows and columns from 2^-40 to 2^40, and a matrix whose rows carry all 24 bits.  Each product is within 2^-21.9 of
+    itself (1 unit of 2^-24 for the bound's own rounding, 4 for the parts of the operands that are not multiplied), sums as in
+    `reference`."""
+    from dss_vae_amd import ops
+    for M, N, K in ((70, 50, 33), (300, 260, 600), (129, 600, 2000)):
+        x, w = rnd(M, K, seed=31), rnd(N, K, seed=32)
+        x = x * 2.0 ** torch.arange(-40, 40, 80 / M)[:M, None].round()
+        w = w * 2.0 ** torch.arange(40, -40, -80 / N)[:N, None].round()
+        want, mag = x.double() @ w.double().t(), x.double().abs() @ w.double().abs().t()
+        check(ops.linear_act(x.to(DEV), w.to(DEV)), want, mag, 3 * math.sqrt(K) + 8 + 5, ("range", M, N, K))
+    # 24-bit integers whose products and sums are exact in fp32: (2^23 + odd) x 1, one to a row
+    x = torch.zeros(64, 64)
+    x[torch.arange(64), torch.arange(64)] = (2 ** 23 + 2 * torch.arange(64) + 1).float()
+    assert torch.equal(ops.linear_act(x.to(DEV), torch.eye(64, device=DEV)).cpu(), x)
+    assert torch.equal(ops.linear_act(-x.to(DEV), torch.eye(64, device=DEV) * 2.0 ** -60).cpu(), -x * 2.0 ** -60)
+
+
+def test_fp32_infinities_and_the_largest_values():
+    """infinite, largest finite and overflowing sums come out as fp32 products give them; other rows keep their bits"""
+    from dss_vae_amd import ops
+    big = torch.finfo(torch.float32).max
+    for M, N, K in ((40, 30, 20), (200, 140, 300)):
+        x, w = rnd(M, K, seed=41).to(DEV), rnd(N, K, seed=42).to(DEV).abs() + 0.5
+        x[3] = 0.0
+        x[3, 5] = float("inf")
+        x[7] = 0.0
+        x[7, 2] = big
+        x[9] = big
+        x[11, 0], x[11, 1] = float("inf"), float("-inf")
+        w[:, 2] = 0.75
+        keep = [i for i in range(M) if i not in (3, 7, 9, 11)]
+        y = ops.linear_act(x, w)
+        assert (y[3] == float("inf")).all() and (y[7] == big * 0.75).all() and (y[9] == float("inf")).all() and y[11].isnan().all()
+        finite = x.clone()
+        finite[[3, 7, 9, 11]] = 0.0
+        assert torch.equal(bits(ops.linear_act(finite, w)[keep]), bits(y[keep]))
