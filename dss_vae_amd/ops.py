@@ -1880,6 +1880,28 @@ def _contig(t):
     return None if t is None else t.contiguous()
 
 
+_ACCUMULATE = type(torch.autograd.graph.get_gradient_edge(torch.zeros(1, requires_grad=True)).node)
+
+
+def _leaves_elsewhere(node, stream):
+    """Notes on the leaves behind an autograd node the stream they were first used on -> whether one was noted for another.
+    Autograd makes a leaf's accumulation node on the stream of its first use and keeps it while any graph holds it."""
+    other = False
+    for n, _ in node.next_functions:
+        if type(n) is _ACCUMULATE and n.metadata.setdefault("dssvae_stream", stream) != stream:
+            other = True
+    return other
+
+
+def _record(what, ctx, dev):
+    """Before an operator records its graph: under capture, refuses leaves that an older graph still holds on another stream.
+    Their gradients would be handed over on that stream, which a capture does not survive (the process ends)."""
+    if _leaves_elsewhere(ctx, torch._C._cuda_getCurrentRawStream(dev.index)) and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("%s: this stream is being captured, and a graph that was recorded on another stream still holds a "
+                           "parameter or input of this call: drop that graph (its outputs) first, or record it on the "
+                           "capturing stream" % what)
+
+
 def _layer_norm_fwd(x2, ldx, code, w, b, eps, stats):
     R, D = x2.shape
     y = x2.new_empty((R, D))
@@ -1895,6 +1917,7 @@ class _LayerNormFn(Function):
     @staticmethod
     def forward(ctx, x, w, b, eps, code):
         ctx.set_materialize_grads(False)
+        _record("layer_norm", ctx, x.device)
         x2, ldx = _matrix(_flat(x))
         stats = torch.empty((x2.size(0), 2), device=x.device, dtype=torch.float32)
         y = _layer_norm_fwd(x2, ldx, code, _contig(w), _contig(b), eps, stats)
@@ -1961,6 +1984,14 @@ def _sequence(t):
     return t
 
 
+def _meet(a, b):
+    """do two tensors' spans of memory overlap?"""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (p, m), (q, n) = ((t.data_ptr(), (1 + sum((d - 1) * s for d, s in zip(t.shape, t.stride()))) * t.element_size()) for t in (a, b))
+    return p < q + n and q < p + m
+
+
 def _gated_step(x, ldx, code, h, tanh, out, h_out):
     B, H = x.size(0), x.size(-1) // 2
     _go("dssvae_gated_step", x.device, (x.data_ptr(), ldx, code, _p(h), tanh, B, H, out.data_ptr(), H, h_out.data_ptr()),
@@ -1993,6 +2024,7 @@ class _GatedScanFn(Function):
     @staticmethod
     def forward(ctx, x, h0, lengths, reverse, tanh, code):
         ctx.set_materialize_grads(False)
+        _record("gated_scan", ctx, x.device)
         xs = _sequence(x)
         out, h_last, ckpt = _gated_scan_fwd(xs, _contig(h0), lengths, reverse, tanh, code, True)
         ctx.save_for_backward(xs, lengths, ckpt)
@@ -2061,7 +2093,7 @@ def gated_scan(xproj, h0=None, lengths=None, reverse=False, candidate="tanh"):
 def gated_step(xproj, h=None, candidate="tanh", h_out=None):
     """one step of gated_scan for xproj [B, 2H] and the state h [B, H] float32 (None = zeros) -> (out [B, H] of xproj's
     type, new state [B, H] float32).  h_out: a contiguous float32 buffer the new state is written to; it may be h itself
-    (then the state is updated in place), but must not overlap it otherwise."""
+    (then the state is updated in place), but must not overlap it otherwise, nor xproj."""
     code = _typed("gated_step", xproj)
     tanh = _candidate("gated_step", candidate)
     if xproj.dim() != 2 or xproj.size(1) < 2 or xproj.size(1) % 2:
@@ -2073,6 +2105,9 @@ def gated_step(xproj, h=None, candidate="tanh", h_out=None):
         _expect("gated_step", "h_out", h_out, (B, H), (torch.float32,), xproj.device)
         if not h_out.is_contiguous():
             raise RuntimeError("gated_step: h_out must be contiguous")
+        for name, t in (("h", h), ("xproj", xproj)):
+            if t is not None and not (t is h and t.data_ptr() == h_out.data_ptr()) and _meet(t, h_out):
+                raise RuntimeError("gated_step: h_out overlaps %s" % name)
     if _wants_grad(xproj, h):
         if h_out is not None:
             raise RuntimeError("gated_step: h_out is for serving (no gradients)")
@@ -2115,6 +2150,7 @@ class _DistillFn(Function):
     @staticmethod
     def forward(ctx, logits, ids, teacher, weight, tau, code):
         ctx.set_materialize_grads(False)
+        _record("distill_loss", ctx, logits.device)
         z, ldz = _matrix(_flat(logits))
         total, rows, ctx.dz = _distill(z, ldz, code, ids, teacher, tau, weight, True)
         ctx.shape, ctx.code = logits.shape, code
@@ -2199,6 +2235,7 @@ class _LinearActFn(Function):
     @staticmethod
     def forward(ctx, x, w, b, residual, act, code):
         ctx.set_materialize_grads(False)
+        _record("linear_act", ctx, x.device)
         N = w.size(0)
         x2, ldx = _matrix(_flat(x))
         wc, ldw = _matrix(w)

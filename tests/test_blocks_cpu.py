@@ -125,3 +125,20 @@ def test_backward_runs_on_the_calling_thread():
         out = subprocess.run([sys.executable, "-c", src], env=dict(os.environ, DSSVAE_AUTOGRAD_THREADS=value), capture_output=True, text=True)
         assert out.stdout.strip() == want, out.stderr
     assert isinstance(L.load().dssvae_distill, C._CFuncPtr)
+
+
+def test_leaves_of_older_graphs_are_noticed():
+    """the stream a leaf was first used on is noted while a graph holds it, and forgotten with the graph"""
+    from dss_vae_amd import ops
+    a, b = torch.ones(3, requires_grad=True), torch.ones(3, requires_grad=True)
+    y = a * b
+    assert not ops._leaves_elsewhere(y.grad_fn, 7)
+    z = a * 2
+    assert not ops._leaves_elsewhere(z.grad_fn, 7) and ops._leaves_elsewhere(z.grad_fn, 8)
+    c = b * 3
+    del y, z
+    fresh = a * 2
+    assert not ops._leaves_elsewhere(fresh.grad_fn, 8)
+    assert ops._leaves_elsewhere(c.grad_fn, 8)
+    inner = fresh * 2  # (no leaf right behind it)
+    assert not ops._leaves_elsewhere(inner.grad_fn, 9)

@@ -264,3 +264,21 @@ def test_refusals():
                 lambda: ops.gated_step(x[:, 0].clone().requires_grad_(), h, h_out=h)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+def test_step_refuses_overlapping_buffers():
+    from dss_vae_amd import ops
+    buf = torch.zeros(100, device=DEV)
+    h = buf[:8].view(2, 4)
+    x = torch.ones(2, 8, device=DEV)
+    for h_out in (buf[4:12].view(2, 4), buf[7:15].view(2, 4)):
+        with pytest.raises(RuntimeError, match="h_out overlaps h"):
+            ops.gated_step(x, h, h_out=h_out)
+    with pytest.raises(RuntimeError, match="h_out overlaps xproj"):
+        ops.gated_step(buf[16:32].view(2, 8), h, h_out=buf[30:38].view(2, 4))
+    with pytest.raises(RuntimeError, match="h_out overlaps h"):  # (a transposed view of the same memory)
+        ops.gated_step(x, buf[:8].view(4, 2).t(), h_out=buf[1:9].view(2, 4))
+    want = ops.gated_step(x, h)[1].clone()
+    assert torch.equal(ops.gated_step(x, h, h_out=buf[8:16].view(2, 4))[1], want)
+    ops.gated_step(x, h, h_out=h)
+    assert torch.equal(h, want)

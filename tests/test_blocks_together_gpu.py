@@ -223,3 +223,34 @@ def test_two_graphs_side_by_side():
         torch.cuda.synchronize()
         for a, b in zip(outs, want):
             assert all(torch.equal(p.detach(), q) for p, q in zip(a, b)), k
+
+
+def test_capture_refuses_leaves_of_a_graph_on_another_stream():
+    """an eager graph of the same leaves lives: every operator refuses the capture before it records anything, the capture ends
+    in order, and once that graph is gone the same step is captured and replays"""
+    from dss_vae_amd import ops
+    x = torch.randn(6, 8, 32, device=DEV).requires_grad_()
+    w = torch.randn(32, 32, device=DEV).requires_grad_()
+    ids, t = torch.zeros(6, 8, 1, dtype=torch.int64, device=DEV), torch.zeros(6, 8, 1, device=DEV)
+    calls = {"layer_norm": lambda: ops.layer_norm(x).sum(), "gated_scan": lambda: ops.gated_scan(x)[0].sum(),
+             "linear_act": lambda: ops.linear_act(x, w, None, "tanh").sum(), "distill_loss": lambda: ops.distill_loss(x, ids, t)[0]}
+    for name, call in calls.items():
+        want = torch.autograd.grad(call(), x)[0]
+        held = call()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = torch.ones(4, device=DEV) * 2
+            with pytest.raises(RuntimeError, match="%s: this stream is being captured" % name):
+                call()
+        del held, g, y
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            got = torch.autograd.grad(call(), x)[0]
+        for _ in range(3):
+            got.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want), name
