@@ -261,7 +261,7 @@ struct Loader {
 };
 
 // Eight fp32 values as sums of three bf16 each, x = p0 + p1 + p2 exactly (the first rounded to nearest, so that the rest has
-// either sign, the others cut off; p2 runs out of exponent below 2^-110: what is smaller than 2^-134 is dropped).  Infinities, and
+// either sign, the others cut off; p2 runs out of exponent below 2^-110: what is smaller than 2^-133 is dropped).  Infinities, and
 // the last 0.4 % below the largest finite value, become NaN.
 struct Split {
     Mfma<bf16_t>::V p[3];
