@@ -17,7 +17,8 @@
 // The backward operands that are contiguous the other way (w and x along the summed axis, dz for dw) are transposed into the
 // workspace first: dz in both orders by the pass that forms it, which also leaves the column sums for db.
 // Few output tiles: K is split over blocks, fp32 partials go to the workspace and a second launch adds them in order and
-// applies the epilogue (no atomics: same bits every time).
+// applies the epilogue (no atomics: same bits every time).  Backward is three launches: the transposes, both products, and
+// the partials with db's column sums.
 #include "elem.h"
 
 namespace {
@@ -347,6 +348,11 @@ struct Shape {
     float* part;         // [ksplit][M][N] where ksplit > 1
 };
 
+// A launch makes one or two products (dx and dw of a backward call: one fills the CUs that the other leaves idle): blocks
+// 0 .. first - 1 are the first one's.
+struct Job { Shape s; Epilogue e; int blocks; };
+struct Jobs { Job job[2]; int first; };
+
 // output tile of work item `wid`: groups of 8 tile rows, column by column inside a group, so that the blocks of an XCD that run
 // together share operand panels in its L2
 __device__ __forceinline__ void tile_of(const Shape& s, int t, int& tm, int& tn) {
@@ -500,10 +506,13 @@ __device__ __forceinline__ void tile_product(const Shape& s, int64_t m0, int n0,
 }
 
 template <typename T, int BM, int BN, int WR, int WC>
-__global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, Epilogue e) {
+__global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Jobs jobs) {
     constexpr int MI = BM / WR / 32, NI = BN / WC / 32;
     __shared__ __attribute__((aligned(16))) T buf0[(BM + BN) * BK<T>], buf1[(BM + BN) * BK<T>];
-    const int wid = xcd_remap(blockIdx.x, gridDim.x), tiles = s.tiles_m * s.tiles_n;
+    const int which = (int)blockIdx.x >= jobs.first;
+    const Shape& s = jobs.job[which].s;
+    const Epilogue& e = jobs.job[which].e;
+    const int wid = xcd_remap(blockIdx.x - (which ? jobs.first : 0), jobs.job[which].blocks), tiles = s.tiles_m * s.tiles_n;
     const int split = wid / tiles;
     int tm, tn;
     tile_of(s, wid - split * tiles, tm, tn);
@@ -579,12 +588,40 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Shape s, E
     }
 }
 
-// partials of the K splits, added in order, then the epilogue: 8 columns a thread
+// What is left behind the tile kernel, in one launch: blocks begin[i] .. begin[i + 1] add the partials of product i's K splits in
+// order and apply its epilogue, 8 columns a thread; the last ones add the rows of db's partial sums in a fixed order, 8 columns a
+// block, 32 threads to a column.
+struct Rest {
+    const float* part[2]; int ksplit[2]; int64_t M[2]; int N[2]; Epilogue e[2];
+    const float* sums; int n; int64_t C; void* db; int db_f32;
+    int begin[3];
+};
+
 template <typename T>
-__global__ __launch_bounds__(256) void linear_join_kernel(const float* __restrict__ part, int ksplit, int64_t M, int N,
-                                                          Epilogue e) {
-    const int per = (N + 7) / 8;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void linear_rest_kernel(Rest a) {
+    __shared__ float red[32][9];
+    const int block = (int)blockIdx.x;
+    if (block >= a.begin[2]) {
+        const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
+        const int64_t c = (int64_t)(block - a.begin[2]) * 8 + tx;
+        float s = 0.f;
+        if (c < a.C)
+            for (int i = ty; i < a.n; i += 32) s += a.sums[(int64_t)i * a.C + c];
+        red[ty][tx] = s;
+        __syncthreads();
+        if (ty != 0 || c >= a.C) return;
+#pragma unroll
+        for (int i = 1; i < 32; ++i) s += red[i][tx];
+        if (a.db_f32) reinterpret_cast<float*>(a.db)[c] = s;
+        else reinterpret_cast<T*>(a.db)[c] = (T)s;
+        return;
+    }
+    const int which = block >= a.begin[1];
+    const Epilogue& e = a.e[which];
+    const float* part = a.part[which];
+    const int64_t M = a.M[which];
+    const int N = a.N[which], ksplit = a.ksplit[which], per = (N + 7) / 8;
+    const int64_t i = (int64_t)(block - a.begin[which]) * 256 + threadIdx.x;
     if (i >= M * per) return;
     const int64_t m = i / per;
     const int n = (int)(i % per) * 8;
@@ -594,9 +631,9 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const float* __restric
     for (int k = 0; k < ksplit; ++k) {
         const float* p = part + ((int64_t)k * M + m) * N + n;
         if (n + 8 <= N && N % 4 == 0) {
-            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-            v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-            v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+            const float4 f = reinterpret_cast<const float4*>(p)[0], g = reinterpret_cast<const float4*>(p)[1];
+            v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
+            v[4] += g.x; v[5] += g.y; v[6] += g.z; v[7] += g.w;
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -742,65 +779,77 @@ __global__ __launch_bounds__(256) void linear_turn_kernel(Turns jobs) {
     }
 }
 
-// db [C] = sum of n rows of partial sums in a fixed order: 32 columns per block, 32 threads share a column
-template <typename T>
-__global__ __launch_bounds__(1024) void linear_db_kernel(const float* __restrict__ sums, int n, int64_t C, void* db, int f32) {
-    __shared__ float red[32][33];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int64_t c = (int64_t)blockIdx.x * 32 + tx;
-    float s = 0.f;
-    if (c < C)
-        for (int i = ty; i < n; i += 32) s += sums[(int64_t)i * C + c];
-    red[ty][tx] = s;
-    __syncthreads();
-    if (ty != 0 || c >= C) return;
-#pragma unroll
-    for (int i = 1; i < 32; ++i) s += red[i][tx];
-    if (f32) reinterpret_cast<float*>(db)[c] = s;
-    else reinterpret_cast<T*>(db)[c] = (T)s;
-}
-
 // ---- host ---------------------------------------------------------------------------------------------------------
 inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Tile width and K split: the smallest of a modelled time in microseconds.  u: a 128 x 128 step of a CU at the rate that the
-// 256-wide (fp32: 128-wide) kernel reaches.  Narrower tiles read more LDS per product; a step takes at least the latency of the
-// loads it waits for; every round of blocks has a prologue and an epilogue; partials cost their traffic and a launch.  (A sweep
-// over 17 shapes and all choices in both widths: within 10 % of the best one for all but the smallest.)
+// Tile width and K splits of a launch's products: the smallest of a modelled time in microseconds,
+//   max(work of all blocks over the CUs, the longest block's steps) + prologue and epilogue + partials' traffic,
+// with `per` the time of a step at a CU's full rate and `least` what a step takes a block alone (the latency of its loads).  The
+// work counts as if every CU took as many blocks as the fullest.  (Sweeps of both, 9 forward and 6 backward shapes: within 10 % of
+// the best choice but for the smallest, which one launch's time decides.)
 struct Plan { int tile, ksplit; };
-template <typename T>
-inline Plan plan(int64_t M, int64_t N, int64_t K) {
+struct Extent { int64_t M, N, K; };
+template <typename T> constexpr int MAX_TILE = sizeof(T) == 4 ? 128 : 256;
+template <typename T, int COUNT>
+inline void plan_products(const Extent (&x)[COUNT], Plan (&best)[COUNT]) {
     static const int splits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
     const bool f32 = sizeof(T) == 4;
-    const double cus = device_cus(), u = f32 ? 2.0 : 0.42;
-    const int64_t nk = up(K, BK<T>) / BK<T>;
-    Plan best{64, 1};
-    double least = -1;
-    for (int tile = f32 ? 128 : 256; tile >= 64; tile /= 2)
-        for (int ks : splits) {
-            if (ks > 1 && nk / ks < 4) break;
-            const double per = tile == 256 ? 4 * u : tile == 128 ? (f32 ? u : 1.35 * u) : (f32 ? 0.3 * u : 0.5 * u);
-            const double least_step = tile == 256 ? 1.7 : tile == 128 ? 0.8 : 0.35;  // a step's load latency
-            const double wait = tile == 256 ? 8 : tile == 128 ? 5 : 3;
-            const int resident = tile == 256 ? 1 : tile == 128 ? 2 : 4;
-            const double tiles = (double)(up(M, tile) / tile) * (double)(up(N, tile) / tile) * ks;
-            const double load = (double)(int64_t)((tiles + cus - 1) / cus);  // blocks of the fullest CU
-            const double step = load * per > least_step ? load * per : least_step;
-            double cost = step * (double)((nk + ks - 1) / ks) + (double)(int64_t)((load + resident - 1) / resident) * wait;
-            if (ks > 1) cost += 4 + (double)(2 * ks + 1) * M * N * 4 / 4e6;
-            if (least < 0 || cost < least) {
-                least = cost;
-                best = Plan{tile, ks};
+    const double cus = device_cus();
+    double lowest = -1;
+    for (int tile = MAX_TILE<T>; tile >= 64; tile /= 2) {
+        const double per = f32 ? (tile == 128 ? 1.33 : 0.5) : tile == 256 ? 1.68 : tile == 128 ? 0.57 : 0.3;
+        const double least = f32 ? (tile == 128 ? 1.45 : 0.5) : tile == 256 ? 1.7 : tile == 128 ? 0.8 : 0.35;
+        const double wait = tile == 256 ? 8 : tile == 128 ? 5 : 3;
+        double work = 0;
+        for (const Extent& e : x) work += (double)(up(e.M, tile) / tile) * (double)(up(e.N, tile) / tile) * (double)(up(e.K, BK<T>) / BK<T>);
+        work *= per / cus;
+        double blocks = 0, chain = 0, join = 0;
+        Plan p[COUNT];
+        for (int i = 0; i < COUNT; ++i) {
+            const Extent& e = x[i];
+            const int64_t nk = up(e.K, BK<T>) / BK<T>;
+            double low = -1, chain_i = 0, join_i = 0;
+            for (int ks : splits) {
+                if (ks > 1 && nk / ks < 4) break;
+                const double steps = (double)((nk + ks - 1) / ks) * least;
+                const double more = ks > 1 ? 6 + (double)(2 * ks + 1) * (double)e.M * (double)e.N * 4 / 6e6 : 0;
+                const double cost = (steps > work ? steps : work) + more;
+                if (low < 0 || cost < low) {
+                    low = cost;
+                    chain_i = steps;
+                    join_i = more;
+                    p[i] = Plan{tile, ks};
+                }
             }
+            blocks += (double)(up(e.M, tile) / tile) * (double)(up(e.N, tile) / tile) * p[i].ksplit / cus;
+            chain = chain_i > chain ? chain_i : chain;
+            join += join_i;
         }
-    return best;
+        const double full = blocks > 1 ? work * (double)((int64_t)blocks + (blocks > (double)(int64_t)blocks)) / blocks : work;
+        const double cost = (full > chain ? full : chain) + wait + join;
+        if (lowest < 0 || cost < lowest) {
+            lowest = cost;
+            for (int i = 0; i < COUNT; ++i) best[i] = p[i];
+        }
+    }
 }
-
 template <typename T>
-inline int64_t part_bytes(int64_t M, int64_t N, int64_t K) {
-    const Plan p = plan<T>(M, N, K);
-    return p.ksplit > 1 ? up((int64_t)p.ksplit * M * N * 4, 256) : 0;
+inline Plan plan(int64_t M, int64_t N, int64_t K) {
+    const Extent x[1] = {{M, N, K}};
+    Plan p[1];
+    plan_products<T, 1>(x, p);
+    return p[0];
 }
+// dx [M, K] over N and dw [N, K] over M, whichever of them a call wants (its bits do not depend on that)
+struct Plans { Plan x, w; };
+template <typename T>
+inline Plans plan_bwd(int64_t M, int64_t N, int64_t K) {
+    const Extent x[2] = {{M, K, up(N, GR<T>)}, {N, K, up(M, GR<T>)}};
+    Plan p[2];
+    plan_products<T, 2>(x, p);
+    return Plans{p[0], p[1]};
+}
+inline int64_t part_bytes(const Plan& p, int64_t M, int64_t N) { return p.ksplit > 1 ? up((int64_t)p.ksplit * M * N * 4, 256) : 0; }
 
 // operand rows usable as they are: 16-byte granules, and the 256 rows of a tile within 32-bit byte offsets
 constexpr int64_t MAX_LD = 1 << 21;
@@ -809,37 +858,63 @@ inline bool direct(const void* p, int64_t ld, int64_t K) {
     return aligned_to(p, 16) && ld % GR<T> == 0 && K % GR<T> == 0 && ld <= MAX_LD;
 }
 
+// C [M, N] = A [M, K] . B [N, K]^T and its epilogue, as a list of up to two for one launch
 template <typename T>
-int product(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K, Epilogue e, void* part,
-            hipStream_t st) {
-    if (M == 0 || N == 0) return DSSVAE_OK;
-    const Plan p = plan<T>(M, N, K);
-    const int b = p.tile;
-    Shape s;
-    s.A = A; s.lda = lda; s.B = B; s.ldb = ldb; s.M = M; s.N = (int)N; s.K = K;
-    const int64_t tm = up(M, b) / b, tn = up(N, b) / b;
-    if (tm * tn * p.ksplit > 0x7fffffff) return DSSVAE_ETOOBIG;
-    s.tiles_m = (int)tm; s.tiles_n = (int)tn; s.ksplit = p.ksplit;
-    const int64_t nk = up(K, BK<T>) / BK<T>;
-    s.ktiles = (nk + p.ksplit - 1) / p.ksplit;
-    s.part = (float*)part;
-    const dim3 grid((unsigned)(tm * tn * p.ksplit));
-    if (b == 256) {
-        if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, 4>), grid, dim3(512), 0, st, s, e);
-    } else if (b == 128) {
-        hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, 2>), grid, dim3(256), 0, st, s, e);
-    } else {
-        hipLaunchKernelGGL((linear_tile_kernel<T, 64, 64, 2, 2>), grid, dim3(256), 0, st, s, e);
+struct Products {
+    Jobs jobs{};
+    Rest rest{};
+    int n = 0, tile = 0;
+    int add(const Plan& p, const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K, const Epilogue& e,
+            void* part) {
+        if (M == 0 || N == 0) return DSSVAE_OK;
+        Shape s;
+        s.A = A; s.lda = lda; s.B = B; s.ldb = ldb; s.M = M; s.N = (int)N; s.K = K;
+        const int64_t tm = up(M, p.tile) / p.tile, tn = up(N, p.tile) / p.tile, blocks = tm * tn * p.ksplit;
+        const int64_t join = p.ksplit > 1 ? (M * ((N + 7) / 8) + 255) / 256 : 0;
+        if (blocks > 0x3fffffff || join > 0x3fffffff) return DSSVAE_ETOOBIG;
+        s.tiles_m = (int)tm; s.tiles_n = (int)tn; s.ksplit = p.ksplit;
+        const int64_t nk = up(K, BK<T>) / BK<T>;
+        s.ktiles = (nk + p.ksplit - 1) / p.ksplit;
+        s.part = (float*)part;
+        jobs.job[n] = Job{s, e, (int)blocks};
+        if (n == 0) jobs.first = (int)blocks;
+        rest.part[n] = s.part; rest.ksplit[n] = p.ksplit; rest.M[n] = M; rest.N[n] = (int)N; rest.e[n] = e;
+        rest.begin[n + 1] = rest.begin[n] + (int)join;
+        tile = p.tile;
+        ++n;
+        return DSSVAE_OK;
     }
-    DSSVAE_CHECK_LAUNCH();
-    if (p.ksplit > 1) {
-        const int64_t n = M * ((N + 7) / 8), blocks = (n + 255) / 256;
-        if (blocks > 0x7fffffff) return DSSVAE_ETOOBIG;
-        hipLaunchKernelGGL((linear_join_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, st, s.part, p.ksplit, M, (int)N, e);
+    int run(hipStream_t st) {
+        if (n == 0) return DSSVAE_OK;
+        if (n > 1 && jobs.job[1].s.ktiles > jobs.job[0].s.ktiles) {  // the blocks with more steps start first
+            const Job j = jobs.job[0];
+            jobs.job[0] = jobs.job[1];
+            jobs.job[1] = j;
+            jobs.first = jobs.job[0].blocks;
+        }
+        const dim3 grid((unsigned)(jobs.first + (n > 1 ? jobs.job[1].blocks : 0)));
+        if (tile == 256) {
+            if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, 4>), grid, dim3(512), 0, st, jobs);
+        } else if (tile == 128) {
+            hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, 2>), grid, dim3(256), 0, st, jobs);
+        } else {
+            hipLaunchKernelGGL((linear_tile_kernel<T, 64, 64, 2, 2>), grid, dim3(256), 0, st, jobs);
+        }
         DSSVAE_CHECK_LAUNCH();
+        return DSSVAE_OK;
     }
-    return DSSVAE_OK;
-}
+    // the splits' partials and, with db, its column sums from n_sums rows of partial ones
+    int finish(hipStream_t st, const float* sums = nullptr, int n_sums = 0, int64_t C = 0, void* db = nullptr, int db_f32 = 0) {
+        for (int i = n; i < 2; ++i) rest.begin[i + 1] = rest.begin[i];
+        rest.sums = sums; rest.n = n_sums; rest.C = C; rest.db = db; rest.db_f32 = db_f32;
+        const int64_t blocks = rest.begin[2] + (db ? (C + 7) / 8 : 0);
+        if (blocks > 0x7fffffff) return DSSVAE_ETOOBIG;
+        if (blocks == 0) return DSSVAE_OK;
+        hipLaunchKernelGGL((linear_rest_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, st, rest);
+        DSSVAE_CHECK_LAUNCH();
+        return DSSVAE_OK;
+    }
+};
 
 template <typename T>
 int pack(const void* src, int64_t ld, int64_t R, int64_t C, void* dst, int64_t ldd, hipStream_t st) {
@@ -913,8 +988,13 @@ int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, i
         if (!dry) { const int rc = pack<T>(w, ldw, N, K, d, ldk, st); if (rc) return rc; }
         w = d; ldw = ldk;
     }
-    void* part = sp.take(part_bytes<T>(M, N, ldk));
-    return dry ? DSSVAE_OK : product<T>(x, ldx, w, ldw, M, N, ldk, e, part, st);
+    const Plan p = plan<T>(M, N, ldk);
+    void* part = sp.take(part_bytes(p, M, N));
+    if (dry) return DSSVAE_OK;
+    Products<T> l;
+    int rc = l.add(p, x, ldx, w, ldw, M, N, ldk, e, part);
+    if (!rc) rc = l.run(st);
+    return rc ? rc : l.finish(st);
 }
 
 struct BwdArgs {
@@ -939,29 +1019,28 @@ int backward(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
     float* sums = a.db ? (float*)sp.take(turn_rows(M, N) * N * 4) : nullptr;
     void* wt = a.dx ? sp.take(K * ldn * es) : nullptr;
     void* xt = a.dw ? sp.take(K * ldm * es) : nullptr;
-    void* part_x = a.dx ? sp.take(part_bytes<T>(M, K, ldn)) : nullptr;
-    void* part_w = a.dw ? sp.take(part_bytes<T>(N, K, ldm)) : nullptr;
+    const Plans p = plan_bwd<T>(M, N, K);
+    void* part_x = a.dx ? sp.take(part_bytes(p.x, M, K)) : nullptr;
+    void* part_w = a.dw ? sp.take(part_bytes(p.w, N, K)) : nullptr;
     if (dry) return rc;
     TurnList l{es};
     if (copy || a.dw || a.db) l.add(a.dy, a.lddy, a.z, a.ldz, M, N, dzc, ldn, dzt, ldm, sums);
     if (a.dx) l.add(a.w, a.ldw, nullptr, 0, N, K, nullptr, 0, wt, ldn, nullptr);
     if (a.dw) l.add(a.x, a.ldx, nullptr, 0, M, K, nullptr, 0, xt, ldm, nullptr);
     if ((rc = turn<T>(l, a.act, st))) return rc;
-    if (a.db) {
-        hipLaunchKernelGGL((linear_db_kernel<T>), dim3((unsigned)((N + 31) / 32)), dim3(1024), 0, st, sums, (int)turn_rows(M, N), N, a.db,
-                           a.db_f32);
-        DSSVAE_CHECK_LAUNCH();
-    }
-    Epilogue e{};
+    Products<T> q;
     if (a.dx) {
+        Epilogue e{};
         e.y = a.dx; e.ldy = a.lddx;
-        if ((rc = product<T>(dz, lddz, wt, ldn, M, K, ldn, e, part_x, st))) return rc;
+        if ((rc = q.add(p.x, dz, lddz, wt, ldn, M, K, ldn, e, part_x))) return rc;
     }
     if (a.dw) {
+        Epilogue e{};
         e.y = a.dw; e.ldy = a.lddw;
-        if ((rc = product<T>(dzt, ldm, xt, ldm, N, K, ldm, e, part_w, st))) return rc;
+        if ((rc = q.add(p.w, dzt, ldm, xt, ldm, N, K, ldm, e, part_w))) return rc;
     }
-    return rc;
+    if ((rc = q.run(st))) return rc;
+    return q.finish(st, sums, a.db ? (int)turn_rows(M, N) : 0, N, a.db, a.db_f32);
 }
 
 int bwd_any(int dtype, const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
