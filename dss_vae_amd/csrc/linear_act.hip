@@ -644,12 +644,26 @@ __global__ __launch_bounds__(256) void linear_rest_kernel(Rest a) {
 }
 
 // ---- operands into the form the tile kernel takes -----------------------------------------------------------------
-// dst [R, ldd] = src [R, C], columns C .. ldd zero
+// dst [R, ldd] = src [R, C], columns C .. ldd zero; ldd is a multiple of a granule, src starts and ends anywhere.  A launch
+// copies one or two matrices: blocks 0 .. first - 1 are the first one's.
+struct Pack { const void* src; int64_t ld, R, C; void* dst; int64_t ldd; };
+struct Packs { Pack job[2]; int first; };
+
 template <typename T>
-__global__ __launch_bounds__(256) void linear_pack_kernel(const T* __restrict__ src, int64_t ld, int64_t R, int64_t C,
-                                                          T* __restrict__ dst, int64_t ldd) {
-    for (int64_t r = blockIdx.x; r < R; r += gridDim.x)
-        for (int64_t c = threadIdx.x; c < ldd; c += 256) dst[r * ldd + c] = c < C ? src[r * ld + c] : (T)0.f;
+__global__ __launch_bounds__(256) void linear_pack_kernel(Packs p) {
+    const int which = (int)blockIdx.x >= p.first;
+    const Pack& j = p.job[which];
+    const T* __restrict__ src = (const T*)j.src;
+    T* __restrict__ dst = (T*)j.dst;
+    const int64_t per = j.ldd / GR<T>, n = j.R * per;
+    const int block = (int)blockIdx.x - (which ? p.first : 0), blocks = which ? (int)gridDim.x - p.first : p.first;
+    for (int64_t i = (int64_t)block * 256 + threadIdx.x; i < n; i += (int64_t)blocks * 256) {
+        const int64_t r = i / per;
+        const int c = (int)(i - r * per) * GR<T>;
+        GranU<T, GR<T>> g;
+        load_cols<false, T, GR<T>>(g, src + r * j.ld, c, (int)j.C);
+        g.store(dst + r * j.ldd + c);
+    }
 }
 
 // One pass over a [R, C] matrix in 64 x 64 tiles (a block walks the row tiles first, + stride, .. of one column tile):
@@ -916,12 +930,21 @@ struct Products {
     }
 };
 
+struct PackList {
+    Packs p{};
+    int n = 0, blocks = 0;
+    void add(const void* src, int64_t ld, int64_t R, int64_t C, void* dst, int64_t ldd, int granule) {
+        const int64_t need = (R * (ldd / granule) + 255) / 256, most = 16 * (int64_t)device_cus();
+        p.job[n] = Pack{src, ld, R, C, dst, ldd};
+        if (n == 0) p.first = (int)(need < most ? need : most);
+        blocks += (int)(need < most ? need : most);
+        ++n;
+    }
+};
 template <typename T>
-int pack(const void* src, int64_t ld, int64_t R, int64_t C, void* dst, int64_t ldd, hipStream_t st) {
-    if (R == 0) return DSSVAE_OK;
-    const int64_t most = 16 * (int64_t)device_cus();
-    hipLaunchKernelGGL((linear_pack_kernel<T>), dim3((unsigned)(R < most ? R : most)), dim3(256), 0, st, (const T*)src, ld, R, C,
-                       (T*)dst, ldd);
+int pack(const PackList& l, hipStream_t st) {
+    if (l.blocks == 0) return DSSVAE_OK;
+    hipLaunchKernelGGL((linear_pack_kernel<T>), dim3((unsigned)l.blocks), dim3(256), 0, st, l.p);
     DSSVAE_CHECK_LAUNCH();
     return DSSVAE_OK;
 }
@@ -974,25 +997,29 @@ bool bad_args(int dtype, int act, int64_t M, int N, int K) {
            N > (1 << 30) || K > (1 << 30);
 }
 
+// (`p`: plan of the product, made where the call's workspace is added up and used where it is launched)
 template <typename T>
 int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int N, int K, const Epilogue& e, Space& sp, hipStream_t st,
-          bool dry) {
+            bool dry, Plan& p) {
     const int64_t ldk = up(K, GR<T>), es = sizeof(T);
+    PackList packs;
     if (!direct<T>(x, ldx, K)) {
         void* d = sp.take(M * ldk * es);
-        if (!dry) { const int rc = pack<T>(x, ldx, M, K, d, ldk, st); if (rc) return rc; }
+        packs.add(x, ldx, M, K, d, ldk, GR<T>);
         x = d; ldx = ldk;
     }
     if (!direct<T>(w, ldw, K)) {
         void* d = sp.take((int64_t)N * ldk * es);
-        if (!dry) { const int rc = pack<T>(w, ldw, N, K, d, ldk, st); if (rc) return rc; }
+        packs.add(w, ldw, N, K, d, ldk, GR<T>);
         w = d; ldw = ldk;
     }
-    const Plan p = plan<T>(M, N, ldk);
+    if (dry) p = plan<T>(M, N, ldk);
     void* part = sp.take(part_bytes(p, M, N));
     if (dry) return DSSVAE_OK;
+    int rc = pack<T>(packs, st);
+    if (rc) return rc;
     Products<T> l;
-    int rc = l.add(p, x, ldx, w, ldw, M, N, ldk, e, part);
+    rc = l.add(p, x, ldx, w, ldw, M, N, ldk, e, part);
     if (!rc) rc = l.run(st);
     return rc ? rc : l.finish(st);
 }
@@ -1003,10 +1030,11 @@ struct BwdArgs {
     void *dx, *dw, *db;
     int db_f32, act;
     int64_t M; int N, K;
+    Plans plans;  // made by the pass that adds up the workspace
 };
 
 template <typename T>
-int backward(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
+int backward(BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
     const int64_t M = a.M, N = a.N, K = a.K, ldn = up(N, GR<T>), ldm = up(M, GR<T>), es = sizeof(T);
     int rc = DSSVAE_OK;
     // dz: a copy where it differs from dy or dy's rows cannot be loaded as they are
@@ -1019,7 +1047,8 @@ int backward(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
     float* sums = a.db ? (float*)sp.take(turn_rows(M, N) * N * 4) : nullptr;
     void* wt = a.dx ? sp.take(K * ldn * es) : nullptr;
     void* xt = a.dw ? sp.take(K * ldm * es) : nullptr;
-    const Plans p = plan_bwd<T>(M, N, K);
+    if (dry) a.plans = plan_bwd<T>(M, N, K);
+    const Plans& p = a.plans;
     void* part_x = a.dx ? sp.take(part_bytes(p.x, M, K)) : nullptr;
     void* part_w = a.dw ? sp.take(part_bytes(p.w, N, K)) : nullptr;
     if (dry) return rc;
@@ -1043,20 +1072,27 @@ int backward(const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
     return q.finish(st, sums, a.db ? (int)turn_rows(M, N) : 0, N, a.db, a.db_f32);
 }
 
-int bwd_any(int dtype, const BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
+int bwd_any(int dtype, BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
     if (dtype == DSSVAE_F32) return backward<float>(a, sp, st, dry);
     return dtype == DSSVAE_BF16 ? backward<bf16_t>(a, sp, st, dry) : backward<f16_t>(a, sp, st, dry);
 }
 
 }  // namespace
 
+namespace {
+int64_t fwd_space(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype, int64_t M, int N, int K, Plan& p) {
+    Space sp{nullptr, 0, 0};
+    if (dtype == DSSVAE_F32) forward<float>(x, ldx, w, ldw, M, N, K, Epilogue{}, sp, nullptr, true, p);
+    else forward<bf16_t>(x, ldx, w, ldw, M, N, K, Epilogue{}, sp, nullptr, true, p);  // (fp16: the same sizes)
+    return sp.used;
+}
+}  // namespace
+
 extern "C" int64_t dssvae_linear_act_fwd_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int dtype,
                                                          int64_t M, int N, int K) {
     if (bad_args(dtype, DSSVAE_ACT_NONE, M, N, K)) return DSSVAE_EINVAL;
-    Space sp{nullptr, 0, 0};
-    if (dtype == DSSVAE_F32) forward<float>(x, ldx, w, ldw, M, N, K, Epilogue{}, sp, nullptr, true);
-    else forward<bf16_t>(x, ldx, w, ldw, M, N, K, Epilogue{}, sp, nullptr, true);  // (fp16: the same sizes)
-    return sp.used;
+    Plan p;
+    return fwd_space(x, ldx, w, ldw, dtype, M, N, K, p);
 }
 
 extern "C" int dssvae_linear_act_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int bias_f32,
@@ -1067,15 +1103,16 @@ extern "C" int dssvae_linear_act_fwd(const void* x, int64_t ldx, const void* w, 
     if (M == 0) return DSSVAE_OK;
     if (K > MAX_LD) return DSSVAE_ETOOBIG;
     if (!x || !w || !y || (z && z == y)) return DSSVAE_EINVAL;
-    const int64_t need = dssvae_linear_act_fwd_workspace_bytes(x, ldx, w, ldw, dtype, M, N, K);
+    Plan p;
+    const int64_t need = fwd_space(x, ldx, w, ldw, dtype, M, N, K, p);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned_to(workspace, 16))) return DSSVAE_EINVAL;
     hipStream_t st = (hipStream_t)stream;
     Epilogue e{};
     e.bias = bias; e.bias_f32 = bias_f32 || dtype == DSSVAE_F32; e.res = res; e.ldr = ldr; e.z = z; e.ldz = ldz; e.y = y; e.ldy = ldy; e.act = act;
     Space sp{(char*)workspace, 0, workspace_bytes};
-    if (dtype == DSSVAE_F32) return forward<float>(x, ldx, w, ldw, M, N, K, e, sp, st, false);
-    if (dtype == DSSVAE_BF16) return forward<bf16_t>(x, ldx, w, ldw, M, N, K, e, sp, st, false);
-    return forward<f16_t>(x, ldx, w, ldw, M, N, K, e, sp, st, false);
+    if (dtype == DSSVAE_F32) return forward<float>(x, ldx, w, ldw, M, N, K, e, sp, st, false, p);
+    if (dtype == DSSVAE_BF16) return forward<bf16_t>(x, ldx, w, ldw, M, N, K, e, sp, st, false, p);
+    return forward<f16_t>(x, ldx, w, ldw, M, N, K, e, sp, st, false, p);
 }
 
 extern "C" int64_t dssvae_linear_act_bwd_workspace_bytes(const void* dy, int64_t lddy, int has_z, int dtype, int64_t M, int N, int K,
