@@ -2,17 +2,17 @@
 //
 // A row lives in registers between its one read and its one write: TPR threads hold E elements each, in granules of 16 bytes
 // (granule i of thread t covers columns (i * TPR + t) * VEC ..).  Rows may start anywhere and end inside a granule: loads take
-// any alignment, the last granule goes by elements (27513 x 1581 bf16 with element loads instead: 69 us forward, 136 us
-// backward).  Mean first, then the centred squares: two reductions over
-// registers, no cancellation as in E[x^2] - E[x]^2.  Forward, up to 1024 columns a row belongs to one wave or a quarter of
-// one (shuffles only); wider rows take 256 threads.  Backward keeps E at 8 (its column sums cost 2 E registers more: 16
-// elements spilled) and gives a row up to 512 threads.  Rows wider than 8192 columns are walked three times by a block of
-// 1024 (the repeats hit L2).
+// any alignment, the last granule goes by elements (27513 x 1581 bf16: 50 us forward, 85 us backward; with element loads 69 and
+// 136 us).  Mean first, then the centred squares: two reductions over registers, no cancellation as in E[x^2] - E[x]^2.
+// Forward, up to 1024 columns a row belongs to one wave or a quarter of one (shuffles only); wider rows take 256 threads.
+// Backward keeps E at 8 up to 4096 columns (its column sums cost 2 E registers more) and gives a row up to 512 threads.  Rows
+// wider than 8192 columns are walked three times by a block of 1024 (the repeats hit L2).
 //   xh = (x - mean) rstd ; y = xh w + b
 //   dx = rstd (w dy - mean(w dy) - xh mean(w dy xh)) ; dw = sum_rows dy xh ; db = sum_rows dy
 // The column sums: a block walks rows blockIdx, + gridDim, ... and keeps dw / db of its columns in registers; its row groups
 // meet in LDS, one [2, D] partial per block goes to the workspace and a second launch adds the partials in order
 // (no atomics: the same bits every time).
+// Measured: 32768 x 2048 bf16 forward 49 us (5.5 TB/s), backward 79 us (5.1 TB/s) and 6 us for the partials.
 #include "elem.h"
 
 namespace {
