@@ -4,11 +4,13 @@
 //   row = tau^2 sum_j p_j (log p_j - log q[id_j]) ; total = sum_i w_i row_i ; dlogits = w tau (q - scatter(p))
 //
 // One block per row.  The weight of a row is known at the call, so the gradient leaves in the SAME pass: a row stays in
-// registers (NV granules of 16 bytes per thread) between its read and the store; wider rows than 16 granules x 1024 threads
-// are read twice.  Maximum and sum are one walk, granule by granule as they arrive: two walks left the memory idle for the
-// second where only one block fits a CU (2048 x 100003 bf16, NV = 16: 222 us, now 181 us = 4.3 TB/s).  Up to NV = 8 two
-// blocks share a CU (64 registers) and fill each other's gaps: 7936 x 30000 fp32 in 345 us = 5.2 TB/s.  Rows may start at any element: up to VEC - 1 elements in front of the first
-// 16-byte boundary and behind the last granule are "edge" elements, one per thread.
+// registers (NV granules of 16 bytes per thread) between its read and the store; of rows wider than 16 granules x 1024 threads,
+// 8 granules a thread more stay in LDS, and what is behind those is read twice (2048 x
+// 100003 fp32: 346 us = 4.7 TB/s, 454 us with the whole row read twice).  Without a gradient nothing is kept of them.
+// Maximum and sum are one walk, granule by granule as they arrive: two walks left the memory idle for the second where only
+// one block fits a CU (2048 x 100003 bf16, NV = 16: 222 us, now 185 us = 4.4 TB/s).  Up to NV = 8 two blocks share a CU (64
+// registers) and fill each other's gaps: 7936 x 30000 fp32 in 350 us = 5.4 TB/s.  Rows may start at any element: up to VEC - 1
+// elements in front of the first 16-byte boundary and behind the last granule are "edge" elements, one per thread.
 // The k teacher slots are wave 0's: softmax by shuffles while the block loads.  The k gradient entries are written over the
 // dense store behind a barrier, by the first slot of each distinct id with the sum of its probabilities: no atomics, and
 // repeated ids add up in slot order.
@@ -50,14 +52,17 @@ __device__ __forceinline__ void keep_raw(Gran<T, VEC>& v) {
     v.v = __builtin_bit_cast(typename Gran<T, VEC>::V, r);
 }
 
-// NV granules per thread in registers; NV = 0: any width, the row is read twice
-template <typename T, int NT, int NV>
+// NV granules per thread in registers; HOLD > 0: any width, the next HOLD granules per thread stay in LDS and what is still left
+// is read twice; NV = 0: any width, no gradient
+template <typename T, int NT, int NV, int HOLD>
 __global__ __launch_bounds__(NT, NV == 8 ? 8 : 4) void distill_kernel(
     const T* __restrict__ z, int64_t ldz, int V, const int64_t* __restrict__ ids, const float* __restrict__ teacher, int k,
     float tau, const float* __restrict__ weight, float w_all, T* __restrict__ dz, int64_t lddz, float* __restrict__ rows) {
     constexpr int VEC = 16 / (int)sizeof(T);
-    constexpr int NR = NV > 0 ? NV : 1;
+    constexpr int NR = NV > 0 ? NV : 1, AHEAD = 4;  // loads in flight in the walk over what the registers do not hold
+    static_assert(HOLD % AHEAD == 0, "whole steps of the walk are held");
     __shared__ float2 red[NT / 64];  // (maximum, sum) of each wave
+    __shared__ uint4 held[HOLD > 0 ? HOLD * NT : 1];
     extern __shared__ int s_id[];  // [k], and behind it the probabilities [k]
     float* s_p = reinterpret_cast<float*>(s_id + k);
     __shared__ float s_mass;  // 1, 0 (no valid slot) or NaN (an id outside the vocabulary, a NaN or +inf among the teacher's logits)
@@ -117,10 +122,24 @@ __global__ __launch_bounds__(NT, NV == 8 ? 8 : 4) void distill_kernel(
                 online(v[i], c, m, s);
                 keep_raw(v[i]);
             }
-        } else {
-            for (int64_t g = tid; g < nvec; g += NT) {
-                v[0].load(zb + g * VEC);
-                online(v[0], c, m, s);
+        }
+        if constexpr (NV == 0 || HOLD > 0) {
+            for (int i = 0, g = NV * NT + tid; g < nvec; i += AHEAD, g += AHEAD * NT) {
+                Gran<T, VEC> r[AHEAD];
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    if (g + j * NT < nvec) {
+                        r[j].load(zb + (unsigned)((g + j * NT) * VEC));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) r[j].set(e, NINF);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    online(r[j], c, m, s);
+                    if (HOLD > 0 && i < HOLD) held[(i + j) * NT + tid] = __builtin_bit_cast(uint4, r[j].v);
+                }
             }
         }
     }
@@ -156,10 +175,10 @@ __global__ __launch_bounds__(NT, NV == 8 ? 8 : 4) void distill_kernel(
         part = wave_sum(part);
         if (tid == 0) rows[row] = tau * tau * (part + logf(S)) * mass;
     }
-    if (!dr) return;
+    if (NV == 0 || !dr) return;
     const float a = w * tau * mass / S;
     T* db = dr + head;
-    if constexpr (NV > 0) {
+    {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int g = i * NT + tid;
@@ -169,13 +188,15 @@ __global__ __launch_bounds__(NT, NV == 8 ? 8 : 4) void distill_kernel(
             for (int j = 0; j < VEC; ++j) o.set(j, a * exp2_f((v[i].get(j) - M) * c));
             o.store(db + (unsigned)(g * VEC));
         }
-    } else {
-        for (int64_t g = tid; g < nvec; g += NT) {
-            Gran<T, VEC> o;
-            v[0].load(zb + g * VEC);
+    }
+    if constexpr (HOLD > 0) {
+        for (int i = 0, g = NV * NT + tid; g < nvec; ++i, g += NT) {
+            Gran<T, VEC> r, o;
+            if (i < HOLD) r.v = __builtin_bit_cast(typename Gran<T, VEC>::V, held[i * NT + tid]);
+            else r.load(zb + (unsigned)(g * VEC));
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) o.set(j, a * exp2_f((v[0].get(j) - M) * c));
-            o.store(db + g * VEC);
+            for (int j = 0; j < VEC; ++j) o.set(j, a * exp2_f((r.get(j) - M) * c));
+            o.store(db + (unsigned)(g * VEC));
         }
     }
     if (edge >= 0) dr[edge] = (T)(a * exp2_f((ev - M) * c));
@@ -237,24 +258,25 @@ int launch(const T* z, int64_t ldz, int64_t N, int V, const int64_t* ids, const 
            const float* weight, float w_all, T* dz, int64_t lddz, float* rows, hipStream_t s) {
     constexpr int VEC = 16 / (int)sizeof(T);
     const int64_t gran = ((int64_t)V + VEC - 1) / VEC;
-#define GO(NT, NV)                                                                                                     \
+#define GO(NT, NV, HOLD)                                                                                                   \
     do {                                                                                                               \
-        hipLaunchKernelGGL((distill_kernel<T, NT, NV>), dim3((unsigned)N), dim3(NT), k * 8, s, z, ldz, V, ids, teacher, k, tau, weight, \
+        hipLaunchKernelGGL((distill_kernel<T, NT, NV, HOLD>), dim3((unsigned)N), dim3(NT), k * 8, s, z, ldz, V, ids, teacher, k, tau, weight, \
                            w_all, dz, lddz, rows);                                                                     \
         DSSVAE_CHECK_LAUNCH();                                                                                         \
         return DSSVAE_OK;                                                                                              \
     } while (0)
     // the fewest threads that hold a row in 8 granules each: more rows in flight where a row is short (60000 x 300 bf16: 54 us, with
     // 256 threads a row 117 us; 8000 x 5000 fp32: 35 us, with 1024 threads a row 67 us)
-    if (gran <= 64) GO(64, 1);
-    if (gran <= 64 * 4) GO(64, 4);
-    if (gran <= 64 * 8) GO(64, 8);
-    if (gran <= 128 * 8) GO(128, 8);
-    if (gran <= 256 * 8) GO(256, 8);
-    if (gran <= 512 * 8) GO(512, 8);
-    if (gran <= 1024 * 8) GO(1024, 8);
-    if (gran <= 1024 * 16) GO(1024, 16);
-    GO(1024, 0);
+    if (gran <= 64) GO(64, 1, 0);
+    if (gran <= 64 * 4) GO(64, 4, 0);
+    if (gran <= 64 * 8) GO(64, 8, 0);
+    if (gran <= 128 * 8) GO(128, 8, 0);
+    if (gran <= 256 * 8) GO(256, 8, 0);
+    if (gran <= 512 * 8) GO(512, 8, 0);
+    if (gran <= 1024 * 8) GO(1024, 8, 0);
+    if (!dz) GO(1024, 0, 0);
+    if (gran <= 1024 * 16) GO(1024, 16, 0);
+    GO(1024, 16, 8);
 #undef GO
 }
 
