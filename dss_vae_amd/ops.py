@@ -1883,23 +1883,24 @@ def _contig(t):
 _ACCUMULATE = type(torch.autograd.graph.get_gradient_edge(torch.zeros(1, requires_grad=True)).node)
 
 
-def _leaves_elsewhere(node, stream):
-    """Notes on the leaves behind an autograd node the stream they were first used on -> whether one was noted for another.
-    Autograd makes a leaf's accumulation node on the stream of its first use and keeps it while any graph holds it."""
-    other = False
+def _leaves_on_null(node, stream):
+    """Notes on the leaves behind an autograd node the stream they were first used on -> whether one was noted for the NULL
+    stream (0) and `stream` is another.  Autograd makes a leaf's accumulation node on the stream of its first use and keeps it
+    while any graph holds it."""
+    found = False
     for n, _ in node.next_functions:
-        if type(n) is _ACCUMULATE and n.metadata.setdefault("dssvae_stream", stream) != stream:
-            other = True
-    return other
+        if type(n) is _ACCUMULATE and n.metadata.setdefault("dssvae_stream", stream) == 0 != stream:
+            found = True
+    return found
 
 
 def _record(what, ctx, dev):
-    """Before an operator records its graph: under capture, refuses leaves that an older graph still holds on another stream.
-    Their gradients would be handed over on that stream, which a capture does not survive (the process ends)."""
-    if _leaves_elsewhere(ctx, torch._C._cuda_getCurrentRawStream(dev.index)) and torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("%s: this stream is being captured, and a graph that was recorded on another stream still holds a "
-                           "parameter or input of this call: drop that graph (its outputs) first, or record it on the "
-                           "capturing stream" % what)
+    """Before an operator records its graph: under capture, refuses leaves that an older graph still holds on the NULL stream.
+    Autograd would make that stream wait for the capturing one, which a HIP capture does not survive (the process ends)."""
+    if _leaves_on_null(ctx, torch._C._cuda_getCurrentRawStream(dev.index)) and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("%s: this stream is being captured, and a graph that was recorded on the default stream still holds a "
+                           "parameter or input of this call: drop that graph (its outputs) first, or record it on another "
+                           "stream" % what)
 
 
 def _layer_norm_fwd(x2, ldx, code, w, b, eps, stats):

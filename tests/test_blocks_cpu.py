@@ -132,13 +132,14 @@ def test_leaves_of_older_graphs_are_noticed():
     from dss_vae_amd import ops
     a, b = torch.ones(3, requires_grad=True), torch.ones(3, requires_grad=True)
     y = a * b
-    assert not ops._leaves_elsewhere(y.grad_fn, 7)
+    assert not ops._leaves_on_null(y.grad_fn, 0)
     z = a * 2
-    assert not ops._leaves_elsewhere(z.grad_fn, 7) and ops._leaves_elsewhere(z.grad_fn, 8)
+    assert not ops._leaves_on_null(z.grad_fn, 0) and ops._leaves_on_null(z.grad_fn, 8)
     c = b * 3
     del y, z
     fresh = a * 2
-    assert not ops._leaves_elsewhere(fresh.grad_fn, 8)
-    assert ops._leaves_elsewhere(c.grad_fn, 8)
+    assert not ops._leaves_on_null(fresh.grad_fn, 8)
+    assert ops._leaves_on_null(c.grad_fn, 8)
+    assert not ops._leaves_on_null(fresh.grad_fn, 9)  # (noted for 8: an ordinary stream may join a capture)
     inner = fresh * 2  # (no leaf right behind it)
-    assert not ops._leaves_elsewhere(inner.grad_fn, 9)
+    assert not ops._leaves_on_null(inner.grad_fn, 9)

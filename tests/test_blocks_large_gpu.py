@@ -72,7 +72,8 @@ def test_distill_loss():
     tp, rp = ops.distill_loss(part, ids[-n:], t[-n:], 2.0, w[-n:])
     dp, = torch.autograd.grad(tp, part)
     assert torch.equal(bits(rows[-n:]), bits(rp)) and torch.equal(bits(dz[-n:].contiguous()), bits(dp.contiguous()))
-    assert abs(float(total) - float((rows.double() * 0.5).sum())) <= 2.0 ** -23 * float(total)
+    total = float(total.detach())
+    assert abs(total - float((rows.double() * 0.5).sum())) <= 2.0 ** -23 * total
 
 
 def test_linear_act():

@@ -225,8 +225,8 @@ def test_two_graphs_side_by_side():
             assert all(torch.equal(p.detach(), q) for p, q in zip(a, b)), k
 
 
-def test_capture_refuses_leaves_of_a_graph_on_another_stream():
-    """an eager graph of the same leaves lives: every operator refuses the capture before it records anything, the capture ends
+def test_capture_refuses_leaves_of_a_graph_on_the_default_stream():
+    """an eager graph of the same leaves lives on the default stream: every operator refuses the capture before it records anything, the capture ends
     in order, and once that graph is gone the same step is captured and replays"""
     from dss_vae_amd import ops
     x = torch.randn(6, 8, 32, device=DEV).requires_grad_()
@@ -254,3 +254,37 @@ def test_capture_refuses_leaves_of_a_graph_on_another_stream():
             g.replay()
             torch.cuda.synchronize()
             assert torch.equal(got, want), name
+
+
+def test_capture_after_a_warm_up_on_a_side_stream():
+    """the usual recipe: eager steps on a side stream, whose last loss is still held, then the capture of such a step"""
+    from dss_vae_amd import ops
+    m = Student().to(DEV)
+    x, lengths, ids, t, w = (v.to(DEV) for v in data())
+    params = list(m.parameters())
+
+    def step():
+        total, _ = ops.distill_loss(m.logits(ops, x, lengths), ids, t, 2.0, w)
+        total.backward()
+        return total
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            m.zero_grad(set_to_none=True)
+            loss = step()
+    torch.cuda.current_stream().wait_stream(side)
+    want = [loss.detach().clone()] + [p.grad.clone() for p in params]
+    m.zero_grad(set_to_none=True)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        static = step()
+    for _ in range(3):
+        for p in params:
+            p.grad.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a.detach(), b) for a, b in zip([static] + [p.grad for p in params], want))
+    assert float(loss.detach()) == float(want[0])
