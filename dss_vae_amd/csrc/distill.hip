@@ -296,14 +296,17 @@ extern "C" int dssvae_distill(const void* logits, int64_t ldz, int dtype, int64_
                              (N > 1 && (ldz - lddz) % (16 / es) != 0)))
         return DSSVAE_EINVAL;
     hipStream_t s = (hipStream_t)stream;
-    if (N > 0) {
+    constexpr int64_t PART = 1 << 21;  // rows of a launch: 1024 threads each stay below 2^32
+    for (int64_t r = 0; r < N; r += PART) {
+        const int64_t n = N - r < PART ? N - r : PART;
         int e;
-        if (dtype == DSSVAE_F32)
-            e = launch<float>((const float*)logits, ldz, N, V, ids, teacher, k, tau, weight, weight_all, (float*)dlogits, lddz, rows, s);
-        else if (dtype == DSSVAE_BF16)
-            e = launch<bf16_t>((const bf16_t*)logits, ldz, N, V, ids, teacher, k, tau, weight, weight_all, (bf16_t*)dlogits, lddz, rows, s);
-        else
-            e = launch<f16_t>((const f16_t*)logits, ldz, N, V, ids, teacher, k, tau, weight, weight_all, (f16_t*)dlogits, lddz, rows, s);
+#define GO(T)                                                                                                          \
+    launch<T>((const T*)logits + r * ldz, ldz, n, V, ids + r * k, teacher + r * k, k, tau, weight ? weight + r : nullptr, weight_all, \
+              dlogits ? (T*)dlogits + r * lddz : nullptr, lddz, rows + r, s)
+        if (dtype == DSSVAE_F32) e = GO(float);
+        else if (dtype == DSSVAE_BF16) e = GO(bf16_t);
+        else e = GO(f16_t);
+#undef GO
         if (e != DSSVAE_OK) return e;
     }
     hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(1024), 0, s, rows, weight, weight_all, N, total);

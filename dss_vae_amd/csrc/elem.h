@@ -135,6 +135,9 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
     return v;
 }
 
+// A launch holds fewer than 2^32 threads.
+static inline bool grid_fits(int64_t blocks, int threads) { return blocks >= 0 && blocks <= 0xffffffffLL / threads; }
+
 static inline bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
 
 // Compute units (one kind of device per process; 256 without one: the host-side plans are tested there).

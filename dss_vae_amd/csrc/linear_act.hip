@@ -885,7 +885,7 @@ struct Products {
         s.A = A; s.lda = lda; s.B = B; s.ldb = ldb; s.M = M; s.N = (int)N; s.K = K;
         const int64_t tm = up(M, p.tile) / p.tile, tn = up(N, p.tile) / p.tile, blocks = tm * tn * p.ksplit;
         const int64_t join = p.ksplit > 1 ? (M * ((N + 7) / 8) + 255) / 256 : 0;
-        if (blocks > 0x3fffffff || join > 0x3fffffff) return DSSVAE_ETOOBIG;
+        if (!grid_fits(2 * blocks, 512) || !grid_fits(2 * join, 512)) return DSSVAE_ETOOBIG;  // (two products to a launch)
         s.tiles_m = (int)tm; s.tiles_n = (int)tn; s.ksplit = p.ksplit;
         const int64_t nk = up(K, BK<T>) / BK<T>;
         s.ktiles = (nk + p.ksplit - 1) / p.ksplit;
@@ -922,7 +922,7 @@ struct Products {
         for (int i = n; i < 2; ++i) rest.begin[i + 1] = rest.begin[i];
         rest.sums = sums; rest.n = n_sums; rest.C = C; rest.db = db; rest.db_f32 = db_f32;
         const int64_t blocks = rest.begin[2] + (db ? (C + 7) / 8 : 0);
-        if (blocks > 0x7fffffff) return DSSVAE_ETOOBIG;
+        if (!grid_fits(blocks, 256)) return DSSVAE_ETOOBIG;
         if (blocks == 0) return DSSVAE_OK;
         hipLaunchKernelGGL((linear_rest_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, st, rest);
         DSSVAE_CHECK_LAUNCH();

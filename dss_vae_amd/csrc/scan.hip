@@ -428,7 +428,7 @@ template <typename T, int VEC, bool TANH>
 int fwd_launch(const T* x, Dims d, const float* h0, T* out, float* h_last, float* ckpt, float* maps, hipStream_t s) {
     d.tiles = (d.H + LPR * VEC - 1) / (LPR * VEC);
     const int64_t grid = (int64_t)d.tiles * d.B * d.segs;
-    if (grid > 0x7fffffff) return DSSVAE_ETOOBIG;
+    if (!grid_fits(grid, NT<T, 1>)) return DSSVAE_ETOOBIG;
     if (d.segs > 1) {
         hipLaunchKernelGGL((gated_scan_maps_kernel<T, VEC, TANH, false>), dim3((unsigned)grid), dim3((NT<T, 1>)), 0, s, x,
                            (const T*)nullptr, d, maps);
@@ -450,7 +450,7 @@ int bwd_launch(const T* x, const T* dout, Dims d, const float* ckpt, const float
                hipStream_t s) {
     d.tiles = (d.H + LPR * VEC - 1) / (LPR * VEC);
     const int64_t grid = (int64_t)d.tiles * d.B * d.segs;
-    if (grid > 0x7fffffff) return DSSVAE_ETOOBIG;
+    if (!grid_fits(grid, NT<T, 1>)) return DSSVAE_ETOOBIG;
     if (d.segs > 1) {
         hipLaunchKernelGGL((gated_scan_maps_kernel<T, VEC, false, true>), dim3((unsigned)grid), dim3((NT<T, 1>)), 0, s, x, dout, d,
                            maps);
@@ -558,7 +558,7 @@ namespace {
 template <typename T, int VEC, bool TANH>
 int step_launch(const T* x, int64_t xb, const float* h, int B, int H, T* out, int64_t ob, float* h_out, hipStream_t s) {
     const int64_t n = (int64_t)B * (H / VEC), grid = (n + STEP_THREADS - 1) / STEP_THREADS;
-    if (grid > 0x7fffffff) return DSSVAE_ETOOBIG;
+    if (!grid_fits(grid, STEP_THREADS)) return DSSVAE_ETOOBIG;
     hipLaunchKernelGGL((gated_step_kernel<T, VEC, TANH>), dim3((unsigned)grid), dim3(STEP_THREADS), 0, s, x, xb, h, B, H, out, ob, h_out);
     DSSVAE_CHECK_LAUNCH();
     return DSSVAE_OK;

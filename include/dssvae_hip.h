@@ -620,7 +620,9 @@ int dssvae_scale_rows(void* x, int64_t ld, int dtype, int64_t rows, int V, const
  *   y must not overlap x, w or z; it may be res.  DSSVAE_ACT_GELU is the exact form, z Phi(z).
  * Backward: dz = dy act'(z); dx = dz w; dw = dz^T x; db = sum over rows of dz; dx, dw, db may each be NULL, z only where act
  * is DSSVAE_ACT_NONE.  (The residual's gradient is dy.)  M = 0 clears dw and db.
- * fp32 accumulation in a fixed order; fp32 operands: each product is within 2^-22 of itself (operands below 2^-110: absolute 2^-133); 16-bit types: dz is rounded to the type (the products of backward start from it).  A summed axis (K forward, N for dx, M for dw) has at most 2097152 elements: DSSVAE_ETOOBIG.
+ * fp32 accumulation in a fixed order; fp32 operands: each product is within 2^-22 of itself (operands below 2^-110: absolute
+ * 2^-133); 16-bit types: dz is rounded to the type (the products of backward start from it).  A summed axis (K forward, N for dx,
+ * M for dw) has at most 2097152 elements, and a launch fewer than 2^32 threads: DSSVAE_ETOOBIG.
  * The workspace sizes depend on where the operands start: the query takes the pointers and strides of the call.
  * ------------------------------------------------------------------------------------------- */
 #define DSSVAE_ACT_NONE 0

@@ -143,3 +143,11 @@ def test_leaves_of_older_graphs_are_noticed():
     assert not ops._leaves_on_null(fresh.grad_fn, 9)  # (noted for 8: an ordinary stream may join a capture)
     inner = fresh * 2  # (no leaf right behind it)
     assert not ops._leaves_on_null(inner.grad_fn, 9)
+
+
+def test_launches_beyond_the_grid_are_refused():
+    """2^32 threads or more in a launch: refused before anything is enqueued"""
+    big = (1 << 31) - 1
+    assert call("dssvae_gated_step", STEP, B=big, H=64, xb=128, ob=64) == ETOOBIG
+    assert call("dssvae_gated_scan_fwd", SCAN_FWD, B=big) == ETOOBIG
+    assert call("dssvae_linear_act_fwd", LIN_FWD, M=big, N=1 << 20, ldy=1 << 20, res=None, z=None, n=1 << 62) == ETOOBIG

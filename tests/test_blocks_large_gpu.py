@@ -98,3 +98,20 @@ def test_linear_act():
     v.copy_(fill(3, 64, seed=5))
     w2 = fill(16, 64, seed=6)
     assert torch.equal(bits(ops.linear_act(v, w2)), bits(ops.linear_act(v.contiguous(), w2)))
+
+
+def test_distill_loss_of_many_rows():
+    """more rows than one launch takes"""
+    from dss_vae_amd import ops
+    N, V, n = (1 << 21) + 700, 24, 1000
+    z, ids = fill(N, V).requires_grad_(), torch.randint(0, V, (N, 3), device=DEV)
+    t = torch.randn(N, 3, device=DEV)
+    w = torch.rand(N, device=DEV) / N
+    total, rows = ops.distill_loss(z, ids, t, 2.0, w)
+    dz, = torch.autograd.grad(total, z)
+    part = z[-n:].detach().requires_grad_()
+    tp, rp = ops.distill_loss(part, ids[-n:], t[-n:], 2.0, w[-n:])
+    dp, = torch.autograd.grad(tp, part)
+    assert torch.equal(bits(rows[-n:]), bits(rp)) and torch.equal(bits(dz[-n:]), bits(dp))
+    total, want = float(total.detach()), float((rows.double() * w.double()).sum())
+    assert abs(total - want) <= 2.0 ** -23 * want
