@@ -233,3 +233,21 @@ def test_refusals():
                 lambda: ops.distill_loss(z, ids, t, 1.0, torch.ones(4, device=DEV, requires_grad=True))):
         with pytest.raises(RuntimeError):
             bad()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("granules", [64, 256, 512, 1024, 2048, 4096, 8192, 16384, 24576])
+def test_borders_of_the_row_kernels(dtype, granules):
+    """rows that just fit the registers (or registers and LDS) of each kernel, and one element more"""
+    from dss_vae_amd import ops
+    per = 4 if dtype == torch.float32 else 8
+    for V in (granules * per, granules * per + 1):
+        z, ids, t, w = case(3, V, 9, dtype, seed=V)
+        w = w + 0.1
+        got = run(z, ids, t, 1.5, w)
+        compare(z, ids, t, 1.5, w, got)
+        with torch.no_grad():
+            total, rows = ops.distill_loss(z.to(DEV), ids.to(DEV), t.to(DEV), 1.5, w.to(DEV))
+        want = reference(z, ids, t, 1.5, w)
+        check(total, want[0], want[3], SLACK, "total without a gradient")
+        check(rows, want[1], want[4], SLACK, "rows without a gradient")

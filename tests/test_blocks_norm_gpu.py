@@ -189,3 +189,33 @@ def test_refusals():
     g, = torch.autograd.grad(ops.layer_norm(z).sum(), z, create_graph=True)
     with pytest.raises(RuntimeError):  # no second derivative
         g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,D", [(40, 4), (33, 9), (70, 127), (70, 128), (70, 129), (33, 511), (20, 1023), (9, 2049), (9, 4095),
+                                    (5, 4097), (3, 8191), (600, 1001)])
+def test_ragged_widths(dtype, rows, D):
+    """rows that end inside a granule, at every border of the kernels' shapes; many rows to a block and fewer than a block"""
+    x, w, b = rnd(rows, D, seed=D, shift=0.2, dtype=dtype), rnd(D, seed=1, shift=1.0, dtype=dtype), rnd(D, seed=2, dtype=dtype)
+    dy = rnd(rows, D, seed=3, dtype=dtype)
+    ref = reference(x, w, b, 1e-5, dy)
+    got = run(x.to(DEV), w.to(DEV), b.to(DEV), 1e-5, dy.to(DEV))
+    for name, g, r, s in zip(("y", "dx", "dw", "db"), got, ref[:4], ref[4:]):
+        check(g, r, s, SLACK, (name, rows, D, dtype))
+
+
+def test_ragged_rows_beside_values_that_are_not_finite():
+    """what stands right behind a ragged row (the next row, or the buffer around it) does not reach it"""
+    from dss_vae_amd import ops
+    for dtype in TYPES:
+        for D in (5, 77, 333, 1100):
+            clean = rnd(6, D, seed=D, dtype=dtype).to(DEV)
+            dy = rnd(6, D, seed=1, dtype=dtype).to(DEV)
+            wide = torch.full((6, D + 9), float("inf"), dtype=dtype, device=DEV)
+            gwide = torch.full((6, D + 9), float("nan"), dtype=dtype, device=DEV)
+            wide[:, 4:4 + D], gwide[:, 4:4 + D] = clean, dy
+            a, b = clean.clone().requires_grad_(), wide[:, 4:4 + D].detach().requires_grad_()
+            ya, yb = ops.layer_norm(a), ops.layer_norm(b)
+            ga, = torch.autograd.grad(ya, a, dy)
+            gb, = torch.autograd.grad(yb, b, gwide[:, 4:4 + D])
+            assert torch.equal(bits(ya.detach()), bits(yb.detach())) and torch.equal(bits(ga), bits(gb))

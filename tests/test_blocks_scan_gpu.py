@@ -282,3 +282,13 @@ def test_step_refuses_overlapping_buffers():
     assert torch.equal(ops.gated_step(x, h, h_out=buf[8:16].view(2, 4))[1], want)
     ops.gated_step(x, h, h_out=h)
     assert torch.equal(h, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T", [31, 32, 33, 63, 64, 65])
+def test_sequences_of_part_of_a_chunk(dtype, T):
+    """blocks of a quarter, half and the whole of a chunk's threads, on both sides of their borders"""
+    for H, reverse, candidate in ((35, False, "tanh"), (64, True, "linear")):
+        x, h0, dout, dh = inputs(5, T, H, dtype, seed=T + H)
+        lengths = torch.tensor([T, 0, 1, T - 1, T // 2], dtype=torch.int32)
+        compare(x, h0, lengths, reverse, candidate, dout, dh, run(x, h0, lengths, reverse, candidate, dout, dh))
