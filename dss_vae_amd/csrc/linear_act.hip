@@ -5,8 +5,9 @@
 // fp32 operands are taken apart into three bf16 each (24 bits, exact) as they come out of LDS, and six of the nine products of
 // the parts are added: what is left out is below 2^-22 of a product, and on the mean of random inputs the sums are closer to
 // the exact ones than v_mfma_f32_32x32x2_f32's order gives (K = 7936: 7e-7 of the norm; the library's fp32 product 1.6e-6).  The
-// fp32 instruction does a sixteenth of the bf16 one's work: a library product of 4096^3 takes 0.91 ms, this one 0.70 ms; the 704 vector
-// instructions that take 64 k apart cost as much time as the 96 MFMAs behind them, interleaved or not.
+// fp32 instruction does a sixteenth of the bf16 one's work: a library product of 4096^3 takes 0.91 ms, this one 0.70 ms (the six
+// run at 1170 TFLOP/s; a library product of bf16 operands reaches 1326).  Taking operands apart once per block, on their way
+// into LDS through registers, halves the vector instructions but measured the same: 0.73 ms.
 //
 // The tile kernel: C[M, N] = A[M, K] . B[N, K]^T, both operands contiguous along K.  A BM x BN block walks K in steps of
 // 128 bytes (64 or 32 elements); operand tiles go global -> LDS directly (16 bytes a lane, no registers), double buffered.  LDS row r keeps its
