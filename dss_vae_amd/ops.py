@@ -1,6 +1,7 @@
 """autograd wrappers over the C-ABI (include/dssvae_hip.h).  Every op launches hand-written HIP
 kernels on the current stream; torch is used for memory and tiny glue only.  No CPU path."""
 import ctypes as C
+import functools
 import os
 
 import torch
@@ -1827,6 +1828,12 @@ def _go(name, dev, args, span=None):
         L.check(rc, name)
 
 
+@functools.lru_cache(maxsize=4096)
+def _size(name, *args):
+    """what a size query of the C-ABI answers (functions of sizes, types and alignment alone)"""
+    return getattr(L.load(), name)(*args)
+
+
 def _p(t):
     return None if t is None else t.data_ptr()
 
@@ -1945,7 +1952,7 @@ class _LayerNormFn(Function):
             dw = w.new_empty((D,))
         if need_b and db is None:
             db = b.new_empty((D,))
-        n = L.load().dssvae_layer_norm_bwd_workspace_bytes(R, D) if need_w or need_b else 0
+        n = _size("dssvae_layer_norm_bwd_workspace_bytes", R, D) if need_w or need_b else 0
         ws = _space(n, dev)
         _go("dssvae_layer_norm_bwd", dev,
             (x2.data_ptr(), ldx, ctx.code, dy2.data_ptr(), lddy, _p(wc), int(p is not None and p.dtype == torch.float32),
@@ -2002,16 +2009,16 @@ def _gated_step(x, ldx, code, h, tanh, out, h_out):
 def _gated_scan_fwd(x, h0, lengths, reverse, tanh, code, keep):
     """-> out, h_last, checkpoints (None unless `keep`)"""
     B, T, H2 = x.shape
-    H, dev, lib = H2 // 2, x.device, L.load()
+    H, dev = H2 // 2, x.device
     out = x.new_empty((B, T, H))
     h_last = torch.empty((B, H), device=dev, dtype=torch.float32)
-    ckpt = h_last.new_empty((B, lib.dssvae_gated_scan_chunks(T), H)) if keep else None
+    ckpt = h_last.new_empty((B, _size("dssvae_gated_scan_chunks", T), H)) if keep else None
     if T == 0:
         h_last.zero_() if h0 is None else h_last.copy_(h0)
     elif T == 1 and lengths is None and not keep:
         _gated_step(x, x.stride(0), code, h0, tanh, out, h_last)
     else:
-        n = lib.dssvae_gated_scan_workspace_bytes(B, T, H, code)
+        n = _size("dssvae_gated_scan_workspace_bytes", B, T, H, code)
         ws = _space(n, dev)
         _go("dssvae_gated_scan_fwd", dev,
             (x.data_ptr(), x.stride(0), x.stride(1), code, _p(h0), _p(lengths), reverse, tanh, B, T, H, out.data_ptr(), T * H,
@@ -2040,7 +2047,7 @@ class _GatedScanFn(Function):
         x, lengths, ckpt = ctx.saved_tensors
         reverse, tanh, code = ctx.meta
         B, T, H2 = x.shape
-        H, dev, lib = H2 // 2, x.device, L.load()
+        H, dev = H2 // 2, x.device
         x = _sequence(x)
         dout = None if dout is None else _sequence(dout)
         dh = _contig(dh)
@@ -2050,7 +2057,7 @@ class _GatedScanFn(Function):
             if dh0 is not None:
                 dh0.zero_() if dh is None else dh0.copy_(dh)
         else:
-            n = lib.dssvae_gated_scan_workspace_bytes(B, T, H, code)
+            n = _size("dssvae_gated_scan_workspace_bytes", B, T, H, code)
             ws = _space(n, dev)
             ob, ot = (0, 0) if dout is None else (dout.stride(0), dout.stride(1))
             _go("dssvae_gated_scan_bwd", dev,
@@ -2125,6 +2132,8 @@ def _like_rows(z, ldz):
     """uninitialised [N, V] whose rows start at the same offset from a 16-byte boundary as those of z"""
     N, V = z.shape
     per = 16 // z.element_size()
+    if z.data_ptr() % 16 == 0 and (ldz - V) % per == 0:
+        return z.new_empty((N, V))
     off, pitch = z.data_ptr() % 16 // z.element_size(), V + (ldz - V) % per
     return torch.empty(off + N * pitch, device=z.device, dtype=z.dtype).as_strided((N, V), (pitch, 1), off)
 
@@ -2205,7 +2214,7 @@ def distill_loss(logits, ids, teacher, temperature=1.0, weight=None):
     ids2, t2 = _flat(ids).contiguous(), _flat(teacher).contiguous()
     if t2.dtype != torch.float32:
         t2 = t2.float()
-    w2 = None if weight is None else weight.reshape(-1).contiguous()
+    w2 = None if weight is None else (weight if weight.dim() == 1 else weight.reshape(-1)).contiguous()
     if _wants_grad(logits):
         return _DistillFn.apply(logits, ids2, t2, w2, tau, code)
     z, ldz = _matrix(_flat(logits))
@@ -2222,7 +2231,7 @@ def _linear_act_fwd(x2, ldx, w, ldw, b, act, r, code, keep_z):
     z = torch.empty((M, N), device=dev, dtype=torch.float32 if code == 0 else torch.int16) if keep_z else None
     r, ldr = (None, 0) if r is None else _matrix(r)
     xp, wp = x2.data_ptr(), w.data_ptr()
-    n = L.load().dssvae_linear_act_fwd_workspace_bytes(xp, ldx, wp, ldw, code, M, N, K)
+    n = _size("dssvae_linear_act_fwd_workspace_bytes", xp % 16, ldx, wp % 16, ldw, code, M, N, K)
     ws = _space(n, dev)
     _go("dssvae_linear_act_fwd", dev,
         (xp, ldx, wp, ldw, _p(b), int(b is not None and b.dtype == torch.float32), _p(r), ldr, code, act, M, N, K, y.data_ptr(),
@@ -2267,8 +2276,8 @@ class _LinearActFn(Function):
                 dw = w.new_empty((N, K))
             if need_b and db is None:
                 db = b.new_empty((N,))
-            n = L.load().dssvae_linear_act_bwd_workspace_bytes(dy2.data_ptr(), lddy, int(z is not None), code, M, N, K,
-                                                               int(need_x and M > 0), int(need_w), int(need_b))
+            n = _size("dssvae_linear_act_bwd_workspace_bytes", dy2.data_ptr() % 16, lddy, int(z is not None), code, M, N, K,
+                      int(need_x and M > 0), int(need_w), int(need_b))
             ws = _space(n, dev)
             _go("dssvae_linear_act_bwd", dev,
                 (dy2.data_ptr(), lddy, _p(z), N, x2.data_ptr(), ldx, wc.data_ptr(), ldw, code, act, M, N, K, _p(dx), K, _p(dw), K,
