@@ -589,6 +589,86 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Jobs jobs)
     }
 }
 
+// Few rows (a token or a small batch of them): the time is one read of w.  A block computes 16 columns of y: its eight waves
+// take K in turns of 64 bytes a row, operands straight from memory into the MFMA's registers (16 x 16 x 32, fp32 16 x 16 x 4; rows at
+// any alignment, four turns' loads in flight), and their sums meet in LDS, added in order, where the epilogue follows.  No
+// workspace, one launch.
+template <typename T> struct Mfma16;
+template <> struct Mfma16<float> {
+    static __device__ __forceinline__ f32x4 go(f32x4 a, f32x4 b, f32x4 c) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+        return c;
+    }
+};
+template <> struct Mfma16<bf16_t> {
+    typedef Mfma<bf16_t>::V V;
+    static __device__ __forceinline__ f32x4 go(V a, V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mfma16<f16_t> {
+    typedef Mfma<f16_t>::V V;
+    static __device__ __forceinline__ f32x4 go(V a, V b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+template <typename T, int MI>
+__global__ __launch_bounds__(512) void linear_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w, int64_t ldw, int M,
+                                                          int N, int K, Epilogue e) {
+    constexpr int W = 8, VEC = GR<T>, KS = 4 * VEC, U = 4;
+    typedef typename Mfma<T>::V V;
+    __shared__ __attribute__((aligned(16))) float part[W][MI * 16][16];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int n0 = (int)blockIdx.x * 16;
+    // (rows behind the last are that one, and never stored)
+    const T* wr = w + (int64_t)min(n0 + r, N - 1) * ldw;
+    const T* xr[MI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i) xr[i] = x + (int64_t)min(i * 16 + r, M - 1) * ldx;
+    f32x4 acc[MI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int turns = K / KS;
+    GranU<T, VEC> wv[U], xv[U][MI];
+    // (two turns in a row to a wave: a cache line of every row)
+    const auto turn = [](int s, int u) { return s + u / 2 * (2 * W) + u % 2; };
+    for (int s = 2 * wave; s < turns; s += W * U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = min(turn(s, u), turns - 1) * KS + g * VEC;
+            wv[u].load(wr + k);
+#pragma unroll
+            for (int i = 0; i < MI; ++i) xv[u][i].load(xr[i] + k);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (turn(s, u) >= turns) break;
+#pragma unroll
+            for (int i = 0; i < MI; ++i) acc[i] = Mfma16<T>::go(__builtin_bit_cast(V, wv[u].v), __builtin_bit_cast(V, xv[u][i].v), acc[i]);
+        }
+    }
+    if (K % KS != 0 && wave == turns / 2 % W) {  // the turn that K ends in
+        load_cols<false, T, VEC>(wv[0], wr, turns * KS + g * VEC, K);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            load_cols<false, T, VEC>(xv[0][i], xr[i], turns * KS + g * VEC, K);
+            acc[i] = Mfma16<T>::go(__builtin_bit_cast(V, wv[0].v), __builtin_bit_cast(V, xv[0][i].v), acc[i]);
+        }
+    }
+    // a lane holds columns 4 g .. 4 g + 3 of row r of each 16
+#pragma unroll
+    for (int i = 0; i < MI; ++i) *reinterpret_cast<f32x4*>(&part[wave][i * 16 + r][g * 4]) = acc[i];
+    __syncthreads();
+    const int m = threadIdx.x >> 1, c = (threadIdx.x & 1) * 8;
+    if (m >= M || n0 + c >= N) return;
+    f32x8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = part[0][m][c + j];
+#pragma unroll
+    for (int k = 1; k < W; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += part[k][m][c + j];
+    finish8<T>(e, v, bias8<T>(e, n0 + c, N), m, n0 + c, N);
+}
+
 // What is left behind the tile kernel, in one launch: blocks begin[i] .. begin[i + 1] add the partials of product i's K splits in
 // order and apply its epilogue, 8 columns a thread; the last ones add the rows of db's partial sums in a fixed order, 8 columns a
 // block, 32 threads to a column.
@@ -806,7 +886,7 @@ struct Plan { int tile, ksplit; };
 struct Extent { int64_t M, N, K; };
 template <typename T> constexpr int MAX_TILE = sizeof(T) == 4 ? 128 : 256;
 template <typename T, int COUNT>
-inline void plan_products(const Extent (&x)[COUNT], Plan (&best)[COUNT]) {
+inline double plan_products(const Extent (&x)[COUNT], Plan (&best)[COUNT]) {
     static const int splits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
     const bool f32 = sizeof(T) == 4;
     const double cus = device_cus();
@@ -847,12 +927,22 @@ inline void plan_products(const Extent (&x)[COUNT], Plan (&best)[COUNT]) {
             for (int i = 0; i < COUNT; ++i) best[i] = p[i];
         }
     }
+    return lowest;
 }
+// tile 0: linear_rows_kernel, where its modelled time is the smaller: 3.5 us and 45 GB/s a CU for what its blocks load, 16 rows of
+// w and up to 64 of x each.  Measured against the tiles, bf16, M x K -> N: 1 x 1024 -> 1024 4.4 / 8.0 us, 50 x 600 -> 300 5.9 / 8.2, 50 x 2048
+// -> 2048 12.0 / 13.4, 50 x 4096 -> 4096 23.5 / 16.3 (taken by the tiles); fp32: 1 x 2048 -> 8192 15 / 31, 50 x 8192 -> 2048 72 / 36 (tiles).
+constexpr int64_t FEW_ROWS = 64;
+inline int row_blocks(int64_t M) { return M <= 16 ? 1 : M <= 32 ? 2 : 4; }  // of 16 rows
 template <typename T>
 inline Plan plan(int64_t M, int64_t N, int64_t K) {
     const Extent x[1] = {{M, N, K}};
     Plan p[1];
-    plan_products<T, 1>(x, p);
+    const double tiles = plan_products<T, 1>(x, p);
+    if (M <= FEW_ROWS) {
+        const int64_t cus = device_cus(), turns = (up(N, 16) / 16 + cus - 1) / cus;
+        if (3.5 + (double)turns * (double)(K * (int64_t)sizeof(T)) * 16 * (1 + row_blocks(M)) / 45e3 < tiles) return Plan{0, 1};
+    }
     return p[0];
 }
 // dx [M, K] over N and dw [N, K] over M, whichever of them a call wants (its bits do not depend on that)
@@ -998,11 +1088,27 @@ bool bad_args(int dtype, int act, int64_t M, int N, int K) {
            N > (1 << 30) || K > (1 << 30);
 }
 
+template <typename T>
+int few_rows(const void* x, int64_t ldx, const void* w, int64_t ldw, int M, int N, int K, const Epilogue& e, hipStream_t st) {
+    const int64_t blocks = ((int64_t)N + 15) / 16;
+    if (!grid_fits(blocks, 512)) return DSSVAE_ETOOBIG;
+#define GO(MI)                                                                                                      \
+    hipLaunchKernelGGL((linear_rows_kernel<T, MI>), dim3((unsigned)blocks), dim3(512), 0, st, (const T*)x, ldx, (const T*)w, ldw, M, N, K, e)
+    if (row_blocks(M) == 1) GO(1);
+    else if (row_blocks(M) == 2) GO(2);
+    else GO(4);
+#undef GO
+    DSSVAE_CHECK_LAUNCH();
+    return DSSVAE_OK;
+}
+
 // (`p`: plan of the product, made where the call's workspace is added up and used where it is launched)
 template <typename T>
 int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int N, int K, const Epilogue& e, Space& sp, hipStream_t st,
             bool dry, Plan& p) {
     const int64_t ldk = up(K, GR<T>), es = sizeof(T);
+    if (dry) p = plan<T>(M, N, ldk);
+    if (p.tile == 0) return dry ? DSSVAE_OK : few_rows<T>(x, ldx, w, ldw, (int)M, N, K, e, st);
     PackList packs;
     if (!direct<T>(x, ldx, K)) {
         void* d = sp.take(M * ldk * es);
@@ -1014,7 +1120,6 @@ int forward(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, i
         packs.add(w, ldw, N, K, d, ldk, GR<T>);
         w = d; ldw = ldk;
     }
-    if (dry) p = plan<T>(M, N, ldk);
     void* part = sp.take(part_bytes(p, M, N));
     if (dry) return DSSVAE_OK;
     int rc = pack<T>(packs, st);

@@ -53,8 +53,8 @@ LIN_BWD = dict(dy=P, lddy=16, z=P, ldz=16, x=P, ldx=8, w=P, ldw=8, dtype=1, act=
     ("dssvae_scale_rows", SCALE, [dict(x=None), dict(f=None), dict(ld=8), dict(V=0), dict(rows=-1), dict(dtype=5)]),
     ("dssvae_linear_act_fwd", LIN_FWD, [dict(x=None), dict(w=None), dict(y=None), dict(act=5), dict(act=-1), dict(dtype=3), dict(N=0),
                                         dict(K=0), dict(M=-1), dict(ldx=7), dict(ldw=7), dict(ldy=15), dict(ldr=15), dict(ldz=15),
-                                        dict(z=P + 4096), dict(K=9, ldx=9, ldw=9, n=0), dict(K=9, ldx=9, ldw=9, ws=None),
-                                        dict(K=9, ldx=9, ldw=9, ws=P + 1)]),
+                                        dict(z=P + 4096), dict(M=100, K=9, ldx=9, ldw=9, n=0), dict(M=100, K=9, ldx=9, ldw=9, ws=None),
+                                        dict(M=100, K=9, ldx=9, ldw=9, ws=P + 1)]),
     ("dssvae_linear_act_bwd", LIN_BWD, [dict(dy=None), dict(x=None), dict(w=None), dict(z=None), dict(lddy=15), dict(ldz=15), dict(ldx=7),
                                         dict(ldw=7), dict(lddx=7), dict(lddw=7), dict(ws=None), dict(n=100), dict(act=9), dict(dtype=3)]),
 ])

@@ -284,3 +284,40 @@ def test_fp32_infinities_and_the_largest_values():
         finite = x.clone()
         finite[[3, 7, 9, 11]] = 0.0
         assert torch.equal(bits(ops.linear_act(finite, w)[keep]), bits(y[keep]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 32, 33, 63, 64, 65])
+def test_few_rows(dtype, M):
+    """a token's product at every row count the few-row kernel treats differently: K around its turns and waves, N that ends inside
+    a block or an eight, rows that start anywhere, the pre-activation kept for backward"""
+    from dss_vae_amd import ops
+    for N, K in ((1, 1), (16, 31), (17, 32), (23, 33), (40, 257), (300, 600), (130, 1111)):
+        name = ACTS[(M + N) % 5]
+        x, w, b, res, dy = case(M, N, K, dtype, seed=M + N + K, bias32=N % 2 == 1)
+        compare(x, w, b, res, name, dy, run(x, w, b, res, name, dy))
+        wide_x, wide_w = torch.full((M, K + 5), float("nan"), dtype=dtype, device=DEV), torch.full((N, K + 3), float("nan"), dtype=dtype, device=DEV)
+        wide_x[:, 1:1 + K], wide_w[:, 2:2 + K] = x.to(DEV), w.to(DEV)
+        with torch.no_grad():
+            plain = ops.linear_act(x.to(DEV), w.to(DEV), b.to(DEV), name, res.to(DEV))
+            assert torch.equal(bits(ops.linear_act(wide_x[:, 1:1 + K], wide_w[:, 2:2 + K], b.to(DEV), name, res.to(DEV))), bits(plain))
+
+
+def test_few_rows_in_a_graph_and_beside_values_that_are_not_finite():
+    from dss_vae_amd import ops
+    for dtype in TYPES:
+        x, w, b, res, _ = (t.to(DEV) for t in case(50, 120, 300, dtype, seed=8))
+        want = ops.linear_act(x, w, b, "silu", res)
+        bad = x.clone()
+        bad[7], bad[9, 4] = float("nan"), float("inf")
+        got = ops.linear_act(bad, w, b, "silu", res)
+        keep = [i for i in range(50) if i not in (7, 9)]
+        assert torch.equal(bits(got[keep]), bits(want[keep])) and got[7].isnan().all()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = ops.linear_act(x, w, b, "silu", res)
+        for _ in range(3):
+            y.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(bits(y), bits(want))
