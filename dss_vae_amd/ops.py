@@ -1887,7 +1887,8 @@ def _contig(t):
     return None if t is None else t.contiguous()
 
 
-_ACCUMULATE = type(torch.autograd.graph.get_gradient_edge(torch.zeros(1, requires_grad=True)).node)
+with torch.inference_mode(False), torch.enable_grad():  # (whatever mode the import runs in)
+    _ACCUMULATE = type(torch.autograd.graph.get_gradient_edge(torch.zeros(1, device="cpu", requires_grad=True)).node)
 
 
 def _leaves_on_null(node, stream):

@@ -151,3 +151,12 @@ def test_launches_beyond_the_grid_are_refused():
     assert call("dssvae_gated_step", STEP, B=big, H=64, xb=128, ob=64) == ETOOBIG
     assert call("dssvae_gated_scan_fwd", SCAN_FWD, B=big) == ETOOBIG
     assert call("dssvae_linear_act_fwd", LIN_FWD, M=big, N=1 << 20, ldy=1 << 20, res=None, z=None, n=1 << 62) == ETOOBIG
+
+
+def test_import_in_any_grad_mode():
+    import subprocess
+    import sys
+    for mode in ("torch.inference_mode()", "torch.no_grad()", "torch.device('meta')"):
+        src = "import torch\nwith %s:\n    import dss_vae_amd.ops as o\nprint(o._ACCUMULATE.__name__)" % mode
+        out = subprocess.run([sys.executable, "-c", src], capture_output=True, text=True)
+        assert out.stdout.strip() == "AccumulateGrad", out.stderr
