@@ -17,6 +17,10 @@
 // wave has read all of this one, so its buffer takes the tile after next while the second half multiplies.
 // The backward operands that are contiguous the other way (w and x along the summed axis, dz for dw) are transposed into the
 // workspace first: dz in both orders by the pass that forms it, which also leaves the column sums for db.
+// 16-bit types: that pass leaves dz in two parts of the type (dy act'(z) is not a number of the type: rounded once, its error is as
+// large as that of the results' own rounding), and the products run over both: low parts first, then high ones, into the same
+// accumulators.  The low parts cost the matrix work again (16384 x 2048 -> 8192 bf16 and fp16, gelu, forward and backward: 2.75 ms, products
+// of backward 1.8 and transposes 0.39 of it; with a rounded dz 1.74 ms, 0.9 and 0.29): DSSVAE_ACT_ROUND_DZ does without them.  None and relu need none: their dz is dy, or zero.
 // Few output tiles: K is split over blocks, fp32 partials go to the workspace and a second launch adds them in order and
 // applies the epilogue (no atomics: same bits every time).  Backward is three launches: the transposes, both products, and
 // the partials with db's column sums.
@@ -195,6 +199,32 @@ __device__ __forceinline__ void finish8(const Epilogue& e, f32x8 a, f32x8 b, int
     }
 }
 
+// A number v as two of a 16-bit type, v = (lo LOW + hi) HIGH to 2^-16 of v (bf16) or 2^-22 (fp16).  bf16: hi the number cut off.
+// fp16: of v / 2, which stays in the range (|dy act'| < 1.13 * 65504), and the rest times 1024, which lifts the rest of a number
+// among the smallest.  hi is always below v in magnitude, so that lo is not zero and has its sign: an infinity on the other side of the
+// product stays one.  What is not finite is itself in both.
+template <typename T> struct Apart { static constexpr float LOW = 1.f, HIGH = 1.f; };  // (fp32 stays whole)
+template <> struct Apart<bf16_t> {
+    static constexpr float LOW = 1.f, HIGH = 1.f;
+    static __device__ __forceinline__ void of(float v, bf16_t& lo, bf16_t& hi) {
+        const bool odd = v == 0.f || !(fabsf(v) < __builtin_huge_valf());
+        const float h = odd ? v : __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, v) - 1) & 0xffff0000u);
+        hi = (bf16_t)h;
+        lo = (bf16_t)(odd ? v : v - h);
+    }
+};
+template <> struct Apart<f16_t> {
+    static constexpr float LOW = 1.f / 1024.f, HIGH = 2.f;
+    static __device__ __forceinline__ void of(float v, f16_t& lo, f16_t& hi) {
+        v *= 0.5f;
+        const bool odd = v == 0.f || !(fabsf(v) < __builtin_huge_valf());
+        const auto cut = __builtin_amdgcn_cvt_pkrtz(__builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) - 1), 0.f);
+        const float h = odd ? v : (float)cut[0];
+        hi = (f16_t)h;
+        lo = (f16_t)(odd ? v : (v - h) * 1024.f);
+    }
+};
+
 // ---- the tile kernel -----------------------------------------------------------------------------------------
 typedef __attribute__((address_space(1))) const void* gptr_t;
 typedef __attribute__((address_space(3))) void* lptr_t;
@@ -247,7 +277,11 @@ struct Loader {
     }
     __device__ __forceinline__ void load(T* lds, const T* base) const {
 #pragma unroll
-        for (int i = 0; i < NR; ++i) put(lds, i, reinterpret_cast<const char*>(base) + off[i]);
+        for (int i = 0; i < NR; ++i) {
+            unsigned o = off[i];
+            asm("" : "+v"(o));  // (extended to 64 bits here, which the load does by itself: extended ahead of the loop it took twice the registers)
+            put(lds, i, reinterpret_cast<const char*>(base) + o);
+        }
     }
     // a tile that may reach behind K: granules there come from a granule of zeros
     __device__ __forceinline__ void load_last(T* lds, const T* base, int64_t left) const {
@@ -257,7 +291,7 @@ struct Loader {
             put(lds, i, in ? reinterpret_cast<const char*>(base) + off[i] : reinterpret_cast<const char*>(&zero_granule));
     }
     static __device__ __forceinline__ void put(T* lds, int i, const char* src) {
-        const int wave = threadIdx.x >> 6;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (places in LDS in scalar registers)
         __builtin_amdgcn_global_load_lds((gptr_t)src, (lptr_t)(lds + (i * TH + wave * 64) * GR<T>), 16, 0, 0);
     }
 };
@@ -345,7 +379,9 @@ struct Shape {
     const void* B; int64_t ldb;
     int64_t M; int N; int64_t K;
     int tiles_m, tiles_n, ksplit;
-    int64_t ktiles;      // k-tiles per split
+    int parts;           // of A, `part_at` elements apart: the sum over both, B the same for each; K is then whole k-tiles
+    int64_t part_at;
+    int64_t ktiles;      // k-tiles per split (of those of all parts, one part behind the other)
     float* part;         // [ksplit][M][N] where ksplit > 1
 };
 
@@ -439,19 +475,35 @@ __device__ __forceinline__ void k_step_split(Planes<MI, NI>& p0, Frags<float, MI
     }
 }
 
-// acc = this wave's part of the output tile at (m0, n0), over the k-tiles kt0 .. kt1 - 1
-template <typename T, int BM, int BN, int WR, int WC, bool SPLIT>
-__device__ __forceinline__ void tile_product(const Shape& s, int64_t m0, int n0, int64_t kt0, int64_t kt1, T* __restrict__ buf0,
-                                             T* __restrict__ buf1, f32x16 (&acc)[BM / WR / 32][BN / WC / 32]) {
-    constexpr int TH = 64 * WR * WC, MI = BM / WR / 32, NI = BN / WC / 32;
-    const int wave = threadIdx.x >> 6;
-    const int ra = wave / WC * (BM / WR), rb = wave % WC * (BN / WC);
+template <int MI, int NI>
+__device__ __forceinline__ void clear(f32x16 (&acc)[MI][NI]) {
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+}
+
+template <int MI, int NI>
+__device__ __forceinline__ void times(f32x16 (&acc)[MI][NI], float f) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] *= f;
+}
+
+// acc = this wave's part of the output tile at (m0, n0), over the k-tiles kt0 .. kt1 - 1 of A's parts
+template <typename T, int BM, int BN, int WR, int WC, bool SPLIT>
+__device__ __forceinline__ void tile_product(const Shape& s, int64_t m0, int n0, int64_t kt0, int64_t kt1, T* __restrict__ buf0,
+                                             T* __restrict__ buf1, f32x16 (&acc)[BM / WR / 32][BN / WC / 32]) {
+    constexpr int TH = 64 * WR * WC, MI = BM / WR / 32, NI = BN / WC / 32;
+    constexpr bool PARTS = sizeof(T) == 2, LIFTED = PARTS && Apart<T>::LOW != 1.f;
+    const int wave = threadIdx.x >> 6;
+    const int ra = wave / WC * (BM / WR), rb = wave % WC * (BN / WC);
+    clear(acc);
     if (kt0 >= kt1) return;
     Loader<T, BM, TH> la;
     Loader<T, BN, TH> lb;
@@ -459,15 +511,29 @@ __device__ __forceinline__ void tile_product(const Shape& s, int64_t m0, int n0,
     lb.init(s.ldb, s.N - n0);
     const T* A = (const T*)s.A + m0 * s.lda;
     const T* B = (const T*)s.B + (int64_t)n0 * s.ldb;
-    // The order of the tiles is free: the last one, which alone may reach behind K, goes first, then kt0 .. kt1 - 2, so that
-    // the loop's loads need no test.  A tile behind the end is the one before it again (loaded, never multiplied).
-    const int64_t kl = (kt1 - 1) * BK<T>, n = kt1 - kt0;
-    la.load_last(buf0, A + kl, s.K - kl);
-    lb.load_last(buf0 + BM * BK<T>, B + kl, s.K - kl);
-    const int64_t most = n > 1 ? kt1 - 2 : kt0;
-    if (n > 1) tile_load<T, BM, BN, TH>(buf1, la, lb, A + kt0 * BK<T>, B + kt0 * BK<T>);
+    const int64_t nk = (s.K + BK<T> - 1) / BK<T>, n = kt1 - kt0;
+    const auto at = [&](int64_t t, const T*& a, const T*& b) {  // k-tile t of all parts
+        const bool second = PARTS && t >= nk;
+        const int64_t k = (second ? t - nk : t) * BK<T>;
+        a = A + (second ? s.part_at : 0) + k;
+        b = B + k;
+    };
+    // The order of the tiles of one part is free: the last one, which alone may reach behind K, goes first, then kt0 .. kt1 - 2, so
+    // that the loop's loads need no test.  Two parts: in order.  A tile behind the end is the one before it again (loaded, never
+    // multiplied).
+    const int ordered = PARTS && s.parts > 1;
+    const T *a, *b;
+    const int64_t t0 = ordered ? kt0 : kt1 - 1, left = s.K - (t0 >= nk ? t0 - nk : t0) * BK<T>;
+    at(t0, a, b);
+    la.load_last(buf0, a, left);
+    lb.load_last(buf0 + BM * BK<T>, b, left);
+    const int64_t most = n > 1 ? kt1 - 2 + ordered : kt0;
+    at(min(kt0 + ordered, most), a, b);
+    if (n > 1) tile_load<T, BM, BN, TH>(buf1, la, lb, a, b);
     tile_barrier();
-    // step i multiplies the i-th tile in that order and loads the (i + 2)-th: kt0 + i + 1
+    // step i multiplies the i-th tile in that order and loads the (i + 2)-th: kt0 + i + 1 (+ 1 in order).  The low part's sums are
+    // brought to the high one's scale behind its last tile.
+    const int64_t next = kt0 + 1 + ordered, edge = LIFTED && ordered && kt0 < nk ? min(nk, kt1) - kt0 : -1;  // (tiles of the low part)
     int64_t i = 0;
     if constexpr (SPLIT) {
         Frags<T, MI, NI> f0, f1;
@@ -477,9 +543,10 @@ __device__ __forceinline__ void tile_product(const Shape& s, int64_t m0, int n0,
         p0.of(f0);
         if (n > 1) {
             for (; i + 1 < n; i += 2) {
-                const int64_t k2 = min(kt0 + i + 1, most) * BK<T>, k3 = min(kt0 + i + 2, most) * BK<T>;
-                k_step_split<BM, BN, TH, MI, NI>(p0, f1, acc, la, lb, buf0, buf1, ra, rb, A + k2, B + k2);
-                k_step_split<BM, BN, TH, MI, NI>(p0, f1, acc, la, lb, buf1, buf0, ra, rb, A + k3, B + k3);
+                at(min(next + i, most), a, b);
+                k_step_split<BM, BN, TH, MI, NI>(p0, f1, acc, la, lb, buf0, buf1, ra, rb, a, b);
+                at(min(next + i + 1, most), a, b);
+                k_step_split<BM, BN, TH, MI, NI>(p0, f1, acc, la, lb, buf1, buf0, ra, rb, a, b);
             }
         }
         if (i < n) {
@@ -492,15 +559,29 @@ __device__ __forceinline__ void tile_product(const Shape& s, int64_t m0, int n0,
         f0.read(buf0, BM * BK<T>, ra, rb, 0);
         if (n > 1) {
             for (; i + 1 < n; i += 2) {
-                const int64_t k2 = min(kt0 + i + 1, most) * BK<T>, k3 = min(kt0 + i + 2, most) * BK<T>;
-                k_step<T, BM, BN, TH, MI, NI>(f0, f1, acc, la, lb, buf0, buf1, ra, rb, A + k2, B + k2);
-                k_step<T, BM, BN, TH, MI, NI>(f0, f1, acc, la, lb, buf1, buf0, ra, rb, A + k3, B + k3);
+                at(min(next + i, most), a, b);
+                k_step<T, BM, BN, TH, MI, NI>(f0, f1, acc, la, lb, buf0, buf1, ra, rb, a, b);
+                if constexpr (LIFTED) {
+                    if (i + 1 == edge) times(acc, Apart<T>::LOW);
+                }
+                __builtin_amdgcn_sched_barrier(0);  // (both steps' operands at once do not fit the registers)
+                at(min(next + i + 1, most), a, b);
+                k_step<T, BM, BN, TH, MI, NI>(f0, f1, acc, la, lb, buf1, buf0, ra, rb, a, b);
+                if constexpr (LIFTED) {
+                    if (i + 2 == edge) times(acc, Apart<T>::LOW);
+                }
             }
         }
         if (i < n) {  // an odd tile is left: nothing behind it
             f1.read(buf0, BM * BK<T>, ra, rb, 1);
             f0.multiply(acc);
             f1.multiply(acc);
+            if constexpr (LIFTED) {
+                if (i + 1 == edge) times(acc, Apart<T>::LOW);
+            }
+        }
+        if constexpr (LIFTED) {
+            if (ordered) times(acc, Apart<T>::HIGH);
         }
     }
     tile_barrier();  // operand buffers are free (and no load is in flight)
@@ -521,7 +602,7 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Jobs jobs)
     const int n0 = tn * BN;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int ra = wave / WC * (BM / WR), rb = wave % WC * (BN / WC);
-    const int64_t nk = (s.K + BK<T> - 1) / BK<T>, kt0 = split * s.ktiles, kt1 = min(nk, kt0 + s.ktiles);
+    const int64_t nk = (s.K + BK<T> - 1) / BK<T>, kt0 = split * s.ktiles, kt1 = min(nk * s.parts, kt0 + s.ktiles);
 
     f32x16 acc[MI][NI];
     if constexpr (sizeof(T) == 4) {
@@ -751,7 +832,8 @@ __global__ __launch_bounds__(256) void linear_pack_kernel(Packs p) {
 //   v = src                      (z NULL)
 //   v = src * act'(z)            else (z as linear_tile_kernel's epilogue kept it)
 // out [R, ldo] (NULL: not wanted) gets v, columns C .. ldo zero; outT [C, ldt] (NULL) its transpose, columns R .. ldt zero;
-// sums [stride][C] (NULL) the block's column sums of the unrounded v.
+// sums [stride][C] (NULL) the block's column sums of the unrounded v.  parts = 2 (16-bit types): out and outT get v's low parts, and
+// its high ones `out_part` / `outT_part` elements behind.
 // A thread moves eight neighbouring elements of a row.  The tile keeps its eight (r, chunk) at chunk ^ (r / 8): the eight lanes
 // that gather one column's 64 rows then read eight different banks.
 // A launch makes several such passes (dy, w and x of one backward call): blocks begin[i] .. begin[i + 1] belong to the i-th.
@@ -761,15 +843,30 @@ struct Turn {
     int64_t R, C;
     void* out; int64_t ldo;
     void* outT; int64_t ldt;
+    int parts; int64_t out_part, outT_part;
     float* sums;
     int stride;  // blocks along the rows
     int stream;  // the outputs are larger than what the caches keep until the products read them: streaming stores
 };
 struct Turns { Turn job[3]; int begin[4]; };
 
+// columns c .. c + 7 of a row of ld elements
+template <typename T>
+__device__ __forceinline__ void turn_row(const GranU<T, 8>& g, T* row, int64_t c, int64_t ld, int stream) {
+    if (c + 8 <= ld) {
+        if (stream) g.store_nt(row + c);
+        else g.store(row + c);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (c + j < ld) row[c + j] = g.v[j];
+    }
+}
+
 template <typename T, int ACT>
 __global__ __launch_bounds__(256) void linear_turn_kernel(Turns jobs) {
-    __shared__ __attribute__((aligned(16))) T tile[64 * 64];
+    constexpr bool APART = sizeof(T) == 2 && (ACT == DSSVAE_ACT_GELU || ACT == DSSVAE_ACT_SILU || ACT == DSSVAE_ACT_TANH);
+    __shared__ __attribute__((aligned(16))) T tile[APART ? 2 : 1][64 * 64];
     __shared__ float red[32][64];
     int which = 0;
     while ((int)blockIdx.x >= jobs.begin[which + 1]) ++which;
@@ -826,38 +923,36 @@ __global__ __launch_bounds__(256) void linear_turn_kernel(Turns jobs) {
                 sum[j] += v[j];
                 g.set(j, v[j]);
             }
-            if (out && r < R) {
-                if (c + 8 <= ldo) {
-                    if (t.stream) g.store_nt(out + r * ldo + c);
-                    else g.store(out + r * ldo + c);
-                } else {
+            if constexpr (APART) {
+                if (t.parts == 2) {
+                    GranU<T, 8> hi;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (c + j < ldo) out[r * ldo + c + j] = (T)v[j];
+                    for (int j = 0; j < 8; ++j) {
+                        T l, h;
+                        Apart<T>::of(v[j], l, h);
+                        g.v[j] = l;
+                        hi.v[j] = h;
+                    }
+                    if (out && r < R) turn_row(hi, out + t.out_part + r * ldo, c, ldo, t.stream);
+                    if (outT) hi.store(tile[1] + tr * 64 + (ch ^ (tr >> 3)) * 8);
                 }
             }
-            if (outT) g.store(tile + tr * 64 + (ch ^ (tr >> 3)) * 8);
+            if (out && r < R) turn_row(g, out + r * ldo, c, ldo, t.stream);
+            if (outT) g.store(tile[0] + tr * 64 + (ch ^ (tr >> 3)) * 8);
         }
         if (outT) {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                // lane ch gathers rows 8 ch .. of column i * 32 + rr
-                const int tc = i * 32 + rr;
-                GranU<T, 8> g;
+            for (int q = 0; q < (APART ? 2 : 1); ++q) {
+                if (q > 0 && t.parts < 2) break;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) g.v[j] = tile[(ch * 8 + j) * 64 + ((tc >> 3) ^ ch) * 8 + (tc & 7)];
-                const int64_t r = r0 + ch * 8;
-                T* o = outT + (c0 + tc) * ldt + r;
-                if (c0 + tc < C) {
-                    if (r + 8 <= ldt) {
-                        if (t.stream) g.store_nt(o);
-                        else g.store(o);
-                    } else {
+                for (int i = 0; i < 2; ++i) {
+                    // lane ch gathers rows 8 ch .. of column i * 32 + rr
+                    const int tc = i * 32 + rr;
+                    GranU<T, 8> g;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (r + j < ldt) o[j] = g.v[j];
-                    }
+                    for (int j = 0; j < 8; ++j) g.v[j] = tile[q][(ch * 8 + j) * 64 + ((tc >> 3) ^ ch) * 8 + (tc & 7)];
+                    if (c0 + tc < C) turn_row(g, outT + q * t.outT_part + (c0 + tc) * ldt, r0 + ch * 8, ldt, t.stream);
                 }
             }
             __syncthreads();
@@ -945,11 +1040,11 @@ inline Plan plan(int64_t M, int64_t N, int64_t K) {
     }
     return p[0];
 }
-// dx [M, K] over N and dw [N, K] over M, whichever of them a call wants (its bits do not depend on that)
+// dx [M, K] over N and dw [N, K] over M, whichever of them a call wants (its bits do not depend on that); dz in one or two parts
 struct Plans { Plan x, w; };
 template <typename T>
-inline Plans plan_bwd(int64_t M, int64_t N, int64_t K) {
-    const Extent x[2] = {{M, K, up(N, GR<T>)}, {N, K, up(M, GR<T>)}};
+inline Plans plan_bwd(int64_t M, int64_t N, int64_t K, int parts) {
+    const Extent x[2] = {{M, K, parts * up(N, parts > 1 ? BK<T> : GR<T>)}, {N, K, parts * up(M, parts > 1 ? BK<T> : GR<T>)}};
     Plan p[2];
     plan_products<T, 2>(x, p);
     return Plans{p[0], p[1]};
@@ -970,15 +1065,16 @@ struct Products {
     Rest rest{};
     int n = 0, tile = 0;
     int add(const Plan& p, const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K, const Epilogue& e,
-            void* part) {
+            void* part, int parts = 1) {
         if (M == 0 || N == 0) return DSSVAE_OK;
         Shape s;
         s.A = A; s.lda = lda; s.B = B; s.ldb = ldb; s.M = M; s.N = (int)N; s.K = K;
+        s.parts = parts; s.part_at = M * lda;
         const int64_t tm = up(M, p.tile) / p.tile, tn = up(N, p.tile) / p.tile, blocks = tm * tn * p.ksplit;
         const int64_t join = p.ksplit > 1 ? (M * ((N + 7) / 8) + 255) / 256 : 0;
         if (!grid_fits(2 * blocks, 512) || !grid_fits(2 * join, 512)) return DSSVAE_ETOOBIG;  // (two products to a launch)
         s.tiles_m = (int)tm; s.tiles_n = (int)tn; s.ksplit = p.ksplit;
-        const int64_t nk = up(K, BK<T>) / BK<T>;
+        const int64_t nk = parts * (up(K, BK<T>) / BK<T>);
         s.ktiles = (nk + p.ksplit - 1) / p.ksplit;
         s.part = (float*)part;
         jobs.job[n] = Job{s, e, (int)blocks};
@@ -1050,11 +1146,11 @@ struct TurnList {
     Turns t{};
     int n = 0;
     void add(const void* src, int64_t ld, const void* z, int64_t ldz, int64_t R, int64_t C, void* out, int64_t ldo, void* outT, int64_t ldt,
-             float* sums) {
+             float* sums, int parts = 1) {
         const int64_t rows = turn_rows(R, C);
         // (streaming stores: 8192 x 16384 bf16, two outputs, 302 -> 268 us; at 10-20 MB they cost the product behind it 13 us of 43)
-        const int stream = R * C * es * ((out != nullptr) + (outT != nullptr)) > (int64_t)128 << 20;
-        t.job[n] = Turn{src, ld, z, ldz, R, C, out, ldo, outT, ldt, sums, (int)rows, stream};
+        const int stream = R * C * es * parts * ((out != nullptr) + (outT != nullptr)) > (int64_t)128 << 20;
+        t.job[n] = Turn{src, ld, z, ldz, R, C, out, ldo, outT, ldt, parts, R * ldo, C * ldt, sums, (int)rows, stream};
         t.begin[n + 1] = t.begin[n] + (int)(rows * ((C + 63) / 64));
         ++n;
     }
@@ -1136,30 +1232,31 @@ struct BwdArgs {
     void *dx, *dw, *db;
     int db_f32, act;
     int64_t M; int N, K;
+    int parts;    // of dz: 2 where dy act'(z) is no number of the type
     Plans plans;  // made by the pass that adds up the workspace
 };
 
 template <typename T>
 int backward(BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
-    const int64_t M = a.M, N = a.N, K = a.K, ldn = up(N, GR<T>), ldm = up(M, GR<T>), es = sizeof(T);
+    const int64_t M = a.M, N = a.N, K = a.K, es = sizeof(T), whole = a.parts > 1 ? BK<T> : GR<T>, ldn = up(N, whole), ldm = up(M, whole);
     int rc = DSSVAE_OK;
     // dz: a copy where it differs from dy or dy's rows cannot be loaded as they are
     const bool copy = a.dx && (a.z || !direct<T>(a.dy, a.lddy, N));
     const void* dz = a.dy;
     int64_t lddz = a.lddy;
     void *dzc = nullptr, *dzt = nullptr;
-    if (copy) { dzc = sp.take(M * ldn * es); dz = dzc; lddz = ldn; }
-    if (a.dw) dzt = sp.take(N * ldm * es);
+    if (copy) { dzc = sp.take(a.parts * M * ldn * es); dz = dzc; lddz = ldn; }
+    if (a.dw) dzt = sp.take(a.parts * N * ldm * es);
     float* sums = a.db ? (float*)sp.take(turn_rows(M, N) * N * 4) : nullptr;
     void* wt = a.dx ? sp.take(K * ldn * es) : nullptr;
     void* xt = a.dw ? sp.take(K * ldm * es) : nullptr;
-    if (dry) a.plans = plan_bwd<T>(M, N, K);
+    if (dry) a.plans = plan_bwd<T>(M, N, K, a.parts);
     const Plans& p = a.plans;
     void* part_x = a.dx ? sp.take(part_bytes(p.x, M, K)) : nullptr;
     void* part_w = a.dw ? sp.take(part_bytes(p.w, N, K)) : nullptr;
     if (dry) return rc;
     TurnList l{es};
-    if (copy || a.dw || a.db) l.add(a.dy, a.lddy, a.z, a.ldz, M, N, dzc, ldn, dzt, ldm, sums);
+    if (copy || a.dw || a.db) l.add(a.dy, a.lddy, a.z, a.ldz, M, N, dzc, ldn, dzt, ldm, sums, a.parts);
     if (a.dx) l.add(a.w, a.ldw, nullptr, 0, N, K, nullptr, 0, wt, ldn, nullptr);
     if (a.dw) l.add(a.x, a.ldx, nullptr, 0, M, K, nullptr, 0, xt, ldm, nullptr);
     if ((rc = turn<T>(l, a.act, st))) return rc;
@@ -1167,12 +1264,12 @@ int backward(BwdArgs& a, Space& sp, hipStream_t st, bool dry) {
     if (a.dx) {
         Epilogue e{};
         e.y = a.dx; e.ldy = a.lddx;
-        if ((rc = q.add(p.x, dz, lddz, wt, ldn, M, K, ldn, e, part_x))) return rc;
+        if ((rc = q.add(p.x, dz, lddz, wt, ldn, M, K, ldn, e, part_x, a.parts))) return rc;
     }
     if (a.dw) {
         Epilogue e{};
         e.y = a.dw; e.ldy = a.lddw;
-        if ((rc = q.add(p.w, dzt, ldm, xt, ldm, N, K, ldm, e, part_w))) return rc;
+        if ((rc = q.add(p.w, dzt, ldm, xt, ldm, N, K, ldm, e, part_w, a.parts))) return rc;
     }
     if ((rc = q.run(st))) return rc;
     return q.finish(st, sums, a.db ? (int)turn_rows(M, N) : 0, N, a.db, a.db_f32);
@@ -1228,15 +1325,21 @@ extern "C" int64_t dssvae_linear_act_bwd_workspace_bytes(const void* dy, int64_t
     BwdArgs a{};
     a.dy = dy; a.lddy = lddy; a.z = has_z ? &some : nullptr; a.M = M; a.N = N; a.K = K;
     a.dx = want_dx ? &some : nullptr; a.dw = want_dw ? &some : nullptr; a.db = want_db ? &some : nullptr;
-    Space sp{nullptr, 0, 0};
-    bwd_any(dtype, a, sp, nullptr, true);
-    return sp.used;
+    int64_t most = 0;
+    for (a.parts = 1; a.parts <= (has_z && dtype != DSSVAE_F32 ? 2 : 1); ++a.parts) {  // (whatever the activation)
+        Space sp{nullptr, 0, 0};
+        bwd_any(dtype, a, sp, nullptr, true);
+        most = sp.used > most ? sp.used : most;
+    }
+    return most;
 }
 
 extern "C" int dssvae_linear_act_bwd(const void* dy, int64_t lddy, const void* z, int64_t ldz, const void* x, int64_t ldx,
                                      const void* w, int64_t ldw, int dtype, int act, int64_t M, int N, int K, void* dx,
                                      int64_t lddx, void* dw, int64_t lddw, void* db, int db_f32, void* workspace,
                                      int64_t workspace_bytes, void* stream) {
+    const bool round_dz = act & DSSVAE_ACT_ROUND_DZ;
+    act &= ~DSSVAE_ACT_ROUND_DZ;
     if (bad_args(dtype, act, M, N, K) || lddy < N || (z && ldz < N) || (dw && (ldx < K || lddw < K)) || (dx && (ldw < K || lddx < K)))
         return DSSVAE_EINVAL;
     if (act != DSSVAE_ACT_NONE && !z && M > 0) return DSSVAE_EINVAL;
@@ -1246,6 +1349,7 @@ extern "C" int dssvae_linear_act_bwd(const void* dy, int64_t lddy, const void* z
     a.dy = dy; a.lddy = lddy; a.z = act == DSSVAE_ACT_NONE ? nullptr : z; a.ldz = ldz; a.x = x; a.ldx = ldx; a.w = w; a.ldw = ldw;
     a.dx = M > 0 ? dx : nullptr; a.lddx = lddx; a.dw = dw; a.lddw = lddw; a.db = db; a.db_f32 = db_f32 || dtype == DSSVAE_F32;
     a.act = act; a.M = M; a.N = N; a.K = K;
+    a.parts = dtype != DSSVAE_F32 && act > DSSVAE_ACT_RELU && !round_dz ? 2 : 1;
     Space need{nullptr, 0, 0};
     bwd_any(dtype, a, need, nullptr, true);
     if (need.used > 0 && (!workspace || workspace_bytes < need.used || !aligned_to(workspace, 16))) return DSSVAE_EINVAL;

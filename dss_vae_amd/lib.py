@@ -40,6 +40,7 @@ class GruBwdInst(C.Structure):
 CELL_GRU, CELL_LSTM = 0, 1
 DISTILL_MAX_TOP = 1024
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "tanh": 4}  # DSSVAE_ACT_*
+ACT_ROUND_DZ = 0x100
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # DSSVAE_F32 / _BF16 / _F16
 
 

@@ -2244,7 +2244,7 @@ def _linear_act_fwd(x2, ldx, w, ldw, b, act, r, code, keep_z):
 
 class _LinearActFn(Function):
     @staticmethod
-    def forward(ctx, x, w, b, residual, act, code):
+    def forward(ctx, x, w, b, residual, act, code, round_dz):
         ctx.set_materialize_grads(False)
         _record("linear_act", ctx, x.device)
         N = w.size(0)
@@ -2253,14 +2253,14 @@ class _LinearActFn(Function):
         keep = act != 0 and any(ctx.needs_input_grad[:3])
         y, z = _linear_act_fwd(x2, ldx, wc, ldw, _contig(b), act, None if residual is None else _flat(residual), code, keep)
         ctx.save_for_backward(x2, w, z)
-        ctx.bias_ref, ctx.act, ctx.code, ctx.xshape = b, act, code, x.shape
+        ctx.bias_ref, ctx.act, ctx.code, ctx.xshape = b, act | (L.ACT_ROUND_DZ if round_dz else 0), code, x.shape
         return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         if dy is None:
-            return (None,) * 6
+            return (None,) * 7
         x2, w, z = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dx = dw = db = None
@@ -2287,14 +2287,15 @@ class _LinearActFn(Function):
                          "M=%d N=%d K=%d" % (M, N, K)))
             if dx is not None and len(ctx.xshape) != 2:
                 dx = dx.view(ctx.xshape)
-        return dx, dw, db, dy if need_r else None, None, None
+        return dx, dw, db, dy if need_r else None, None, None, None
 
 
-def linear_act(x, w, b=None, act="none", residual=None):
+def linear_act(x, w, b=None, act="none", residual=None, round_dz=False):
     """act(x w^T + b) + residual: x [..., K], w [N, K] and residual [..., N] of one type (float32, bfloat16, float16),
     b [N] of that type or float32; act "none", "relu", "gelu" (the exact form), "silu" or "tanh".  Products accumulate in
     fp32 in a fixed order and every output is rounded once.  For training in 16 bits the slope's argument is kept in 16 bits
-    (evenly spaced, finer than either type where slopes move) and the products of backward take dy act'(z) rounded to the type."""
+    (evenly spaced, finer than either type where slopes move), and the products of backward take dz = dy act'(z) unrounded, in two
+    16-bit parts; round_dz=True rounds it to the type instead: half the matrix work of backward, sqrt(2) times the error of dx and dw."""
     code = _typed("linear_act", x)
     if act not in L.ACTIVATIONS:
         raise RuntimeError("linear_act: act must be one of %s, got %r" % (sorted(L.ACTIVATIONS), act))
@@ -2308,7 +2309,7 @@ def linear_act(x, w, b=None, act="none", residual=None):
         _expect("linear_act", "residual", residual, tuple(x.shape[:-1]) + (N,), (x.dtype,), x.device)
     a = L.ACTIVATIONS[act]
     if _wants_grad(x, w, b, residual):
-        return _LinearActFn.apply(x, w, b, residual, a, code)
+        return _LinearActFn.apply(x, w, b, residual, a, code, bool(round_dz))
     x2, ldx = _matrix(_flat(x))
     w2, ldw = _matrix(w)
     y, _ = _linear_act_fwd(x2, ldx, w2, ldw, _contig(b), a, None if residual is None else _flat(residual), code, False)
