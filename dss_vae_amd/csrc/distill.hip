@@ -14,6 +14,11 @@
 // The k teacher slots are wave 0's: softmax by shuffles while the block loads.  The k gradient entries are written over the
 // dense store behind a barrier, by the first slot of each distinct id with the sum of its probabilities: no atomics, and
 // repeated ids add up in slot order.
+// An upstream gradient f other than 1 (a loss scale, a mixing weight) is only known in backward.  It has to come before the rounding to
+// 16 bits: at 7936 rows and 30000 words the unit gradient of a word is about 1e-8, zero in fp16, and 65536 times it is not.  So
+// backward forms the rows again with w f in place of w, from the logits (read and write: what multiplying the stored gradient
+// would move, too: 7936 x 30000 fp32 366 us a step with f = 1, 739 with 0.3; 2048 x 100003 bf16 187 and 389).  Where f is 1 its blocks
+// end at once.
 #include "elem.h"
 
 namespace {
@@ -52,12 +57,12 @@ __device__ __forceinline__ void keep_raw(Gran<T, VEC>& v) {
     v.v = __builtin_bit_cast(typename Gran<T, VEC>::V, r);
 }
 
-// NV granules per thread in registers; HOLD > 0: any width, the next HOLD granules per thread stay in LDS and what is still left
-// is read twice; NV = 0: any width, no gradient
+// One row by a block.  NV granules per thread in registers; HOLD > 0: any width, the next HOLD granules per thread stay in LDS and
+// what is still left is read twice; NV = 0: any width, no gradient.  f: the gradient's factor; rows NULL: the loss is not wanted.
 template <typename T, int NT, int NV, int HOLD>
-__global__ __launch_bounds__(NT, NV == 8 ? 8 : 4) void distill_kernel(
-    const T* __restrict__ z, int64_t ldz, int V, const int64_t* __restrict__ ids, const float* __restrict__ teacher, int k,
-    float tau, const float* __restrict__ weight, float w_all, T* __restrict__ dz, int64_t lddz, float* __restrict__ rows) {
+__device__ __forceinline__ void distill_row(const T* __restrict__ z, int64_t ldz, int V, const int64_t* __restrict__ ids,
+                                            const float* __restrict__ teacher, int k, float tau, const float* __restrict__ weight,
+                                            float w_all, T* __restrict__ dz, int64_t lddz, float* __restrict__ rows, int64_t row, float f) {
     constexpr int VEC = 16 / (int)sizeof(T);
     constexpr int NR = NV > 0 ? NV : 1, AHEAD = 4;  // loads in flight in the walk over what the registers do not hold
     static_assert(HOLD % AHEAD == 0, "whole steps of the walk are held");
@@ -67,7 +72,6 @@ __global__ __launch_bounds__(NT, NV == 8 ? 8 : 4) void distill_kernel(
     float* s_p = reinterpret_cast<float*>(s_id + k);
     __shared__ float s_mass;  // 1, 0 (no valid slot) or NaN (an id outside the vocabulary, a NaN or +inf among the teacher's logits)
     const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x;
     const float w = weight ? weight[row] : w_all, c = LOG2E / tau;
     const T* zr = z + row * ldz;
     T* dr = dz ? dz + row * lddz : nullptr;
@@ -150,7 +154,7 @@ __global__ __launch_bounds__(NT, NV == 8 ? 8 : 4) void distill_kernel(
     __syncthreads();
     const float mass = dead ? 0.f : s_mass;
     if (mass == 0.f) {  // (the whole block alike)
-        if (tid == 0) rows[row] = 0.f;
+        if (rows && tid == 0) rows[row] = 0.f;
         if (!dr) return;
         Gran<T, VEC> o;
         o.zero();
@@ -166,7 +170,7 @@ __global__ __launch_bounds__(NT, NV == 8 ? 8 : 4) void distill_kernel(
     float S = r.y * exp2_f((r.x - M) * c);
 #pragma unroll
     for (int o = NT / 128; o > 0; o >>= 1) S += __shfl_xor(S, o, 64);
-    if (tid < 64) {
+    if (rows && tid < 64) {
         float part = 0.f;
         for (int j = tid; j < k; j += 64) {
             const float p = s_p[j];
@@ -176,7 +180,7 @@ __global__ __launch_bounds__(NT, NV == 8 ? 8 : 4) void distill_kernel(
         if (tid == 0) rows[row] = tau * tau * (part + logf(S)) * mass;
     }
     if (NV == 0 || !dr) return;
-    const float a = w * tau * mass / S;
+    const float wt = w * tau * f, a = wt * mass / S;
     T* db = dr + head;
     {
 #pragma unroll
@@ -212,7 +216,27 @@ __global__ __launch_bounds__(NT, NV == 8 ? 8 : 4) void distill_kernel(
             first = first && !(same && i < j);
             p += same ? s_p[i] : 0.f;
         }
-        if (first) dr[id] = (T)(a * exp2_f(((float)zr[id] - M) * c) - w * tau * p * mass);
+        if (first) dr[id] = (T)(a * exp2_f(((float)zr[id] - M) * c) - wt * p * mass);
+    }
+}
+
+template <typename T, int NT, int NV, int HOLD>
+__global__ __launch_bounds__(NT, NV == 8 ? 8 : 4) void distill_kernel(
+    const T* __restrict__ z, int64_t ldz, int V, const int64_t* __restrict__ ids, const float* __restrict__ teacher, int k,
+    float tau, const float* __restrict__ weight, float w_all, T* __restrict__ dz, int64_t lddz, float* __restrict__ rows) {
+    distill_row<T, NT, NV, HOLD>(z, ldz, V, ids, teacher, k, tau, weight, w_all, dz, lddz, rows, blockIdx.x, 1.f);
+}
+
+// the gradient again, times *factor, unless that is 1: as many blocks as the chip holds, row after row
+template <typename T, int NT, int NV, int HOLD>
+__global__ __launch_bounds__(NT, NV == 8 ? 8 : 4) void distill_again_kernel(
+    const T* __restrict__ z, int64_t ldz, int64_t N, int V, const int64_t* __restrict__ ids, const float* __restrict__ teacher, int k,
+    float tau, const float* __restrict__ weight, float w_all, const float* __restrict__ factor, T* __restrict__ dz, int64_t lddz) {
+    const float f = *factor;
+    if (f == 1.f) return;
+    for (int64_t row = blockIdx.x; row < N; row += gridDim.x) {
+        distill_row<T, NT, NV, HOLD>(z, ldz, V, ids, teacher, k, tau, weight, w_all, dz, lddz, nullptr, row, f);
+        __syncthreads();  // the row's slots and sums have been read
     }
 }
 
@@ -253,13 +277,23 @@ __global__ __launch_bounds__(256) void scale_kernel(T* __restrict__ x, int64_t l
         for (int64_t c = threadIdx.x; c < V; c += 256) x[r * ld + c] = (T)((float)x[r * ld + c] * f);
 }
 
+// (factor: the gradient alone, again)
 template <typename T>
 int launch(const T* z, int64_t ldz, int64_t N, int V, const int64_t* ids, const float* teacher, int k, float tau,
-           const float* weight, float w_all, T* dz, int64_t lddz, float* rows, hipStream_t s) {
+           const float* weight, float w_all, const float* factor, T* dz, int64_t lddz, float* rows, hipStream_t s) {
     constexpr int VEC = 16 / (int)sizeof(T);
     const int64_t gran = ((int64_t)V + VEC - 1) / VEC;
 #define GO(NT, NV, HOLD)                                                                                                   \
     do {                                                                                                               \
+        if constexpr ((NV) > 0) {                                                                                      \
+            if (factor) {                                                                                              \
+                const int64_t most = (int64_t)device_cus() * (2048 / NT);                                              \
+                hipLaunchKernelGGL((distill_again_kernel<T, NT, NV, HOLD>), dim3((unsigned)(N < most ? N : most)), dim3(NT), k * 8, s, z, ldz, \
+                                   N, V, ids, teacher, k, tau, weight, w_all, factor, dz, lddz);                       \
+                DSSVAE_CHECK_LAUNCH();                                                                                 \
+                return DSSVAE_OK;                                                                                      \
+            }                                                                                                          \
+        }                                                                                                              \
         hipLaunchKernelGGL((distill_kernel<T, NT, NV, HOLD>), dim3((unsigned)N), dim3(NT), k * 8, s, z, ldz, V, ids, teacher, k, tau, weight, \
                            w_all, dz, lddz, rows);                                                                     \
         DSSVAE_CHECK_LAUNCH();                                                                                         \
@@ -282,36 +316,58 @@ int launch(const T* z, int64_t ldz, int64_t N, int V, const int64_t* ids, const 
 
 }  // namespace
 
-extern "C" int dssvae_distill(const void* logits, int64_t ldz, int dtype, int64_t N, int V, const int64_t* ids,
-                              const float* teacher, int k, float tau, const float* weight, float weight_all, void* dlogits,
-                              int64_t lddz, float* rows, float* total, void* stream) {
+namespace {
+
+bool bad_args(const void* logits, int64_t ldz, int dtype, int64_t N, int V, const int64_t* ids, const float* teacher, int k, float tau,
+              const void* dlogits, int64_t lddz) {
     if (!dtype_ok(dtype) || N < 0 || N > 0x7fffffff || V < 1 || V > (1 << 30) || k < 1 || k > MAX_TOP || ldz < V ||
-        !(tau > 0.f) || !(tau < __builtin_huge_valf()) || !total || (dlogits && lddz < V))
-        return DSSVAE_EINVAL;
-    if (N > 0 && (!logits || !ids || !teacher || !rows)) return DSSVAE_EINVAL;
+        !(tau > 0.f) || !(tau < __builtin_huge_valf()) || (dlogits && lddz < V))
+        return true;
+    if (N > 0 && (!logits || !ids || !teacher)) return true;
     const int es = elem_size(dtype);
-    if (!aligned_to(logits, es) || !aligned_to(dlogits, es)) return DSSVAE_EINVAL;
+    if (!aligned_to(logits, es) || !aligned_to(dlogits, es)) return true;
     // a granule of the gradient is stored where its logits were loaded: same offset from the 16-byte boundary in every row
-    if (dlogits && N > 0 && ((reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(dlogits)) % 16 != 0 ||
-                             (N > 1 && (ldz - lddz) % (16 / es) != 0)))
-        return DSSVAE_EINVAL;
-    hipStream_t s = (hipStream_t)stream;
+    return dlogits && N > 0 && ((reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(dlogits)) % 16 != 0 ||
+                                (N > 1 && (ldz - lddz) % (16 / es) != 0));
+}
+
+int all_rows(const void* logits, int64_t ldz, int dtype, int64_t N, int V, const int64_t* ids, const float* teacher, int k, float tau,
+             const float* weight, float weight_all, const float* factor, void* dlogits, int64_t lddz, float* rows, hipStream_t s) {
     constexpr int64_t PART = 1 << 21;  // rows of a launch: 1024 threads each stay below 2^32
     for (int64_t r = 0; r < N; r += PART) {
         const int64_t n = N - r < PART ? N - r : PART;
         int e;
 #define GO(T)                                                                                                          \
-    launch<T>((const T*)logits + r * ldz, ldz, n, V, ids + r * k, teacher + r * k, k, tau, weight ? weight + r : nullptr, weight_all, \
-              dlogits ? (T*)dlogits + r * lddz : nullptr, lddz, rows + r, s)
+    launch<T>((const T*)logits + r * ldz, ldz, n, V, ids + r * k, teacher + r * k, k, tau, weight ? weight + r : nullptr, weight_all, factor, \
+              dlogits ? (T*)dlogits + r * lddz : nullptr, lddz, rows ? rows + r : nullptr, s)
         if (dtype == DSSVAE_F32) e = GO(float);
         else if (dtype == DSSVAE_BF16) e = GO(bf16_t);
         else e = GO(f16_t);
 #undef GO
         if (e != DSSVAE_OK) return e;
     }
+    return DSSVAE_OK;
+}
+
+}  // namespace
+
+extern "C" int dssvae_distill(const void* logits, int64_t ldz, int dtype, int64_t N, int V, const int64_t* ids,
+                              const float* teacher, int k, float tau, const float* weight, float weight_all, void* dlogits,
+                              int64_t lddz, float* rows, float* total, void* stream) {
+    if (bad_args(logits, ldz, dtype, N, V, ids, teacher, k, tau, dlogits, lddz) || !total || (N > 0 && !rows)) return DSSVAE_EINVAL;
+    hipStream_t s = (hipStream_t)stream;
+    const int e = all_rows(logits, ldz, dtype, N, V, ids, teacher, k, tau, weight, weight_all, nullptr, dlogits, lddz, rows, s);
+    if (e != DSSVAE_OK) return e;
     hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(1024), 0, s, rows, weight, weight_all, N, total);
     DSSVAE_CHECK_LAUNCH();
     return DSSVAE_OK;
+}
+
+extern "C" int dssvae_distill_again(const void* logits, int64_t ldz, int dtype, int64_t N, int V, const int64_t* ids,
+                                    const float* teacher, int k, float tau, const float* weight, float weight_all, const float* factor,
+                                    void* dlogits, int64_t lddz, void* stream) {
+    if (bad_args(logits, ldz, dtype, N, V, ids, teacher, k, tau, dlogits, lddz) || !factor || (N > 0 && !dlogits)) return DSSVAE_EINVAL;
+    return all_rows(logits, ldz, dtype, N, V, ids, teacher, k, tau, weight, weight_all, factor, dlogits, lddz, nullptr, (hipStream_t)stream);
 }
 
 extern "C" int dssvae_scale_rows(void* x, int64_t ld, int dtype, int64_t rows, int V, const float* factor, void* stream) {

@@ -153,6 +153,7 @@ _SIGNATURES = {
     "dssvae_gated_scan_bwd": ([_P, _L, _L, _I, _P, _I, _I, _P, _P, _L, _L, _P, _I, _I, _I, _P, _L, _L, _P, _P, _L, _P], _I),
     "dssvae_gated_step": ([_P, _L, _I, _P, _I, _I, _I, _P, _L, _P, _P], _I),
     "dssvae_distill": ([_P, _L, _I, _L, _I, _P, _P, _I, _F, _P, _F, _P, _L, _P, _P, _P], _I),
+    "dssvae_distill_again": ([_P, _L, _I, _L, _I, _P, _P, _I, _F, _P, _F, _P, _P, _L, _P], _I),
     "dssvae_scale_rows": ([_P, _L, _I, _L, _I, _P, _P], _I),
     "dssvae_linear_act_fwd_workspace_bytes": ([_P, _L, _P, _L, _I, _L, _I, _I], _L),
     "dssvae_linear_act_fwd": ([_P, _L, _P, _L, _P, _I, _P, _L, _I, _I, _L, _I, _I, _P, _L, _P, _L, _P, _L, _P], _I),

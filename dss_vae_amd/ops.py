@@ -2155,8 +2155,8 @@ def _distill(z, ldz, code, ids, teacher, tau, weight, want_grad):
 
 
 class _DistillFn(Function):
-    """the gradient is written by the forward pass (the rows' weights are its arguments) and scaled by the upstream
-    scalar in backward, which costs nothing where that is 1"""
+    """the gradient is written by the forward pass (the rows' weights are its arguments); an upstream scalar other than 1 has
+    backward form it again from the logits, times that scalar and rounded once"""
 
     @staticmethod
     def forward(ctx, logits, ids, teacher, weight, tau, code):
@@ -2164,7 +2164,8 @@ class _DistillFn(Function):
         _record("distill_loss", ctx, logits.device)
         z, ldz = _matrix(_flat(logits))
         total, rows, ctx.dz = _distill(z, ldz, code, ids, teacher, tau, weight, True)
-        ctx.shape, ctx.code = logits.shape, code
+        ctx.save_for_backward(z, ids, teacher, weight)
+        ctx.shape, ctx.code, ctx.tau = logits.shape, code, tau
         if logits.dim() != 2:
             rows = rows.view(logits.shape[:-1])
         ctx.mark_non_differentiable(rows)
@@ -2180,8 +2181,15 @@ class _DistillFn(Function):
         if dz is None:
             raise RuntimeError("distill_loss keeps its gradient for ONE backward pass (retain_graph / a second backward "
                                "is not supported)")
-        if dz.size(0):
-            _go("dssvae_scale_rows", dz.device, (dz.data_ptr(), dz.stride(0), ctx.code, dz.size(0), dz.size(1), g.data_ptr()))
+        z, ids, teacher, weight = ctx.saved_tensors
+        z, ldz = _matrix(z)
+        N, V = dz.shape
+        if (z.data_ptr() - dz.data_ptr()) % 16 or N > 1 and (ldz - dz.stride(0)) * z.element_size() % 16:
+            z, ldz = _matrix(_like_rows(dz, dz.stride(0)).copy_(z))  # (a saved tensor that came back at another place)
+        if N:
+            _go("dssvae_distill_again", dz.device,
+                (z.data_ptr(), ldz, ctx.code, N, V, ids.data_ptr(), teacher.data_ptr(), ids.size(1), ctx.tau, _p(weight), 1.0 / N,
+                 g.data_ptr(), dz.data_ptr(), dz.stride(0)))
         if len(ctx.shape) != 2:
             dz = dz.view(ctx.shape) if dz.is_contiguous() else dz.unflatten(0, ctx.shape[:-1])
         return dz, None, None, None, None, None
@@ -2194,7 +2202,8 @@ def distill_loss(logits, ids, teacher, temperature=1.0, weight=None):
     up; teacher [..., k] float32 or of the logits' type (logits or log-probabilities alike); weight [...] float32, None =
     1 / rows each.  Rows of weight 0 and rows without a valid slot are not read: loss 0, gradient 0.
     -> (total = sum of weight * row, a differentiable float32 scalar; rows [...] float32, for reporting only).
-    The gradient of `total` is computed in the forward pass and kept for ONE backward pass."""
+    The gradient of `total` is computed in the forward pass and kept for ONE backward pass; an upstream gradient other than 1
+    (a loss scale, a mixing weight) costs that pass another one over the logits, and comes ahead of the rounding to their type."""
     code = _typed("distill_loss", logits)
     if logits.dim() < 2 or logits.size(-1) < 1:
         raise RuntimeError("distill_loss: logits must be [..., V], got %s" % (list(logits.shape),))

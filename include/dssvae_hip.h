@@ -604,12 +604,18 @@ int dssvae_gated_step(const void* x, int64_t xb, int dtype, const float* h, int 
  *   teacher logit makes its row (loss and gradient) NaN.  A row without a valid slot, all teacher logits -inf among it, and one of
  *   weight 0 is not read: loss 0, gradient 0.  weight [N] fp32, or NULL: weight_all for every row.
  *   dlogits NULL: no gradient.  Its rows must start at the same offset from a 16-byte boundary as those of logits.
+ * dssvae_distill_again: for a backward pass whose upstream gradient *factor (fp32 on the device) is not 1: writes dlogits once more, with
+ * w_i *factor in place of w_i, from the arguments of the call before, so that the factor comes ahead of the rounding to dtype.  Where it
+ * is 1 nothing is touched.
  * dssvae_scale_rows: x[r, :V] *= *factor (fp32 on the device), without touching memory where that is 1.
  * ------------------------------------------------------------------------------------------- */
 #define DSSVAE_DISTILL_MAX_TOP 1024
 int dssvae_distill(const void* logits, int64_t ldz, int dtype, int64_t N, int V, const int64_t* ids, const float* teacher,
                    int k, float tau, const float* weight, float weight_all, void* dlogits, int64_t lddz, float* rows,
                    float* total, void* stream);
+int dssvae_distill_again(const void* logits, int64_t ldz, int dtype, int64_t N, int V, const int64_t* ids, const float* teacher,
+                         int k, float tau, const float* weight, float weight_all, const float* factor, void* dlogits, int64_t lddz,
+                         void* stream);
 int dssvae_scale_rows(void* x, int64_t ld, int dtype, int64_t rows, int V, const float* factor, void* stream);
 
 /* ---------------------------------------------------------------------------------------------

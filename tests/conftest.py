@@ -15,6 +15,21 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
 
 
+# tests whose expected value is wrong, with the reason; each still runs and must go on failing
+WRONG_VALUES = {
+    "test_blocks_distill_gpu.py::test_upstream_factor[dtype2]":
+        "fp16: expects 4 times the unit gradient as rounded to the type.  Among subnormal numbers that is a multiple of 4 smallest steps (2^-24), up to 2 "
+        "of them off; 4 times the exact gradient rounded once is within half a step (test_blocks_distill_factor_gpu.py holds it to that)",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        for name, reason in WRONG_VALUES.items():
+            if item.nodeid.endswith(name):
+                item.add_marker(pytest.mark.xfail(reason=reason, strict=True, raises=AssertionError))
+
+
 def load_golden(name):
     return torch.load(os.path.join(GOLDEN, name + ".pt"), weights_only=True)
 
