@@ -31,8 +31,14 @@ template <typename T> constexpr int KT = sizeof(T) == 4 ? 16 : 8;
 template <typename T, int DIV> constexpr int NT = CHUNK / DIV * LPR / KT<T>;
 constexpr int STEP_THREADS = 256;
 
-__device__ __forceinline__ float sigmoid_f(float x) {
-    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+// a = sigmoid(z) and b = 1 - a, each to its own accuracy: long memories are gates whose 1 - a is small, and the update and both
+// gradients are proportional to it.  With u = exp(-z), a = 1 / (1 + u) and b = u a; a subtraction leaves 1 - a with a few bits (off by
+// 1e-3 at z = 10, all of it at 17).  a close to 1 is 1 - b, which is rounded to nearest: what 1 + u and the reciprocal lose
+// would add up over thousands of steps.  z = +inf gives 1 and 0 exactly, z = -inf (u overflows) 0 and 1, NaN stays.
+__device__ __forceinline__ void gate_f(float z, float& a, float& b) {
+    const float u = __builtin_amdgcn_exp2f(-1.4426950408889634f * z), r = __builtin_amdgcn_rcpf(1.f + u);
+    b = u > 0x1p126f ? 1.f : u * r;
+    a = u < 1.f ? 1.f - b : r;
 }
 // (absolute error ~2e-7: hardware exp2 and rcp)
 __device__ __forceinline__ float tanh_f(float x) {
@@ -212,12 +218,13 @@ __global__ __launch_bounds__((NT<T, 1>)) void gated_scan_maps_kernel(const T* __
             const int k = BWD ? K - 1 - kk : kk;
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                const float a = sigmoid_f(s.z[k].get(v));
+                float a, b;
+                gate_f(s.z[k].get(v), a, b);
                 if constexpr (BWD) {
                     B[v] = a * (s.g[k].get(v) + B[v]);
                 } else {
                     const float n = TANH ? tanh_f(s.v[k].get(v)) : s.v[k].get(v);
-                    B[v] = a * B[v] + (1.f - a) * n;
+                    B[v] = a * B[v] + b * n;
                 }
                 A[v] *= a;
             }
@@ -243,9 +250,10 @@ __device__ __forceinline__ void fwd_chunk(const Steps<T, VEC, false, false>& s, 
     for (int k = 0; k < K; ++k) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            const float ak = sigmoid_f(s.z[k].get(v)), n = TANH ? tanh_f(s.v[k].get(v)) : s.v[k].get(v);
-            a[k][v] = ak;
-            bn[k][v] = (1.f - ak) * n;
+            const float n = TANH ? tanh_f(s.v[k].get(v)) : s.v[k].get(v);
+            float b;
+            gate_f(s.z[k].get(v), a[k][v], b);
+            bn[k][v] = b * n;
             B[v] = a[k][v] * B[v] + bn[k][v];
             A[v] *= a[k][v];
         }
@@ -296,16 +304,16 @@ template <typename T, int VEC, bool TANH, int DIV>
 __device__ __forceinline__ void bwd_chunk(const Steps<T, VEC, false, true>& s, const Thread<T, VEC>& th,
                                           const Dims& d, int chunk, float hc, float& E, float2* lds0, float2* lds1, T* dx) {
     constexpr int NW = NT<T, DIV> / 64, K = KT<T>;
-    float a[K][VEC], n[K][VEC], A[VEC], B[VEC], F[VEC], G[VEC], y[VEC], e[VEC];
+    float a[K][VEC], b[K][VEC], n[K][VEC], A[VEC], B[VEC], F[VEC], G[VEC], y[VEC], e[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) { A[v] = 1.f; B[v] = 0.f; G[v] = 0.f; }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            a[k][v] = sigmoid_f(s.z[k].get(v));
+            gate_f(s.z[k].get(v), a[k][v], b[k][v]);
             n[k][v] = TANH ? tanh_f(s.v[k].get(v)) : s.v[k].get(v);
-            B[v] = a[k][v] * B[v] + (1.f - a[k][v]) * n[k][v];
+            B[v] = a[k][v] * B[v] + b[k][v] * n[k][v];
             A[v] *= a[k][v];
         }
     }
@@ -324,7 +332,7 @@ __device__ __forceinline__ void bwd_chunk(const Steps<T, VEC, false, true>& s, c
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             h[k][v] = a[k][v] * (y[v] - n[k][v]);
-            y[v] = h[k][v] + n[k][v];
+            y[v] = a[k][v] * y[v] + b[k][v] * n[k][v];  // (h[k] + n would carry n's roundings into a small state)
         }
     }
     const int64_t dgs = d.reverse ? -d.gt : d.gt;
@@ -336,7 +344,7 @@ __device__ __forceinline__ void bwd_chunk(const Steps<T, VEC, false, true>& s, c
         Gran<T, VEC> oz, on_;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            const float D = s.g[k].get(v) + e[v], q = D * (1.f - a[k][v]);
+            const float D = s.g[k].get(v) + e[v], q = D * b[k][v];
             oz.set(v, q * h[k][v]);
             on_.set(v, TANH ? q * (1.f - n[k][v] * n[k][v]) : q);
             e[v] = a[k][v] * D;
@@ -394,8 +402,10 @@ __global__ __launch_bounds__(STEP_THREADS) void gated_step_kernel(const T* __res
     for (int j = 0; j < VEC; ++j) hv[j] = h ? h[b * H + c + j] : 0.f;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-        const float a = sigmoid_f(z.get(j)), n = TANH ? tanh_f(v.get(j)) : v.get(j);
-        hv[j] = a * hv[j] + (1.f - a) * n;
+        const float n = TANH ? tanh_f(v.get(j)) : v.get(j);
+        float a, b;
+        gate_f(z.get(j), a, b);
+        hv[j] = a * hv[j] + b * n;
         o.set(j, hv[j]);
     }
     o.store(out + b * ob + c);
