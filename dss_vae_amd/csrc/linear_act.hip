@@ -38,9 +38,6 @@ typedef float f32x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ float sigmoid_f(float x) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
 }
-__device__ __forceinline__ float tanh_f(float x) {
-    return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.8853900817779268f * x));
-}
 // Phi(z) of the normal distribution, given e = exp(-z^2 / 2): the five-term rational form of Abramowitz & Stegun 7.1.26
 // (|error of erf| <= 1.5e-7).  The epilogue is bound by the vector ALUs: this is 20 lane cycles where erff is about 45.
 __device__ __forceinline__ float normal_cdf(float z, float e) {
@@ -71,8 +68,9 @@ __device__ __forceinline__ float act_slope(int act, float z) {
             return s * (1.f + z * (1.f - s));
         }
         case DSSVAE_ACT_TANH: {
-            const float t = tanh_f(z);
-            return 1.f - t * t;
+            float slope;
+            tanh_f(z, slope);
+            return slope;
         }
         default: return 1.f;
     }

@@ -40,10 +40,6 @@ __device__ __forceinline__ void gate_f(float z, float& a, float& b) {
     b = u > 0x1p126f ? 1.f : u * r;
     a = u < 1.f ? 1.f - b : r;
 }
-// (absolute error ~2e-7: hardware exp2 and rcp)
-__device__ __forceinline__ float tanh_f(float x) {
-    return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(2.8853900817779268f * x));
-}
 
 struct Dims {
     const int32_t* lengths;
@@ -304,7 +300,7 @@ template <typename T, int VEC, bool TANH, int DIV>
 __device__ __forceinline__ void bwd_chunk(const Steps<T, VEC, false, true>& s, const Thread<T, VEC>& th,
                                           const Dims& d, int chunk, float hc, float& E, float2* lds0, float2* lds1, T* dx) {
     constexpr int NW = NT<T, DIV> / 64, K = KT<T>;
-    float a[K][VEC], b[K][VEC], n[K][VEC], A[VEC], B[VEC], F[VEC], G[VEC], y[VEC], e[VEC];
+    float a[K][VEC], b[K][VEC], n[K][VEC], dn[TANH ? K : 1][VEC], A[VEC], B[VEC], F[VEC], G[VEC], y[VEC], e[VEC];
 #pragma unroll
     for (int v = 0; v < VEC; ++v) { A[v] = 1.f; B[v] = 0.f; G[v] = 0.f; }
 #pragma unroll
@@ -312,7 +308,8 @@ __device__ __forceinline__ void bwd_chunk(const Steps<T, VEC, false, true>& s, c
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             gate_f(s.z[k].get(v), a[k][v], b[k][v]);
-            n[k][v] = TANH ? tanh_f(s.v[k].get(v)) : s.v[k].get(v);
+            if constexpr (TANH) n[k][v] = tanh_f(s.v[k].get(v), dn[k][v]);
+            else n[k][v] = s.v[k].get(v);
             B[v] = a[k][v] * B[v] + b[k][v] * n[k][v];
             A[v] *= a[k][v];
         }
@@ -346,7 +343,7 @@ __device__ __forceinline__ void bwd_chunk(const Steps<T, VEC, false, true>& s, c
         for (int v = 0; v < VEC; ++v) {
             const float D = s.g[k].get(v) + e[v], q = D * b[k][v];
             oz.set(v, q * h[k][v]);
-            on_.set(v, TANH ? q * (1.f - n[k][v] * n[k][v]) : q);
+            on_.set(v, TANH ? q * dn[TANH ? k : 0][v] : q);
             e[v] = a[k][v] * D;
         }
         if (!ok) {

@@ -38,7 +38,7 @@ def magnitudes(x, h0, dout, candidate):
     return torch.stack(hs, 1), torch.stack(D, 1), n, a, oma
 
 
-@pytest.mark.parametrize("candidate", ["linear"])
+@pytest.mark.parametrize("candidate", ["linear", "tanh"])
 @pytest.mark.parametrize("B,T,H", [(2, 60, 50), (3, 2000, 48), (40, 300, 130)])
 def test_long_memory(candidate, B, T, H):
     """fp32, gates at 8, 10, 12, 16, 20.  u = exp(-z) is off by |z| units of 2^-24 (its argument's rounding) and 2 of the instruction, 1 - a = u a by
