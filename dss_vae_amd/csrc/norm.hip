@@ -3,10 +3,12 @@
 // A row lives in registers between its one read and its one write: TPR threads hold E elements each, in granules of 16 bytes
 // (granule i of thread t covers columns (i * TPR + t) * VEC ..).  Rows may start anywhere and end inside a granule: loads take
 // any alignment, the last granule goes by elements (27513 x 1581 bf16: 50 us forward, 85 us backward; with element loads 69 and
-// 136 us).  Mean first, then the centred squares: two reductions over registers, no cancellation as in E[x^2] - E[x]^2.
+// 136 us).  Mean first, then the centred squares, no cancellation as in E[x^2] - E[x]^2.  The mean takes two reductions: partial sums of
+// values with a common offset are rounded to the offset's bits, and the mean of a row of 99999.9 came out 0.01 off; the deviations from it
+// are exact and their mean corrects it to half a step.
 // Forward, up to 1024 columns a row belongs to one wave or a quarter of one (shuffles only); wider rows take 256 threads.
 // Backward keeps E at 8 up to 4096 columns (its column sums cost 2 E registers more) and gives a row up to 512 threads.  Rows
-// wider than 8192 columns are walked three times by a block of 1024 (the repeats hit L2).
+// wider than 8192 columns are walked four times (backward twice) by a block of 1024 (the repeats hit L2).
 //   xh = (x - mean) rstd ; y = xh w + b
 //   dx = rstd (w dy - mean(w dy) - xh mean(w dy xh)) ; dw = sum_rows dy xh ; db = sum_rows dy
 // The column sums: a block walks rows blockIdx, + gridDim, ... and keeps dw / db of its columns in registers; its row groups
@@ -20,6 +22,18 @@ namespace {
 constexpr int FWD_THREADS = 256;
 constexpr int BWD_THREADS = 512;
 constexpr int LOOP_THREADS = 1024;
+
+// f(x - mean) for the granule's columns in front of D
+template <bool WHOLE, typename T, int VEC, typename F>
+__device__ __forceinline__ void deviations(const GranU<T, VEC>& g, int c, int D, float mean, F f) {
+    if (WHOLE ? c < D : c + VEC <= D) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f(g.get(j) - mean);
+    } else if (!WHOLE) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f(c + j < D ? g.get(j) - mean : 0.f);
+    }
+}
 
 template <typename T, int TPR, int E, bool WHOLE>
 __global__ __launch_bounds__(FWD_THREADS) void layer_norm_fwd_kernel(const T* __restrict__ x, int64_t ldx,
@@ -36,7 +50,7 @@ __global__ __launch_bounds__(FWD_THREADS) void layer_norm_fwd_kernel(const T* __
         load_param<WHOLE, T, VEC>(wv[i], w, param_f32, (i * TPR + t) * VEC, D, 1.f);
         load_param<WHOLE, T, VEC>(bv[i], b, param_f32, (i * TPR + t) * VEC, D, 0.f);
     }
-    const float n = (float)D;  // (divided by, not multiplied with 1 / n: the mean of equal values is that value)
+    const float n = (float)D;
     // (every row group of the block makes the same number of trips: the row sums may hold barriers)
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
         const int64_t r = r0 + g;
@@ -50,25 +64,15 @@ __global__ __launch_bounds__(FWD_THREADS) void layer_norm_fwd_kernel(const T* __
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) s += v[i].get(j);
-        const float mean = row_sum<TPR>(s, red) / n;
-        float q = 0.f;
+        float mean = row_sum<TPR>(s, red) / n, q = 0.f;
+        s = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * TPR + t) * VEC;
-            if (WHOLE ? c < D : c + VEC <= D) {
+        for (int i = 0; i < NV; ++i)
+            deviations<WHOLE, T, VEC>(v[i], (i * TPR + t) * VEC, D, mean, [&](float d) { s += d; });
+        mean += row_sum<TPR>(s, red) / n;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float d = v[i].get(j) - mean;
-                    q += d * d;
-                }
-            } else if (!WHOLE) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const float d = c + j < D ? v[i].get(j) - mean : 0.f;
-                    q += d * d;
-                }
-            }
-        }
+        for (int i = 0; i < NV; ++i)
+            deviations<WHOLE, T, VEC>(v[i], (i * TPR + t) * VEC, D, mean, [&](float d) { q += d * d; });
         const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red) / n + eps);
         if (!live) continue;
         T* yr = y + r * ldy;
@@ -86,7 +90,7 @@ __global__ __launch_bounds__(FWD_THREADS) void layer_norm_fwd_kernel(const T* __
     }
 }
 
-// rows too wide for the registers: one block per row, three walks
+// rows too wide for the registers: one block per row, four walks
 template <typename T>
 __global__ __launch_bounds__(LOOP_THREADS) void layer_norm_fwd_wide_kernel(const T* __restrict__ x, int64_t ldx,
                                                                             const void* __restrict__ w,
@@ -100,8 +104,10 @@ __global__ __launch_bounds__(LOOP_THREADS) void layer_norm_fwd_wide_kernel(const
         T* yr = y + r * ldy;
         float s = 0.f;
         for (int64_t c = threadIdx.x; c < D; c += LOOP_THREADS) s += (float)xr[c];
-        const float mean = row_sum<LOOP_THREADS>(s, red) / (float)D;
-        float q = 0.f;
+        float mean = row_sum<LOOP_THREADS>(s, red) / (float)D, q = 0.f;
+        s = 0.f;
+        for (int64_t c = threadIdx.x; c < D; c += LOOP_THREADS) s += (float)xr[c] - mean;
+        mean += row_sum<LOOP_THREADS>(s, red) / (float)D;
         for (int64_t c = threadIdx.x; c < D; c += LOOP_THREADS) {
             const float d = (float)xr[c] - mean;
             q += d * d;
