@@ -311,26 +311,28 @@ __global__ __launch_bounds__(256) void layer_norm_cols_kernel(const T* __restric
     part[(int64_t)blockIdx.y * 2 * D + D + c] = db;
 }
 
-// dw / db [D] = sum over n partials [2, D]: 32 columns per block, 32 threads share a column
+// dw / db [D] = sum over n partials [2, D]: 32 columns per block (and the next 32 a grid behind them), 32 threads share a column
 template <typename T>
 __global__ __launch_bounds__(1024) void layer_norm_sum_kernel(const float* __restrict__ part, int n, int D, void* dw,
                                                               void* db, int param_f32) {
     __shared__ float red[32][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int64_t c = (int64_t)blockIdx.x * 32 + tx;  // column of [dw | db]
-    float s = 0.f;
-    if (c < 2 * (int64_t)D)
-        for (int i = ty; i < n; i += 32) s += part[(int64_t)i * 2 * D + c];
-    red[ty][tx] = s;
-    __syncthreads();
-    if (ty != 0 || c >= 2 * (int64_t)D) return;
+    for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < 2 * (int64_t)D; c0 += (int64_t)gridDim.x * 32) {
+        const int64_t c = c0 + tx;  // column of [dw | db]
+        float s = 0.f;
+        if (c < 2 * (int64_t)D)
+            for (int i = ty; i < n; i += 32) s += part[(int64_t)i * 2 * D + c];
+        __syncthreads();  // the sums of the columns before have been read
+        red[ty][tx] = s;
+        __syncthreads();
+        void* o = c < D ? dw : db;
+        if (ty != 0 || c >= 2 * (int64_t)D || !o) continue;
 #pragma unroll
-    for (int i = 1; i < 32; ++i) s += red[i][tx];
-    void* o = c < D ? dw : db;
-    const int64_t k = c < D ? c : c - D;
-    if (!o) return;
-    if (param_f32) reinterpret_cast<float*>(o)[k] = s;
-    else reinterpret_cast<T*>(o)[k] = (T)s;
+        for (int i = 1; i < 32; ++i) s += red[i][tx];
+        const int64_t k = c < D ? c : c - D;
+        if (param_f32) reinterpret_cast<float*>(o)[k] = s;
+        else reinterpret_cast<T*>(o)[k] = (T)s;
+    }
 }
 
 // Which kernel a width takes: the first shape that covers D columns; {0, 0}: the wide form.
@@ -405,7 +407,9 @@ int bwd_launch(const T* x, int64_t ldx, const T* dy, int64_t lddy, const void* w
         DSSVAE_CHECK_LAUNCH();
     }
     if (part) {
-        hipLaunchKernelGGL((layer_norm_sum_kernel<T>), dim3((unsigned)((2 * (int64_t)D + 31) / 32)), dim3(1024), 0, s, part,
+        // (a launch holds fewer than 2^32 threads, 64 to a column here: rows of 2^26 and more columns take several trips)
+        const int64_t groups = (2 * (int64_t)D + 31) / 32, most = 1 << 20;
+        hipLaunchKernelGGL((layer_norm_sum_kernel<T>), dim3((unsigned)(groups < most ? groups : most)), dim3(1024), 0, s, part,
                            (int)blocks, D, dw, db, pf);
         DSSVAE_CHECK_LAUNCH();
     }
