@@ -5,7 +5,7 @@ import functools
 import os
 
 import torch
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import lib as L
@@ -1875,7 +1875,13 @@ def _flat(t):
     return t if t.dim() == 2 else t.reshape(-1, t.size(-1))
 
 
-def _wants_grad(*tensors):
+def _wants_grad(what, *tensors):
+    """does a call record a graph?  Dual tensors are refused: they do not require grad, and an output without a tangent would pass
+    for one whose derivative is zero."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("%s: no forward-mode derivatives" % what)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -1978,7 +1984,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
             _expect("layer_norm", name, p, (D,), (x.dtype, torch.float32), x.device)
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise RuntimeError("layer_norm: weight is %s, bias is %s" % (weight.dtype, bias.dtype))
-    if _wants_grad(x, weight, bias):
+    if _wants_grad("layer_norm", x, weight, bias):
         return _LayerNormFn.apply(x, weight, bias, float(eps), code)
     x2, ldx = _matrix(_flat(x))
     y = _layer_norm_fwd(x2, ldx, code, _contig(weight), _contig(bias), float(eps), None)
@@ -2094,7 +2100,7 @@ def gated_scan(xproj, h0=None, lengths=None, reverse=False, candidate="tanh"):
         _expect("gated_scan", "h0", h0, (B, H), (torch.float32,), xproj.device)
     if lengths is not None:
         lengths = _expect("gated_scan", "lengths", lengths, (B,), (torch.int32,), xproj.device).contiguous()
-    if _wants_grad(xproj, h0):
+    if _wants_grad("gated_scan", xproj, h0):
         return _GatedScanFn.apply(xproj, h0, lengths, int(bool(reverse)), tanh, code)
     return _gated_scan_fwd(_sequence(xproj), _contig(h0), lengths, int(bool(reverse)), tanh, code, False)[:2]
 
@@ -2117,7 +2123,7 @@ def gated_step(xproj, h=None, candidate="tanh", h_out=None):
         for name, t in (("h", h), ("xproj", xproj)):
             if t is not None and not (t is h and t.data_ptr() == h_out.data_ptr()) and _meet(t, h_out):
                 raise RuntimeError("gated_step: h_out overlaps %s" % name)
-    if _wants_grad(xproj, h):
+    if _wants_grad("gated_step", xproj, h):
         if h_out is not None:
             raise RuntimeError("gated_step: h_out is for serving (no gradients)")
         out, hn = gated_scan(xproj.unsqueeze(1), h, None, False, candidate)
@@ -2219,13 +2225,13 @@ def distill_loss(logits, ids, teacher, temperature=1.0, weight=None):
     tau = float(temperature)
     if not 0.0 < tau < float("inf"):
         raise RuntimeError("distill_loss: temperature must be positive and finite, got %r" % (temperature,))
-    if _wants_grad(teacher, weight):
+    if _wants_grad("distill_loss", teacher, weight):
         raise RuntimeError("distill_loss: gradients go to the logits only (detach teacher and weight)")
     ids2, t2 = _flat(ids).contiguous(), _flat(teacher).contiguous()
     if t2.dtype != torch.float32:
         t2 = t2.float()
     w2 = None if weight is None else (weight if weight.dim() == 1 else weight.reshape(-1)).contiguous()
-    if _wants_grad(logits):
+    if _wants_grad("distill_loss", logits):
         return _DistillFn.apply(logits, ids2, t2, w2, tau, code)
     z, ldz = _matrix(_flat(logits))
     total, rows, _ = _distill(z, ldz, code, ids2, t2, tau, w2, False)
@@ -2317,7 +2323,7 @@ def linear_act(x, w, b=None, act="none", residual=None, round_dz=False):
     if residual is not None:
         _expect("linear_act", "residual", residual, tuple(x.shape[:-1]) + (N,), (x.dtype,), x.device)
     a = L.ACTIVATIONS[act]
-    if _wants_grad(x, w, b, residual):
+    if _wants_grad("linear_act", x, w, b, residual):
         return _LinearActFn.apply(x, w, b, residual, a, code, bool(round_dz))
     x2, ldx = _matrix(_flat(x))
     w2, ldw = _matrix(w)
