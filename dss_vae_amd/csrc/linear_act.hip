@@ -4,7 +4,9 @@
 // Products run on one tile kernel: v_mfma_f32_32x32x16 for bf16 / fp16, fp32 accumulation, one rounding per output.
 // fp32 operands are taken apart into three bf16 each (24 bits, exact) as they come out of LDS, and six of the nine products of
 // the parts are added: what is left out is below 2^-22 of a product, and on the mean of random inputs the sums are closer to
-// the exact ones than v_mfma_f32_32x32x2_f32's order gives (K = 7936: 7e-7 of the norm; the library's fp32 product 1.6e-6).  The
+// the exact ones than v_mfma_f32_32x32x2_f32's order gives (K = 7936: 7e-7 of the norm; the library's fp32 product 1.6e-6).  Sums of
+// at most 32 products, where that would show (a single product came out up to four times as far off as one fp32 rounding), take the
+// fp32 instruction.  The
 // fp32 instruction does a sixteenth of the bf16 one's work: a library product of 4096^3 takes 0.91 ms, this one 0.70 ms (the six
 // run at 1170 TFLOP/s; a library product of bf16 operands reaches 1326).  Taking operands apart once per block, on their way
 // into LDS through registers, halves the vector instructions but measured the same: 0.73 ms.
@@ -474,13 +476,13 @@ __device__ __forceinline__ void k_step_split(Planes<MI, NI>& p0, Frags<float, MI
 }
 
 template <int MI, int NI>
-__device__ __forceinline__ void clear(f32x16 (&acc)[MI][NI]) {
+__device__ __forceinline__ void fill(f32x16 (&acc)[MI][NI], float f) {
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = f;
 }
 
 template <int MI, int NI>
@@ -501,7 +503,7 @@ __device__ __forceinline__ void tile_product(const Shape& s, int64_t m0, int n0,
     constexpr bool PARTS = sizeof(T) == 2, LIFTED = PARTS && Apart<T>::LOW != 1.f;
     const int wave = threadIdx.x >> 6;
     const int ra = wave / WC * (BM / WR), rb = wave % WC * (BN / WC);
-    clear(acc);
+    fill(acc, 0.f);
     if (kt0 >= kt1) return;
     Loader<T, BM, TH> la;
     Loader<T, BN, TH> lb;
@@ -604,15 +606,21 @@ __global__ __launch_bounds__(64 * WR * WC, 2) void linear_tile_kernel(Jobs jobs)
 
     f32x16 acc[MI][NI];
     if constexpr (sizeof(T) == 4) {
-        tile_product<T, BM, BN, WR, WC, true>(s, m0, n0, kt0, kt1, buf0, buf1, acc);
-        float odd = 0.f;  // NaN once a sum is not finite
+        int redo = 1;
+        if (s.K > BK<T>) {
+            tile_product<T, BM, BN, WR, WC, true>(s, m0, n0, kt0, kt1, buf0, buf1, acc);
+            float odd = 0.f;  // NaN once a sum is not finite
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
+            for (int i = 0; i < MI; ++i)
 #pragma unroll
-            for (int j = 0; j < NI; ++j)
+                for (int j = 0; j < NI; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) odd += 0.f * acc[i][j][r];
-        if (__syncthreads_or(odd != odd)) {  // infinities have no triple: those sums, and no others, from fp32 products
+                    for (int r = 0; r < 16; ++r) odd += 0.f * acc[i][j][r];
+            redo = __syncthreads_or(odd != odd);  // infinities have no triple: those sums, and no others, from fp32 products
+        } else {  // sums of one k-tile: too few terms for what the triples leave out to be lost among their roundings
+            fill(acc, __builtin_huge_valf());
+        }
+        if (redo) {
             f32x16 whole[MI][NI];
             tile_product<T, BM, BN, WR, WC, false>(s, m0, n0, kt0, kt1, buf0, buf1, whole);
 #pragma unroll

@@ -626,8 +626,8 @@ int dssvae_scale_rows(void* x, int64_t ld, int dtype, int64_t rows, int V, const
  *   y must not overlap x, w or z; it may be res.  DSSVAE_ACT_GELU is the exact form, z Phi(z).
  * Backward: dz = dy act'(z); dx = dz w; dw = dz^T x; db = sum over rows of dz; dx, dw, db may each be NULL, z only where act
  * is DSSVAE_ACT_NONE.  (The residual's gradient is dy.)  M = 0 clears dw and db.
- * fp32 accumulation in a fixed order; fp32 operands: each product is within 2^-22 of itself (operands below 2^-110: absolute
- * 2^-133); 16-bit types: dz goes into the products of backward in two parts, good to 2^-16 (bf16) or 2^-22 (fp16) of it, or, with
+ * fp32 accumulation in a fixed order; fp32 operands: in sums of more than 32 each product is within 2^-22 of itself (operands below
+ * 2^-110: absolute 2^-133); 16-bit types: dz goes into the products of backward in two parts, good to 2^-16 (bf16) or 2^-22 (fp16) of it, or, with
  * DSSVAE_ACT_ROUND_DZ or-ed into backward's act, rounded to the type for half the matrix work.  A summed axis (K forward, N for dx,
  * M for dw) has at most 2097152 elements, and a launch fewer than 2^32 threads: DSSVAE_ETOOBIG.
  * The workspace sizes depend on where the operands start: the query takes the pointers and strides of the call.
