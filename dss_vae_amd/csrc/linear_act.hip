@@ -40,30 +40,35 @@ typedef float f32x8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ float sigmoid_f(float x) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
 }
-// Phi(z) of the normal distribution, given e = exp(-z^2 / 2): the five-term rational form of Abramowitz & Stegun 7.1.26
-// (|error of erf| <= 1.5e-7).  The epilogue is bound by the vector ALUs: this is 20 lane cycles where erff is about 45.
+// Phi(z) of the normal distribution, given e = exp(-z^2 / 2).  fp32: from the complementary error function.  16-bit types: the five-term
+// rational form of Abramowitz & Stegun 7.1.26 (|error of erf| <= 1.5e-7, a thousandth of their half step): their epilogue is bound by the
+// vector ALUs, and this is 20 lane cycles where erff is about 45.
+template <typename T>
 __device__ __forceinline__ float normal_cdf(float z, float e) {
+    if constexpr (sizeof(T) == 4) return 0.5f * erfcf(-0.70710678118654752f * z);
     const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678118654752f * fabsf(z));
     const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
     const float q = 0.5f * p * e;
     return z < 0.f ? q : 1.f - q;
 }
 __device__ __forceinline__ float normal_exp(float z) { return __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z); }
+template <typename T>
 __device__ __forceinline__ float act_f(int act, float z) {
     switch (act) {
         case DSSVAE_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
-        case DSSVAE_ACT_GELU: return z * normal_cdf(z, normal_exp(z));
+        case DSSVAE_ACT_GELU: return z * normal_cdf<T>(z, normal_exp(z));
         case DSSVAE_ACT_SILU: return z * sigmoid_f(z);
         case DSSVAE_ACT_TANH: return tanh_f(z);
         default: return z;
     }
 }
+template <typename T>
 __device__ __forceinline__ float act_slope(int act, float z) {
     switch (act) {
         case DSSVAE_ACT_RELU: return z > 0.f ? 1.f : (z != z ? z : 0.f);
         case DSSVAE_ACT_GELU: {
             const float e = normal_exp(z);
-            return normal_cdf(z, e) + z * 0.3989422804014327f * e;
+            return normal_cdf<T>(z, e) + z * 0.3989422804014327f * e;
         }
         case DSSVAE_ACT_SILU: {
             const float s = sigmoid_f(z);
@@ -112,8 +117,8 @@ __device__ __forceinline__ float decode(int act, int16_t q) {
 // act'(z) from what forward kept
 template <typename T, int ACT>
 __device__ __forceinline__ float slope_kept(const T* z, int64_t i) {
-    if constexpr (sizeof(T) == 4) return act_slope(ACT, (float)z[i]);
-    else return act_slope(ACT, decode(ACT, reinterpret_cast<const int16_t*>(z)[i]));
+    if constexpr (sizeof(T) == 4) return act_slope<T>(ACT, (float)z[i]);
+    else return act_slope<T>(ACT, decode(ACT, reinterpret_cast<const int16_t*>(z)[i]));
 }
 
 // What happens to an accumulated element on its way out
@@ -153,7 +158,7 @@ __device__ __forceinline__ void finish8_act(const Epilogue& e, f32x8 a, f32x8 b,
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             zz[j] = a[j] + b[j];
-            gy.set(j, act_f(ACT, zz[j]) + g.get(j));
+            gy.set(j, act_f<T>(ACT, zz[j]) + g.get(j));
         }
         if (z) {
             if constexpr (sizeof(T) == 4) {
@@ -183,7 +188,7 @@ __device__ __forceinline__ void finish8_act(const Epilogue& e, f32x8 a, f32x8 b,
                 if constexpr (sizeof(T) == 4) z[j] = zz[j];
                 else reinterpret_cast<int16_t*>(z)[j] = q[j];
             }
-            y[j] = (T)(act_f(ACT, zz[j]) + (r ? (float)r[j] : 0.f));
+            y[j] = (T)(act_f<T>(ACT, zz[j]) + (r ? (float)r[j] : 0.f));
         }
     }
 }
@@ -907,12 +912,12 @@ __global__ __launch_bounds__(256) void linear_turn_kernel(Turns jobs) {
                         if constexpr (sizeof(T) == 4) {
                             g.load(z + r * ldz + c);
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) v[j] *= act_slope(ACT, g.get(j));
+                            for (int j = 0; j < 8; ++j) v[j] *= act_slope<T>(ACT, g.get(j));
                         } else {
                             GranU<int16_t, 8> gq;
                             gq.load(reinterpret_cast<const int16_t*>(z) + r * ldz + c);
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) v[j] *= act_slope(ACT, decode(ACT, gq.v[j]));
+                            for (int j = 0; j < 8; ++j) v[j] *= act_slope<T>(ACT, decode(ACT, gq.v[j]));
                         }
                     }
                 } else {
