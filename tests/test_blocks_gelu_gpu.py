@@ -29,3 +29,30 @@ def test_relative_accuracy():
     got, want = g.cpu().double().view(-1), cdf + d * pdf
     err = (got - want).abs() / (cdf + (d * pdf).abs())
     assert (err <= units * U32).all(), float((err / units / U32).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_every_value_of_the_16_bit_types(dtype):
+    """one rounding: half a step of the type, and a twentieth of it for what comes before (1e-6 of the rational form; exp2's argument z^2 / 2 log2 e,
+    off by 2.3 roundings: 1.2 z^2 units of 2^-24, 1.4e-5 at z = -14).  The slope comes from a code of z that is off by up to 8 / 65534:
+    0.8 times that, and the product over one column is rounded to the type."""
+    from dss_vae_amd import ops
+    every = torch.arange(-32768, 32768, dtype=torch.int32).to(torch.int16).view(dtype)
+    z = every[every.isfinite() & (every.abs() < 13) & ((every.abs() > 1e-30) | (every == 0))]
+    for rows in (z.numel(), 1):  # z along the rows: the tiles; along the columns of one row: the few-row kernel
+        x = z.to(DEV).view(-1, 1) if rows > 1 else torch.ones(1, 1, device=DEV, dtype=dtype)
+        w = torch.ones(1, 1, device=DEV, dtype=dtype) if rows > 1 else z.to(DEV).view(-1, 1)
+        x.requires_grad_(rows > 1)
+        y = ops.linear_act(x, w, None, "gelu")
+        d = z.double()
+        cdf = 0.5 * torch.special.erfc(-d / math.sqrt(2))
+        want = d * cdf
+        smallest = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+        bound = torch.finfo(dtype).eps / 2 * 1.05 * want.abs() + smallest
+        err = (y.detach().cpu().double().view(-1) - want).abs()
+        assert (err <= bound).all(), float((err / bound).max())
+        if rows > 1:
+            g, = torch.autograd.grad(y, x, torch.ones_like(y))
+            slope = cdf + d * torch.exp(-d * d / 2) / math.sqrt(2 * math.pi)
+            err = (g.cpu().double().view(-1) - slope).abs()
+            assert (err <= torch.finfo(dtype).eps / 2 * 1.01 * slope.abs() + 0.8 * 8 / 65534 + 2e-6).all()
