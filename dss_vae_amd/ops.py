@@ -1,5 +1,6 @@
 """autograd wrappers over the C-ABI (include/dssvae_hip.h).  Every op launches hand-written HIP
 kernels on the current stream; torch is used for memory and tiny glue only.  No CPU path."""
+import contextlib
 import ctypes as C
 import functools
 import os
@@ -10,12 +11,21 @@ from torch.autograd.function import once_differentiable
 
 from . import lib as L
 
-# Backward passes run on the thread that asks for them.  One process drives one GPU here: autograd's worker thread per device has
-# nothing to run beside, and the two hand-overs per backward call (the caller sleeps meanwhile) cost 50-70 us of a small step:
-# layer_norm forward and backward of 7936 x 300 fp32 125 -> 57 us, gated_scan of 256 x 90 x 300 114 -> 54 us.  The setting belongs to
-# the importing thread; DSSVAE_AUTOGRAD_THREADS=1 (or torch.autograd.set_multithreading_enabled(True) later) keeps torch's default.
-if os.environ.get("DSSVAE_AUTOGRAD_THREADS", "0") != "1":
+# DSSVAE_AUTOGRAD_THREADS=0 in the environment: every backward pass of the importing thread as under backward_on_caller().
+if os.environ.get("DSSVAE_AUTOGRAD_THREADS", "1") == "0":
     torch.autograd.set_multithreading_enabled(False)
+
+
+@contextlib.contextmanager
+def backward_on_caller():
+    """`with ops.backward_on_caller(): loss.backward()` runs the backward pass on the calling thread.  One process drives one GPU here:
+    autograd's worker thread per device has nothing to run beside, and the two hand-overs per backward call (the caller sleeps
+    meanwhile) cost 40-60 us of a small step: layer_norm forward and backward of 7936 x 300 fp32 112 -> 56 us, gated_scan of 256 x 90 x
+    300 110 -> 54, distill_loss of 50 x 30000 93 -> 50; steps whose kernels take longer than that gain nothing.  The framework's
+    trainer does so; other code of the process keeps torch's setting."""
+    with torch.autograd.set_multithreading_enabled(False):
+        yield
+
 
 _CUS = None
 

@@ -267,7 +267,8 @@ def train_iteration(model, optimizer, examples, train_iter, adv_syn=False, adv_s
         if on:
             ret = model.get_loss(examples=examples, train_iter=train_iter, is_dis=True)
             optimizer.zero_grad(tag)
-            (ret[key] * float(world) if world > 1 else ret[key]).backward()
+            with ops.backward_on_caller():
+                (ret[key] * float(world) if world > 1 else ret[key]).backward()
             optimizer.step()
     return train_step(model, optimizer, examples, train_iter, global_batch)
 
@@ -280,7 +281,8 @@ def train_step(model, optimizer, examples, train_iter, global_batch=None):
     world = getattr(optimizer, "world", 1)
     if world > 1 and global_batch is not None and len(examples) * world != global_batch:
         loss = loss * (len(examples) * world / float(global_batch))  # unequal shards stay exact
-    loss.backward()
+    with ops.backward_on_caller():
+        loss.backward()
     optimizer.step()
     # the caller gets numbers, not a graph: a loss dictionary that still referenced the step's autograd nodes would
     # keep every parameter's AccumulateGrad node (and the stream it was made on) alive into the next step
@@ -397,7 +399,8 @@ class GraphedTrainer(object):
                 with torch.cuda.graph(g1, pool=self.pool, stream=self.stream, capture_error_mode=CAPTURE_MODE):
                     opt.zero_grad("main")
                     rec["ret"] = model.get_loss(rec["static"], train_iter)
-                    torch.mean(rec["ret"]["Loss"]).backward()
+                    with ops.backward_on_caller():
+                        torch.mean(rec["ret"]["Loss"]).backward()
                 if self.pool is None:
                     self.pool = g1.pool()
                 with torch.cuda.graph(g2, pool=self.pool, stream=self.stream, capture_error_mode=CAPTURE_MODE):
