@@ -2180,7 +2180,8 @@ class _DistillFn(Function):
         _record("distill_loss", ctx, logits.device)
         z, ldz = _matrix(_flat(logits))
         total, rows, ctx.dz = _distill(z, ldz, code, ids, teacher, tau, weight, True)
-        ctx.save_for_backward(z, ids, teacher, weight)
+        # (a teacher's forward pass often runs in inference mode, whose tensors autograd does not save)
+        ctx.save_for_backward(z, *(t.clone() if t is not None and t.is_inference() else t for t in (ids, teacher, weight)))
         ctx.shape, ctx.code, ctx.tau = logits.shape, code, tau
         if logits.dim() != 2:
             rows = rows.view(logits.shape[:-1])

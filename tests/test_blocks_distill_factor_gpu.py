@@ -133,3 +133,15 @@ def test_refusals_of_the_second_pass():
         bad = list(good)
         bad[i] = v
         assert L.load().dssvae_distill_again(*bad) == -1, (i, v)
+
+
+def test_a_teacher_in_inference_mode():
+    from dss_vae_amd import ops
+    z, ids, t, w = case(6, 333, 9, torch.float32, seed=9)
+    want = reference(z, ids, t, 2.0, w)
+    with torch.inference_mode():
+        ids, t, w = ids.to(DEV), t.to(DEV), w.to(DEV)
+    leaf = z.to(DEV).requires_grad_()
+    total, _ = ops.distill_loss(leaf, ids, t, 2.0, w)
+    g, = torch.autograd.grad(total * 3, leaf)
+    check(g, want[2] * 3, want[5] * 3, MORE, "inference mode")
