@@ -2130,6 +2130,8 @@ def gated_step(xproj, h=None, candidate="tanh", h_out=None):
         _expect("gated_step", "h_out", h_out, (B, H), (torch.float32,), xproj.device)
         if not h_out.is_contiguous():
             raise RuntimeError("gated_step: h_out must be contiguous")
+        if h_out.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("gated_step: h_out requires grad (its buffer is written; run under no_grad or pass h_out.detach())")
         for name, t in (("h", h), ("xproj", xproj)):
             if t is not None and not (t is h and t.data_ptr() == h_out.data_ptr()) and _meet(t, h_out):
                 raise RuntimeError("gated_step: h_out overlaps %s" % name)
@@ -2141,6 +2143,8 @@ def gated_step(xproj, h=None, candidate="tanh", h_out=None):
     x, ldx = _matrix(xproj)
     out = x.new_empty((B, H))
     hn = torch.empty((B, H), device=x.device, dtype=torch.float32) if h_out is None else h_out
+    if h_out is not None:
+        torch.autograd.graph.increment_version(h_out)  # (a graph that saved it has to notice, as with any write in place)
     _gated_step(x, ldx, code, _contig(h), tanh, out, hn)
     return out, hn
 
