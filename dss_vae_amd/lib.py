@@ -41,6 +41,7 @@ CELL_GRU, CELL_LSTM = 0, 1
 DISTILL_MAX_TOP = 1024
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "tanh": 4}  # DSSVAE_ACT_*
 ACT_ROUND_DZ = 0x100
+LINEAR_MAX_SUM = 1 << 21  # elements of an axis that linear_act sums over
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # DSSVAE_F32 / _BF16 / _F16
 
 

@@ -2323,7 +2323,8 @@ class _LinearActFn(Function):
 def linear_act(x, w, b=None, act="none", residual=None, round_dz=False):
     """act(x w^T + b) + residual: x [..., K], w [N, K] and residual [..., N] of one type (float32, bfloat16, float16),
     b [N] of that type or float32; act "none", "relu", "gelu" (the exact form), "silu" or "tanh".  Products accumulate in
-    fp32 in a fixed order and every output is rounded once.  For training in 16 bits the slope's argument is kept in 16 bits
+    fp32 in a fixed order and every output is rounded once; a summed axis (K; N for x's gradient, the rows for w's) has at most 2097152
+    elements.  For training in 16 bits the slope's argument is kept in 16 bits
     (evenly spaced, finer than either type where slopes move), and the products of backward take dz = dy act'(z) unrounded, in two
     16-bit parts; round_dz=True rounds it to the type instead: half the matrix work of backward, sqrt(2) times the error of dx and dw."""
     code = _typed("linear_act", x)
@@ -2339,6 +2340,10 @@ def linear_act(x, w, b=None, act="none", residual=None, round_dz=False):
         _expect("linear_act", "residual", residual, tuple(x.shape[:-1]) + (N,), (x.dtype,), x.device)
     a = L.ACTIVATIONS[act]
     if _wants_grad("linear_act", x, w, b, residual):
+        # (what backward would refuse is refused before the forward pass)
+        for name, t, axis, n in (("x", x, "N", N), ("w", w, "rows", x.numel() // K)):
+            if t.requires_grad and n > L.LINEAR_MAX_SUM:
+                raise RuntimeError("linear_act: the gradient of %s sums over %s = %d, at most %d" % (name, axis, n, L.LINEAR_MAX_SUM))
         return _LinearActFn.apply(x, w, b, residual, a, code, bool(round_dz))
     x2, ldx = _matrix(_flat(x))
     w2, ldw = _matrix(w)
