@@ -1920,11 +1920,13 @@ def _leaves_on_null(node, stream):
 
 def _record(what, ctx, dev):
     """Before an operator records its graph: under capture, refuses leaves that an older graph still holds on the NULL stream.
-    Autograd would make that stream wait for the capturing one, which a HIP capture does not survive (the process ends)."""
+    Autograd would make that stream wait for the capturing one, which a HIP capture does not survive (the process ends).  Known are the
+    streams that these operators saw a leaf on first: autograd does not tell a node's stream, so a leaf that another operation's
+    graph holds on the NULL stream is not noticed."""
     if _leaves_on_null(ctx, torch._C._cuda_getCurrentRawStream(dev.index)) and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("%s: this stream is being captured, and a graph that was recorded on the default stream still holds a "
                            "parameter or input of this call: drop that graph (its outputs) first, or record it on another "
-                           "stream" % what)
+                           "stream; a capture of the forward pass alone goes under no_grad" % what)
 
 
 def _layer_norm_fwd(x2, ldx, code, w, b, eps, stats):
