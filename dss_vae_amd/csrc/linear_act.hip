@@ -6,8 +6,7 @@
 // the parts are added: what is left out is below 2^-22 of a product, and on the mean of random inputs the sums are closer to
 // the exact ones than v_mfma_f32_32x32x2_f32's order gives (K = 7936: 7e-7 of the norm; the library's fp32 product 1.6e-6).  Sums of
 // at most 32 products, where that would show (a single product came out up to four times as far off as one fp32 rounding), take the
-// fp32 instruction.  The
-// fp32 instruction does a sixteenth of the bf16 one's work: a library product of 4096^3 takes 0.91 ms, this one 0.70 ms (the six
+// fp32 instruction, which does a sixteenth of the bf16 one's work: a library product of 4096^3 takes 0.91 ms, this one 0.70 ms (the six
 // run at 1170 TFLOP/s; a library product of bf16 operands reaches 1326).  Taking operands apart once per block, on their way
 // into LDS through registers, halves the vector instructions but measured the same: 0.73 ms.
 //
@@ -21,8 +20,9 @@
 // workspace first: dz in both orders by the pass that forms it, which also leaves the column sums for db.
 // 16-bit types: that pass leaves dz in two parts of the type (dy act'(z) is not a number of the type: rounded once, its error is as
 // large as that of the results' own rounding), and the products run over both: low parts first, then high ones, into the same
-// accumulators.  The low parts cost the matrix work again (16384 x 2048 -> 8192 bf16 and fp16, gelu, forward and backward: 2.75 ms, products
-// of backward 1.8 and transposes 0.39 of it; with a rounded dz 1.74 ms, 0.9 and 0.29): DSSVAE_ACT_ROUND_DZ does without them.  None and relu need none: their dz is dy, or zero.
+// accumulators.  The low parts cost the matrix work again (16384 x 2048 -> 8192 bf16 and fp16, gelu, forward and backward: 2.7 ms,
+// products of backward 1.8 and transposes 0.39 of it; with a rounded dz 1.74 ms, 0.9 and 0.29): DSSVAE_ACT_ROUND_DZ does without
+// them.  None and relu need none: their dz is dy, or zero.
 // Few output tiles: K is split over blocks, fp32 partials go to the workspace and a second launch adds them in order and
 // applies the epilogue (no atomics: same bits every time).  Backward is three launches: the transposes, both products, and
 // the partials with db's column sums.

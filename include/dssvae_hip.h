@@ -630,7 +630,8 @@ int dssvae_scale_rows(void* x, int64_t ld, int dtype, int64_t rows, int V, const
  * 2^-110: absolute 2^-133); 16-bit types: dz goes into the products of backward in two parts, good to 2^-16 (bf16) or 2^-22 (fp16) of it, or, with
  * DSSVAE_ACT_ROUND_DZ or-ed into backward's act, rounded to the type for half the matrix work.  A summed axis (K forward, N for dx,
  * M for dw) has at most 2097152 elements, and a launch fewer than 2^32 threads: DSSVAE_ETOOBIG.
- * The workspace sizes depend on where the operands start: the query takes the pointers and strides of the call.
+ * The workspace sizes depend on where the operands start: the query takes the pointers and strides of the call (backward's is enough
+ * for every activation).
  * ------------------------------------------------------------------------------------------- */
 #define DSSVAE_ACT_NONE 0
 #define DSSVAE_ACT_RELU 1
