@@ -135,6 +135,33 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
     return v;
 }
 
+// The same of two values behind one pair of barriers; `red` holds two floats per wave
+template <int TPR>
+__device__ __forceinline__ void row_sums(float& a, float& b, float* red) {
+    constexpr int W = TPR < 64 ? TPR : 64;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) {
+        a += __shfl_xor(a, o, 64);
+        b += __shfl_xor(b, o, 64);
+    }
+    if constexpr (TPR > 64) {
+        constexpr int NW = TPR / 64;
+        const int wave = threadIdx.x >> 6, w0 = wave / NW * NW;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) {
+            red[2 * wave] = a;
+            red[2 * wave + 1] = b;
+        }
+        __syncthreads();
+        a = b = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            a += red[2 * (w0 + i)];
+            b += red[2 * (w0 + i) + 1];
+        }
+    }
+}
+
 // tanh and its slope from u = exp(-2 |x|), both to their own accuracy: tanh = (1 - u) / (1 + u), which cancels near 0 (1 - 2 / (1 + exp(2 x))
 // is off by 1e-3 of itself at 1e-4): below 0.3 an odd polynomial takes its place (x^3 (c0 + c1 x^2 + c2 x^4), fitted for the least
 // relative error, 1.2e-8); slope = 4 u / (1 + u)^2, which 1 - tanh^2 loses where tanh saturates (6 % off at 8).

@@ -3,9 +3,10 @@
 // A row lives in registers between its one read and its one write: TPR threads hold E elements each, in granules of 16 bytes
 // (granule i of thread t covers columns (i * TPR + t) * VEC ..).  Rows may start anywhere and end inside a granule: loads take
 // any alignment, the last granule goes by elements (27513 x 1581 bf16: 50 us forward, 85 us backward; with element loads 69 and
-// 136 us).  Mean first, then the centred squares, no cancellation as in E[x^2] - E[x]^2.  The mean takes two reductions: partial sums of
-// values with a common offset are rounded to the offset's bits, and the mean of a row of 99999.9 came out 0.01 off; the deviations from it
-// are exact and their mean corrects it to half a step.
+// 136 us).  Mean first, then the deviations and their squares, no cancellation as in E[x^2] - E[x]^2.  Partial sums of values with a
+// common offset are rounded to the offset's bits, and the mean of a row of 99999.9 comes out 0.01 off: the deviations from it are exact, and
+// their mean corrects it to half a step.  The squares are corrected by it too, or, where it is not small beside them (equal values), taken
+// again about the new mean (32768 x 2048 bf16: 56 us, 50 with the first mean, 58 with the squares always taken again).
 // Forward, up to 1024 columns a row belongs to one wave or a quarter of one (shuffles only); wider rows take 256 threads.
 // Backward keeps E at 8 up to 4096 columns (its column sums cost 2 E registers more) and gives a row up to 512 threads.  Rows
 // wider than 8192 columns are walked four times (backward twice) by a block of 1024 (the repeats hit L2).
@@ -14,7 +15,7 @@
 // The column sums: a block walks rows blockIdx, + gridDim, ... and keeps dw / db of its columns in registers; its row groups
 // meet in LDS, one [2, D] partial per block goes to the workspace and a second launch adds the partials in order
 // (no atomics: the same bits every time).
-// Measured: 32768 x 2048 bf16 forward 49 us (5.5 TB/s), backward 79 us (5.1 TB/s) and 6 us for the partials.
+// Measured: 32768 x 2048 bf16 forward 56 us (4.8 TB/s), backward 78 us (5.2 TB/s) and 6 us for the partials.
 #include "elem.h"
 
 namespace {
@@ -42,7 +43,7 @@ __global__ __launch_bounds__(FWD_THREADS) void layer_norm_fwd_kernel(const T* __
                                                                       int64_t rows, int D, float eps, T* __restrict__ y,
                                                                       int64_t ldy, float* __restrict__ stats) {
     constexpr int VEC = 16 / (int)sizeof(T), NV = E / VEC, RPB = FWD_THREADS / TPR;
-    __shared__ float red[FWD_THREADS / 64];
+    __shared__ float red[2 * FWD_THREADS / 64];
     const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
     float wv[NV][VEC], bv[NV][VEC];
 #pragma unroll
@@ -68,12 +69,22 @@ __global__ __launch_bounds__(FWD_THREADS) void layer_norm_fwd_kernel(const T* __
         s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            deviations<WHOLE, T, VEC>(v[i], (i * TPR + t) * VEC, D, mean, [&](float d) { s += d; });
-        mean += row_sum<TPR>(s, red) / n;
+            deviations<WHOLE, T, VEC>(v[i], (i * TPR + t) * VEC, D, mean, [&](float d) {
+                s += d;
+                q += d * d;
+            });
+        row_sums<TPR>(s, q, red);
+        const float off = s / n;
+        mean += off;
+        float var = q / n - off * off;
+        if (!(off * off <= 0.01f * var)) {  // (the row alike) hardly any spread beside the first mean's error: squares about the new one
+            q = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-            deviations<WHOLE, T, VEC>(v[i], (i * TPR + t) * VEC, D, mean, [&](float d) { q += d * d; });
-        const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red) / n + eps);
+            for (int i = 0; i < NV; ++i)
+                deviations<WHOLE, T, VEC>(v[i], (i * TPR + t) * VEC, D, mean, [&](float d) { q += d * d; });
+            var = row_sum<TPR>(q, red) / n;
+        }
+        const float rstd = 1.f / sqrtf(var + eps);
         if (!live) continue;
         T* yr = y + r * ldy;
 #pragma unroll
@@ -188,32 +199,9 @@ __global__ __launch_bounds__(BWD_THREADS, E > 8 ? 2 : 4) void layer_norm_bwd_ker
                 s2 += d * wv[i][j] * xh;
             }
         }
-        if constexpr (TPR <= 64) {
-            s1 = row_sum<TPR>(s1, red) * inv;
-            s2 = row_sum<TPR>(s2, red) * inv;
-        } else {  // both sums behind one pair of barriers
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) {
-                s1 += __shfl_xor(s1, o, 64);
-                s2 += __shfl_xor(s2, o, 64);
-            }
-            constexpr int NW = TPR / 64;
-            const int wave = threadIdx.x >> 6, w0 = wave / NW * NW;
-            __syncthreads();
-            if ((threadIdx.x & 63) == 0) {
-                red[2 * wave] = s1;
-                red[2 * wave + 1] = s2;
-            }
-            __syncthreads();
-            s1 = s2 = 0.f;
-#pragma unroll
-            for (int i = 0; i < NW; ++i) {
-                s1 += red[2 * (w0 + i)];
-                s2 += red[2 * (w0 + i) + 1];
-            }
-            s1 *= inv;
-            s2 *= inv;
-        }
+        row_sums<TPR>(s1, s2, red);
+        s1 *= inv;
+        s2 *= inv;
         if (!live || !dx) continue;
         T* o = dx + r * lddx;
 #pragma unroll
