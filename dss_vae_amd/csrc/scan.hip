@@ -13,7 +13,7 @@
 // rebuilds h inside the chunk from it, in fp32, and never reads out.
 // A granule is only 4 bytes: the scan costs log2(64 / LPR) shuffled compositions per channel and thread, so many steps per
 // thread (KT = 8, fp32 16) beat wide granules (16-byte ones leave 2: 265 us for backward over 2 x 16384 x 2048 bf16, 8-byte
-// ones 213 us, this form 150 us = 4.5 TB/s; forward 109 / 97 / 81 us = 4.9 TB/s).
+// ones 213 us, this form 153 us = 4.4 TB/s; forward 109 / 97 / 87 us = 4.6 TB/s).
 // Too few tiles (128 bytes of channels each) to fill the chip: the time axis is cut into segments; a first launch reads the
 // segment's inputs for its (A, B) per channel, the second starts each segment from the composition of those before it
 // (backward: behind it).  Narrower tiles instead (32 bytes: no second read, but four blocks per cache line) took 192 us
@@ -32,13 +32,13 @@ template <typename T, int DIV> constexpr int NT = CHUNK / DIV * LPR / KT<T>;
 constexpr int STEP_THREADS = 256;
 
 // a = sigmoid(z) and b = 1 - a, each to its own accuracy: long memories are gates whose 1 - a is small, and the update and both
-// gradients are proportional to it.  With u = exp(-z), a = 1 / (1 + u) and b = u a; a subtraction leaves 1 - a with a few bits (off by
-// 1e-3 at z = 10, all of it at 17).  a close to 1 is 1 - b, which is rounded to nearest: what 1 + u and the reciprocal lose
-// would add up over thousands of steps.  z = +inf gives 1 and 0 exactly, z = -inf (u overflows) 0 and 1, NaN stays.
+// gradients are proportional to it.  With w = exp(-|z|) the smaller of the two is w / (1 + w) and the larger one 1 minus it, rounded to
+// nearest; 1 - a from a rounded a keeps a few bits (off by 1e-3 at z = 10, by all of it at 17), and what 1 + w and the reciprocal lose in
+// an a close to 1 would add up over thousands of steps.  z = +-inf gives 1 and 0 exactly; NaN stays.
 __device__ __forceinline__ void gate_f(float z, float& a, float& b) {
-    const float u = __builtin_amdgcn_exp2f(-1.4426950408889634f * z), r = __builtin_amdgcn_rcpf(1.f + u);
-    b = u > 0x1p126f ? 1.f : u * r;
-    a = u < 1.f ? 1.f - b : r;
+    const float w = __builtin_amdgcn_exp2f(-1.4426950408889634f * fabsf(z)), less = w * __builtin_amdgcn_rcpf(1.f + w), more = 1.f - less;
+    a = z < 0.f ? less : more;
+    b = z < 0.f ? more : less;
 }
 
 struct Dims {
