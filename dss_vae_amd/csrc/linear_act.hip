@@ -986,8 +986,9 @@ inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 // Tile width and K splits of a launch's products: the smallest of a modelled time in microseconds,
 //   max(work of all blocks over the CUs, the longest block's steps) + prologue and epilogue + partials' traffic,
 // with `per` the time of a step at a CU's full rate and `least` what a step takes a block alone (the latency of its loads).  The
-// work counts as if every CU took as many blocks as the fullest.  (Sweeps of both, 9 forward and 6 backward shapes: within 10 % of
-// the best choice but for the smallest, which one launch's time decides.)
+// work counts as if every CU took as many blocks as the fullest.  (Every width and split of 46 forward shapes,
+// profiles/blocks_plan_sweep.txt: within 13 % of the best choice but for four with few tiles and a long K, bf16 300 x 7936 -> 600 22.6 us
+// against 16.7 and 256 x 16384 -> 256 19.4 against 16.2, fp32 512 x 4096 -> 4096 134 against 105 and 300 x 7936 -> 600 44 against 37.)
 struct Plan { int tile, ksplit; };
 struct Extent { int64_t M, N, K; };
 template <typename T> constexpr int MAX_TILE = sizeof(T) == 4 ? 128 : 256;
@@ -1036,8 +1037,8 @@ inline double plan_products(const Extent (&x)[COUNT], Plan (&best)[COUNT]) {
     return lowest;
 }
 // tile 0: linear_rows_kernel, where its modelled time is the smaller: 3.5 us and 45 GB/s a CU for what its blocks load, 16 rows of
-// w and up to 64 of x each.  Measured against the tiles, bf16, M x K -> N: 1 x 1024 -> 1024 4.4 / 8.0 us, 50 x 600 -> 300 5.9 / 8.2, 50 x 2048
-// -> 2048 12.0 / 13.4, 50 x 4096 -> 4096 23.5 / 16.3 (taken by the tiles); fp32: 1 x 2048 -> 8192 15 / 31, 50 x 8192 -> 2048 72 / 36 (tiles).
+// w and up to 64 of x each.  Measured against the tiles, bf16, M x K -> N: 1 x 1024 -> 1024 4.1 / 7.3 us, 50 x 600 -> 300 5.4 / 7.2, 50 x 2048
+// -> 2048 10.8 / 10.1, 50 x 4096 -> 4096 21 / 15 (taken by the tiles); fp32: 1 x 2048 -> 8192 14.6 / 24.7, 50 x 8192 -> 2048 67 / 29 (tiles).
 constexpr int64_t FEW_ROWS = 64;
 inline int row_blocks(int64_t M) { return M <= 16 ? 1 : M <= 32 ? 2 : 4; }  // of 16 rows
 template <typename T>
