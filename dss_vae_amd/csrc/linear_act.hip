@@ -62,17 +62,19 @@ __device__ __forceinline__ float act_f(int act, float z) {
         default: return z;
     }
 }
+// (an infinite z has the slope it tends to, not inf * 0; what NaN turns into here meets a NaN)
+__device__ __forceinline__ float finite(float z) { return __builtin_amdgcn_fmed3f(z, -1000.f, 1000.f); }
 template <typename T>
 __device__ __forceinline__ float act_slope(int act, float z) {
     switch (act) {
         case DSSVAE_ACT_RELU: return z > 0.f ? 1.f : (z != z ? z : 0.f);
         case DSSVAE_ACT_GELU: {
             const float e = normal_exp(z);
-            return normal_cdf<T>(z, e) + z * 0.3989422804014327f * e;
+            return normal_cdf<T>(z, e) + finite(z) * 0.3989422804014327f * e;
         }
         case DSSVAE_ACT_SILU: {
             const float s = sigmoid_f(z);
-            return s * (1.f + z * (1.f - s));
+            return s * (1.f + finite(z) * (1.f - s));
         }
         case DSSVAE_ACT_TANH: {
             float slope;
@@ -83,15 +85,15 @@ __device__ __forceinline__ float act_slope(int act, float z) {
     }
 }
 
-// The pre-activation as backward needs it.  fp32: itself.  16-bit types: a 16-bit code of the slope's argument, evenly spaced over
-// the range in which the slope moves (beyond it the slope is 0 or 1 to 2e-6): |z| <= 8, silu 16, in steps of range / 32767,
-// i.e. off by at most 1.2e-4 (silu 2.4e-4).  z rounded to bf16 would be off by 4e-3 at |z| = 2 and z rounded to fp16 lost a
-// gradient's last bit; the code takes one instruction for two values.  relu keeps z > 0 only.  NaN has a code of its own.
+// What backward needs of the pre-activation z.  fp32: z.  16-bit types: a 16-bit code of act'(z), its signed fourth root in steps of
+// 1 / 31744 (the largest slope, gelu's 1.129, fits; 0 and 1 are exact): a slope s is off by at most 6.3e-5 |s|^(3/4), that is 6e-5 of
+// itself at 1, 2e-4 at 0.01, 2e-3 at 1e-6 (fp16's half step: 2.4e-4 to 4.9e-4).  Even steps of z (8 / 32767) were off by 1e-4 in s wherever it bends, more than
+// the type's rounding where s is below 0.2; z rounded to the type loses 4e-3 (bf16).  Forward has the slope's exponential at hand
+// and backward decodes with four multiplications.  relu keeps z > 0 only.  NaN has a code of its own.
 constexpr int16_t CODE_NAN = -32768;
-__device__ __forceinline__ float code_range(int act) { return act == DSSVAE_ACT_SILU ? 16.f : 8.f; }
-template <int ACT>
+constexpr float CODE_ONE = 31744.f;
+template <typename T, int ACT>
 __device__ __forceinline__ void encode8(const float (&z)[8], int16_t (&q)[8]) {
-    const float c = 1.f / code_range(ACT);
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
@@ -101,7 +103,13 @@ __device__ __forceinline__ void encode8(const float (&z)[8], int16_t (&q)[8]) {
             q[j + 1] = z[j + 1] > 0.f;
         } else {
             typedef short s16x2 __attribute__((ext_vector_type(2)));
-            const s16x2 p = __builtin_bit_cast(s16x2, __builtin_amdgcn_cvt_pknorm_i16(z[j] * c, z[j + 1] * c));
+            float c[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float s = act_slope<T>(ACT, z[j + i]);
+                c[i] = copysignf(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(fabsf(s))) * (CODE_ONE / 32767.f), s);
+            }
+            const s16x2 p = __builtin_bit_cast(s16x2, __builtin_amdgcn_cvt_pknorm_i16(c[0], c[1]));
             q[j] = p.x;
             q[j + 1] = p.y;
         }
@@ -111,14 +119,18 @@ __device__ __forceinline__ void encode8(const float (&z)[8], int16_t (&q)[8]) {
         for (int j = 0; j < 8; ++j) q[j] = z[j] != z[j] ? CODE_NAN : q[j];
     }
 }
-__device__ __forceinline__ float decode(int act, int16_t q) {
-    return q == CODE_NAN ? __builtin_nanf("") : (float)q * (code_range(act) / 32767.f);
+template <int ACT>
+__device__ __forceinline__ float decode(int16_t q) {
+    if (q == CODE_NAN) return __builtin_nanf("");
+    if constexpr (ACT == DSSVAE_ACT_RELU) return q ? 1.f : 0.f;
+    const float c = (float)q * (1.f / CODE_ONE);
+    return c * c * (c * fabsf(c));
 }
 // act'(z) from what forward kept
 template <typename T, int ACT>
 __device__ __forceinline__ float slope_kept(const T* z, int64_t i) {
     if constexpr (sizeof(T) == 4) return act_slope<T>(ACT, (float)z[i]);
-    else return act_slope<T>(ACT, decode(ACT, reinterpret_cast<const int16_t*>(z)[i]));
+    else return decode<ACT>(reinterpret_cast<const int16_t*>(z)[i]);
 }
 
 // What happens to an accumulated element on its way out
@@ -167,7 +179,7 @@ __device__ __forceinline__ void finish8_act(const Epilogue& e, f32x8 a, f32x8 b,
                 g.store(z);
             } else {
                 int16_t q[8];
-                encode8<ACT>(zz, q);
+                encode8<T, ACT>(zz, q);
                 GranU<int16_t, 8> gq;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) gq.v[j] = q[j];
@@ -180,7 +192,7 @@ __device__ __forceinline__ void finish8_act(const Epilogue& e, f32x8 a, f32x8 b,
         int16_t q[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) zz[j] = a[j] + b[j];
-        if constexpr (sizeof(T) == 2) encode8<ACT>(zz, q);
+        if constexpr (sizeof(T) == 2) encode8<T, ACT>(zz, q);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             if (n + j >= N) continue;
@@ -917,7 +929,7 @@ __global__ __launch_bounds__(256) void linear_turn_kernel(Turns jobs) {
                             GranU<int16_t, 8> gq;
                             gq.load(reinterpret_cast<const int16_t*>(z) + r * ldz + c);
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) v[j] *= act_slope<T>(ACT, decode(ACT, gq.v[j]));
+                            for (int j = 0; j < 8; ++j) v[j] *= decode<ACT>(gq.v[j]);
                         }
                     }
                 } else {
@@ -986,8 +998,8 @@ inline int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 // Tile width and K splits of a launch's products: the smallest of a modelled time in microseconds,
 //   max(work of all blocks over the CUs, the longest block's steps) + prologue and epilogue + partials' traffic,
 // with `per` the time of a step at a CU's full rate and `least` what a step takes a block alone (the latency of its loads).  The
-// work counts as if every CU took as many blocks as the fullest.  (Every width and split of 46 forward shapes,
-// profiles/blocks_plan_sweep.txt: within 13 % of the best choice but for four with few tiles and a long K, bf16 300 x 7936 -> 600 22.6 us
+// work counts as if every CU took as many blocks as the fullest.  (Every width and split of 46 forward
+// shapes: within 13 % of the best choice but for four with few tiles and a long K, bf16 300 x 7936 -> 600 22.6 us
 // against 16.7 and 256 x 16384 -> 256 19.4 against 16.2, fp32 512 x 4096 -> 4096 134 against 105 and 300 x 7936 -> 600 44 against 37.)
 struct Plan { int tile, ksplit; };
 struct Extent { int64_t M, N, K; };

@@ -2326,8 +2326,8 @@ def linear_act(x, w, b=None, act="none", residual=None, round_dz=False):
     """act(x w^T + b) + residual: x [..., K], w [N, K] and residual [..., N] of one type (float32, bfloat16, float16),
     b [N] of that type or float32; act "none", "relu", "gelu" (the exact form), "silu" or "tanh".  Products accumulate in
     fp32 in a fixed order and every output is rounded once; a summed axis (K; N for x's gradient, the rows for w's) has at most 2097152
-    elements.  For training in 16 bits the slope's argument is kept in 16 bits
-    (evenly spaced, finer than either type where slopes move), and the products of backward take dz = dy act'(z) unrounded, in two
+    elements.  For training in 16 bits act'(z) is kept in 16 bits (its fourth root, in even steps:
+    finer than either type), and the products of backward take dz = dy act'(z) unrounded, in two
     16-bit parts; round_dz=True rounds it to the type instead: half the matrix work of backward, sqrt(2) times the error of dx and dw."""
     code = _typed("linear_act", x)
     if act not in L.ACTIVATIONS:

@@ -622,7 +622,7 @@ int dssvae_scale_rows(void* x, int64_t ld, int dtype, int64_t rows, int V, const
  * Linear layer with bias, activation and residual:  z = x w^T + bias,  y = act(z) + res
  *   x [M, K], w [N, K], res / y / z [M, N] of `dtype` with their row strides; bias [N] fp32 if bias_f32 else `dtype`, or
  *   NULL; res NULL: none; z NULL: the pre-activation is not kept (backward needs it unless act is DSSVAE_ACT_NONE).
- *   What z holds is between forward and backward (fp32: the values; 16-bit types: 16-bit codes of the slope's argument).
+ *   What z holds is between forward and backward (fp32: the values; 16-bit types: 16-bit codes of act'(z)).
  *   y must not overlap x, w or z; it may be res.  DSSVAE_ACT_GELU is the exact form, z Phi(z).
  * Backward: dz = dy act'(z); dx = dz w; dw = dz^T x; db = sum over rows of dz; dx, dw, db may each be NULL, z only where act
  * is DSSVAE_ACT_NONE.  (The residual's gradient is dy.)  M = 0 clears dw and db.

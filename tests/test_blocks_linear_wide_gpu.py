@@ -12,17 +12,6 @@ pytestmark = pytest.mark.gpu
 TYPES16 = [torch.bfloat16, torch.float16]
 
 
-def curve(z, name):
-    """act''(z) in 64 bits"""
-    if name == "gelu":
-        return (2 - z * z) * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
-    s = torch.sigmoid(z)
-    if name == "silu":
-        return s * (1 - s) * (2 + z * (1 - 2 * s))
-    t = torch.tanh(z)
-    return -2 * t * (1 - t * t)
-
-
 def operands(M, N, K, dtype, dy_scale=1.0, w_scale=1.0):
     return (rnd(M, K, seed=70, dtype=dtype), rnd(N, K, seed=71, scale=w_scale * K ** -0.5, dtype=dtype), rnd(N, seed=72, scale=0.3, dtype=dtype),
             rnd(M, N, seed=73, scale=dy_scale, dtype=dtype))
@@ -35,14 +24,14 @@ def gradients(x, w, b, name, dy, **more):
 
 
 def off(x, w, b, name, dy, got):
-    """per gradient: (error of `got`, error of the exact values rounded once, what the 16-bit codes of z add), each as a norm.
-    A code is off by up to half of range / 32767 (range 8, silu 16), evenly spread: step / sqrt(12) in the mean square, which moves
-    dz by dy act'' times that, independently from element to element."""
+    """per gradient: (error of `got`, error of the exact values rounded once, what the 16-bit codes of act'(z) add), each as a
+    norm.  A code is the fourth root in steps of 1 / 31744, off by 1 / sqrt(12) of one in the mean square, which moves the slope s by
+    4 |s|^(3/4) times that, independently from element to element."""
     x, w, b, d = x.double(), w.double(), b.double(), dy.double()
     z = x @ w.t() + b
-    dz = d * act(z, name)[1]
-    step = (16.0 if name == "silu" else 8.0) / 32767 / math.sqrt(12)
-    c = (d * curve(z, name) * step) ** 2
+    slope = act(z, name)[1]
+    dz = d * slope
+    c = (d * 4 * slope.abs() ** 0.75 / 31744 / math.sqrt(12)) ** 2
     out = []
     for g, want, code in zip(got, (dz @ w, dz.t() @ x, dz.sum(0)), (c @ (w * w), c.t() @ (x * x), c.sum(0))):
         out.append((float((g.double() - want).norm()), float((want.to(g.dtype).double() - want).norm()), float(code.sum().sqrt())))
@@ -91,7 +80,7 @@ def test_values_that_are_not_finite(dtype):
     rows = [i for i in range(150) if i not in (3, 4, 9)]
     assert torch.equal(bits(dx[rows]), bits(clean[0][rows]))
     assert torch.equal(bits(dw[[0, 1, 2, 8]]), bits(clean[1][[0, 1, 2, 8]]))
-    # an infinite input column whose dz are exact in the type (slope 1 at z > 8 in the codes): inf of their sign, not NaN
+    # an infinite input column whose dz are exact in the type (slope 1): inf of their sign, not NaN
     x2, d2 = x.abs() + 2.0, dy.abs() + 0.5
     w2 = torch.zeros_like(w)
     w2[:, 0] = 20.0
@@ -139,3 +128,28 @@ def test_same_bits_whichever_gradient_is_wanted(dtype):
         assert torch.equal(bits(g.cpu()), bits(full[which])), which
     again = gradients(x, w, b, "silu", dy)
     assert all(torch.equal(bits(p), bits(q)) for p, q in zip(full, again))
+
+
+@pytest.mark.parametrize("dtype", TYPES16)
+@pytest.mark.parametrize("name", ["gelu", "silu", "tanh"])
+def test_slopes_that_are_kept(dtype, name):
+    """every z of the type: the slope backward sees is off by half a step h = 1 / 63488 of its code (c = |s|^(1/4), 1 % on h for the root's
+    roundings: t^4 is convex, so the slope by at most (c + h)^4 - c^4) and the roundings of its formula (20 units of 2^-24 of the terms it
+    adds, at most 1.2; tanh's slope 2 |z| + 16 of itself), then rounded to the type; 0 and 1 are exact, infinite z have the slope they tend to, NaN stays"""
+    from dss_vae_amd import ops
+    every = torch.arange(-32768, 32768, dtype=torch.int32).to(torch.int16).view(dtype)
+    x = every.to(DEV).view(-1, 1).requires_grad_()
+    y = ops.linear_act(x, torch.ones(1, 1, device=DEV, dtype=dtype), None, name)
+    g = torch.autograd.grad(y, x, torch.ones_like(y))[0].cpu().double().view(-1)
+    z = every.double()
+    ok = z.isfinite()
+    slope = torch.cosh(z[ok].clamp(-300, 300)) ** -2 if name == "tanh" else act(z[ok].clamp(-700, 700), name)[1]  # (1 - tanh^2 cancels in 64 bits)
+    units = (2 * z[ok].abs() + 16) * slope if name == "tanh" else torch.full_like(slope, 24.0)
+    tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    code = (slope.abs() ** 0.25 + 1.01 / 63488) ** 4 - slope.abs()
+    bound = torch.finfo(dtype).eps / 2 * 1.01 * slope.abs() + code + units * 2.0 ** -24 + tiny
+    err = (g[ok] - slope).abs()
+    assert (err <= bound).all(), (float((err / bound).max()), z[ok][(err / bound).argmax()])
+    assert (g[z == math.inf] == (0 if name == "tanh" else 1)).all() and (g[z == -math.inf] == 0).all() and g[z.isnan()].isnan().all()
+    if name != "tanh":
+        assert (g[(z > 20) & ok] == 1).all()
