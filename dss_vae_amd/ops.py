@@ -4,6 +4,7 @@ import contextlib
 import ctypes as C
 import functools
 import os
+import threading
 
 import torch
 from torch.autograd import Function, forward_ad
@@ -11,20 +12,66 @@ from torch.autograd.function import once_differentiable
 
 from . import lib as L
 
-# DSSVAE_AUTOGRAD_THREADS=0 in the environment: every backward pass of the importing thread as under backward_on_caller().
-if os.environ.get("DSSVAE_AUTOGRAD_THREADS", "1") == "0":
+# Backward passes on the calling thread.  One process drives one GPU here: autograd's worker thread per device has nothing to run
+# beside, and the two hand-overs per backward call (the caller sleeps meanwhile) cost 40-60 us of a small step: layer_norm forward and
+# backward of 7936 x 300 fp32 112 -> 56 us, gated_scan of 256 x 90 x 300 110 -> 54, distill_loss of 50 x 30000 93 -> 50; steps whose
+# kernels take longer than that gain nothing.  Nothing of it outlasts the graphs it is for: backward_on_caller() is a scope, and the
+# sequence-block operators hold such a setting for the thread that recorded a graph of theirs while that graph lives (_lease).
+# DSSVAE_AUTOGRAD_THREADS in the environment: 1 keeps autograd's threads throughout (but for explicit scopes), 0 sets the importing
+# thread for good.
+_AUTOGRAD_THREADS = os.environ.get("DSSVAE_AUTOGRAD_THREADS", "")
+if _AUTOGRAD_THREADS == "0":
     torch.autograd.set_multithreading_enabled(False)
 
 
 @contextlib.contextmanager
 def backward_on_caller():
-    """`with ops.backward_on_caller(): loss.backward()` runs the backward pass on the calling thread.  One process drives one GPU here:
-    autograd's worker thread per device has nothing to run beside, and the two hand-overs per backward call (the caller sleeps
-    meanwhile) cost 40-60 us of a small step: layer_norm forward and backward of 7936 x 300 fp32 112 -> 56 us, gated_scan of 256 x 90 x
-    300 110 -> 54, distill_loss of 50 x 30000 93 -> 50; steps whose kernels take longer than that gain nothing.  The framework's
-    trainer does so; other code of the process keeps torch's setting."""
+    """`with ops.backward_on_caller(): loss.backward()` runs the backward pass on the calling thread (the framework's trainer does)"""
     with torch.autograd.set_multithreading_enabled(False):
         yield
+
+
+class _Thread(threading.local):
+    """graphs of the sequence-block operators that live and were recorded on this thread; whether autograd's threads are off for them"""
+
+    def __init__(self):
+        self.home = [threading.get_ident(), 0, False]
+
+
+_THREAD = _Thread()
+
+
+class _Lease(object):
+    """kept by a graph's node; the last one to go, on its own thread, turns autograd's threads on again"""
+    __slots__ = ("home",)
+
+    def __init__(self, home):
+        self.home = home
+        home[1] += 1
+
+    def __del__(self, ident=threading.get_ident, switch=torch._C._set_multithreading_enabled):
+        home = self.home
+        home[1] -= 1
+        if home[1] <= 0 and home[2] and ident() == home[0]:
+            home[1], home[2] = 0, False
+            switch(True)
+
+
+@functools.lru_cache(maxsize=1)
+def _gpus():
+    return torch.cuda.device_count()
+
+
+def _lease():
+    """-> what a graph's node keeps (None where nothing is to be given back: autograd's threads are off by the user's choice, on by
+    the environment's, or the process sees several GPUs, whose backward passes they run side by side)"""
+    home = _THREAD.home
+    if not home[2]:
+        if _AUTOGRAD_THREADS == "1" or not torch._C._is_multithreading_enabled() or _gpus() > 1:
+            return None
+        torch._C._set_multithreading_enabled(False)
+        home[2] = True
+    return _Lease(home)
 
 
 _CUS = None
@@ -1919,14 +1966,15 @@ def _leaves_on_null(node, stream):
 
 
 def _record(what, ctx, dev):
-    """Before an operator records its graph: under capture, refuses leaves that an older graph still holds on the NULL stream.
-    Autograd would make that stream wait for the capturing one, which a HIP capture does not survive (the process ends).  Known are the
+    """Before an operator records its graph, which then holds a lease of its thread: under capture, refuses leaves that an older graph
+    still holds on the NULL stream.  Autograd would make that stream wait for the capturing one, which a HIP capture does not survive (the process ends).  Known are the
     streams that these operators saw a leaf on first: autograd does not tell a node's stream, so a leaf that another operation's
     graph holds on the NULL stream is not noticed."""
     if _leaves_on_null(ctx, torch._C._cuda_getCurrentRawStream(dev.index)) and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("%s: this stream is being captured, and a graph that was recorded on the default stream still holds a "
                            "parameter or input of this call: drop that graph (its outputs) first, or record it on another "
                            "stream; a capture of the forward pass alone goes under no_grad" % what)
+    ctx.lease = _lease()
 
 
 def _layer_norm_fwd(x2, ldx, code, w, b, eps, stats):
