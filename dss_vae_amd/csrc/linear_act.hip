@@ -20,8 +20,8 @@
 // workspace first: dz in both orders by the pass that forms it, which also leaves the column sums for db.
 // 16-bit types: that pass leaves dz in two parts of the type (dy act'(z) is not a number of the type: rounded once, its error is as
 // large as that of the results' own rounding), and the products run over both: low parts first, then high ones, into the same
-// accumulators.  The low parts cost the matrix work again (16384 x 2048 -> 8192 bf16 and fp16, gelu, forward and backward: 2.7 ms,
-// products of backward 1.8 and transposes 0.39 of it; with a rounded dz 1.74 ms, 0.9 and 0.29): DSSVAE_ACT_ROUND_DZ does without
+// accumulators.  The low parts cost the matrix work again (16384 x 2048 -> 8192 bf16 and fp16, gelu, forward and backward: 2.75 ms,
+// products of backward 1.8 and transposes 0.39 of it; with a rounded dz 1.76 ms, 0.9 and 0.29): DSSVAE_ACT_ROUND_DZ does without
 // them.  None and relu need none: their dz is dy, or zero.
 // Few output tiles: K is split over blocks, fp32 partials go to the workspace and a second launch adds them in order and
 // applies the epilogue (no atomics: same bits every time).  Backward is three launches: the transposes, both products, and

@@ -35,7 +35,7 @@ class _Thread(threading.local):
     """graphs of the sequence-block operators that live and were recorded on this thread; whether autograd's threads are off for them"""
 
     def __init__(self):
-        self.home = [threading.get_ident(), 0, False]
+        self.home = [0, False]
 
 
 _THREAD = _Thread()
@@ -47,13 +47,13 @@ class _Lease(object):
 
     def __init__(self, home):
         self.home = home
-        home[1] += 1
+        home[0] += 1
 
-    def __del__(self, ident=threading.get_ident, switch=torch._C._set_multithreading_enabled):
+    def __del__(self, thread=_THREAD, switch=torch._C._set_multithreading_enabled):
         home = self.home
-        home[1] -= 1
-        if home[1] <= 0 and home[2] and ident() == home[0]:
-            home[1], home[2] = 0, False
+        home[0] -= 1
+        if home[0] <= 0 and home[1] and thread.home is home:
+            home[:] = 0, False
             switch(True)
 
 
@@ -66,11 +66,11 @@ def _lease():
     """-> what a graph's node keeps (None where nothing is to be given back: autograd's threads are off by the user's choice, on by
     the environment's, or the process sees several GPUs, whose backward passes they run side by side)"""
     home = _THREAD.home
-    if not home[2]:
+    if not home[1]:
         if _AUTOGRAD_THREADS == "1" or not torch._C._is_multithreading_enabled() or _gpus() > 1:
             return None
         torch._C._set_multithreading_enabled(False)
-        home[2] = True
+        home[1] = True
     return _Lease(home)
 
 
@@ -1967,9 +1967,9 @@ def _leaves_on_null(node, stream):
 
 def _record(what, ctx, dev):
     """Before an operator records its graph, which then holds a lease of its thread: under capture, refuses leaves that an older graph
-    still holds on the NULL stream.  Autograd would make that stream wait for the capturing one, which a HIP capture does not survive (the process ends).  Known are the
-    streams that these operators saw a leaf on first: autograd does not tell a node's stream, so a leaf that another operation's
-    graph holds on the NULL stream is not noticed."""
+    still holds on the NULL stream.  Autograd would make that stream wait for the capturing one, which a HIP capture does not survive
+    (the process ends).  Known are the streams that these operators saw a leaf on first: autograd does not tell a node's stream, so a
+    leaf that another operation's graph holds on the NULL stream is not noticed."""
     if _leaves_on_null(ctx, torch._C._cuda_getCurrentRawStream(dev.index)) and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("%s: this stream is being captured, and a graph that was recorded on the default stream still holds a "
                            "parameter or input of this call: drop that graph (its outputs) first, or record it on another "
@@ -2374,9 +2374,8 @@ def linear_act(x, w, b=None, act="none", residual=None, round_dz=False):
     """act(x w^T + b) + residual: x [..., K], w [N, K] and residual [..., N] of one type (float32, bfloat16, float16),
     b [N] of that type or float32; act "none", "relu", "gelu" (the exact form), "silu" or "tanh".  Products accumulate in
     fp32 in a fixed order and every output is rounded once; a summed axis (K; N for x's gradient, the rows for w's) has at most 2097152
-    elements.  For training in 16 bits act'(z) is kept in 16 bits (its fourth root, in even steps:
-    finer than either type), and the products of backward take dz = dy act'(z) unrounded, in two
-    16-bit parts; round_dz=True rounds it to the type instead: half the matrix work of backward, sqrt(2) times the error of dx and dw."""
+    elements.  For training in 16 bits act'(z) is kept in 16 bits (its fourth root, in even steps: finer than either type), and the
+    products of backward take dz = dy act'(z) unrounded, in two 16-bit parts; round_dz=True rounds it to the type instead: half the matrix work of backward, sqrt(2) times the error of dx and dw."""
     code = _typed("linear_act", x)
     if act not in L.ACTIVATIONS:
         raise RuntimeError("linear_act: act must be one of %s, got %r" % (sorted(L.ACTIVATIONS), act))
